@@ -53,6 +53,16 @@ class Block(ctypes.Structure):
                 ("A_log", _vp), ("D", _vp)]
 
 
+class DecayAttn(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("zero_tail", ctypes.c_int)] + [
+        (n, _c_i64) for n in ("batch", "seqlen", "heads", "q_heads", "k_heads", "v_heads", "dk",
+                              "dv")] + [
+        (n, _vp) for n in ("q", "k", "v", "g", "o")] + [
+        (n, _c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "g_stride", "o_stride")] + [
+        ("h0", _vp), ("h_last", _vp), ("cu_seqlens", _vp), ("n_seqs", _c_i64),
+        ("scale", ctypes.c_float)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "mb2_version": (ctypes.c_int, []),
@@ -127,6 +137,9 @@ _SIGS = {
                                           _vp]),
     "mb2_peer_status": (ctypes.c_int, [ctypes.POINTER(PeerGroup), ctypes.POINTER(ctypes.c_int),
                                        ctypes.c_int]),
+    "mb2_decay_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecayAttn)]),
+    "mb2_decay_attention": (ctypes.c_int, [ctypes.POINTER(DecayAttn), _vp, ctypes.c_size_t, _vp]),
+    "mb2_decay_attention_step": (ctypes.c_int, [ctypes.POINTER(DecayAttn), _vp, _vp]),
     "mb2_fold_norm": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
     "mb2_stack_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Block), _c_i64, _c_i64,
                                                     _c_i64]),

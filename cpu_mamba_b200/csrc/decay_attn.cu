@@ -1,0 +1,498 @@
+// Decay attention: linear attention whose state decays by a scalar per head,
+//   S_t = e^{g_t} S_{t-1} + k_t v_t^T          (S: Dk x Dv, fp32)
+//   o_t = scale * S_t^T q_t
+// for whole prompts (dense (B, T, ...) or packed sequences) and for one token
+// with the state updated in place.  q, k and v may have fewer heads than the
+// H decays; head h reads q head h / (H / Hq) and so on.
+//
+// This file: argument checks, the choice of kernel, the recurrent prompt
+// kernel (any width up to 256, any stride, fp32 arithmetic) and the one-token
+// kernel.
+#include "decay.cuh"
+
+namespace mb2 {
+namespace decay {
+
+// ------------------------------------------------------- recurrent prompt
+// One CTA walks one (sequence, head, column tile) token by token, the state in
+// registers: thread (kg, vg) of a warp owns VT columns and the KT rows
+// dk = 32 i + 4 kg + (0..3), so the eight row groups of a warp read 128
+// consecutive bytes of k and q per shared-memory load.
+//
+// Deferred decay: the registers hold u_t = S_t / A_t, A_t the product of the
+// decays since the last renormalisation.  Then u += k (v / A_t)^T and
+// o = (scale A_t) u^T q: two FMAs per state element and token instead of
+// three operations.  A run ends (u *= A, A = 1) when log A leaves
+// [-5.5, 5.5], so v / A grows by 2^8 at most (|v| > 1e36 would overflow) and
+// every product has the relative precision it has without the factor.
+//
+// Bound: the FP32 pipe, 2 Dk Dv FMAs per token and head.
+constexpr int L = 16;                 // tokens staged at a time
+constexpr float kRun = 5.5f;          // bound on |log A| within a run
+
+template <typename T, int KT, int VT> struct Rec {
+    static constexpr int DK = 8 * KT;       // padded rows
+    static constexpr int WV = 4 * VT;       // columns per warp
+    static constexpr int MAXW = 4;          // warps per CTA
+    static constexpr int PK = DK + 16 / (int)sizeof(T);   // row pitch of q and k in shared memory
+};
+
+template <typename T>
+__device__ __forceinline__ void ld4(const T *p, float (&r)[4]);
+template <> __device__ __forceinline__ void ld4<float>(const float *p, float (&r)[4]) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+}
+template <> __device__ __forceinline__ void ld4<__nv_bfloat16>(const __nv_bfloat16 *p, float (&r)[4]) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    r[0] = __uint_as_float(v.x << 16); r[1] = __uint_as_float(v.x & 0xffff0000u);
+    r[2] = __uint_as_float(v.y << 16); r[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+// p aligned to VT elements
+template <typename T, int VT>
+__device__ __forceinline__ void ldv(const T *p, float (&r)[VT]) {
+    if constexpr (VT == 4) {
+        ld4<T>(p, r);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VT; ++i) r[i] = io<T>::to_f(p[i]);
+    }
+}
+
+// rows [0, n) x cols of a strided matrix into shared memory (pitch `pitch`):
+// 16-byte asynchronous copies where the rows allow them, else element copies
+template <typename T>
+__device__ __forceinline__ void stage(T *dst, int pitch, const T *src, int64_t ld, int n, int cols,
+                                      bool vec) {
+    if (vec) {
+        constexpr int E = 16 / (int)sizeof(T);
+        const int per = cols / E;
+        for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
+            const int r = i / per, c = (i - r * per) * E;
+            cp_async16(dst + r * pitch + c, src + r * ld + c);
+        }
+    } else {
+        for (int i = threadIdx.x; i < n * cols; i += blockDim.x) {
+            const int r = i / cols, c = i - r * cols;
+            dst[r * pitch + c] = src[r * ld + c];
+        }
+    }
+}
+
+template <typename T, int KT, int VT>
+__global__ void __launch_bounds__(128)
+decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec_v) {
+    using R = Rec<T, KT, VT>;
+    constexpr int KI = KT / 4;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const int pv = vtile + 16 / (int)sizeof(T);
+    T *const qs = reinterpret_cast<T *>(smem_raw);         // [2][L][PK]
+    T *const ks = qs + 2 * L * R::PK;                      // [2][L][PK]
+    T *const vs = ks + 2 * L * R::PK;                      // [2][L][pv]
+    __shared__ float s_ren[2][L], s_inv[2][L], s_out[2][L];
+
+    const int tiles = (int)ceil_div(a.dv, vtile);
+    int64_t id = blockIdx.x;
+    const int tile = (int)(id % tiles);
+    id /= tiles;
+    const int h = (int)(id % a.heads);
+    const int64_t seq = id / a.heads;
+    int64_t row0, len;
+    bounds(a, seq, row0, len);
+    const int64_t bq = a.cu ? 0 : seq;
+    const T *q = static_cast<const T *>(a.q) + bq * a.qs[0] + row0 * a.qs[1] + (h / a.q_rep) * a.qs[2];
+    const T *k = static_cast<const T *>(a.k) + bq * a.ks[0] + row0 * a.ks[1] + (h / a.k_rep) * a.ks[2];
+    const int c0 = tile * vtile;
+    const int cols = (int)(a.dv - c0 < vtile ? a.dv - c0 : vtile);
+    const T *v = static_cast<const T *>(a.v) + bq * a.vs[0] + row0 * a.vs[1] +
+                 (h / a.v_rep) * a.vs[2] + c0;
+    const float *g = a.g + bq * a.gs[0] + row0 * a.gs[1] + h * a.gs[2];
+    T *o = static_cast<T *>(a.o) + bq * a.os[0] + row0 * a.os[1] + h * a.os[2] + c0;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int kg = lane & 7, vg = lane >> 3;
+    const int col = warp * R::WV + vg * VT;
+
+    // columns past Dk and Dv are zero for the whole walk
+    for (int i = threadIdx.x; i < 2 * L * R::PK; i += blockDim.x) {
+        qs[i] = io<T>::from_f(0.0f);
+        ks[i] = io<T>::from_f(0.0f);
+    }
+    for (int i = threadIdx.x; i < 2 * L * pv; i += blockDim.x) vs[i] = io<T>::from_f(0.0f);
+
+    float u[KI][4][VT];
+#pragma unroll
+    for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int dk = 32 * i + 4 * kg + j;
+#pragma unroll
+            for (int c = 0; c < VT; ++c)
+                u[i][j][c] = (a.h0 && dk < a.dk && col + c < cols)
+                                 ? a.h0[((seq * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c]
+                                 : 0.0f;
+        }
+    __syncthreads();
+
+    const int nchunks = (int)ceil_div(len, (int64_t)L);
+    auto load = [&](int n) {
+        const int b = n & 1;
+        const int64_t t0 = (int64_t)n * L;
+        const int m = (int)(len - t0 < L ? len - t0 : L);
+        stage<T>(qs + b * L * R::PK, R::PK, q + t0 * a.qs[1], a.qs[1], m, (int)a.dk, vec_q);
+        stage<T>(ks + b * L * R::PK, R::PK, k + t0 * a.ks[1], a.ks[1], m, (int)a.dk, vec_k);
+        stage<T>(vs + b * L * pv, pv, v + t0 * a.vs[1], a.vs[1], m, cols, vec_v);
+        cp_async_commit();
+    };
+    // Per token: the factor on u before it (1: none), 1 / A and scale * A.
+    // log A is a 64-bit sum: a head that forgets over thousands of tokens adds
+    // as many equal decays, whose roundings in 32 bits all point one way.
+    double run = 0.0;                 // log A after the chunk (warp 0)
+    auto factors = [&](int n) {
+        const int b = n & 1;
+        const int64_t t0 = (int64_t)n * L;
+        const int m = (int)(len - t0 < L ? len - t0 : L);
+        const float gt = lane < m ? g[(t0 + lane) * a.gs[1]] : 0.0f;
+        double cum = gt;
+        float ren = 0.0f;
+        bool r = false;
+#pragma unroll
+        for (int s = 1; s < L; s <<= 1) {
+            const double below = __shfl_up_sync(0xffffffffu, cum, s);
+            if (lane >= s) cum += below;
+        }
+        cum += run;
+        // false for NaN and infinities too
+        if (__all_sync(0xffffffffu, lane >= m || fabs(cum) <= kRun)) {
+            run = __shfl_sync(0xffffffffu, cum, m - 1);
+        } else {
+            for (int t = 0; t < m; ++t) {
+                const double next = run + (double)__shfl_sync(0xffffffffu, gt, t);
+                const bool keep = fabs(next) <= kRun;
+                run = keep ? next : 0.0;
+                if (lane == t) { cum = run; ren = (float)next; r = !keep; }
+            }
+        }
+        if (lane < L) {
+            const float hi = (float)cum, lo = (float)(cum - (double)hi);
+            const float dn = expf(-hi), up = expf(hi);
+            s_ren[b][lane] = r ? expf(ren) : 1.0f;
+            s_inv[b][lane] = fmaf(dn, -lo, dn);
+            s_out[b][lane] = fmaf(up, lo, up) * a.scale;
+        }
+    };
+
+    if (nchunks > 0) {
+        load(0);
+        if (warp == 0) factors(0);
+    }
+    for (int n = 0; n < nchunks; ++n) {
+        const int b = n & 1;
+        cp_async_wait<0>();
+        __syncthreads();              // chunk n staged; chunk n - 1 read by every warp
+        if (n + 1 < nchunks) {
+            load(n + 1);
+            if (warp == 0) factors(n + 1);
+        }
+        const int64_t t0 = (int64_t)n * L;
+        const int m = (int)(len - t0 < L ? len - t0 : L);
+        const T *qb = qs + b * L * R::PK + 4 * kg;
+        const T *kb = ks + b * L * R::PK + 4 * kg;
+        const T *vb = vs + b * L * pv + col;
+        for (int t = 0; t < m; ++t) {
+            const float ren = s_ren[b][t];
+            if (ren != 1.0f) {
+#pragma unroll
+                for (int i = 0; i < KI; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int c = 0; c < VT; ++c) u[i][j][c] *= ren;
+            }
+            float w[VT], acc[VT];
+            ldv<T, VT>(vb + t * pv, w);
+            const float inv = s_inv[b][t];
+#pragma unroll
+            for (int c = 0; c < VT; ++c) { w[c] *= inv; acc[c] = 0.0f; }
+#pragma unroll
+            for (int i = 0; i < KI; ++i) {
+                float kv[4], qv[4];
+                ld4<T>(kb + t * R::PK + 32 * i, kv);
+                ld4<T>(qb + t * R::PK + 32 * i, qv);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int c = 0; c < VT; ++c) {
+                        u[i][j][c] = fmaf(kv[j], w[c], u[i][j][c]);
+                        acc[c] = fmaf(qv[j], u[i][j][c], acc[c]);
+                    }
+            }
+#pragma unroll
+            for (int s = 1; s < 8; s <<= 1)
+#pragma unroll
+                for (int c = 0; c < VT; ++c) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], s);
+            float r = acc[0];
+#pragma unroll
+            for (int c = 1; c < VT; ++c) r = kg == c ? acc[c] : r;
+            if (kg < VT && col + kg < cols)
+                o[(t0 + t) * a.os[1] + col + kg] = io<T>::from_f(r * s_out[b][t]);
+        }
+    }
+    if (a.h_last) {
+        // the last run's decay: every thread needs log A of the last token
+        __shared__ float s_last;
+        if (threadIdx.x == 0) s_last = (float)exp(run);
+        __syncthreads();
+        const float f = s_last;
+#pragma unroll
+        for (int i = 0; i < KI; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int dk = 32 * i + 4 * kg + j;
+#pragma unroll
+                for (int c = 0; c < VT; ++c)
+                    if (dk < a.dk && col + c < cols)
+                        a.h_last[((seq * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c] =
+                            u[i][j][c] * f;
+            }
+    }
+}
+
+template <typename T>
+static bool vec16(const void *p, const int64_t (&s)[3], int64_t cols) {
+    constexpr int64_t E = 16 / (int64_t)sizeof(T);
+    return aligned(p, 16) && s[0] % E == 0 && s[1] % E == 0 && s[2] % E == 0 && cols % E == 0;
+}
+
+template <typename T, int KT, int VT>
+static int launch_recurrent(const Args &a, cudaStream_t st) {
+    using R = Rec<T, KT, VT>;
+    const int warps = (int)(ceil_div(a.dv, R::WV) < R::MAXW ? ceil_div(a.dv, R::WV) : R::MAXW);
+    const int vtile = warps * R::WV;
+    const int64_t grid = ceil_div(a.dv, vtile) * a.heads * a.seqs;
+    MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
+    const size_t smem = sizeof(T) * 2 * L * (2 * R::PK + vtile + 16 / sizeof(T));
+    auto kern = decay_recurrent_kernel<T, KT, VT>;
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)smem);
+        if (e != cudaSuccess)
+            return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
+    }
+    kern<<<(unsigned)grid, warps * 32, smem, st>>>(a, vtile, vec16<T>(a.q, a.qs, a.dk),
+                                                   vec16<T>(a.k, a.ks, a.dk),
+                                                   vec16<T>(a.v, a.vs, a.dv));
+    return check_launch("decay_recurrent_kernel");
+}
+
+template <typename T>
+static int recurrent(const Args &a, cudaStream_t st) {
+    if (a.dk <= 32) return launch_recurrent<T, 4, 4>(a, st);
+    if (a.dk <= 64) return launch_recurrent<T, 8, 4>(a, st);
+    if (a.dk <= 128) return launch_recurrent<T, 16, 4>(a, st);
+    return launch_recurrent<T, 32, 2>(a, st);
+}
+
+// rows of o behind the last packed sequence (a freshly allocated o)
+template <typename T>
+__global__ void zero_tail_kernel(const Args a) {
+    const int64_t end = clamp_row(a.cu[a.seqs], a.seqlen);
+    const int64_t per = a.heads * a.dv;
+    T *o = static_cast<T *>(a.o);
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (a.seqlen - end) * per;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t t = end + i / per, r = i % per;
+        o[t * a.os[1] + (r / a.dv) * a.os[2] + r % a.dv] = io<T>::from_f(0.0f);
+    }
+}
+
+// -------------------------------------------------------------- one token
+// HBM-bound: the state is read and written once (8 Dk Dv bytes per head), all
+// else is small.  A CTA takes one (sequence, head, column tile): `lanes`
+// threads per state row of VEC columns each, the CTA's row slots stepping
+// through the Dk rows with ROWS rows' loads in flight per thread.  Partial
+// sums of o over the row slots meet in shared memory, added in a fixed order.
+constexpr int STEP_THREADS = 256;
+template <int VEC> struct vecf;
+template <> struct vecf<4> { using t = float4; };
+template <> struct vecf<1> { using t = float; };
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(STEP_THREADS)
+decay_step_kernel(const Args a, float *__restrict__ state, int lanes) {
+    constexpr int ROWS = 8;
+    using V = typename vecf<VEC>::t;
+    __shared__ float part[STEP_THREADS * VEC];
+    __shared__ float sq[256], sk[256];
+    const int ctile = lanes * VEC;
+    const int tiles = (int)ceil_div(a.dv, ctile);
+    int64_t id = blockIdx.x;
+    const int tile = (int)(id % tiles);
+    id /= tiles;
+    const int h = (int)(id % a.heads);
+    const int64_t b = id / a.heads;
+    const int lane = threadIdx.x % lanes, slot = threadIdx.x / lanes;
+    const int slots = STEP_THREADS / lanes;
+    const int c = tile * ctile + lane * VEC;
+    const bool live = slot < slots && c < a.dv;
+
+    float *const s = state + ((b * a.heads + h) * a.dk) * a.dv + c;
+    const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + (h / a.q_rep) * a.qs[2];
+    const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + (h / a.k_rep) * a.ks[2];
+    const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + (h / a.v_rep) * a.vs[2];
+    // the first rows' loads are issued before q and k are waited for
+    V x[ROWS];
+    const int dk = (int)a.dk;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = slot + i * slots;
+        if (live && r < dk) x[i] = *reinterpret_cast<const V *>(s + (int64_t)r * a.dv);
+    }
+    for (int i = threadIdx.x; i < dk; i += STEP_THREADS) {
+        sq[i] = io<T>::to_f(q[i]) * a.scale;
+        sk[i] = io<T>::to_f(k[i]);
+    }
+    const float dec = expf(a.g[b * a.gs[0] + h * a.gs[2]]);
+    float vv[VEC], acc[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        vv[j] = live ? io<T>::to_f(v[c + j]) : 0.0f;
+        acc[j] = 0.0f;
+    }
+    __syncthreads();
+    if (live) {
+        for (int r0 = slot; r0 < dk; r0 += ROWS * slots) {
+            if (r0 != slot) {
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) {
+                    const int r = r0 + i * slots;
+                    if (r < dk) x[i] = *reinterpret_cast<const V *>(s + (int64_t)r * a.dv);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const int r = r0 + i * slots;
+                if (r < dk) {
+                    float *e = reinterpret_cast<float *>(&x[i]);
+                    const float kr = sk[r], qr = sq[r];
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        e[j] = fmaf(kr, vv[j], dec * e[j]);
+                        acc[j] = fmaf(qr, e[j], acc[j]);
+                    }
+                    *reinterpret_cast<V *>(s + (int64_t)r * a.dv) = x[i];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) part[threadIdx.x * VEC + j] = acc[j];
+    __syncthreads();
+    T *o = static_cast<T *>(a.o) + b * a.os[0] + h * a.os[2];
+    for (int i = threadIdx.x; i < ctile; i += STEP_THREADS) {
+        const int cc = tile * ctile + i;
+        if (cc < a.dv) {
+            float sum = 0.0f;
+            for (int j = 0; j < slots; ++j) sum += part[j * ctile + i];
+            o[cc] = io<T>::from_f(sum);
+        }
+    }
+}
+
+template <typename T>
+static int step(const Args &a, float *state, cudaStream_t st) {
+    const bool vec = a.dv % 4 == 0 && aligned(state, 16);
+    const int per = vec ? 4 : 1;
+    int lanes = (int)(ceil_div(a.dv, per) < 64 ? ceil_div(a.dv, per) : 64);
+    const int64_t grid = ceil_div(a.dv, lanes * per) * a.heads * a.seqs;
+    MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention_step: batch x heads too large");
+    if (vec)
+        decay_step_kernel<T, 4><<<(unsigned)grid, STEP_THREADS, 0, st>>>(a, state, lanes);
+    else
+        decay_step_kernel<T, 1><<<(unsigned)grid, STEP_THREADS, 0, st>>>(a, state, lanes);
+    return check_launch("decay_step_kernel");
+}
+
+static int to_args(const mb2_decay_attn *d, bool one, Args &a) {
+    const char *what = one ? "decay_attention_step" : "decay_attention";
+    MB2_REQUIRE(d, MB2_ERR_ARG, "%s: null descriptor", what);
+    MB2_REQUIRE(d->dtype == MB2_F32 || d->dtype == MB2_BF16, MB2_ERR_ARG, "%s: bad dtype", what);
+    MB2_REQUIRE(d->batch >= 0 && d->seqlen >= 0 && d->n_seqs >= 0, MB2_ERR_SHAPE,
+                "%s: negative size", what);
+    MB2_REQUIRE(d->heads > 0 && d->dk > 0 && d->dv > 0, MB2_ERR_SHAPE,
+                "%s: heads, dk and dv must be positive", what);
+    MB2_REQUIRE(d->heads <= (1 << 20) && d->dv <= (1 << 20), MB2_ERR_SHAPE,
+                "%s: heads or dv above 2^20", what);
+    MB2_REQUIRE(d->dk <= 256, MB2_ERR_SHAPE, "%s: dk %lld > 256 not supported", what,
+                (long long)d->dk);
+    MB2_REQUIRE(d->q_heads > 0 && d->k_heads > 0 && d->v_heads > 0 &&
+                    d->heads % d->q_heads == 0 && d->heads % d->k_heads == 0 &&
+                    d->heads % d->v_heads == 0,
+                MB2_ERR_SHAPE, "%s: the heads of q, k and v must divide the %lld decays", what,
+                (long long)d->heads);
+    MB2_REQUIRE(!d->cu_seqlens || (!one && d->batch == 1), MB2_ERR_SHAPE,
+                "%s: packed sequences need batch 1", what);
+    a.dtype = d->dtype;
+    a.seqs = d->cu_seqlens ? d->n_seqs : d->batch;
+    a.seqlen = d->seqlen;
+    a.heads = d->heads;
+    a.dk = d->dk;
+    a.dv = d->dv;
+    a.q_rep = (int)(d->heads / d->q_heads);
+    a.k_rep = (int)(d->heads / d->k_heads);
+    a.v_rep = (int)(d->heads / d->v_heads);
+    a.q = d->q; a.k = d->k; a.v = d->v; a.g = d->g; a.o = d->o;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = d->q_stride[i];
+        a.ks[i] = d->k_stride[i];
+        a.vs[i] = d->v_stride[i];
+        a.gs[i] = d->g_stride[i];
+        a.os[i] = d->o_stride[i];
+    }
+    a.h0 = d->h0;
+    a.h_last = d->h_last;
+    a.cu = d->cu_seqlens;
+    a.scale = d->scale;
+    return MB2_OK;
+}
+
+}  // namespace decay
+}  // namespace mb2
+
+using namespace mb2;
+
+extern "C" size_t mb2_decay_attention_workspace_bytes(const mb2_decay_attn *d) {
+    (void)d;
+    return 0;
+}
+
+extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, size_t workspace_bytes,
+                                   mb2_stream_t stream) {
+    (void)workspace;
+    (void)workspace_bytes;
+    decay::Args a;
+    MB2_TRY(decay::to_args(d, false, a));
+    if (a.seqs == 0) return MB2_OK;
+    MB2_REQUIRE((a.q && a.k && a.v && a.g && a.o) || a.seqlen == 0, MB2_ERR_ARG,
+                "decay_attention: null pointer");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a.cu && d->zero_tail && a.seqlen > 0) {
+        if (a.dtype == MB2_F32)
+            decay::zero_tail_kernel<float><<<64, 256, 0, st>>>(a);
+        else
+            decay::zero_tail_kernel<__nv_bfloat16><<<64, 256, 0, st>>>(a);
+        MB2_TRY(check_launch("zero_tail_kernel"));
+    }
+    return a.dtype == MB2_F32 ? decay::recurrent<float>(a, st)
+                              : decay::recurrent<__nv_bfloat16>(a, st);
+}
+
+extern "C" int mb2_decay_attention_step(const mb2_decay_attn *d, float *state, mb2_stream_t stream) {
+    decay::Args a;
+    MB2_TRY(decay::to_args(d, true, a));
+    if (a.seqs == 0) return MB2_OK;
+    MB2_REQUIRE(a.q && a.k && a.v && a.g && a.o && state, MB2_ERR_ARG,
+                "decay_attention_step: null pointer");
+    return a.dtype == MB2_F32 ? decay::step<float>(a, state, (cudaStream_t)stream)
+                              : decay::step<__nv_bfloat16>(a, state, (cudaStream_t)stream);
+}

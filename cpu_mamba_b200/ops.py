@@ -7,12 +7,14 @@ stages of the block for tests and for callers composing their own pipeline.
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, lib, ptr, require_cuda, stream_of
+from ._lib import DecayAttn, check, dtype_code, lib, ptr, require_cuda, stream_of
 
 
 def selective_scan(x, dt, A, B, C, D, h0: Optional[torch.Tensor] = None,
@@ -262,3 +264,144 @@ def qlinear(x: torch.Tensor, scheme: str, weight_q: torch.Tensor, scale: torch.T
                             _lib.EPI_SOFTPLUS if softplus else _lib.EPI_NONE, stream_of(x)),
           f"qlinear_{scheme}")
     return y.reshape(*lead, N)
+
+
+# ------------------------------------------------------------ decay attention
+def _one_device(what: str, first: torch.Tensor, *others) -> None:
+    require_cuda(first, *others, what=what)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _on(t: torch.Tensor):
+    """The device of ``t`` as the current one for a launch."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its last index contiguous."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool) -> DecayAttn:
+    """Argument checks shared by the prompt and the one-token form, and the
+    descriptor.  ``tokens``: q, k, v and o carry a token index after the batch."""
+    lead = 2 if tokens else 1
+    names = "(batch, tokens, heads, width)" if tokens else "(batch, heads, width)"
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != lead + 2:
+            raise RuntimeError(f"{what}: {n} must be {names}, got {tuple(t.shape)}")
+        if t.dtype != v.dtype:
+            raise RuntimeError(f"{what}: q, k and v must share a dtype")
+    d = DecayAttn()
+    d.dtype = dtype_code(v.dtype)
+    if g.dtype != torch.float32:
+        raise RuntimeError(f"{what}: g must be float32")
+    if q.shape[:lead] != v.shape[:lead] or k.shape[:lead] != v.shape[:lead] or (
+            q.shape[-1] != k.shape[-1]):
+        raise RuntimeError(f"{what}: shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, "
+                           f"v {tuple(v.shape)}")
+    H = g.shape[-1] if g.dim() else 0
+    if g.dim() != 1 and g.shape != v.shape[:lead] + (H,):
+        raise RuntimeError(f"{what}: g must be (heads,) or {names[:-8]}), got {tuple(g.shape)}")
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.shape[-2] == 0 or t.shape[-1] == 0 or H == 0 or H % t.shape[-2]:
+            raise RuntimeError(f"{what}: the {t.shape[-2]} heads of {n} (width {t.shape[-1]}) "
+                               f"must divide the {H} decays of g")
+    d.batch, d.seqlen = v.shape[0], v.shape[1] if tokens else 1
+    d.heads, d.q_heads, d.k_heads, d.v_heads = H, q.shape[-2], k.shape[-2], v.shape[-2]
+    d.dk, d.dv = q.shape[-1], v.shape[-1]
+    if o.shape != v.shape[:lead] + (H, d.dv) or o.dtype != v.dtype or (
+            o.stride(-1) != 1 and o.shape[-1] > 1):
+        raise RuntimeError(f"{what}: out must be {tuple(v.shape[:lead]) + (H, d.dv)} in "
+                           f"{v.dtype} with its last index contiguous")
+    for n, t in (("q", q), ("k", k), ("v", v), ("o", o)):
+        s = t.stride()
+        setattr(d, n, t.data_ptr())
+        setattr(d, n + "_stride", (s[0], s[1] if tokens else 0, s[-2]))
+    d.g = g.data_ptr()
+    s = g.stride()
+    d.g_stride = (0, 0, s[0]) if g.dim() == 1 else (s[0], s[1] if tokens else 0, s[-1])
+    d.scale = scale
+    return d
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                    scale: float = 1.0, initial_state: Optional[torch.Tensor] = None,
+                    cu_seqlens: Optional[torch.Tensor] = None, return_final_state: bool = False,
+                    out: Optional[torch.Tensor] = None):
+    """Linear attention with a decay for each head, over whole prompts:
+
+        S_t = exp(g_t) S_{t-1} + k_t v_t^T,     o_t = scale * S_t^T q_t
+
+    q: (B, T, Hq, Dk), k: (B, T, Hk, Dk), v: (B, T, Hv, Dv), float32 or bfloat16
+    (any strides with a contiguous last index); g: float32 log decays (B, T, H)
+    or (H,); Hq, Hk and Hv divide H, and head h reads q head h // (H // Hq).
+    Dk <= 256.  initial_state: float32 (N, H, Dk, Dv), zeros when None.
+
+    cu_seqlens (int, N + 1 offsets on the device) packs N sequences along T with
+    B = 1; rows behind the last one are zero in a new output and untouched in
+    ``out``.  Otherwise N = B.
+
+    Returns o (B, T, H, Dv), with the final state (N, H, Dk, Dv) float32 when
+    ``return_final_state``.  An empty sequence's final state is its initial one;
+    g = -inf forgets the state.  Forward only."""
+    what = "decay_attention"
+    _one_device(what, q, k, v, g, initial_state, cu_seqlens, out)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if v.dim() != 4 or g.dim() not in (1, 3):
+        raise RuntimeError(f"{what}: v must be (batch, tokens, heads, width) and g (heads,) or "
+                           f"(batch, tokens, heads), got {tuple(v.shape)} and {tuple(g.shape)}")
+    H = g.shape[-1]
+    o = out if out is not None else torch.empty(*v.shape[:2], H, v.shape[3], device=v.device,
+                                                dtype=v.dtype)
+    d = _decay_descriptor(what, q, k, v, g, scale, o, True)
+    n = d.batch
+    if cu_seqlens is not None:
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or d.batch != 1 or (
+                cu_seqlens.dtype not in (torch.int32, torch.int64)):
+            raise RuntimeError(f"{what}: cu_seqlens must hold N + 1 integer offsets into a "
+                               "batch of 1")
+        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        n = cu_seqlens.shape[0] - 1
+        d.cu_seqlens, d.n_seqs, d.zero_tail = cu_seqlens.data_ptr(), n, int(out is None)
+    shape = (n, H, d.dk, d.dv)
+    if initial_state is not None:
+        if initial_state.shape != shape or initial_state.dtype != torch.float32:
+            raise RuntimeError(f"{what}: initial_state must be float32 {shape}")
+        initial_state = initial_state.contiguous()
+        d.h0 = initial_state.data_ptr()
+    h_last = None
+    if return_final_state:
+        h_last = torch.empty(shape, device=v.device, dtype=torch.float32)
+        d.h_last = h_last.data_ptr()
+    with _on(v):
+        nbytes = lib().mb2_decay_attention_workspace_bytes(ctypes.byref(d))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=v.device) if nbytes else None
+        check(lib().mb2_decay_attention(ctypes.byref(d), ptr(ws), nbytes, stream_of(v)), what)
+    return (o, h_last) if return_final_state else o
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                         state: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """decay_attention for one token: q (B, Hq, Dk), k (B, Hk, Dk), v (B, Hv, Dv),
+    g (B, H) or (H,); ``state`` (B, H, Dk, Dv) float32 contiguous is advanced in
+    place.  Returns o (B, H, Dv)."""
+    what = "decay_attention_step"
+    _one_device(what, q, k, v, g, state)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if v.dim() != 3 or g.dim() not in (1, 2):
+        raise RuntimeError(f"{what}: v must be (batch, heads, width) and g (heads,) or "
+                           f"(batch, heads), got {tuple(v.shape)} and {tuple(g.shape)}")
+    o = torch.empty(v.shape[0], g.shape[-1], v.shape[2], device=v.device, dtype=v.dtype)
+    d = _decay_descriptor(what, q, k, v, g, scale, o, False)
+    if (state.shape != (d.batch, d.heads, d.dk, d.dv) or state.dtype != torch.float32
+            or not state.is_contiguous()):
+        raise RuntimeError(f"{what}: state must be contiguous float32 "
+                           f"{(d.batch, d.heads, d.dk, d.dv)}")
+    with _on(v):
+        check(lib().mb2_decay_attention_step(ctypes.byref(d), ptr(state), stream_of(v)), what)
+    return o

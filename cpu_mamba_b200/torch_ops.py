@@ -13,6 +13,8 @@ torch custom ops, callable as ``torch.ops.mamba_b200.<name>`` and traceable
   qlinear(x, weight_q, scale, bias?, scheme, in_dim, group_size=0) -> y
   mamba_step(x, h, conv_state, in_proj_w, conv_w, conv_b?, x_proj_w, dt_proj_w,
              dt_proj_b?, A_log, D, out_proj_w) -> y   (h, conv_state updated in place)
+  decay_attention(q, k, v, g, scale=1, h0?, cu_seqlens?) -> (o, h_last)
+  decay_attention_step(q, k, v, g, state, scale=1) -> o       (state updated in place)
 
 Each runs the C-ABI kernels on the inputs' CUDA device and current stream
 (no CPU implementation: CPU tensors raise, as the rest of the package does).
@@ -151,3 +153,31 @@ def mamba_step(x: torch.Tensor, h: torch.Tensor, conv_state: torch.Tensor,
 def _(x, h, conv_state, in_proj_w, conv_w, conv_b, x_proj_w, dt_proj_w, dt_proj_b, A_log, D,
       out_proj_w):
     return torch.empty_like(x)
+
+
+@torch.library.custom_op(f"{NS}::decay_attention", mutates_args=())
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                    scale: float = 1.0, h0: Optional[torch.Tensor] = None,
+                    cu_seqlens: Optional[torch.Tensor] = None) -> tuple[torch.Tensor,
+                                                                        torch.Tensor]:
+    return ops.decay_attention(q, k, v, g, scale=scale, initial_state=h0, cu_seqlens=cu_seqlens,
+                               return_final_state=True)
+
+
+@decay_attention.register_fake
+def _(q, k, v, g, scale=1.0, h0=None, cu_seqlens=None):
+    H = g.shape[-1]
+    n = v.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    return (v.new_empty(*v.shape[:2], H, v.shape[3]),
+            v.new_empty(n, H, q.shape[3], v.shape[3], dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{NS}::decay_attention_step", mutates_args=("state",))
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                         state: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    return ops.decay_attention_step(q, k, v, g, state, scale=scale)
+
+
+@decay_attention_step.register_fake
+def _(q, k, v, g, state, scale=1.0):
+    return v.new_empty(v.shape[0], g.shape[-1], v.shape[2])

@@ -412,6 +412,45 @@ int mb2_peer_status(const mb2_peer_group *g, int *code, int clear);
 int mb2_block_step_static(const mb2_block *blk, const void *x, void *out, float *h,
                           void *conv_state, int64_t batch, mb2_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Decay attention: linear attention whose state decays by a scalar per head.
+ * No counterpart in the reference, whose scan decays per channel and state
+ * (src/cpu_mamba/selective_scan_cpu.cpp:19-87).
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T      S: (dk, dv), fp32
+ *   o_t = scale * S_t^T q_t
+ * q (batch, seqlen, q_heads, dk), k (.., k_heads, dk), v (.., v_heads, dv),
+ * o (.., heads, dv) in dtype; g fp32 (batch, seqlen, heads).  Strides are in
+ * elements, ordered batch, token, head; the last index is contiguous; a zero
+ * g_stride repeats a decay.  heads is a multiple of q_heads, k_heads and
+ * v_heads; head h reads q head h / (heads / q_heads).  dk <= 256.
+ * h0 (or NULL: zeros) and h_last (or NULL): (sequences, heads, dk, dv) fp32
+ * contiguous.  A g of -inf resets the state.
+ * cu_seqlens (device, n_seqs + 1 offsets): batch must be 1 and sequence i is
+ * rows cu[i] .. cu[i+1]-1 of the seqlen rows; rows behind the last sequence
+ * are zeroed when zero_tail is set and left alone otherwise.  Offsets are
+ * clamped to 0 .. seqlen; a sequence whose end is not behind its start is
+ * empty (its h_last is its h0). */
+typedef struct mb2_decay_attn {
+    int dtype;
+    int zero_tail;
+    int64_t batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv;
+    const void *q, *k, *v;
+    const float *g;
+    void *o;
+    int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], o_stride[3];
+    const float *h0;
+    float *h_last;
+    const int32_t *cu_seqlens;
+    int64_t n_seqs;
+    float scale;
+} mb2_decay_attn;
+size_t mb2_decay_attention_workspace_bytes(const mb2_decay_attn *d);
+int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, size_t workspace_bytes,
+                        mb2_stream_t stream);
+/* One token: seqlen and the token strides are ignored, state (batch, heads,
+ * dk, dv) fp32 is advanced in place. */
+int mb2_decay_attention_step(const mb2_decay_attn *d, float *state, mb2_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,380 @@
+"""Decay attention, S_t = e^{g_t} S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t:
+the prompt form (dense and packed) and the one-token form, against the
+recurrence in 64 bits; refusals on the CPU."""
+import pytest
+import torch
+
+from cpu_mamba_b200 import _lib, ops
+
+gpu = pytest.mark.gpu
+
+
+def reference(q, k, v, g, scale, h0=None):
+    """(o, final state, bound): the recurrence in 64 bits for (B, T, H, width)
+    inputs with all heads spelled out, and the same recurrence on absolute
+    values, which bounds the sum of the magnitudes of an output's terms."""
+    q, k, v = q.double(), k.double(), v.double()
+    B, T, H, dv = v.shape
+    s = torch.zeros(B, H, q.shape[-1], dv, dtype=torch.float64) if h0 is None else h0.double()
+    m = s.abs()
+    o, ob = torch.empty(B, T, H, dv, dtype=torch.float64), torch.empty(B, T, H, dv).double()
+    for t in range(T):
+        a = torch.exp(g[:, t].double())[..., None, None]
+        kv = k[:, t].unsqueeze(-1) * v[:, t].unsqueeze(-2)
+        s, m = a * s + kv, a * m + kv.abs()
+        o[:, t] = scale * (q[:, t].unsqueeze(-1) * s).sum(-2)
+        ob[:, t] = abs(scale) * (q[:, t].abs().unsqueeze(-1) * m).sum(-2)
+    return o, s, ob, m
+
+
+def spread(x, H):
+    return x.repeat_interleave(H // x.shape[2], dim=2)
+
+
+def make(B, T, H, Hq, Hk, Hv, dk, dv, dtype, seed, per_head=False, strong=False):
+    r = torch.Generator().manual_seed(seed)
+    q = torch.randn(B, T, Hq, dk, generator=r).to(dtype)
+    k = torch.randn(B, T, Hk, dk, generator=r).to(dtype)
+    v = torch.randn(B, T, Hv, dv, generator=r).to(dtype)
+    top = 30.0 if strong else 0.3
+    g = -torch.rand(H, generator=r) * top if per_head else -torch.rand(B, T, H, generator=r) * top
+    h0 = torch.randn(B, H, dk, dv, generator=r) * 2
+    return q, k, v, g, h0
+
+
+def tolerance(dtype, T, dk, o, ob):
+    """fp32: an output is a sum of terms that pass through at most 3 roundings a
+    token (decay, product, sum), dk additions and a few factors, each off by
+    2^-24 relative: (3 T + dk + 32) 2^-24 times the sum of the terms' sizes.
+    bf16 adds the output's rounding (2^-8 of it) and, on the tensor cores, the
+    rounding to bf16 of the decayed scores and of the carried state (2^-8 of
+    each term)."""
+    f = (3 * T + dk + 32) * 2.0 ** -24
+    if dtype == torch.float32:
+        return f * ob
+    return 2.0 ** -8 * (1 + 2.0 ** -8) * (o.abs() + ob) + f * ob
+
+
+def state_tolerance(T, m):
+    # fp32 throughout: 3 roundings a token and a few factors; bf16 inputs whose
+    # decayed values are split into three bf16 parts lose 2^-26 more of a term
+    return (3 * T + 32) * 2.0 ** -24 * m + 1e-30
+
+
+def check(o, s, ref, dtype, T, dk):
+    ro, rs, ob, m = ref
+    d = (o.double().cpu() - ro).abs()
+    assert bool((d <= tolerance(dtype, T, dk, ro, ob) + 1e-30).all()), (
+        d / (tolerance(dtype, T, dk, ro, ob) + 1e-30)).max().item()
+    if s is not None:
+        d = (s.double().cpu() - rs).abs()
+        assert bool((d <= state_tolerance(T, m)).all()), (d / state_tolerance(T, m)).max().item()
+
+
+SHAPES = [  # B, T, H, Hq, Hk, Hv, dk, dv
+    (1, 1, 1, 1, 1, 1, 1, 1),
+    (2, 2, 2, 1, 2, 2, 3, 5),
+    (2, 15, 4, 2, 1, 4, 16, 16),
+    (1, 16, 2, 2, 2, 1, 32, 64),
+    (3, 17, 6, 3, 6, 2, 20, 36),
+    (2, 64, 2, 1, 1, 2, 64, 64),
+    (1, 127, 2, 2, 2, 2, 128, 128),
+    (1, 128, 3, 1, 1, 3, 128, 64),
+    (2, 129, 2, 1, 1, 2, 64, 72),
+    (1, 300, 2, 2, 1, 2, 24, 64),
+    (1, 257, 1, 1, 1, 1, 104, 200),
+    (1, 70, 1, 1, 1, 1, 200, 33),
+    (1, 40, 2, 1, 2, 2, 256, 130),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_prompt_matches_the_recurrence(shape, dtype):
+    B, T, H, Hq, Hk, Hv, dk, dv = shape
+    q, k, v, g, h0 = make(*shape, dtype, seed=T + dk, per_head=T % 2 == 0)
+    ref = reference(spread(q, H), spread(k, H), spread(v, H), g.expand(B, T, H), 0.7, h0)
+    o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), scale=0.7,
+                               initial_state=h0.cuda(), return_final_state=True)
+    assert o.dtype == dtype and o.shape == (B, T, H, dv) and s.dtype == torch.float32
+    check(o, s, ref, dtype, T, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strong_decays_and_resets(dtype):
+    """Decays down to e^-30 a token, a reset (g = -inf) in the middle, no
+    initial state."""
+    B, T, H, dk, dv = 2, 150, 2, 64, 64
+    q, k, v, g, _ = make(B, T, H, 1, 2, 2, dk, dv, dtype, seed=3, strong=True)
+    g[:, :50] *= 0.01
+    g[0, 70, 0] = float("-inf")
+    g[1, 0, 1] = float("-inf")
+    g[:, 100:] = 0.0
+    ref = reference(spread(q, H), spread(k, H), v, g, 1.0)
+    o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), return_final_state=True)
+    check(o, s, ref, dtype, T, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weak_decay_over_a_long_sequence(dtype):
+    """A head that forgets over 4096 tokens: the products of thousands of equal
+    decays hold (all terms positive, so nothing hides in cancellation)."""
+    B, T, H, dk, dv = 1, 6000, 1, 8, 8
+    r = torch.Generator().manual_seed(1)
+    q = torch.rand(B, T, H, dk, generator=r).to(dtype)
+    k = torch.rand(B, T, H, dk, generator=r).to(dtype)
+    v = torch.rand(B, T, H, dv, generator=r).to(dtype)
+    g = torch.log1p(torch.tensor([-2.0 ** -12]))
+    ref = reference(q, k, v, g.expand(B, T, H), 1.0)
+    o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), return_final_state=True)
+    rel = ((s.double().cpu() - ref[1]) / ref[1]).abs().max().item()
+    # 6000 sums of positive terms in fp32, each rounding within 2^-24 and of either
+    # sign: 5 sqrt(6000) 2^-24 = 2.3e-5 bounds their random walk
+    assert rel <= 2.3e-5, rel
+    check(o, s, ref, dtype, T, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_packed_sequences(dtype):
+    """Lengths 0, 1, odd, over several tiles; rows behind the last sequence."""
+    lens = [5, 0, 1, 130, 63, 200, 17]
+    H, dk, dv = 4, 64, 48
+    T = sum(lens) + 9
+    q, k, v, g, _ = make(1, T, H, 2, 1, 4, dk, dv, dtype, seed=11)
+    h0 = torch.randn(len(lens), H, dk, dv, generator=torch.Generator().manual_seed(2))
+    cu = torch.tensor([0] + lens).cumsum(0)
+    # what stands behind the last sequence must not matter
+    for t in (q, k, v):
+        t[:, -9:] = float("nan")
+    out = torch.full((1, T, H, dv), 7.0, dtype=dtype, device="cuda")
+    args = [t.cuda() for t in (q, k, v, g)]
+    o, s = ops.decay_attention(*args, initial_state=h0.cuda(), cu_seqlens=cu.cuda(),
+                               return_final_state=True, out=out)
+    assert o.data_ptr() == out.data_ptr() and bool((out[:, -9:] == 7).all())
+    new = ops.decay_attention(*args, initial_state=h0.cuda(), cu_seqlens=cu.cuda().int())
+    assert bool((new[:, -9:] == 0).all()) and torch.equal(new[:, :-9], out[:, :-9])
+    for i, n in enumerate(lens):
+        a, b = int(cu[i]), int(cu[i + 1])
+        if n == 0:
+            assert torch.equal(s[i].cpu(), h0[i])
+            continue
+        ref = reference(spread(q[:, a:b], H), spread(k[:, a:b], H), v[:, a:b], g[:, a:b], 1.0,
+                        h0[i:i + 1])
+        check(o[:, a:b], s[i:i + 1], ref, dtype, n, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_column_slices(dtype):
+    """q, k, v as slices of one projection's rows, and transposed (heads before
+    tokens) inputs, give the bits of contiguous ones."""
+    B, T, H, dk, dv = 2, 140, 2, 64, 64
+    r = torch.Generator().manual_seed(9)
+    x = torch.randn(B, T, 2 * dk + H * dv + 8, generator=r).to(dtype).cuda()
+    q, k = x[..., :dk].unsqueeze(2), x[..., dk:2 * dk].unsqueeze(2)
+    v = x[..., 2 * dk:2 * dk + H * dv].unflatten(-1, (H, dv))
+    g = (-torch.rand(B, T, H, generator=r)).cuda()
+    a = ops.decay_attention(q, k, v, g)
+    b = ops.decay_attention(q.contiguous(), k.contiguous(), v.contiguous(), g)
+    assert torch.equal(a, b)
+    vt = v.transpose(1, 2).contiguous().transpose(1, 2)
+    gt = g.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(ops.decay_attention(q, k, vt, gt), a)
+    odd = torch.randn(B, T, 1 + H * dv, generator=r).to(dtype).cuda()
+    vo = odd[..., 1:].unflatten(-1, (H, dv))                 # rows off every 16-byte boundary
+    check(ops.decay_attention(q, k, vo, g), None,
+          reference(spread(q.cpu(), H), spread(k.cpu(), H), vo.cpu(), g.cpu(), 1.0), dtype, T, dk)
+    rev = v.transpose(2, 3).contiguous().transpose(2, 3)     # last index not contiguous
+    assert torch.equal(ops.decay_attention(q, k, rev, g), a)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_later_tokens_do_not_reach_back(dtype):
+    """Infinities and NaN in a token leave every earlier output as it was."""
+    B, T, H, dk, dv = 1, 200, 2, 64, 64
+    q, k, v, g, h0 = make(B, T, H, 1, 1, 2, dk, dv, dtype, seed=4)
+    args = [t.cuda() for t in (q, k, v, g)]
+    clean = ops.decay_attention(*args, initial_state=h0.cuda())
+    v[:, 150, 0] = float("inf")
+    k[:, 170] = float("nan")
+    got = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), initial_state=h0.cuda())
+    ref = reference(spread(q, H), spread(k, H), v, g, 1.0, h0)
+    check(got[:, :150], None, tuple(t[:, :150] if t.dim() == 4 and t.shape[1] == T else t
+                                    for t in ref), dtype, T, dk)
+    assert bool(torch.isfinite(got[:, :150]).all())
+    assert bool(torch.isfinite(got[:, 150:170, 1]).all())
+    assert not bool(torch.isfinite(got[:, 150:, 0]).any())
+    assert bool(torch.isnan(got[:, 170:]).all())
+    assert torch.equal(clean[:, :128], got[:, :128])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 1, 1), (3, 6, 3, 1, 2, 20, 36),
+                                   (5, 4, 4, 4, 4, 128, 128), (2, 2, 1, 1, 2, 64, 300),
+                                   (70, 8, 1, 1, 8, 128, 64), (1, 2, 1, 2, 1, 256, 33)])
+def test_one_token(shape, dtype):
+    B, H, Hq, Hk, Hv, dk, dv = shape
+    q, k, v, g, h0 = make(B, 1, H, Hq, Hk, Hv, dk, dv, dtype, seed=dk)
+    ref = reference(spread(q, H), spread(k, H), spread(v, H), g, 0.5, h0)
+    s = h0.cuda()
+    o = ops.decay_attention_step(q[:, 0].cuda(), k[:, 0].cuda(), v[:, 0].cuda(), g[:, 0].cuda(), s,
+                                 scale=0.5)
+    assert o.shape == (B, H, dv) and o.dtype == dtype
+    check(o.unsqueeze(1), s, ref, dtype, 1, dk)
+    s2 = h0.cuda()
+    gh = g[0, 0].clone()
+    o2 = ops.decay_attention_step(q[:1, 0].cuda(), k[:1, 0].cuda(), v[:1, 0].cuda(), gh.cuda(),
+                                  s2[:1], scale=0.5)
+    assert torch.equal(o2[0], o[0]) and torch.equal(s2[0], s[0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompt_then_tokens(dtype):
+    """A prompt's final state continued token by token, on a side stream and as a
+    replayed graph, gives the outputs of the whole sequence."""
+    B, T, n, H, dk, dv = 2, 90, 4, 2, 64, 64
+    q, k, v, g, _ = make(B, T, H, 1, 1, 2, dk, dv, dtype, seed=6)
+    ref = reference(spread(q, H), spread(k, H), v, g, 1.0)
+    q, k, v, g = (t.cuda() for t in (q, k, v, g))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o, s = ops.decay_attention(*(t[:, :T - n] for t in (q, k, v, g)), return_final_state=True)
+        outs = [o]
+        outs += [ops.decay_attention_step(q[:, T - n], k[:, T - n], v[:, T - n], g[:, T - n],
+                                          s).unsqueeze(1)]
+    torch.cuda.current_stream().wait_stream(side)
+    cur = [t[:, 0].clone() for t in (q, k, v, g)]
+    graph = torch.cuda.CUDAGraph()
+    keep = s.clone()
+    with torch.cuda.graph(graph):
+        y = ops.decay_attention_step(*cur, s)
+    assert torch.equal(s, keep)
+    for t in range(T - n + 1, T):
+        for c, x in zip(cur, (q, k, v, g)):
+            c.copy_(x[:, t])
+        graph.replay()
+        outs.append(y.clone().unsqueeze(1))
+    check(torch.cat(outs, 1), s, ref, dtype, T, dk)
+
+
+@gpu
+def test_prompt_in_a_graph_matches_eager():
+    q, k, v, g, h0 = (t.cuda() for t in make(2, 300, 4, 1, 1, 4, 64, 64, torch.bfloat16, seed=8))
+    cu = torch.tensor([0, 100, 300], device="cuda", dtype=torch.int32)
+    a = ops.decay_attention(q, k, v, g, initial_state=h0)
+    p = ops.decay_attention(q[:1], k[:1], v[:1], g[:1], cu_seqlens=cu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ya = ops.decay_attention(q, k, v, g, initial_state=h0)
+        yp = ops.decay_attention(q[:1], k[:1], v[:1], g[:1], cu_seqlens=cu)
+    for _ in range(2):
+        ya.fill_(3)
+        yp.fill_(3)
+        graph.replay()
+        assert torch.equal(ya, a) and torch.equal(yp, p)
+
+
+@gpu
+def test_broken_offsets_stay_inside():
+    """Offsets out of order or out of range address no row outside the tensors
+    (they are clamped); no sequence at all leaves zeros."""
+    q, k, v, g, _ = (t.cuda() for t in make(1, 50, 2, 1, 1, 2, 32, 32, torch.float32, seed=5))
+    for cu in ([0, 40, 20, 99], [-5, 10, 10, 50], [50, 50]):
+        o = ops.decay_attention(q, k, v, g, cu_seqlens=torch.tensor(cu, device="cuda"))
+        assert o.shape == v.shape
+    z, s = ops.decay_attention(q, k, v, g, cu_seqlens=torch.zeros(1, device="cuda").int(),
+                               return_final_state=True)
+    assert s.shape[0] == 0
+
+
+@gpu
+def test_empty_prompt_returns_the_state():
+    q, k, v, g, h0 = (t.cuda() for t in make(2, 0, 2, 1, 1, 2, 32, 32, torch.float32, seed=5))
+    o, s = ops.decay_attention(q, k, v, g, initial_state=h0, return_final_state=True)
+    assert o.shape == (2, 0, 2, 32) and torch.equal(s, h0)
+    _, s = ops.decay_attention(q, k, v, g, return_final_state=True)
+    assert bool((s == 0).all())
+
+
+@gpu
+def test_torch_ops():
+    q, k, v, g, h0 = (t.cuda() for t in make(1, 20, 2, 1, 1, 2, 16, 16, torch.float32, seed=5))
+    o, s = ops.decay_attention(q, k, v, g, initial_state=h0, return_final_state=True)
+    o2, s2 = torch.ops.mamba_b200.decay_attention(q, k, v, g, 1.0, h0, None)
+    assert torch.equal(o, o2) and torch.equal(s, s2)
+    st = s.clone()
+    y = torch.ops.mamba_b200.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], st, 1.0)
+    assert torch.equal(y, ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], s))
+    assert torch.equal(s, st)
+
+
+# ------------------------------------------------------------- refusals (CPU)
+def desc(**kw):
+    d = _lib.DecayAttn()
+    d.batch, d.seqlen, d.heads, d.q_heads, d.k_heads, d.v_heads, d.dk, d.dv = 1, 4, 2, 1, 1, 2, 8, 8
+    for n, x in kw.items():
+        setattr(d, n, x)
+    return d
+
+
+@pytest.mark.parametrize("kw,code", [({"dtype": 5}, 1), ({"batch": -1}, 2), ({"dk": 257}, 2),
+                                     ({"dk": 0}, 2), ({"dv": 0}, 2), ({"q_heads": 3}, 2),
+                                     ({"v_heads": 0}, 2), ({"heads": 0}, 2), ({}, 1),
+                                     ({"batch": 2, "cu_seqlens": 16, "n_seqs": 1}, 2)])
+def test_c_entry_refuses(kw, code):
+    import ctypes
+    lib = _lib.lib()
+    assert lib.mb2_decay_attention(ctypes.byref(desc(**kw)), None, 0, None) == code
+    assert b"decay_attention" in lib.mb2_last_error()
+    assert lib.mb2_decay_attention_step(ctypes.byref(desc(**kw)), None, None) == code
+    assert lib.mb2_decay_attention(None, None, 0, None) == 1
+
+
+def test_c_entry_nothing_to_do():
+    import ctypes
+    lib = _lib.lib()
+    assert lib.mb2_decay_attention(ctypes.byref(desc(batch=0)), None, 0, None) == 0
+    assert lib.mb2_decay_attention_step(ctypes.byref(desc(batch=0)), None, None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    q, k, v, g, h0 = make(1, 4, 2, 1, 1, 2, 8, 8, torch.float32, seed=1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.decay_attention(q, k, v, g)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], h0)
+
+
+@gpu
+def test_refusals():
+    q, k, v, g, h0 = (t.cuda() for t in make(2, 6, 4, 1, 2, 4, 8, 8, torch.float32, seed=1))
+    f = ops.decay_attention
+    bad = [
+        lambda: f(q[0], k, v, g), lambda: f(q, k.bfloat16(), v, g), lambda: f(q, k, v, g.double()),
+        lambda: f(q[:, :5], k, v, g), lambda: f(q[..., :7], k, v, g), lambda: f(q, k, v, g[..., :3]),
+        lambda: f(q, k, v, g[:, :, 0]), lambda: f(q, k, v, g, initial_state=h0[:1]),
+        lambda: f(q, k, v, g, initial_state=h0.bfloat16()),
+        lambda: f(q, k, v, g, cu_seqlens=torch.tensor([0, 6], device="cuda")),
+        lambda: f(q[:1], k[:1], v[:1], g[:1], cu_seqlens=torch.tensor([0., 6.], device="cuda")),
+        lambda: f(q, k, v, g, out=v.bfloat16()), lambda: f(q, k, v, g, out=v[:, :5]),
+        lambda: f(q, k, v.cpu(), g),
+        lambda: ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], h0[:, :3]),
+        lambda: ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], h0.transpose(2, 3)),
+        lambda: ops.decay_attention_step(q, k, v, g, h0),
+    ]
+    for call in bad:
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(TypeError):
+        f(q.double(), k.double(), v.double(), g)
+    wide = torch.zeros(1, 3, 1, 257, device="cuda")
+    with pytest.raises(RuntimeError, match="257"):
+        f(wide, wide, wide, torch.zeros(1, device="cuda"))
