@@ -63,6 +63,16 @@ class DecayAttn(ctypes.Structure):
         ("scale", ctypes.c_float)]
 
 
+class GatedNorm(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("residual_dtype", ctypes.c_int)] + [
+        (n, _c_i64) for n in ("rows", "width", "group")] + [
+        (n, _vp) for n in ("x", "gate", "weight", "residual", "residual_scale", "next_weight",
+                           "out", "next_out")] + [
+        (n, _c_i64) for n in ("ld_x", "ld_gate", "ld_residual", "ld_out", "ld_next")] + [
+        ("scale", ctypes.c_float), ("eps", ctypes.c_float)] + [
+        (n, ctypes.c_int) for n in ("norm_before_gate", "weight_f32", "scale_f32", "next_f32")]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "mb2_version": (ctypes.c_int, []),
@@ -140,6 +150,11 @@ _SIGS = {
     "mb2_decay_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecayAttn)]),
     "mb2_decay_attention": (ctypes.c_int, [ctypes.POINTER(DecayAttn), _vp, ctypes.c_size_t, _vp]),
     "mb2_decay_attention_step": (ctypes.c_int, [ctypes.POINTER(DecayAttn), _vp, _vp]),
+    "mb2_gated_norm": (ctypes.c_int, [ctypes.POINTER(GatedNorm), _vp]),
+    "mb2_beam_select_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] + [_c_i64] * 4),
+    "mb2_beam_select": (ctypes.c_int, [ctypes.c_int, _vp, _c_i64, _c_i64, _vp, _vp] + [_c_i64] * 5 +
+                        [_vp] * 4 + [ctypes.c_size_t, _vp]),
+    "mb2_reorder_rows": (ctypes.c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp]),
     "mb2_fold_norm": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
     "mb2_stack_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Block), _c_i64, _c_i64,
                                                     _c_i64]),

@@ -1,0 +1,478 @@
+// Beam search on the GPU: the selection over beams and vocabulary, and the
+// reordering of the beams' recurrent states.
+//
+// beam_select: candidate (k, v) of a batch has the value
+//   scores[k] + logits[k, v] - log sum_v' exp(logits[k, v'])
+// and the best `num` of all K V candidates come out in order, ties to the
+// lowest beam, then the lowest token.  Two kernels:
+//   beam_rows   one CTA per (row, slice of 8192 logits or so): the slice stays
+//               in registers, so the logits are read once; its maximum, its sum
+//               of exponentials and its best `num` (value, token) pairs
+//   beam_merge  one CTA per batch: the rows' normalisers (64-bit sums of the
+//               slices') and a merge of the slices' sorted lists, comparing the
+//               candidates' 64-bit values
+// Bound: the logits' read (HBM).
+#include "common.cuh"
+
+namespace mb2 {
+namespace {
+
+constexpr int ROW_THREADS = 256;
+constexpr int EPT = 32;                       // logits per thread
+constexpr int SLICE = ROW_THREADS * EPT;
+constexpr int LIST = 1024;                    // candidates above a slice's threshold
+constexpr int MAX_NUM = 64;
+constexpr int MAX_BEAMS = 32;
+constexpr int MAX_VOCAB = 1 << 20;
+
+// fp32 ordered as unsigned, 0 below every value; NaN orders as -inf
+__device__ __forceinline__ uint32_t order_key(float v) {
+    if (v != v) v = -INFINITY;
+    const uint32_t b = __float_as_uint(v + 0.0f);           // -0 -> +0
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
+
+struct RowArgs {
+    const void *logits;
+    int64_t s_batch, s_beam;                  // strides
+    int beams, vocab, num, splits;
+    const uint8_t *finished;
+    float *part_max, *part_sum;               // (rows, splits)
+    uint64_t *part_list;                      // (rows, splits, num): key << 32 | ~token, 0: none
+};
+
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS)
+beam_rows_kernel(const RowArgs a) {
+    constexpr int VEC = 16 / (int)sizeof(T), NV = EPT / VEC;
+    __shared__ uint64_t list[LIST];
+    __shared__ uint64_t best[ROW_THREADS / 32];
+    __shared__ float redf[2][ROW_THREADS / 32];
+    __shared__ int count;
+    const int split = blockIdx.x, row = blockIdx.y;
+    if (a.finished && a.finished[row]) return;              // beam_merge writes its candidates
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    const T *p = static_cast<const T *>(a.logits) + (int64_t)(row / a.beams) * a.s_batch +
+                 (int64_t)(row % a.beams) * a.s_beam;
+    // 16-byte loads from the aligned address at or below the row's start; the
+    // elements outside the row are dropped (their 16 bytes hold one inside it)
+    const int lead = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+    const T *base = p - lead;
+    const int nvec = (a.vocab + lead + VEC - 1) / VEC;
+    const int v0 = split * (ROW_THREADS * NV) + tid;
+    if (tid == 0) count = 0;
+
+    uint32_t key[EPT];
+    float tmax = -INFINITY;
+    uint32_t kmax = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int v = v0 + j * ROW_THREADS;
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (v < nvec) raw = __ldcs(reinterpret_cast<const uint4 *>(base) + v);
+        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int tok = v * VEC + i - lead;
+            const bool in = tok >= 0 && tok < a.vocab;
+            const float x = io<T>::to_f(e[i]);
+            // kept as the value; what is not a logit gets key 0 below
+            key[j * VEC + i] = in ? __float_as_uint(x) : 0xffffffffu;   // a NaN pattern
+            if (in) tmax = fmaxf(tmax, x);
+        }
+    }
+    float m = tmax;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) redf[0][wid] = m;
+    __syncthreads();
+    m = redf[0][0];
+#pragma unroll
+    for (int w = 1; w < ROW_THREADS / 32; ++w) m = fmaxf(m, redf[0][w]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int tok = (v0 + j * ROW_THREADS) * VEC + i - lead;
+            const bool in = tok >= 0 && tok < a.vocab;
+            const float x = __uint_as_float(key[j * VEC + i]);
+            // all masked: no term; a NaN or +inf makes the sum NaN
+            if (in) sum += x == -INFINITY ? 0.0f : __expf(x - m);
+            const uint32_t k = in ? order_key(x) : 0u;
+            key[j * VEC + i] = k;
+            kmax = k > kmax ? k : kmax;
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) redf[1][wid] = sum;
+
+    // A threshold that at least `num` threads reach (each by its largest key),
+    // so that the slice's best `num` are among the keys at or above it: bisection
+    // of the key's bits, stopped once few more threads than needed reach it.
+    uint32_t thr = 1;
+    const int reach = __syncthreads_count(kmax > 0);
+    if (reach > a.num) {
+        thr = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t t = thr | (1u << bit);
+            const int c = __syncthreads_count(kmax >= t);
+            if (c >= a.num) thr = t;
+            if (c >= a.num && c <= a.num + 8) break;
+        }
+    }
+    if (kmax >= thr) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (key[j * VEC + i] >= thr) {
+                    const int at = atomicAdd(&count, 1);
+                    const uint32_t tok = (uint32_t)((v0 + j * ROW_THREADS) * VEC + i - lead);
+                    if (at < LIST) list[at] = (uint64_t)key[j * VEC + i] << 32 | (uint32_t)~tok;
+                }
+    }
+    __syncthreads();
+    const int64_t part = (int64_t)row * a.splits + split;
+    uint64_t *out = a.part_list + part * a.num;
+    if (tid == 0) {
+        float s = redf[1][0];
+        for (int w = 1; w < ROW_THREADS / 32; ++w) s += redf[1][w];
+        a.part_max[part] = m;
+        a.part_sum[part] = s;
+    }
+    const int c = count;
+    if (c <= LIST) {
+        // distinct entries: each one's rank is the number of larger ones
+        for (int i = tid; i < c; i += ROW_THREADS) {
+            const uint64_t mine = list[i];
+            int rank = 0;
+            for (int j = 0; j < c; ++j) rank += list[j] > mine;
+            if (rank < a.num) out[rank] = mine;
+        }
+        for (int i = c + tid; i < a.num; i += ROW_THREADS) out[i] = 0;
+        return;
+    }
+    // many equal logits at the threshold: pick one after the other
+    uint64_t last = ~0ull;
+    for (int n = 0; n < a.num; ++n) {
+        uint64_t b = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const uint32_t tok = (uint32_t)((v0 + j * ROW_THREADS) * VEC + i - lead);
+                const uint64_t e = (uint64_t)key[j * VEC + i] << 32 | (uint32_t)~tok;
+                if (key[j * VEC + i] && e < last && e > b) b = e;
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t x = __shfl_xor_sync(0xffffffffu, b, o);
+            b = x > b ? x : b;
+        }
+        if (lane == 0) best[wid] = b;
+        __syncthreads();
+        last = best[0];
+        for (int w = 1; w < ROW_THREADS / 32; ++w) last = best[w] > last ? best[w] : last;
+        if (tid == 0) out[n] = last;
+        __syncthreads();
+    }
+}
+
+struct MergeArgs {
+    int beams, vocab, num, splits;
+    int64_t pad;
+    const float *scores;
+    const uint8_t *finished;
+    const float *part_max, *part_sum;
+    const uint64_t *part_list;
+    float *out_scores;
+    int64_t *out_parents, *out_tokens;
+};
+
+// better: the larger value, then the lower flat index (NaN never reaches here)
+__device__ __forceinline__ bool better(double v, int64_t at, double v2, int64_t at2) {
+    return v > v2 || (v == v2 && at < at2);
+}
+
+__global__ void __launch_bounds__(1024)
+beam_merge_kernel(const MergeArgs a) {
+    extern __shared__ int heads[];            // per list: entries taken
+    // a beam's score, largest logit and log sum of exp(logit - largest): a large
+    // common offset of the logits must cancel before the other terms join
+    __shared__ double s_score[MAX_BEAMS], s_max[MAX_BEAMS], s_logsum[MAX_BEAMS];
+    __shared__ int s_kind[MAX_BEAMS];         // 0 live, 1 finished, 2 no continuation
+    __shared__ double w_val[2][32];
+    __shared__ int64_t w_at[2][32];
+    __shared__ int w_list[2][32];
+    const int batch = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    const int warps = blockDim.x >> 5, lists = a.beams * a.splits;
+
+    for (int l = tid; l < lists; l += blockDim.x) heads[l] = 0;
+    for (int k = wid; k < a.beams; k += warps) {
+        const int row = batch * a.beams + k;
+        const double sc = (double)a.scores[row];
+        int kind = a.finished && a.finished[row] ? 1 : 0;
+        double top = 0.0, logsum = 0.0;
+        if (kind == 0) {
+            const float *pm = a.part_max + (int64_t)row * a.splits;
+            const float *ps = a.part_sum + (int64_t)row * a.splits;
+            float m = -INFINITY;
+            for (int i = lane; i < a.splits; i += 32) m = fmaxf(m, pm[i]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            double s = 0.0;
+            for (int i = lane; i < a.splits; i += 32)
+                if (ps[i] != 0.0f) s += (double)ps[i] * exp((double)pm[i] - (double)m);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            top = (double)m;
+            logsum = log(s);
+        }
+        if (!isfinite(top) || !isfinite(logsum) || !isfinite(sc)) kind = 2;
+        if (lane == 0) {
+            s_kind[k] = kind;
+            s_score[k] = sc;
+            s_max[k] = top;
+            s_logsum[k] = logsum;
+        }
+    }
+    __syncthreads();
+
+    // entry `h` of a list: false when it has none
+    auto entry = [&](int l, int h, double &val, int64_t &at) {
+        const int k = l / a.splits, sp = l - k * a.splits;
+        const int kind = s_kind[k];
+        const int64_t flat = (int64_t)k * a.vocab;
+        if (kind != 0) {
+            // a finished beam continues with the pad token alone; every other
+            // token, and all of a beam without continuation, are worth -inf
+            if (sp != 0 || h >= a.vocab) return false;
+            const int64_t tok = kind == 2 ? h : (h == 0 ? a.pad : h - 1 + (h - 1 >= a.pad));
+            val = kind == 1 && h == 0 ? s_score[k] : -INFINITY;
+            at = flat + tok;
+            return true;
+        }
+        if (h >= a.num) return false;
+        const uint64_t e = a.part_list[((int64_t)(batch * a.beams + k) * a.splits + sp) * a.num + h];
+        if (e == 0) return false;
+        val = s_score[k] + (((double)key_value((uint32_t)(e >> 32)) - s_max[k]) - s_logsum[k]);
+        at = flat + (uint32_t)~(uint32_t)e;
+        return true;
+    };
+    // this thread's best head over its lists
+    double val;
+    int64_t at;
+    int which;
+    auto refresh = [&]() {
+        which = -1;
+        val = -INFINITY;
+        at = INT64_MAX;
+        for (int l = tid; l < lists; l += blockDim.x) {
+            double v;
+            int64_t p;
+            if (entry(l, heads[l], v, p) && (which < 0 || better(v, p, val, at))) {
+                val = v;
+                at = p;
+                which = l;
+            }
+        }
+    };
+    refresh();
+    for (int n = 0; n < a.num; ++n) {
+        double bv = val;
+        int64_t ba = at;
+        int bl = which;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const double v = __shfl_xor_sync(0xffffffffu, bv, o);
+            const int64_t p = __shfl_xor_sync(0xffffffffu, ba, o);
+            const int l = __shfl_xor_sync(0xffffffffu, bl, o);
+            if (better(v, p, bv, ba)) { bv = v; ba = p; bl = l; }
+        }
+        if (warps > 1) {
+            if (lane == 0) { w_val[n & 1][wid] = bv; w_at[n & 1][wid] = ba; w_list[n & 1][wid] = bl; }
+            __syncthreads();
+            bv = w_val[n & 1][0]; ba = w_at[n & 1][0]; bl = w_list[n & 1][0];
+            for (int w = 1; w < warps; ++w)
+                if (better(w_val[n & 1][w], w_at[n & 1][w], bv, ba)) {
+                    bv = w_val[n & 1][w]; ba = w_at[n & 1][w]; bl = w_list[n & 1][w];
+                }
+        }
+        if (bl < 0) break;                    // num <= beams x vocab: not reached
+        if (which == bl) {                    // the thread that offered it
+            const int64_t i = (int64_t)batch * a.num + n;
+            a.out_scores[i] = (float)bv;
+            a.out_parents[i] = ba / a.vocab;
+            a.out_tokens[i] = ba % a.vocab;
+            ++heads[bl];
+            refresh();
+        }
+    }
+}
+
+// ------------------------------------------------------------ state reorder
+// Row b K + j of every tensor becomes row b K + parents[b, j], in place: one
+// thread holds the same bytes of all K rows of a batch, so it has read every
+// source before it writes.  Rows that stay are neither read nor written.  All
+// tensors of a call share one launch.  Bound: HBM, the moved rows once each way.
+constexpr int MAX_TENSORS = 64;
+struct Reorder {
+    struct Item { uint8_t *p; int64_t row_bytes; int vec; int block0; } item[MAX_TENSORS];
+    int n, beams;
+    const int64_t *parents;
+};
+constexpr int MOVE_THREADS = 128;
+
+template <typename V, int KMAX>
+__device__ __forceinline__ void move_rows(uint8_t *p, int64_t row_bytes, int64_t i, int K,
+                                          const int *src) {
+    const int64_t n = row_bytes / (int64_t)sizeof(V);
+    if (i >= n) return;
+    V x[KMAX];
+#pragma unroll
+    for (int j = 0; j < KMAX; ++j)
+        if (j < K && src[j] != j) x[j] = reinterpret_cast<const V *>(p + src[j] * row_bytes)[i];
+#pragma unroll
+    for (int j = 0; j < KMAX; ++j)
+        if (j < K && src[j] != j) reinterpret_cast<V *>(p + j * row_bytes)[i] = x[j];
+}
+
+template <int KMAX>
+__global__ void __launch_bounds__(MOVE_THREADS)
+reorder_kernel(const __grid_constant__ Reorder r) {
+    __shared__ int src[MAX_BEAMS];
+    int t = 0;
+    while (t + 1 < r.n && (int)blockIdx.x >= r.item[t + 1].block0) ++t;
+    const int64_t row_bytes = r.item[t].row_bytes;
+    const int vec = r.item[t].vec, K = r.beams, batch = blockIdx.y;
+    if ((int)threadIdx.x < K) {
+        // a parent outside the beams leaves its row as it is
+        const int64_t s = r.parents[(int64_t)batch * K + threadIdx.x];
+        src[threadIdx.x] = s >= 0 && s < K ? (int)s : (int)threadIdx.x;
+    }
+    __syncthreads();
+    uint8_t *p = r.item[t].p + (int64_t)batch * K * row_bytes;
+    const int64_t i = (int64_t)((int)blockIdx.x - r.item[t].block0) * MOVE_THREADS + threadIdx.x;
+    if (vec == 16) move_rows<uint4, KMAX>(p, row_bytes, i, K, src);
+    else if (vec == 4) move_rows<uint32_t, KMAX>(p, row_bytes, i, K, src);
+    else if (vec == 2) move_rows<uint16_t, KMAX>(p, row_bytes, i, K, src);
+    else move_rows<uint8_t, KMAX>(p, row_bytes, i, K, src);
+}
+
+// slices of a row; one more element vector where the row may start off a
+// 16-byte boundary
+int beam_splits(int64_t vocab, size_t e) {
+    const int64_t vec = 16 / (int64_t)e;
+    return (int)ceil_div(ceil_div(vocab + vec - 1, vec), SLICE / vec);
+}
+
+}  // namespace
+}  // namespace mb2
+
+using namespace mb2;
+
+extern "C" size_t mb2_beam_select_workspace_bytes(int dtype, int64_t batch, int64_t beams,
+                                                  int64_t vocab, int64_t num) {
+    if (batch <= 0 || beams <= 0 || vocab <= 0 || num <= 0 || vocab > MAX_VOCAB) return 0;
+    const size_t lists = (size_t)(batch * beams) * beam_splits(vocab, dtype_size(dtype));
+    return lists * ((size_t)num * 8 + 8);
+}
+
+extern "C" int mb2_beam_select(int dtype, const void *logits, int64_t batch_stride,
+                               int64_t beam_stride, const float *scores, const uint8_t *finished,
+                               int64_t pad_token, int64_t batch, int64_t beams, int64_t vocab,
+                               int64_t num, float *out_scores, int64_t *out_parents,
+                               int64_t *out_tokens, void *workspace, size_t workspace_bytes,
+                               mb2_stream_t stream) {
+    MB2_REQUIRE(dtype == MB2_F32 || dtype == MB2_BF16, MB2_ERR_ARG, "beam_select: bad dtype");
+    MB2_REQUIRE(batch >= 0 && beams > 0 && vocab > 0 && num > 0, MB2_ERR_SHAPE,
+                "beam_select: bad size");
+    MB2_REQUIRE(beams <= MAX_BEAMS && num <= MAX_NUM && vocab <= MAX_VOCAB, MB2_ERR_SHAPE,
+                "beam_select: at most %d beams, %d continuations and a vocabulary of %d",
+                MAX_BEAMS, MAX_NUM, MAX_VOCAB);
+    MB2_REQUIRE(num <= beams * vocab, MB2_ERR_SHAPE, "beam_select: more continuations than tokens");
+    MB2_REQUIRE(pad_token >= 0 && pad_token < vocab, MB2_ERR_SHAPE,
+                "beam_select: pad token outside the vocabulary");
+    MB2_REQUIRE(batch * beams < 65536, MB2_ERR_SHAPE, "beam_select: batch x beams %lld >= 65536",
+                (long long)(batch * beams));
+    if (batch == 0) return MB2_OK;
+    MB2_REQUIRE(logits && scores && out_scores && out_parents && out_tokens, MB2_ERR_ARG,
+                "beam_select: null pointer");
+    MB2_REQUIRE(workspace_bytes >= mb2_beam_select_workspace_bytes(dtype, batch, beams, vocab, num) &&
+                    workspace,
+                MB2_ERR_WORKSPACE, "beam_select: workspace too small");
+    MB2_REQUIRE(aligned(workspace, 8), MB2_ERR_ALIGN, "beam_select: misaligned workspace");
+    const int splits = beam_splits(vocab, dtype_size(dtype));
+    const int64_t rows = batch * beams;
+    RowArgs r;
+    r.logits = logits;
+    r.s_batch = batch_stride;
+    r.s_beam = beam_stride;
+    r.beams = (int)beams; r.vocab = (int)vocab; r.num = (int)num; r.splits = splits;
+    r.finished = finished;
+    r.part_list = static_cast<uint64_t *>(workspace);
+    r.part_max = reinterpret_cast<float *>(r.part_list + rows * splits * num);
+    r.part_sum = r.part_max + rows * splits;
+    cudaStream_t st = (cudaStream_t)stream;
+    const dim3 grid((unsigned)splits, (unsigned)rows);
+    if (dtype == MB2_F32) beam_rows_kernel<float><<<grid, ROW_THREADS, 0, st>>>(r);
+    else beam_rows_kernel<__nv_bfloat16><<<grid, ROW_THREADS, 0, st>>>(r);
+    MB2_TRY(check_launch("beam_rows_kernel"));
+    MergeArgs g;
+    g.beams = r.beams; g.vocab = r.vocab; g.num = r.num; g.splits = splits;
+    g.pad = pad_token;
+    g.scores = scores;
+    g.finished = finished;
+    g.part_max = r.part_max; g.part_sum = r.part_sum; g.part_list = r.part_list;
+    g.out_scores = out_scores; g.out_parents = out_parents; g.out_tokens = out_tokens;
+    const int lists = (int)beams * splits;
+    const int threads = (int)(round_up(lists, 32) < 1024 ? round_up(lists, 32) : 1024);
+    beam_merge_kernel<<<(unsigned)batch, threads, sizeof(int) * lists, st>>>(g);
+    return check_launch("beam_merge_kernel");
+}
+
+extern "C" int mb2_reorder_rows(void *const *tensors, const int64_t *row_bytes, int64_t n_tensors,
+                                const int64_t *parents, int64_t batch, int64_t beams,
+                                mb2_stream_t stream) {
+    MB2_REQUIRE(n_tensors >= 0 && batch >= 0 && beams > 0, MB2_ERR_SHAPE, "reorder_rows: bad size");
+    MB2_REQUIRE(beams <= MAX_BEAMS, MB2_ERR_SHAPE, "reorder_rows: at most %d beams", MAX_BEAMS);
+    MB2_REQUIRE(batch < 65536, MB2_ERR_SHAPE, "reorder_rows: batch %lld >= 65536", (long long)batch);
+    if (n_tensors == 0 || batch == 0) return MB2_OK;
+    MB2_REQUIRE(tensors && row_bytes && parents, MB2_ERR_ARG, "reorder_rows: null pointer");
+    for (int64_t i = 0; i < n_tensors; ++i)
+        MB2_REQUIRE(row_bytes[i] >= 0 && (tensors[i] || row_bytes[i] == 0), MB2_ERR_ARG,
+                    "reorder_rows: bad tensor %lld", (long long)i);
+    for (int64_t t0 = 0; t0 < n_tensors; t0 += MAX_TENSORS) {
+        Reorder r;
+        r.n = 0;
+        r.beams = (int)beams;
+        r.parents = parents;
+        int64_t blocks = 0;
+        for (int64_t i = t0; i < n_tensors && i < t0 + MAX_TENSORS; ++i) {
+            const int64_t rb = row_bytes[i];
+            if (rb == 0) continue;
+            int vec = 16;
+            while (vec > 1 && (rb % vec || !aligned(tensors[i], vec))) vec = vec == 16 ? 4 : vec / 2;
+            r.item[r.n].p = static_cast<uint8_t *>(tensors[i]);
+            r.item[r.n].row_bytes = rb;
+            r.item[r.n].vec = vec;
+            r.item[r.n].block0 = (int)blocks;
+            ++r.n;
+            blocks += ceil_div(rb / vec, MOVE_THREADS);
+            MB2_REQUIRE(blocks <= 0x7fffffff, MB2_ERR_SHAPE, "reorder_rows: rows too long");
+        }
+        if (blocks == 0) continue;
+        const dim3 grid((unsigned)blocks, (unsigned)batch);
+        cudaStream_t st = (cudaStream_t)stream;
+        if (beams <= 4) reorder_kernel<4><<<grid, MOVE_THREADS, 0, st>>>(r);
+        else if (beams <= 8) reorder_kernel<8><<<grid, MOVE_THREADS, 0, st>>>(r);
+        else if (beams <= 16) reorder_kernel<16><<<grid, MOVE_THREADS, 0, st>>>(r);
+        else reorder_kernel<32><<<grid, MOVE_THREADS, 0, st>>>(r);
+        MB2_TRY(check_launch("reorder_kernel"));
+    }
+    return MB2_OK;
+}

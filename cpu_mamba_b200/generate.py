@@ -19,6 +19,8 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from . import ops
+
 
 class TiedEmbeddingSampler:
     """Token choice through an LM head tied to the input embedding (the
@@ -132,3 +134,132 @@ def generate(model, sampler, prompt: torch.Tensor, max_new_tokens: int,
         return tok0[:, None], state
     loop = DecodeLoop(model, sampler, state, x, min(steps_per_graph, rest))
     return torch.cat([tok0[:, None], loop.run(rest)], dim=1), state
+
+
+class BeamLoop:
+    """``steps_per_graph`` beam-search steps (model step, logits, selection over
+    beams and vocabulary, reordering of the states) captured as one CUDA graph.
+
+    state: the decode state of B * K sequences, beam j of request b in row
+    b * K + j; ``tokens`` and ``scores`` (B, K): each beam's first token and its
+    score.  A beam that emits ``eos_token`` is finished: it keeps its score and
+    is padded with it.  ``run(n)`` takes n steps; ``result()`` returns the beams
+    so far."""
+
+    def __init__(self, model, sampler, state, tokens: torch.Tensor, scores: torch.Tensor,
+                 eos_token: Optional[int] = None, steps_per_graph: int = 16,
+                 dtype: Optional[torch.dtype] = None):
+        if steps_per_graph < 1:
+            raise ValueError("steps_per_graph must be >= 1")
+        self.model, self.sampler, self.state = model, sampler, state
+        self.K = int(steps_per_graph)
+        self.dtype = sampler.E.dtype if dtype is None else dtype      # of the model's inputs
+        self.eos = -1 if eos_token is None else int(eos_token)
+        self.scores = scores.clone()
+        self.last = tokens.clone()                    # each beam's newest token
+        self.finished = self.last == self.eos
+        self.history = [(None, tokens.clone())]       # (parents, tokens) of every step
+        shape = (self.K,) + tuple(tokens.shape)
+        self.parents = torch.empty(shape, dtype=torch.long, device=tokens.device)
+        self.tokens = torch.empty_like(self.parents)
+        dev = tokens.device
+        self.graph = None
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side), torch.no_grad():
+            # warm-up on copies (library set-up outside the capture)
+            kept = self.state, self.scores, self.last, self.finished
+            self.state = _clone_state(state)
+            self.scores, self.last, self.finished = (t.clone() for t in kept[1:])
+            self._steps(1)
+            self.state, self.scores, self.last, self.finished = kept
+        torch.cuda.current_stream(dev).wait_stream(side)
+
+    def _steps(self, n):
+        E = self.sampler.E
+        B, K = self.scores.shape
+        for i in range(n):
+            x = E[self.last.flatten()].to(self.dtype)
+            y, _ = self.model.forward_step(x, self.state)
+            logits = self.sampler.logits(y).reshape(B, K, -1)
+            best, par, tok = ops.beam_select(logits, self.scores, finished=self.finished,
+                                             pad_token=max(self.eos, 0))
+            ops.reorder_states(self.state, par)
+            self.finished.copy_(self.finished.gather(1, par) | (tok == self.eos))
+            self.scores.copy_(best)
+            self.last.copy_(tok)
+            self.parents[i].copy_(par)
+            self.tokens[i].copy_(tok)
+
+    def _keep(self, n):
+        self.history += zip(self.parents[:n].clone().unbind(0), self.tokens[:n].clone().unbind(0))
+
+    @torch.no_grad()
+    def run(self, n: int) -> None:
+        full, rest = divmod(n, self.K)
+        if full and self.graph is None:
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
+                self._steps(self.K)
+        for _ in range(full):
+            self.graph.replay()
+            self._keep(self.K)
+        if rest:
+            self._steps(rest)
+            self._keep(rest)
+
+    def result(self) -> tuple:
+        """(tokens (B, K, steps), scores (B, K)), each batch's best beam first."""
+        B, K = self.scores.shape
+        at = torch.arange(K, device=self.scores.device).expand(B, K)
+        out = []
+        for par, tok in reversed(self.history):
+            out.append(tok.gather(1, at))
+            if par is not None:
+                at = par.gather(1, at)
+        return torch.stack(out[::-1], -1), self.scores.clone()
+
+
+def _repeat_state(state, n: int):
+    if isinstance(state, dict):
+        return {k: v.repeat_interleave(n, 0) for k, v in state.items()}
+    return [_repeat_state(s, n) for s in state]
+
+
+@torch.no_grad()
+def beam_search(model, sampler, prompt: torch.Tensor, max_new_tokens: int, beams: int,
+                eos_token: Optional[int] = None, length_penalty: float = 0.0,
+                steps_per_graph: int = 16) -> tuple:
+    """Beam search on the GPU: prefill ``prompt`` (B, T, d_model) once, then keep
+    the ``beams`` best continuations of each request by total log probability
+    (``sampler.logits`` through log-softmax), the beams' recurrent states
+    following them.  Beams that emit ``eos_token`` keep their score and are
+    padded with it.  ``length_penalty`` a > 0 ranks the final beams by score /
+    length^a, length counting up to the first ``eos_token``.
+
+    Returns (tokens (B, beams, max_new_tokens), scores (B, beams)), the best
+    beam of each request first."""
+    if max_new_tokens < 1:
+        raise ValueError("max_new_tokens must be >= 1")
+    if beams < 1:
+        raise ValueError("beams must be >= 1")
+    y, state = model.forward_with_final_state(prompt)
+    logits = sampler.logits(y[:, -1])
+    B, V = logits.shape
+    if eos_token is not None and not 0 <= eos_token < V:
+        raise ValueError(f"eos_token {eos_token} outside the vocabulary of {V}")
+    if beams > V:
+        raise ValueError(f"{beams} beams from a vocabulary of {V}")
+    scores, _, tokens = ops.beam_select(logits.unsqueeze(1), logits.new_zeros(B, 1), num=beams)
+    rest = max_new_tokens - 1
+    loop = BeamLoop(model, sampler, _repeat_state(state, beams), tokens, scores, eos_token,
+                    max(1, min(steps_per_graph, rest)), prompt.dtype)
+    loop.run(rest)
+    out, scores = loop.result()
+    if length_penalty:
+        done = out == (-1 if eos_token is None else eos_token)
+        length = max_new_tokens - (done.cumsum(-1) > 0).sum(-1) + done.any(-1)
+        order = (scores / length.to(scores.dtype) ** length_penalty).argsort(-1, descending=True)
+        out = out.gather(1, order[..., None].expand_as(out))
+        scores = scores.gather(1, order)
+    return out, scores

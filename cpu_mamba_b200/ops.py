@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import DecayAttn, check, dtype_code, lib, ptr, require_cuda, stream_of
+from ._lib import DecayAttn, GatedNorm, check, dtype_code, lib, ptr, require_cuda, stream_of
 
 
 def selective_scan(x, dt, A, B, C, D, h0: Optional[torch.Tensor] = None,
@@ -405,3 +405,176 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: t
     with _on(v):
         check(lib().mb2_decay_attention_step(ctypes.byref(d), ptr(state), stream_of(v)), what)
     return o
+
+
+# ------------------------------------------------------- norms around a block
+def gated_norm(x: torch.Tensor, gate: Optional[torch.Tensor] = None,
+               weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+               residual_scale=None, next_weight: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, group_size: Optional[int] = None,
+               norm_before_gate: bool = True, out: Optional[torch.Tensor] = None):
+    """The norm after a block, its gate, the residual add and the norm before
+    the next block, in one pass over the rows of x (..., width):
+
+        u = RMSNorm(x) * weight * silu(gate)      (norm_before_gate)
+        u = RMSNorm(x * silu(gate)) * weight      (otherwise)
+        r = residual + residual_scale * u
+        n = RMSNorm(r) * next_weight
+
+    Without ``weight`` there is no first norm, without ``gate`` no gate; the
+    first norm runs over groups of ``group_size`` columns (None: all of them).
+    x and gate share a dtype (float32 or bfloat16); residual is in it or in
+    float32; residual_scale is a number (default 1) or a (width,) tensor, and
+    the (width,) tensors are in x's dtype or float32.  width <= 16384.
+
+    Returns u without a residual, r with one, (r, n) with ``next_weight``; r in
+    residual's dtype, u and n in x's, n computed from the unrounded r.  ``out``
+    receives the first result; it may be ``residual`` itself.  Forward only."""
+    what = "gated_norm"
+    vec_scale = isinstance(residual_scale, torch.Tensor)
+    _one_device(what, x, gate, weight, residual, residual_scale if vec_scale else None,
+                next_weight, out)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"{what}: x must be (..., width), got {tuple(x.shape)}")
+    W = x.shape[-1]
+    if residual is None and (residual_scale is not None or next_weight is not None):
+        raise RuntimeError(f"{what}: residual_scale and next_weight need a residual")
+    d = GatedNorm()
+    d.dtype = d.residual_dtype = dtype_code(x.dtype)
+    if group_size is not None and (group_size < 1 or W % group_size):
+        raise RuntimeError(f"{what}: group_size {group_size} does not divide width {W}")
+    d.rows, d.width, d.group = x.numel() // W, W, group_size or 0
+    d.eps, d.norm_before_gate, d.scale = eps, int(norm_before_gate), 1.0
+    keep = []
+
+    def rows_of(name, t):
+        if t.shape != x.shape:
+            raise RuntimeError(f"{what}: {name} {tuple(t.shape)} does not match x "
+                               f"{tuple(x.shape)}")
+        t2 = _rows(t).reshape(-1, W)
+        keep.append(t2)
+        return t2.data_ptr(), t2.stride(0)
+
+    def vector(name, t):
+        if t.shape != (W,) or t.dtype not in (x.dtype, torch.float32):
+            raise RuntimeError(f"{what}: {name} must be ({W},) in {x.dtype} or float32")
+        t = t.contiguous()
+        keep.append(t)
+        return t.data_ptr(), int(t.dtype == torch.float32)
+
+    d.x, d.ld_x = rows_of("x", x)
+    if gate is not None:
+        if gate.dtype != x.dtype:
+            raise RuntimeError(f"{what}: gate must be in {x.dtype}")
+        d.gate, d.ld_gate = rows_of("gate", gate)
+    if weight is not None:
+        d.weight, d.weight_f32 = vector("weight", weight)
+    first = x.dtype
+    if residual is not None:
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise RuntimeError(f"{what}: residual must be in {x.dtype} or float32")
+        first = residual.dtype
+        d.residual_dtype = dtype_code(first)
+        d.residual, d.ld_residual = rows_of("residual", residual)
+        if vec_scale:
+            d.residual_scale, d.scale_f32 = vector("residual_scale", residual_scale)
+        elif residual_scale is not None:
+            d.scale = residual_scale
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=first)
+    elif out.shape != x.shape or out.dtype != first or not out.is_contiguous():
+        raise RuntimeError(f"{what}: out must be contiguous {tuple(x.shape)} in {first}")
+    d.out, d.ld_out = out.data_ptr(), W
+    n = None
+    if next_weight is not None:
+        d.next_weight, d.next_f32 = vector("next_weight", next_weight)
+        n = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        d.next_out, d.ld_next = n.data_ptr(), W
+    with _on(x):
+        check(lib().mb2_gated_norm(ctypes.byref(d), stream_of(x)), what)
+    return out if n is None else (out, n)
+
+
+# ---------------------------------------------------------------- beam search
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] = None,
+                finished: Optional[torch.Tensor] = None, pad_token: int = 0
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The best ``num`` continuations of each batch over its beams and the
+    vocabulary: the candidates scores[b, k] + log_softmax(logits[b, k])[v] in
+    order, ties to the lowest beam and then the lowest token.
+
+    logits: (B, K, V) float32 or bfloat16 (strided batch and beams; an expanded
+    beam index is fine); scores: (B, K) float32.  ``num`` defaults to K.  A beam
+    flagged in ``finished`` (B, K) bool has the one continuation ``pad_token``
+    at its own score.  A beam whose score or normaliser is not finite has none;
+    such candidates and masked (-inf or NaN) logits are worth -inf and come
+    last, lowest index first.  K <= 32, num <= 64, V <= 2^20.
+
+    Returns (scores (B, num) float32, parents (B, num), tokens (B, num)), the
+    last two int64, parents being beams 0 .. K-1."""
+    what = "beam_select"
+    _one_device(what, logits, scores, finished)
+    if logits.dim() != 3 or logits.shape[1] == 0 or logits.shape[2] == 0:
+        raise RuntimeError(f"{what}: logits must be (batch, beams, vocab), got "
+                           f"{tuple(logits.shape)}")
+    B, K, V = logits.shape
+    if scores.shape != (B, K) or scores.dtype != torch.float32:
+        raise RuntimeError(f"{what}: scores must be float32 {(B, K)}")
+    if finished is not None and (finished.shape != (B, K) or finished.dtype != torch.bool):
+        raise RuntimeError(f"{what}: finished must be bool {(B, K)}")
+    num = K if num is None else int(num)
+    code = dtype_code(logits.dtype)
+    logits, scores = _rows(logits), scores.contiguous()
+    finished = None if finished is None else finished.contiguous()
+    with _on(logits):
+        n = max(num, 0)
+        best = torch.empty(B, n, device=logits.device, dtype=torch.float32)
+        parents = torch.empty(B, n, device=logits.device, dtype=torch.int64)
+        tokens = torch.empty_like(parents)
+        nbytes = lib().mb2_beam_select_workspace_bytes(code, B, K, V, num)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+        check(lib().mb2_beam_select(code, ptr(logits), logits.stride(0), logits.stride(1),
+                                    ptr(scores), ptr(finished), pad_token, B, K, V, num,
+                                    ptr(best), ptr(parents), ptr(tokens), ptr(ws), nbytes,
+                                    stream_of(logits)), what)
+    return best, parents, tokens
+
+
+def _leaves(states):
+    if isinstance(states, torch.Tensor):
+        yield states
+    else:
+        for s in states.values() if isinstance(states, dict) else states:
+            yield from _leaves(s)
+
+
+def reorder_states(states, parents: torch.Tensor):
+    """Beams follow their parents, in place: row b * K + j of every tensor in
+    ``states`` (a tensor, or nested lists, tuples and dicts of them, such as
+    MambaStack's or CPUMamba's decode states) becomes row b * K + parents[b, j].
+
+    Each tensor is contiguous with B * K rows (its first index) of any dtype;
+    parents: (B, K) int64 or int32 beams, K <= 32; a parent outside 0 .. K-1
+    leaves its row as it is.  Tensors that overlap one another are not
+    supported.  Returns ``states``."""
+    what = "reorder_states"
+    if parents.dim() != 2 or parents.shape[1] == 0 or (
+            parents.dtype not in (torch.int64, torch.int32)):
+        raise RuntimeError(f"{what}: parents must be (batch, beams) int64 or int32, got "
+                           f"{tuple(parents.shape)} {parents.dtype}")
+    B, K = parents.shape
+    rows, dev = B * K, parents.device
+    tensors = list(_leaves(states))
+    require_cuda(parents, *tensors, what=what)
+    n = len(tensors)
+    ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
+    for i, t in enumerate(tensors):
+        if t.dim() < 1 or t.shape[0] != rows or not t.is_contiguous() or t.device != dev:
+            raise RuntimeError(f"{what}: states must be contiguous with {rows} rows on {dev}, got "
+                               f"{tuple(t.shape)} on {t.device}")
+        ptrs[i] = t.data_ptr()
+        sizes[i] = t.numel() * t.element_size() // rows if rows else 0
+    parents = parents.to(torch.int64).contiguous()
+    with _on(parents):
+        check(lib().mb2_reorder_rows(ptrs, sizes, n, ptr(parents), B, K, stream_of(parents)), what)
+    return states

@@ -15,6 +15,11 @@ torch custom ops, callable as ``torch.ops.mamba_b200.<name>`` and traceable
              dt_proj_b?, A_log, D, out_proj_w) -> y   (h, conv_state updated in place)
   decay_attention(q, k, v, g, scale=1, h0?, cu_seqlens?) -> (o, h_last)
   decay_attention_step(q, k, v, g, state, scale=1) -> o       (state updated in place)
+  gated_norm(x, gate?, weight?, group_size=0, eps, norm_before_gate=True) -> u
+  gated_norm_residual(x, gate?, weight?, residual, residual_scale?, next_weight,
+                      group_size=0, eps, norm_before_gate=True) -> (r, n)
+  beam_select(logits, scores, num, finished?, pad_token=0) -> (scores, parents, tokens)
+  reorder_states(states, parents)                             (states: Tensor[], in place)
 
 Each runs the C-ABI kernels on the inputs' CUDA device and current stream
 (no CPU implementation: CPU tensors raise, as the rest of the package does).
@@ -181,3 +186,57 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: t
 @decay_attention_step.register_fake
 def _(q, k, v, g, state, scale=1.0):
     return v.new_empty(v.shape[0], g.shape[-1], v.shape[2])
+
+
+@torch.library.custom_op(f"{NS}::gated_norm", mutates_args=())
+def gated_norm(x: torch.Tensor, gate: Optional[torch.Tensor], weight: Optional[torch.Tensor],
+               group_size: int = 0, eps: float = 1e-5,
+               norm_before_gate: bool = True) -> torch.Tensor:
+    return ops.gated_norm(x, gate=gate, weight=weight, eps=eps, group_size=group_size or None,
+                          norm_before_gate=norm_before_gate)
+
+
+@gated_norm.register_fake
+def _(x, gate, weight, group_size=0, eps=1e-5, norm_before_gate=True):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{NS}::gated_norm_residual", mutates_args=())
+def gated_norm_residual(x: torch.Tensor, gate: Optional[torch.Tensor],
+                        weight: Optional[torch.Tensor], residual: torch.Tensor,
+                        residual_scale: Optional[torch.Tensor], next_weight: torch.Tensor,
+                        group_size: int = 0, eps: float = 1e-5,
+                        norm_before_gate: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.gated_norm(x, gate=gate, weight=weight, residual=residual,
+                          residual_scale=residual_scale, next_weight=next_weight, eps=eps,
+                          group_size=group_size or None, norm_before_gate=norm_before_gate)
+
+
+@gated_norm_residual.register_fake
+def _(x, gate, weight, residual, residual_scale, next_weight, group_size=0, eps=1e-5,
+      norm_before_gate=True):
+    return residual.new_empty(x.shape), x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{NS}::beam_select", mutates_args=())
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: int,
+                finished: Optional[torch.Tensor] = None, pad_token: int = 0
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.beam_select(logits, scores, num=num, finished=finished, pad_token=pad_token)
+
+
+@beam_select.register_fake
+def _(logits, scores, num, finished=None, pad_token=0):
+    B = logits.shape[0]
+    i = logits.new_empty(B, num, dtype=torch.int64)
+    return logits.new_empty(B, num, dtype=torch.float32), i, torch.empty_like(i)
+
+
+@torch.library.custom_op(f"{NS}::reorder_states", mutates_args=("states",))
+def reorder_states(states: list[torch.Tensor], parents: torch.Tensor) -> None:
+    ops.reorder_states(states, parents)
+
+
+@reorder_states.register_fake
+def _(states, parents):
+    return None

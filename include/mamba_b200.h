@@ -451,6 +451,63 @@ int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, size_t workspa
  * dk, dv) fp32 is advanced in place. */
 int mb2_decay_attention_step(const mb2_decay_attn *d, float *state, mb2_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * The norms around a block, with its gate and the residual add, in one pass
+ * (no counterpart in the reference, which leaves the norm between blocks to
+ * the model):
+ *   u = RMSNorm(x) weight silu(gate)   (norm_before_gate)
+ *   u = RMSNorm(x silu(gate)) weight   (otherwise)
+ *   out = residual + scale u           (scale: residual_scale (width) or `scale`)
+ *   next_out = RMSNorm(out) next_weight
+ * weight NULL: no first norm; gate NULL: no gate; residual NULL: out = u (in
+ * dtype; then no residual_scale or next_weight).  The first norm runs over
+ * groups of `group` columns (0: all).  x, gate, next_out in dtype; residual and
+ * out in residual_dtype (dtype or fp32); each vector operand in dtype, or fp32
+ * with its _f32 flag.  Rows have leading dimensions in elements; width <=
+ * 16384.  out may be residual itself. */
+typedef struct mb2_gated_norm_desc {
+    int dtype, residual_dtype;
+    int64_t rows, width, group;
+    const void *x, *gate, *weight, *residual, *residual_scale, *next_weight;
+    void *out, *next_out;
+    int64_t ld_x, ld_gate, ld_residual, ld_out, ld_next;
+    float scale, eps;
+    int norm_before_gate;
+    int weight_f32, scale_f32, next_f32;
+} mb2_gated_norm_desc;
+int mb2_gated_norm(const mb2_gated_norm_desc *d, mb2_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Beam search (no counterpart in the reference, which leaves the choice of
+ * tokens to the caller, README.md:75-86).
+ *
+ * mb2_beam_select: of the candidates
+ *   scores[b, k] + logits[b, k, v] - log sum exp(logits[b, k, :])
+ * the best `num` per batch, in order, ties to the lowest beam and then the
+ * lowest token: out_scores fp32, out_parents (the beam k) and out_tokens
+ * int64, each (batch, num).  logits (batch, beams, vocab) in dtype, strides in
+ * elements, last index contiguous; scores fp32 (batch, beams).  finished
+ * (batch, beams; or NULL): a beam with a non-zero flag has the one candidate
+ * (pad_token, its score) and its logits are not read.  A beam whose score or
+ * normaliser is not finite has no continuation; that and a logit of -inf or
+ * NaN are worth -inf, chosen last, lowest index first.  beams <= 32, num <= 64
+ * and <= beams x vocab, vocab <= 2^20.  The workspace is 8-byte aligned.
+ *
+ * mb2_reorder_rows: row b beams + j of each of n_tensors contiguous tensors
+ * (batch x beams rows of row_bytes[i] bytes) becomes row b beams +
+ * parents[b, j], in place, in one launch per 64 tensors.  tensors and
+ * row_bytes are host arrays, parents a device one; a parent outside 0 ..
+ * beams-1 leaves its row as it is.  The tensors do not overlap. */
+size_t mb2_beam_select_workspace_bytes(int dtype, int64_t batch, int64_t beams, int64_t vocab,
+                                       int64_t num);
+int mb2_beam_select(int dtype, const void *logits, int64_t batch_stride, int64_t beam_stride,
+                    const float *scores, const uint8_t *finished, int64_t pad_token,
+                    int64_t batch, int64_t beams, int64_t vocab, int64_t num, float *out_scores,
+                    int64_t *out_parents, int64_t *out_tokens, void *workspace,
+                    size_t workspace_bytes, mb2_stream_t stream);
+int mb2_reorder_rows(void *const *tensors, const int64_t *row_bytes, int64_t n_tensors,
+                     const int64_t *parents, int64_t batch, int64_t beams, mb2_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
