@@ -38,5 +38,9 @@ __device__ __forceinline__ void bounds(const Args &a, int64_t seq, int64_t &row0
     }
 }
 
+// decay_tc.cu: the tensor-core prompt kernel; *used = false (and nothing
+// launched) when it does not take the call
+int chunked(const Args &a, cudaStream_t st, bool *used);
+
 }  // namespace decay
 }  // namespace mb2

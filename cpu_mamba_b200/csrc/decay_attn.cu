@@ -483,6 +483,9 @@ extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, siz
             decay::zero_tail_kernel<__nv_bfloat16><<<64, 256, 0, st>>>(a);
         MB2_TRY(check_launch("zero_tail_kernel"));
     }
+    bool used = false;
+    MB2_TRY(decay::chunked(a, st, &used));
+    if (used) return MB2_OK;
     return a.dtype == MB2_F32 ? decay::recurrent<float>(a, st)
                               : decay::recurrent<__nv_bfloat16>(a, st);
 }
