@@ -23,10 +23,13 @@
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone.
 //
-// Roles (16 warps): 0 TMA loads, 1 MMA issue, 4-7 decays, V~ and the state,
-// 8-15 P and the output rows.  Every mbarrier completes once per chunk (twice
-// staged ones once per two), so its phase follows from the chunk count.  All
-// waits are bounded; a wait that expires sets the device status.
+// Roles (19 warps): 0-3 the state, 4-11 P, 12-15 V~ and the output rows, 16 TMA
+// loads, 17 MMA issue, 18 decays.  A chunk's products are issued as
+//   Q S0 (n), Q K^T (n + 1), P V (n), K^T V~ (n + 1)
+// so that P (n + 1) and the state update overlap the others' MMAs.  Every
+// mbarrier completes once per chunk (staged ones once per two), so its phase
+// follows from the chunk count.  All waits are bounded; a wait that expires sets
+// the device status.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -40,7 +43,7 @@ using namespace tc;
 
 constexpr int C = 128;                       // tokens per chunk
 constexpr int DV = 64;                       // columns of v per CTA
-constexpr int THREADS = 512;
+constexpr int THREADS = 608;
 constexpr uint32_t SUB = 128 * 128;          // one 128-row x 128-byte operand tile
 // shared memory (bytes from a 1024-aligned base)
 constexpr uint32_t OFF_Q = 0;                            // [2][2 SUB]
@@ -49,11 +52,17 @@ constexpr uint32_t OFF_V = OFF_K + 4 * SUB;              // [2][SUB]
 constexpr uint32_t OFF_VT = OFF_V + 2 * SUB;             // [3][SUB]
 constexpr uint32_t OFF_H = OFF_VT + 3 * SUB;             // [SUB]
 constexpr uint32_t OFF_COLF = OFF_H + SUB;               // float [2][128]
-constexpr uint32_t OFF_TOT = OFF_COLF + 2 * C * 4;       // double [2][4]
-constexpr uint32_t OFF_BARS = OFF_TOT + 2 * 4 * 8;
-constexpr int NBARS = 6 + 6 + 11;
+constexpr uint32_t OFF_G2 = OFF_COLF + 2 * C * 4;        // float [2][128]
+constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
+constexpr uint32_t OFF_BARS = OFF_SC + 2 * 16 * 4;
+constexpr int NBARS = 6 + 6 + 4 + 9 + 1;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
+// scalars of a chunk (OFF_SC), all e^sums of whole blocks' decays
+constexpr int SC_BEFORE = 0;     // [4] blocks before block w
+constexpr int SC_AFTER = 4;      // [4] blocks after it
+constexpr int SC_ALL = 8;        // the chunk
+constexpr int SC_1 = 9, SC_12 = 10, SC_2 = 11;   // block 1; blocks 1 and 2; block 2
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 // TMEM columns
 constexpr uint32_t T_S = 0, T_P = 128, T_PV = 192, T_QH = 256, T_D = 320;
@@ -92,6 +101,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
           "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
           "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                   "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld8_async(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+// waits for the loads into r: the registers pass through, so that no use of
+// them can be scheduled before the wait
+template <int N>
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[N]) {
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -135,32 +164,54 @@ struct Item {
     int tile, h;
     int64_t seq, row0, len;
 };
-__device__ __forceinline__ Item item_of(const Args &a, int tiles, int64_t id) {
+__device__ __forceinline__ Item item_of(const Args &a, int tiles, uint32_t id) {
     Item it;
-    it.tile = (int)(id % tiles);
-    id /= tiles;
-    it.h = (int)(id % a.heads);
-    it.seq = id / a.heads;
+    const uint32_t n = id / (uint32_t)tiles, heads = (uint32_t)a.heads;
+    it.tile = (int)(id - n * (uint32_t)tiles);
+    it.seq = n / heads;
+    it.h = (int)(n - (uint32_t)it.seq * heads);
     bounds(a, it.seq, it.row0, it.len);
     return it;
 }
-// g of token t of an item's chunk (0 behind its end); below -256 e^g is 0 for
-// every fp32 product, and a finite sum keeps later differences
+// the chunks of a CTA's items, in order
+struct Walk {
+    const Args &a;
+    const int tiles;
+    const uint32_t items;
+    uint32_t id;
+    int64_t t0;
+    Item it;
+    uint32_t c;                          // chunks before this one
+    __device__ __forceinline__ Walk(const Args &a_, int tiles_, uint32_t items_)
+        : a(a_), tiles(tiles_), items(items_), id(blockIdx.x), t0(0), c(0) {
+        find();
+    }
+    __device__ __forceinline__ bool valid() const { return id < items; }
+    __device__ __forceinline__ void find() {     // the next item with tokens
+        for (; id < items; id += gridDim.x) {
+            it = item_of(a, tiles, id);
+            if (it.len > 0) break;
+        }
+    }
+    __device__ __forceinline__ void next() {
+        ++c;
+        t0 += C;
+        if (t0 >= it.len) {
+            t0 = 0;
+            id += gridDim.x;
+            find();
+        }
+    }
+};
+// g of token t of an item (0 behind its end)
 __device__ __forceinline__ float load_g(const Args &a, const Item &it, int64_t t) {
     if (t >= it.len) return 0.0f;
     const int64_t bq = a.cu ? 0 : it.seq;
-    const float g = a.g[bq * a.gs[0] + (it.row0 + t) * a.gs[1] + it.h * a.gs[2]];
-    return g < -256.0f ? -256.0f : g;
+    return a.g[bq * a.gs[0] + (it.row0 + t) * a.gs[1] + it.h * a.gs[2]];
 }
-__device__ __forceinline__ double scan32(float g) {
-    double x = g;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, x, s);
-        if ((int)(threadIdx.x & 31) >= s) x += y;
-    }
-    return x;
-}
+// below -256, e^g is 0 for every fp32 product, and a finite sum keeps later
+// differences; NaN stays
+__device__ __forceinline__ float clamp_g(float g) { return g < -256.0f ? -256.0f : g; }
 
 // a bounded wait of a whole warp; every lane gets the same answer
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int where) {
@@ -170,12 +221,12 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int whe
 // sum_j P_ij v_j of row t over its own tokens j <= t of the chunk, from global
 // memory: for rows that met an infinity or a NaN, perhaps in a masked token
 __device__ __forceinline__ void masked_row(const Args &a, const Item &it, int64_t t0, int64_t t,
-                                           int col, float (&y)[32]) {
+                                           int col, float (&y)[16]) {
     const int64_t bq = a.cu ? 0 : it.seq;
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + bq * a.qs[0] +
                              (it.row0 + t) * a.qs[1] + (it.h / a.q_rep) * a.qs[2];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) y[i] = 0.0f;
+    for (int i = 0; i < 16; ++i) y[i] = 0.0f;
     double sum = 0.0;
     for (int64_t j = t; j >= t0; --j) {
         const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(a.k) + bq * a.ks[0] +
@@ -187,9 +238,9 @@ __device__ __forceinline__ void masked_row(const Args &a, const Item &it, int64_
             d = fmaf(__bfloat162float(q[e]), __bfloat162float(k[e]), d);
         const float p = io<__nv_bfloat16>::round(d * __expf((float)sum));
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 16; ++i)
             if (col + i < a.dv) y[i] = fmaf(p, __bfloat162float(v[i]), y[i]);
-        sum += load_g(a, it, j);
+        sum += clamp_g(load_g(a, it, j));
     }
 }
 
@@ -197,11 +248,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a,
-                   int tiles, int64_t items) {
+                   int tiles, uint32_t items) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     float *const colf = reinterpret_cast<float *>(smem + OFF_COLF);
-    double *const tot = reinterpret_cast<double *>(smem + OFF_TOT);
+    float *const g2 = reinterpret_cast<float *>(smem + OFF_G2);
+    float *const sc = reinterpret_cast<float *>(smem + OFF_SC);
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(smem + OFF_TMEM);
     auto bar = [&](int i) { return base + OFF_BARS + 8u * i; };
     auto full_q = [&](int s) { return bar(s); };
@@ -210,37 +262,31 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     auto empty_q = [&](int s) { return bar(6 + s); };
     auto empty_k = [&](int s) { return bar(8 + s); };
     auto empty_v = [&](int s) { return bar(10 + s); };
-    const uint32_t s_full = bar(12);    // Q K^T in TMEM
-    const uint32_t vt_full = bar(13);   // V~ and the decays of a chunk in shared memory
-    const uint32_t d_full = bar(14);    // K^T V~ in TMEM
-    const uint32_t d_free = bar(15);    // ... read
-    const uint32_t h_full = bar(16);    // S0 (bf16) in shared memory
-    const uint32_t h_free = bar(17);    // ... read
-    const uint32_t p_full = bar(18);    // P in TMEM, S read
-    const uint32_t o_full = bar(19);    // P V and Q S0 in TMEM
-    const uint32_t o_free = bar(20);    // ... read
-    const uint32_t t_full = bar(21);    // the four blocks' decay totals in shared memory
-    const uint32_t drain = bar(22);     // every MMA complete (once, at the end)
+    auto g_full = [&](int s) { return bar(12 + s); };    // a chunk's decays in shared memory
+    auto g_free = [&](int s) { return bar(14 + s); };    // ... read
+    const uint32_t s_full = bar(16);    // Q K^T in TMEM
+    const uint32_t vt_full = bar(17);   // V~ in shared memory
+    const uint32_t d_full = bar(18);    // K^T V~ in TMEM, V~ read
+    const uint32_t d_free = bar(19);    // ... read
+    const uint32_t h_full = bar(20);    // S0 (bf16) in shared memory
+    const uint32_t h_free = bar(21);    // ... read
+    const uint32_t p_full = bar(22);    // P in TMEM, S read
+    const uint32_t o_full = bar(23);    // P V and Q S0 in TMEM, P read
+    const uint32_t o_free = bar(24);    // ... read
+    const uint32_t drain = bar(25);     // every MMA complete (once, at the end)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool wide = a.dk > 64;                         // two 64-column operand tiles
     const int ks = (int)ceil_div(a.dk, 16);              // MMA steps over Dk
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 12; ++i) mbar_init(bar(i), 1);
-        mbar_init(s_full, 1);
-        mbar_init(vt_full, 128);
-        mbar_init(d_full, 1);
-        mbar_init(d_free, 128);
-        mbar_init(h_full, 128);
-        mbar_init(h_free, 1);
-        mbar_init(p_full, 256);
-        mbar_init(o_full, 1);
-        mbar_init(o_free, 256);
-        mbar_init(t_full, 128);
-        mbar_init(drain, 1);
+        for (int i = 0; i < NBARS; ++i) {
+            const int n = (i == 12 || i == 13) ? 32 : (i == 14 || i == 15) ? 256 :
+                          (i == 17 || i == 19 || i == 20 || i == 24) ? 128 : i == 22 ? 256 : 1;
+            mbar_init(bar(i), n);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(base + OFF_TMEM), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -250,183 +296,173 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
+    if (warp == 16) {
         // -------------------------------------------------------- TMA loads
         if (lane == 0) {
-            uint32_t c = 0;
-            bool ok = true;
-            for (int64_t id = blockIdx.x; id < items && ok; id += gridDim.x) {
-                const Item it = item_of(a, tiles, id);
-                const int bq = a.cu ? 0 : (int)it.seq;
-                for (int64_t t0 = 0; t0 < it.len; t0 += C, ++c) {
-                    const int s = c & 1;
-                    const uint32_t ph = ((c >> 1) & 1) ^ 1;
-                    const int tok = (int)(it.row0 + t0);
-                    const uint32_t qk = wide ? 2 * SUB : SUB;
-                    const uint32_t dk_ = base + OFF_K + s * 2 * SUB, dq = base + OFF_Q + s * 2 * SUB;
-                    if (!(ok = mbar_wait(empty_k(s), ph, 0x401))) break;
-                    mbar_expect_tx(full_k(s), qk);
-                    tma_load_4d(dk_, &map_k, full_k(s), 0, it.h / a.k_rep, tok, bq);
-                    if (wide) tma_load_4d(dk_ + SUB, &map_k, full_k(s), 64, it.h / a.k_rep, tok, bq);
-                    if (!(ok = mbar_wait(empty_q(s), ph, 0x402))) break;
-                    mbar_expect_tx(full_q(s), qk);
-                    tma_load_4d(dq, &map_q, full_q(s), 0, it.h / a.q_rep, tok, bq);
-                    if (wide) tma_load_4d(dq + SUB, &map_q, full_q(s), 64, it.h / a.q_rep, tok, bq);
-                    if (!(ok = mbar_wait(empty_v(s), ph, 0x403))) break;
-                    mbar_expect_tx(full_v(s), SUB);
-                    tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), it.tile * DV,
-                                it.h / a.v_rep, tok, bq);
-                }
+            Walk k(a, tiles, items);
+            const uint32_t qk = wide ? 2 * SUB : SUB;
+            for (; k.valid(); k.next()) {
+                const int s = k.c & 1;
+                const uint32_t ph = ((k.c >> 1) & 1) ^ 1;
+                const int tok = (int)(k.it.row0 + k.t0), bq = a.cu ? 0 : (int)k.it.seq;
+                const int hq = k.it.h / a.q_rep, hk = k.it.h / a.k_rep, hv = k.it.h / a.v_rep;
+                const uint32_t dk = base + OFF_K + s * 2 * SUB, dq = base + OFF_Q + s * 2 * SUB;
+                if (!mbar_wait(empty_k(s), ph, 0x401)) break;
+                mbar_expect_tx(full_k(s), qk);
+                tma_load_4d(dk, &map_k, full_k(s), 0, hk, tok, bq);
+                if (wide) tma_load_4d(dk + SUB, &map_k, full_k(s), 64, hk, tok, bq);
+                if (!mbar_wait(empty_q(s), ph, 0x402)) break;
+                mbar_expect_tx(full_q(s), qk);
+                tma_load_4d(dq, &map_q, full_q(s), 0, hq, tok, bq);
+                if (wide) tma_load_4d(dq + SUB, &map_q, full_q(s), 64, hq, tok, bq);
+                if (!mbar_wait(empty_v(s), ph, 0x403)) break;
+                mbar_expect_tx(full_v(s), SUB);
+                tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
             }
             // no load is in flight when the CTA ends (its consumers may have given up)
-            for (uint32_t n = c > 2 ? c - 2 : 0; n < c; ++n) {
+            for (uint32_t n = k.c > 2 ? k.c - 2 : 0; n < k.c; ++n) {
                 mbar_wait(full_k(n & 1), (n >> 1) & 1, 0x404);
                 mbar_wait(full_q(n & 1), (n >> 1) & 1, 0x404);
                 mbar_wait(full_v(n & 1), (n >> 1) & 1, 0x404);
             }
         }
-    } else if (warp == 1) {
+        __syncwarp();
+    } else if (warp == 17) {
         // -------------------------------------------------------- MMA issue
         if (lane == 0) {
-            uint32_t c = 0;
-            bool ok = true;
-            for (int64_t id = blockIdx.x; id < items && ok; id += gridDim.x) {
-                const Item it = item_of(a, tiles, id);
-                for (int64_t t0 = 0; t0 < it.len && ok; t0 += C, ++c) {
-                    const int s = c & 1;
-                    const uint32_t ph2 = (c >> 1) & 1, ph = c & 1, prev = ph ^ 1;
-                    const uint32_t q = base + OFF_Q + s * 2 * SUB, k = base + OFF_K + s * 2 * SUB;
-                    const uint32_t v = base + OFF_V + s * SUB;
-                    // S = Q K^T (P of the chunk before read the last S before p_full)
-                    if (!(ok = mbar_wait(full_k(s), ph2, 0x411) && mbar_wait(full_q(s), ph2, 0x412)))
-                        break;
-                    fence_after();
-                    for (int i = 0; i < ks; ++i) {
-                        const uint32_t off = (i >> 2) * SUB + (i & 3) * 32;
-                        mma_ss(tmem + T_S, smem_desc(q + off), smem_desc(k + off),
-                               idesc(128, false, false), i > 0);
-                    }
-                    mma_commit(s_full);
-                    // K^T V~, three parts side by side
-                    if (!(ok = mbar_wait(vt_full, ph, 0x413) && mbar_wait(d_free, prev, 0x414))) break;
-                    fence_after();
-#pragma unroll
-                    for (int i = 0; i < C / 16; ++i)
-                        mma_ss(tmem + T_D, smem_desc_mn(k + i * 2048),
-                               smem_desc_mn(base + OFF_VT + i * 2048), idesc(192, true, true), i > 0);
-                    mma_commit(d_full);
-                    mma_commit(empty_k(s));
-                    // Q S0
-                    if (!(ok = mbar_wait(h_full, ph, 0x415) && mbar_wait(o_free, prev, 0x416))) break;
-                    fence_after();
-                    for (int i = 0; i < ks; ++i)
-                        mma_ss(tmem + T_QH, smem_desc(q + (i >> 2) * SUB + (i & 3) * 32),
-                               smem_desc_mn(base + OFF_H + i * 2048), idesc(64, false, true), i > 0);
-                    mma_commit(h_free);
-                    mma_commit(empty_q(s));
-                    // P V
-                    if (!(ok = mbar_wait(p_full, ph, 0x417))) break;
-                    fence_after();
-#pragma unroll
-                    for (int i = 0; i < C / 16; ++i)
-                        mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, smem_desc_mn(v + i * 2048),
-                                    idesc(64, false, true), i > 0);
-                    mma_commit(o_full);
-                    mma_commit(empty_v(s));
+            uint32_t total = 0;
+            for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
+                total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
+            const uint64_t dq0 = smem_desc(base + OFF_Q), dk0 = smem_desc(base + OFF_K);
+            const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
+            const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
+            constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
+            // S = Q K^T of chunk c
+            auto qk = [&](uint32_t c) {
+                const int s = c & 1;
+                const uint32_t ph = (c >> 1) & 1;
+                if (!mbar_wait(full_k(s), ph, 0x411) || !mbar_wait(full_q(s), ph, 0x412))
+                    return false;
+                fence_after();
+#pragma unroll 1
+                for (int i = 0; i < ks; ++i) {
+                    const uint64_t off = s * STAGE + (i >> 2) * (SUB >> 4) + (i & 3) * 2;
+                    mma_ss(tmem + T_S, dq0 + off, dk0 + off, idesc(128, false, false), i > 0);
                 }
+                mma_commit(s_full);
+                return true;
+            };
+            // K^T V~ of chunk c, the three parts of V~ side by side
+            auto ktv = [&](uint32_t c) {
+                if (!mbar_wait(vt_full, c & 1, 0x413) || !mbar_wait(d_free, (c & 1) ^ 1, 0x414))
+                    return false;
+                fence_after();
+#pragma unroll 1
+                for (int i = 0; i < C / 16; ++i)
+                    mma_ss(tmem + T_D, kt0 + (c & 1) * STAGE + i * ROWS16, vt0 + i * ROWS16,
+                           idesc(192, true, true), i > 0);
+                mma_commit(d_full);
+                mma_commit(empty_k(c & 1));
+                return true;
+            };
+            bool ok = total > 0 && qk(0) && ktv(0);
+            for (uint32_t c = 0; ok && c < total; ++c) {
+                const int s = c & 1;
+                if (!(ok = mbar_wait(h_full, c & 1, 0x415) && mbar_wait(o_free, (c & 1) ^ 1, 0x416)))
+                    break;
+                fence_after();
+#pragma unroll 1
+                for (int i = 0; i < ks; ++i)
+                    mma_ss(tmem + T_QH, dq0 + s * STAGE + (i >> 2) * (SUB >> 4) + (i & 3) * 2,
+                           h0 + i * ROWS16, idesc(64, false, true), i > 0);
+                mma_commit(h_free);
+                mma_commit(empty_q(s));
+                if (!(ok = mbar_wait(p_full, c & 1, 0x417))) break;
+                fence_after();
+                if (c + 1 < total && !(ok = qk(c + 1))) break;
+#pragma unroll 1
+                for (int i = 0; i < C / 16; ++i)
+                    mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8,
+                                v0 + s * (SUB >> 4) + i * ROWS16, idesc(64, false, true), i > 0);
+                mma_commit(o_full);
+                mma_commit(empty_v(s));
+                if (c + 1 < total) ok = ktv(c + 1);
             }
             mma_commit(drain);                           // before TMEM is given back
             mbar_wait(drain, 0, 0x418);
         }
         __syncwarp();
-    } else if (warp >= 4 && warp < 8) {
-        // ------------------------------------------- decays, V~ and the state
-        const int w = warp & 3, r = 32 * w + lane;        // token of a chunk, row of the state
+    } else if (warp == 18) {
+        // ----------------------------------------------------------- decays
+        Walk k(a, tiles, items);
+        float gn[4];
+        if (k.valid()) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
+        }
+        while (k.valid()) {
+            const uint32_t c = k.c;
+            const int s = c & 1;
+            double g[4], t[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) g[b] = (double)clamp_g(gn[b]);
+            k.next();                                    // the next chunk's loads
+            if (k.valid()) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const double y = __shfl_up_sync(0xffffffffu, g[b], d);
+                    if (lane >= d) g[b] += y;
+                }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) t[b] = __shfl_sync(0xffffffffu, g[b], 31);
+            // lane l: the blocks whose decays scalar l of OFF_SC multiplies
+            constexpr uint64_t sets = 0x462F08CE7310ull;
+            const uint32_t set = lane < 12 ? (uint32_t)(sets >> (4 * lane)) & 15u : 0u;
+            double sum = 0.0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                if (set >> b & 1u) sum += t[b];
+            const float mine = exp_of(sum);
+            float cf[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) cf[b] = exp_of(t[b] - g[b]);
+            if (!wait_warp(g_free(s), ((c >> 1) & 1) ^ 1, 0x451)) break;
+            if (lane < 16) sc[s * 16 + lane] = mine;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                colf[s * C + 32 * b + lane] = cf[b];
+                g2[s * C + 32 * b + lane] = (float)(g[b] * 1.4426950408889634);
+            }
+            mbar_arrive(g_full(s));
+        }
+    } else if (warp < 4) {
+        // -------------------------------------------------------- the state
+        const int w = warp & 3, r = 32 * w + lane;        // row of the state
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
+        uint8_t *const hrow = smem + OFF_H + r * 128;
         uint32_t c = 0;
         bool ok = true;
-        for (int64_t id = blockIdx.x; id < items && ok; id += gridDim.x) {
+        for (uint32_t id = blockIdx.x; id < items && ok; id += gridDim.x) {
             const Item it = item_of(a, tiles, id);
             const int c0 = it.tile * DV;
             const int64_t at = ((it.seq * a.heads + it.h) * a.dk + r) * a.dv + c0;
             float h[DV];
-            if (a.h0 && r < a.dk) {
 #pragma unroll
-                for (int i = 0; i < DV; i += 4) {
-                    float4 x = make_float4(0, 0, 0, 0);
-                    if (c0 + i < a.dv) x = *reinterpret_cast<const float4 *>(a.h0 + at + i);
-                    h[i] = x.x; h[i + 1] = x.y; h[i + 2] = x.z; h[i + 3] = x.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < DV; ++i) h[i] = 0.0f;
+            for (int i = 0; i < DV; i += 4) {
+                float4 x = make_float4(0, 0, 0, 0);
+                if (a.h0 && r < a.dk && c0 + i < a.dv)
+                    x = *reinterpret_cast<const float4 *>(a.h0 + at + i);
+                h[i] = x.x; h[i + 1] = x.y; h[i + 2] = x.z; h[i + 3] = x.w;
             }
-            float gn = load_g(a, it, r);
             for (int64_t t0 = 0; t0 < it.len; t0 += C, ++c) {
                 const int s = c & 1;
-                const uint32_t ph = c & 1, prev = ph ^ 1;
-                const int m = (int)(it.len - t0 < C ? it.len - t0 : C);
-                const double gl = scan32(gn);
-                gn = load_g(a, it, t0 + C + r);
-                const double bt = __shfl_sync(0xffffffffu, gl, 31);
-                const float cf = exp_of(bt - gl);
-                colf[s * C + r] = cf;
-                if (lane == 0) tot[s * 4 + w] = bt;
-                mbar_arrive(t_full);
-                if (!(ok = wait_warp(t_full, ph, 0x420))) break;
-                double later = 0.0, all = 0.0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const double x = tot[s * 4 + b];
-                    all += x;
-                    if (b > w) later += x;
-                }
-                const float dec = exp_of(all);            // e^{G_C}
-                const float wj = cf * exp_of(later);      // e^{G_C - G_j}
-                if (!(ok = wait_warp(full_v(s), (c >> 1) & 1, 0x421))) break;
-                uint8_t *const vrow = smem + OFF_V + s * SUB + r * 128;
-                uint8_t *const trow = smem + OFF_VT + r * 128;
-                if (m < C && !(ok = wait_warp(full_k(s), (c >> 1) & 1, 0x422))) break;
-                if (r < m) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t off = (uint32_t)((i ^ (r & 7)) << 4);
-                        const uint4 x4 = *reinterpret_cast<const uint4 *>(vrow + off);
-                        const uint32_t *x = reinterpret_cast<const uint32_t *>(&x4);
-                        uint32_t p0[4], p1[4], p2[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float lo = bf_lo(x[e]) * wj, hi = bf_hi(x[e]) * wj;
-                            p0[e] = pack_bf16(lo, hi);
-                            lo -= bf_lo(p0[e]);
-                            hi -= bf_hi(p0[e]);
-                            p1[e] = pack_bf16(lo, hi);
-                            p2[e] = pack_bf16(lo - bf_lo(p1[e]), hi - bf_hi(p1[e]));
-                        }
-                        *reinterpret_cast<uint4 *>(trow + off) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-                        *reinterpret_cast<uint4 *>(trow + SUB + off) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
-                        *reinterpret_cast<uint4 *>(trow + 2 * SUB + off) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
-                    }
-                } else {
-                    // rows behind the sequence (another one's, or nothing): zero in
-                    // V, V~ and K, whose values a product would otherwise meet
-                    const uint4 z = make_uint4(0, 0, 0, 0);
-                    uint8_t *const krow = smem + OFF_K + s * 2 * SUB + r * 128;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        *reinterpret_cast<uint4 *>(vrow + i * 16) = z;
-                        *reinterpret_cast<uint4 *>(trow + i * 16) = z;
-                        *reinterpret_cast<uint4 *>(trow + SUB + i * 16) = z;
-                        *reinterpret_cast<uint4 *>(trow + 2 * SUB + i * 16) = z;
-                        *reinterpret_cast<uint4 *>(krow + i * 16) = z;
-                        *reinterpret_cast<uint4 *>(krow + SUB + i * 16) = z;
-                    }
-                }
-                fence_async_smem();
-                mbar_arrive(vt_full);
                 // S0 of this chunk for Q S0
-                if (!(ok = wait_warp(h_free, prev, 0x423))) break;
-                uint8_t *const hrow = smem + OFF_H + r * 128;
+                if (!(ok = wait_warp(h_free, (c & 1) ^ 1, 0x423))) break;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     uint4 x;
@@ -439,21 +475,25 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 fence_async_smem();
                 mbar_arrive(h_full);
                 // S = e^{G_C} S0 + K^T V~
-                if (!(ok = wait_warp(d_full, ph, 0x424))) break;
+                if (!(ok = wait_warp(g_full(s), (c >> 1) & 1, 0x424))) break;
+                const float dec = sc[s * 16 + SC_ALL];
+                mbar_arrive(g_free(s));
+                if (!(ok = wait_warp(d_full, c & 1, 0x425))) break;
                 fence_after();
 #pragma unroll
-                for (int half = 0; half < 4; ++half) {
-                    uint32_t d0[16], d1[16], d2[16];
-                    tmem_ld16_async(quarter + T_D + half * 16, d0);
-                    tmem_ld16_async(quarter + T_D + 64 + half * 16, d1);
-                    tmem_ld16_async(quarter + T_D + 128 + half * 16, d2);
-                    tmem_wait_ld();
+                for (int i = 0; i < DV; i += 8) {
+                    uint32_t d0[8], d1[8], d2[8];
+                    tmem_ld8_async(quarter + T_D + i, d0);
+                    tmem_ld8_async(quarter + T_D + 64 + i, d1);
+                    tmem_ld8_async(quarter + T_D + 128 + i, d2);
+                    tmem_loaded(d0);
+                    tmem_loaded(d1);
+                    tmem_loaded(d2);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        h[half * 16 + i] =
-                            fmaf(dec, h[half * 16 + i],
-                                 __uint_as_float(d0[i]) +
-                                     (__uint_as_float(d1[i]) + __uint_as_float(d2[i])));
+                    for (int e = 0; e < 8; ++e)
+                        h[i + e] = fmaf(dec, h[i + e],
+                                        __uint_as_float(d0[e]) +
+                                            (__uint_as_float(d1[e]) + __uint_as_float(d2[e])));
                 }
                 fence_before();
                 mbar_arrive(d_free);
@@ -466,106 +506,174 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                             make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
             }
         }
-    } else if (warp >= 8) {
-        // --------------------------------------------------- P and the outputs
-        const int w = warp & 3, half = (warp - 8) >> 2, r = 32 * w + lane;
+    } else if (warp < 12) {
+        // ---------------------------------------------------------------- P
+        // rows 32 w + lane; the first four warps take blocks 0 and 2, the others
+        // 1 and 3.  Blocks above the diagonal stay the zeros written here.
+        const int w = warp & 3, odd = (warp - 4) >> 2, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
-        uint32_t c = 0;
-        bool ok = true;
-        for (int64_t id = blockIdx.x; id < items && ok; id += gridDim.x) {
-            const Item it = item_of(a, tiles, id);
-            const int64_t bq = a.cu ? 0 : it.seq;
-            const int col = it.tile * DV + 32 * half;
-            __nv_bfloat16 *const o = static_cast<__nv_bfloat16 *>(a.o) + bq * a.os[0] +
-                                     it.row0 * a.os[1] + it.h * a.os[2] + col;
-            float gn = load_g(a, it, r);
-            for (int64_t t0 = 0; t0 < it.len; t0 += C, ++c) {
-                const int s = c & 1;
-                const uint32_t ph = c & 1;
-                const double gl = scan32(gn);
-                gn = load_g(a, it, t0 + C + r);
-                const float ghi = (float)gl, glo = (float)(gl - (double)ghi);
-                if (!(ok = wait_warp(vt_full, ph, 0x431))) break;
-                // e^{G_i - (G at the end of block b)} for the blocks before this
-                // one, and e^{G_i}
-                double sum = gl;
-                float f[3] = {0.0f, 0.0f, 0.0f};
+        {
+            uint32_t z[16];
 #pragma unroll
-                for (int b = 2; b >= 0; --b)
-                    if (b < w) {
-                        f[b] = __expf((float)sum);
-                        sum += tot[s * 4 + b];
+            for (int i = 0; i < 16; ++i) z[i] = 0u;
+            tmem_st16(quarter + T_P + 16 * odd, z);
+            tmem_st16(quarter + T_P + 16 * (odd + 2), z);
+            tmem_wait_st();
+        }
+        uint32_t total = 0;
+        for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
+            total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
+        for (uint32_t c = 0; c < total; ++c) {
+            const int s = c & 1;
+            if (!wait_warp(g_full(s), (c >> 1) & 1, 0x431)) break;
+            const float gr = g2[s * C + r];
+            const float rowf = ex2(gr);
+            // e^{blocks between}: block b's columns for the rows of block w
+            const float f0 = rowf * (w == 2 ? sc[s * 16 + SC_1] : w == 3 ? sc[s * 16 + SC_12] : 1.0f);
+            const float f1 = rowf * (w == 3 ? sc[s * 16 + SC_2] : 1.0f);
+            if (!wait_warp(s_full, c & 1, 0x432)) break;
+            fence_after();
+            // P of the chunk before has been read
+            if (!wait_warp(o_full, (c & 1) ^ 1, 0x433)) break;
+            fence_after();
+#pragma unroll 1
+            for (int n = 2 * odd; n < 2 * w + 2; n += (n & 1) ? 3 : 1) {   // 16 columns
+                uint32_t x[16], p[8];
+                tmem_ld16_async(quarter + T_S + 16 * n, x);
+                const int b = n >> 1;
+                if (b < w) {
+                    const float fb = b == 0 ? f0 : b == 1 ? f1 : rowf;
+                    const float4 *cf = reinterpret_cast<const float4 *>(colf + s * C + 16 * n);
+                    tmem_loaded(x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 y = cf[i];
+                        p[2 * i] = pack_bf16(__uint_as_float(x[4 * i]) * (y.x * fb),
+                                             __uint_as_float(x[4 * i + 1]) * (y.y * fb));
+                        p[2 * i + 1] = pack_bf16(__uint_as_float(x[4 * i + 2]) * (y.z * fb),
+                                                 __uint_as_float(x[4 * i + 3]) * (y.w * fb));
                     }
-                const float ei = __expf((float)sum) * a.scale;
-                if (!(ok = wait_warp(s_full, ph, 0x432))) break;
-                fence_after();
+                } else {
+                    const float4 *gj = reinterpret_cast<const float4 *>(g2 + s * C + 16 * n);
+                    const int last = lane - 16 * (n & 1);            // the diagonal's column
+                    tmem_loaded(x);
 #pragma unroll
-                for (int bb = 0; bb < 2; ++bb) {
-                    const int b = 2 * half + bb;
-                    uint32_t p[16];
-                    if (b > w) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) p[i] = 0u;
-                    } else {
-                        uint32_t x[32];
-                        tmem_ld32_async(quarter + T_S + 32 * b, x);
-                        tmem_wait_ld();
-                        if (b < w) {
-                            const float fb = b == 0 ? f[0] : b == 1 ? f[1] : f[2];
-                            const float4 *cf = reinterpret_cast<const float4 *>(colf + s * C + 32 * b);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float4 y = cf[i];
-                                p[2 * i] = pack_bf16(__uint_as_float(x[4 * i]) * (y.x * fb),
-                                                     __uint_as_float(x[4 * i + 1]) * (y.y * fb));
-                                p[2 * i + 1] = pack_bf16(__uint_as_float(x[4 * i + 2]) * (y.z * fb),
-                                                         __uint_as_float(x[4 * i + 3]) * (y.w * fb));
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                float e[2];
-#pragma unroll
-                                for (int z = 0; z < 2; ++z) {
-                                    const int j = 2 * i + z;
-                                    const float d = (ghi - __shfl_sync(0xffffffffu, ghi, j)) +
-                                                    (glo - __shfl_sync(0xffffffffu, glo, j));
-                                    e[z] = j <= lane ? __uint_as_float(x[j]) * __expf(d) : 0.0f;
-                                }
-                                p[i] = pack_bf16(e[0], e[1]);
-                            }
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 y = gj[i];
+                        const float e0 = __uint_as_float(x[4 * i]) * ex2(gr - y.x);
+                        const float e1 = __uint_as_float(x[4 * i + 1]) * ex2(gr - y.y);
+                        const float e2 = __uint_as_float(x[4 * i + 2]) * ex2(gr - y.z);
+                        const float e3 = __uint_as_float(x[4 * i + 3]) * ex2(gr - y.w);
+                        p[2 * i] = pack_bf16(4 * i <= last ? e0 : 0.0f, 4 * i + 1 <= last ? e1 : 0.0f);
+                        p[2 * i + 1] =
+                            pack_bf16(4 * i + 2 <= last ? e2 : 0.0f, 4 * i + 3 <= last ? e3 : 0.0f);
                     }
-                    tmem_st16(quarter + T_P + 16 * b, p);
                 }
-                tmem_wait_st();
-                fence_before();
-                mbar_arrive(p_full);
-
-                if (!(ok = wait_warp(o_full, ph, 0x433))) break;
-                fence_after();
-                uint32_t pv[32], qh[32];
-                tmem_ld32_async(quarter + T_PV + 32 * half, pv);
-                tmem_ld32_async(quarter + T_QH + 32 * half, qh);
-                tmem_wait_ld();
-                fence_before();
-                mbar_arrive(o_free);
-                const int64_t t = t0 + r;
+                tmem_st8(quarter + T_P + 8 * n, p);
+            }
+            tmem_wait_st();
+            fence_before();
+            mbar_arrive(p_full);
+        }
+    } else {
+        // ------------------------------------------- V~ and the output rows
+        const int w = warp & 3, r = 32 * w + lane;
+        const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
+        // iteration n: V~ of chunk n, the rows of V times e^{G_C - G_j} in three
+        // bf16 parts; then the outputs of chunk n - 1
+        Walk k(a, tiles, items);
+        Item it = k.it;
+        int64_t t0 = 0;
+        for (uint32_t n = 0;; ++n) {
+          const bool more = k.valid();
+          if (more) {
+            const int s = n & 1;
+            const uint32_t ph2 = (n >> 1) & 1;
+            const int64_t left = k.it.len - k.t0;
+            const int m = (int)(left < C ? left : C);
+            if (!wait_warp(g_full(s), ph2, 0x441)) break;
+            const float wj = colf[s * C + r] * sc[s * 16 + SC_AFTER + w];
+            if (!wait_warp(full_v(s), ph2, 0x442)) break;
+            if (m < C && !wait_warp(full_k(s), ph2, 0x443)) break;
+            if (!wait_warp(d_full, (n & 1) ^ 1, 0x444)) break;             // V~ (n - 1) read
+            uint8_t *const vrow = smem + OFF_V + s * SUB + r * 128;
+            uint8_t *const trow = smem + OFF_VT + r * 128;
+            if (r < m) {
+#pragma unroll 2
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t off = (uint32_t)((i ^ (r & 7)) << 4);
+                    const uint4 x4 = *reinterpret_cast<const uint4 *>(vrow + off);
+                    const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+                    uint32_t p0[4], p1[4], p2[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float lo = bf_lo(x[e]) * wj, hi = bf_hi(x[e]) * wj;
+                        p0[e] = pack_bf16(lo, hi);
+                        lo -= bf_lo(p0[e]);
+                        hi -= bf_hi(p0[e]);
+                        p1[e] = pack_bf16(lo, hi);
+                        p2[e] = pack_bf16(lo - bf_lo(p1[e]), hi - bf_hi(p1[e]));
+                    }
+                    *reinterpret_cast<uint4 *>(trow + off) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+                    *reinterpret_cast<uint4 *>(trow + SUB + off) =
+                        make_uint4(p1[0], p1[1], p1[2], p1[3]);
+                    *reinterpret_cast<uint4 *>(trow + 2 * SUB + off) =
+                        make_uint4(p2[0], p2[1], p2[2], p2[3]);
+                }
+            } else {
+                // rows behind the sequence (another one's, or nothing): zero in
+                // V, V~ and K, whose values a product would otherwise meet
+                const uint4 z = make_uint4(0, 0, 0, 0);
+                uint8_t *const krow = smem + OFF_K + s * 2 * SUB + r * 128;
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {
+                    *reinterpret_cast<uint4 *>(vrow + i * 16) = z;
+                    *reinterpret_cast<uint4 *>(trow + i * 16) = z;
+                    *reinterpret_cast<uint4 *>(trow + SUB + i * 16) = z;
+                    *reinterpret_cast<uint4 *>(trow + 2 * SUB + i * 16) = z;
+                    *reinterpret_cast<uint4 *>(krow + i * 16) = z;
+                    *reinterpret_cast<uint4 *>(krow + SUB + i * 16) = z;
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(vt_full);
+          }
+          if (n > 0) {
+            const int s = (n - 1) & 1;
+            const float ei = ex2(g2[s * C + r]) * sc[s * 16 + SC_BEFORE + w] * a.scale;
+            if (!wait_warp(o_full, (n - 1) & 1, 0x445)) break;
+            mbar_arrive(g_free(s));                      // P (n - 1) has read them too
+            fence_after();
+            const int64_t bq = a.cu ? 0 : it.seq;
+            const int64_t t = t0 + r;
+#pragma unroll 1
+            for (int part = 0; part < 4; ++part) {
+                const int col = it.tile * DV + 16 * part;
+                uint32_t pv[16], qh[16];
+                tmem_ld16_async(quarter + T_PV + 16 * part, pv);
+                tmem_ld16_async(quarter + T_QH + 16 * part, qh);
+                tmem_loaded(pv);
+                tmem_loaded(qh);
+                if (part == 3) {
+                    fence_before();
+                    mbar_arrive(o_free);
+                }
                 if (t < it.len) {
-                    float y[32];
+                    float y[16];
                     float bad = 0.0f;                     // 0, or NaN
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         y[i] = __uint_as_float(pv[i]);
                         bad = fmaf(0.0f, y[i], bad);
                     }
                     if (bad != 0.0f) masked_row(a, it, t0, t, col, y);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    for (int i = 0; i < 16; ++i)
                         y[i] = fmaf(y[i], a.scale, __uint_as_float(qh[i]) * ei);
-                    __nv_bfloat16 *const row = o + t * a.os[1];
+                    __nv_bfloat16 *const row = static_cast<__nv_bfloat16 *>(a.o) + bq * a.os[0] +
+                                               (it.row0 + t) * a.os[1] + it.h * a.os[2] + col;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8)
+                    for (int i = 0; i < 16; i += 8)
                         if (col + i < a.dv) {
                             uint4 x;
                             x.x = pack_bf16(y[i], y[i + 1]);
@@ -575,14 +683,20 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                             *reinterpret_cast<uint4 *>(row + i) = x;
                         }
                 }
+                __syncwarp();
             }
+          }
+          if (!more) break;
+          it = k.it;
+          t0 = k.t0;
+          k.next();
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 1) {
+    if (warp == 17) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
@@ -654,8 +768,9 @@ int chunked(const Args &a, cudaStream_t st, bool *used) {
     if (e != cudaSuccess) return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
     const int tiles = (int)ceil_div(a.dv, DV);
     const int64_t items = (int64_t)tiles * a.heads * a.seqs;
+    MB2_REQUIRE(items < (1ll << 31), MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
     const unsigned grid = (unsigned)(items < sms ? items : sms);
-    decay_chunk_kernel<<<grid, THREADS, SMEM_BYTES, st>>>(mq, mk, mv, a, tiles, items);
+    decay_chunk_kernel<<<grid, THREADS, SMEM_BYTES, st>>>(mq, mk, mv, a, tiles, (uint32_t)items);
     return check_launch("decay_chunk_kernel");
 }
 
