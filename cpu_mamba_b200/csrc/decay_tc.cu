@@ -1,6 +1,6 @@
 // Decay attention over prompts on the tensor cores (bf16): chunks of 128 tokens,
 // one CTA walking the chunks of a (sequence, head, 64 columns of v) with the
-// state S (Dk x 64) in fp32 registers.  Within a chunk, with G_i the sum of the
+// state S (Dk x 64) in fp32 in TMEM.  Within a chunk, with G_i the sum of the
 // log decays up to token i and S0 the state before it,
 //   P_ij = e^{G_i - G_j} (q_i . k_j)  for j <= i, else 0
 //   o_i  = scale (sum_j P_ij v_j + e^{G_i} q_i^T S0)
@@ -17,19 +17,24 @@
 //
 // Roundings to bf16: P and S0 as MMA operands (the products of a flash-attention
 // style kernel; outputs are bf16 anyway).  V~ is held as three bf16 parts
-// (24 bits), multiplied side by side as one N = 192 MMA, because the state is an
-// fp32 output and lives for many chunks.
+// (24 bits), because the state is an fp32 output and lives for many chunks.
 //
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone.
 //
-// Roles (19 warps): 0-3 the state, 4-11 P, 12-15 V~ and the output rows, 16 TMA
-// loads, 17 MMA issue, 18 decays.  A chunk's products are issued as
-//   Q S0 (n), Q K^T (n + 1), P V (n), K^T V~ (n + 1)
+// Roles (23 warps): 0-3 the state, 4-11 P, 12-15 V~, 16-19 the output rows, 20 TMA
+// loads, 21 MMA issue, 22 decays.  A chunk's products are issued as
+//   Q S0 (n), P V (n), Q K^T (n + 1), K^T V~ (n + 1)
 // so that P (n + 1) and the state update overlap the others' MMAs.  Every
 // mbarrier completes once per chunk (staged ones once per two), so its phase
 // follows from the chunk count.  All waits are bounded; a wait that expires sets
 // the device status.
+//
+// Instruction supply is what this layout is built around: five roles' warps
+// share each scheduler's small instruction cache, and with straight-line bodies
+// (the state in registers, 500 instructions a role) a chunk took 11,000 cycles,
+// half of them stalled for instructions.  So each role's chunk is a short loop
+// over 16-column pieces, and the state lives in TMEM.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -43,7 +48,7 @@ using namespace tc;
 
 constexpr int C = 128;                       // tokens per chunk
 constexpr int DV = 64;                       // columns of v per CTA
-constexpr int THREADS = 608;
+constexpr int THREADS = 736;
 constexpr uint32_t SUB = 128 * 128;          // one 128-row x 128-byte operand tile
 // shared memory (bytes from a 1024-aligned base)
 constexpr uint32_t OFF_Q = 0;                            // [2][2 SUB]
@@ -65,7 +70,8 @@ constexpr int SC_ALL = 8;        // the chunk
 constexpr int SC_1 = 9, SC_12 = 10, SC_2 = 11;   // block 1; blocks 1 and 2; block 2
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 // TMEM columns
-constexpr uint32_t T_S = 0, T_P = 128, T_PV = 192, T_QH = 256, T_D = 320;
+// (T_D: K^T V~ of V~'s first part, then of the other two)
+constexpr uint32_t T_S = 0, T_P = 128, T_PV = 192, T_QH = 256, T_D = 320, T_H = 448;
 
 // UMMA descriptor of an MN-major operand, 128-byte swizzle: rows are the
 // contraction index (128 bytes of 64 MN elements each), 8-row groups 1024 B
@@ -143,6 +149,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(head), "r"(tok),
           "r"(b)
         : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap *map, int32_t x, int32_t head,
+                                                int32_t tok, int32_t b) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(b)
+                 : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
@@ -277,7 +295,6 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool wide = a.dk > 64;                         // two 64-column operand tiles
-    const int ks = (int)ceil_div(a.dk, 16);              // MMA steps over Dk
     if (threadIdx.x == 0) {
         for (int i = 0; i < NBARS; ++i) {
             const int n = (i == 12 || i == 13) ? 32 : (i == 14 || i == 15) ? 256 :
@@ -286,7 +303,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 17) {
+    if (warp == 21) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(base + OFF_TMEM), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -296,11 +313,12 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 16) {
+    if (warp == 20) {
         // -------------------------------------------------------- TMA loads
         if (lane == 0) {
-            Walk k(a, tiles, items);
+            Walk k(a, tiles, items), ahead(a, tiles, items);
             const uint32_t qk = wide ? 2 * SUB : SUB;
+            if (ahead.valid()) ahead.next();
             for (; k.valid(); k.next()) {
                 const int s = k.c & 1;
                 const uint32_t ph = ((k.c >> 1) & 1) ^ 1;
@@ -318,6 +336,17 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (!mbar_wait(empty_v(s), ph, 0x403)) break;
                 mbar_expect_tx(full_v(s), SUB);
                 tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
+                // the chunk that these stages take next comes from L2
+                if (ahead.valid()) ahead.next();
+                if (ahead.valid()) {
+                    const Item &it = ahead.it;
+                    const int tk = (int)(it.row0 + ahead.t0), b = a.cu ? 0 : (int)it.seq;
+                    tma_prefetch_4d(&map_k, 0, it.h / a.k_rep, tk, b);
+                    if (wide) tma_prefetch_4d(&map_k, 64, it.h / a.k_rep, tk, b);
+                    tma_prefetch_4d(&map_q, 0, it.h / a.q_rep, tk, b);
+                    if (wide) tma_prefetch_4d(&map_q, 64, it.h / a.q_rep, tk, b);
+                    tma_prefetch_4d(&map_v, it.tile * DV, it.h / a.v_rep, tk, b);
+                }
             }
             // no load is in flight when the CTA ends (its consumers may have given up)
             for (uint32_t n = k.c > 2 ? k.c - 2 : 0; n < k.c; ++n) {
@@ -327,72 +356,85 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             }
         }
         __syncwarp();
-    } else if (warp == 17) {
+    } else if (warp == 21) {
         // -------------------------------------------------------- MMA issue
-        if (lane == 0) {
-            uint32_t total = 0;
-            for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
-                total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
-            const uint64_t dq0 = smem_desc(base + OFF_Q), dk0 = smem_desc(base + OFF_K);
-            const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
-            const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
-            constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
-            // S = Q K^T of chunk c
-            auto qk = [&](uint32_t c) {
-                const int s = c & 1;
-                const uint32_t ph = (c >> 1) & 1;
-                if (!mbar_wait(full_k(s), ph, 0x411) || !mbar_wait(full_q(s), ph, 0x412))
-                    return false;
+        // the whole warp walks the chunks (descriptors stay uniform); one lane
+        // issues
+        const bool leader = elect_one();
+        uint32_t total = 0;
+        for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
+            total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
+        const uint64_t dq0 = smem_desc(base + OFF_Q), dk0 = smem_desc(base + OFF_K);
+        const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
+        const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
+        constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
+        const int steps = wide ? 8 : 4;                  // of 16 columns of q and k
+        // iteration n: Q S0 and P V of chunk n - 1, then Q K^T and K^T V~ of chunk n
+        for (uint32_t n = 0; n <= total; ++n) {
+            if (n > 0) {
+                const uint32_t c = n - 1, ph = c & 1;
+                const uint64_t q = dq0 + ph * STAGE, v = v0 + ph * (SUB >> 4);
+                if (!wait_warp(h_full, ph, 0x415) || !wait_warp(o_free, ph ^ 1, 0x416)) break;
                 fence_after();
-#pragma unroll 1
-                for (int i = 0; i < ks; ++i) {
-                    const uint64_t off = s * STAGE + (i >> 2) * (SUB >> 4) + (i & 3) * 2;
-                    mma_ss(tmem + T_S, dq0 + off, dk0 + off, idesc(128, false, false), i > 0);
+                if (leader) {
+#pragma unroll 2
+                    for (int i = 0; i < steps; ++i)
+                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h0 + i * ROWS16,
+                               idesc(64, false, true), i != 0);
+                    mma_commit(h_free);
+                    mma_commit(empty_q(ph));
                 }
-                mma_commit(s_full);
-                return true;
-            };
-            // K^T V~ of chunk c, the three parts of V~ side by side
-            auto ktv = [&](uint32_t c) {
-                if (!mbar_wait(vt_full, c & 1, 0x413) || !mbar_wait(d_free, (c & 1) ^ 1, 0x414))
-                    return false;
+                __syncwarp();
+                if (!wait_warp(p_full, ph, 0x417)) break;
                 fence_after();
-#pragma unroll 1
-                for (int i = 0; i < C / 16; ++i)
-                    mma_ss(tmem + T_D, kt0 + (c & 1) * STAGE + i * ROWS16, vt0 + i * ROWS16,
-                           idesc(192, true, true), i > 0);
-                mma_commit(d_full);
-                mma_commit(empty_k(c & 1));
-                return true;
-            };
-            bool ok = total > 0 && qk(0) && ktv(0);
-            for (uint32_t c = 0; ok && c < total; ++c) {
-                const int s = c & 1;
-                if (!(ok = mbar_wait(h_full, c & 1, 0x415) && mbar_wait(o_free, (c & 1) ^ 1, 0x416)))
-                    break;
-                fence_after();
-#pragma unroll 1
-                for (int i = 0; i < ks; ++i)
-                    mma_ss(tmem + T_QH, dq0 + s * STAGE + (i >> 2) * (SUB >> 4) + (i & 3) * 2,
-                           h0 + i * ROWS16, idesc(64, false, true), i > 0);
-                mma_commit(h_free);
-                mma_commit(empty_q(s));
-                if (!(ok = mbar_wait(p_full, c & 1, 0x417))) break;
-                fence_after();
-                if (c + 1 < total && !(ok = qk(c + 1))) break;
-#pragma unroll 1
-                for (int i = 0; i < C / 16; ++i)
-                    mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8,
-                                v0 + s * (SUB >> 4) + i * ROWS16, idesc(64, false, true), i > 0);
-                mma_commit(o_full);
-                mma_commit(empty_v(s));
-                if (c + 1 < total) ok = ktv(c + 1);
+                if (leader) {
+#pragma unroll 2
+                    for (int i = 0; i < C / 16; ++i)
+                        mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, v + i * ROWS16,
+                                    idesc(64, false, true), i != 0);
+                    mma_commit(o_full);
+                    mma_commit(empty_v(ph));
+                }
+                __syncwarp();
             }
+            if (n < total) {
+                const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
+                const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE, kt = kt0 + s * STAGE;
+                if (!wait_warp(full_k(s), ph2, 0x411) || !wait_warp(full_q(s), ph2, 0x412)) break;
+                fence_after();
+                if (leader) {
+#pragma unroll 2
+                    for (int i = 0; i < steps; ++i) {
+                        const uint64_t off = (i >> 2) * (SUB >> 4) + (i & 3) * 2;
+                        mma_ss(tmem + T_S, q + off, k + off, idesc(128, false, false), i != 0);
+                    }
+                    mma_commit(s_full);
+                }
+                __syncwarp();
+                if (!wait_warp(vt_full, s, 0x413) || !wait_warp(d_free, s ^ 1, 0x414)) break;
+                fence_after();
+                if (leader) {
+                    // V~'s first two parts side by side, the third added to the second's
+#pragma unroll 2
+                    for (int i = 0; i < C / 16; ++i)
+                        mma_ss(tmem + T_D, kt + i * ROWS16, vt0 + i * ROWS16, idesc(128, true, true),
+                               i != 0);
+#pragma unroll 2
+                    for (int i = 0; i < C / 16; ++i)
+                        mma_ss(tmem + T_D + 64, kt + i * ROWS16, vt0 + (2 * SUB >> 4) + i * ROWS16,
+                               idesc(64, true, true), 1);
+                    mma_commit(d_full);
+                    mma_commit(empty_k(s));
+                }
+                __syncwarp();
+            }
+        }
+        if (leader) {
             mma_commit(drain);                           // before TMEM is given back
             mbar_wait(drain, 0, 0x418);
         }
         __syncwarp();
-    } else if (warp == 18) {
+    } else if (warp == 22) {
         // ----------------------------------------------------------- decays
         Walk k(a, tiles, items);
         float gn[4];
@@ -411,7 +453,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
                 for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
             }
-#pragma unroll
+#pragma unroll 1
             for (int d = 1; d < 32; d <<= 1)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
@@ -428,83 +470,105 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             for (int b = 0; b < 4; ++b)
                 if (set >> b & 1u) sum += t[b];
             const float mine = exp_of(sum);
-            float cf[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) cf[b] = exp_of(t[b] - g[b]);
             if (!wait_warp(g_free(s), ((c >> 1) & 1) ^ 1, 0x451)) break;
             if (lane < 16) sc[s * 16 + lane] = mine;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                colf[s * C + 32 * b + lane] = cf[b];
+                colf[s * C + 32 * b + lane] = exp_of(t[b] - g[b]);
                 g2[s * C + 32 * b + lane] = (float)(g[b] * 1.4426950408889634);
             }
             mbar_arrive(g_full(s));
         }
     } else if (warp < 4) {
         // -------------------------------------------------------- the state
-        const int w = warp & 3, r = 32 * w + lane;        // row of the state
+        // Row r of the state, 16 columns at a time: from h0 at an item's start, else
+        // e^{G_C} S0 + K^T V~ of the chunk just done; to TMEM and (bf16, for Q S0)
+        // to shared memory, or to h_last behind an item's last chunk.
+        const int w = warp & 3, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
         uint8_t *const hrow = smem + OFF_H + r * 128;
-        uint32_t c = 0;
-        bool ok = true;
-        for (uint32_t id = blockIdx.x; id < items && ok; id += gridDim.x) {
+        Walk k(a, tiles, items);
+        bool fresh = true;
+        while (k.valid()) {
+            const uint32_t c = k.c;                      // the chunk to start, or just done
+            const bool last = !fresh && k.t0 + C >= k.it.len;
+            float dec = 0.0f;
+            if (!fresh) {
+                if (!wait_warp(g_full(c & 1), (c >> 1) & 1, 0x424)) break;
+                dec = sc[(c & 1) * 16 + SC_ALL];
+                if (!wait_warp(d_full, c & 1, 0x425)) break;
+                fence_after();
+            }
+            // Q S0 of the chunk before the one this state is for
+            const uint32_t m = fresh ? c : c + 1;
+            if (!last && !wait_warp(h_free, (m & 1) ^ 1, 0x423)) break;
+            const int c0 = k.it.tile * DV;
+            const int64_t at = ((k.it.seq * a.heads + k.it.h) * a.dk + r) * a.dv + c0;
+            const bool row = r < a.dk;
+#pragma unroll 1
+            for (int i = 0; i < DV; i += 16) {
+                uint32_t h[16];
+                if (fresh) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (a.h0 && row && c0 + i + j < a.dv)
+                            x = *reinterpret_cast<const uint4 *>(a.h0 + at + i + j);
+                        h[j] = x.x; h[j + 1] = x.y; h[j + 2] = x.z; h[j + 3] = x.w;
+                    }
+                } else {
+                    uint32_t d0[16], d1[16];
+                    tmem_ld16_async(quarter + T_H + i, h);
+                    tmem_ld16_async(quarter + T_D + i, d0);
+                    tmem_ld16_async(quarter + T_D + 64 + i, d1);
+                    tmem_loaded(h);
+                    tmem_loaded(d0);
+                    tmem_loaded(d1);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        h[j] = __float_as_uint(fmaf(dec, __uint_as_float(h[j]),
+                                                    __uint_as_float(d0[j]) + __uint_as_float(d1[j])));
+                }
+                if (last) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        if (a.h_last && row && c0 + i + j < a.dv)
+                            *reinterpret_cast<uint4 *>(a.h_last + at + i + j) =
+                                make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
+                } else {
+                    tmem_st16(quarter + T_H + i, h);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint4 x;
+                        x.x = pack_bf16(__uint_as_float(h[8 * j]), __uint_as_float(h[8 * j + 1]));
+                        x.y = pack_bf16(__uint_as_float(h[8 * j + 2]), __uint_as_float(h[8 * j + 3]));
+                        x.z = pack_bf16(__uint_as_float(h[8 * j + 4]), __uint_as_float(h[8 * j + 5]));
+                        x.w = pack_bf16(__uint_as_float(h[8 * j + 6]), __uint_as_float(h[8 * j + 7]));
+                        *reinterpret_cast<uint4 *>(hrow + (((i / 8 + j) ^ (r & 7)) << 4)) = x;
+                    }
+                }
+            }
+            if (!fresh) {
+                fence_before();
+                mbar_arrive(d_free);
+                mbar_arrive(g_free(c & 1));              // V~ (c) has read its decays too
+                k.next();
+            }
+            if (!last) {
+                tmem_wait_st();
+                fence_async_smem();
+                mbar_arrive(h_full);
+            }
+            fresh = last;
+        }
+        // items without tokens keep their state
+        for (uint32_t id = blockIdx.x; a.h_last && id < items; id += gridDim.x) {
             const Item it = item_of(a, tiles, id);
             const int c0 = it.tile * DV;
             const int64_t at = ((it.seq * a.heads + it.h) * a.dk + r) * a.dv + c0;
-            float h[DV];
-#pragma unroll
-            for (int i = 0; i < DV; i += 4) {
-                float4 x = make_float4(0, 0, 0, 0);
-                if (a.h0 && r < a.dk && c0 + i < a.dv)
-                    x = *reinterpret_cast<const float4 *>(a.h0 + at + i);
-                h[i] = x.x; h[i + 1] = x.y; h[i + 2] = x.z; h[i + 3] = x.w;
-            }
-            for (int64_t t0 = 0; t0 < it.len; t0 += C, ++c) {
-                const int s = c & 1;
-                // S0 of this chunk for Q S0
-                if (!(ok = wait_warp(h_free, (c & 1) ^ 1, 0x423))) break;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint4 x;
-                    x.x = pack_bf16(h[8 * i], h[8 * i + 1]);
-                    x.y = pack_bf16(h[8 * i + 2], h[8 * i + 3]);
-                    x.z = pack_bf16(h[8 * i + 4], h[8 * i + 5]);
-                    x.w = pack_bf16(h[8 * i + 6], h[8 * i + 7]);
-                    *reinterpret_cast<uint4 *>(hrow + ((i ^ (r & 7)) << 4)) = x;
-                }
-                fence_async_smem();
-                mbar_arrive(h_full);
-                // S = e^{G_C} S0 + K^T V~
-                if (!(ok = wait_warp(g_full(s), (c >> 1) & 1, 0x424))) break;
-                const float dec = sc[s * 16 + SC_ALL];
-                mbar_arrive(g_free(s));
-                if (!(ok = wait_warp(d_full, c & 1, 0x425))) break;
-                fence_after();
-#pragma unroll
-                for (int i = 0; i < DV; i += 8) {
-                    uint32_t d0[8], d1[8], d2[8];
-                    tmem_ld8_async(quarter + T_D + i, d0);
-                    tmem_ld8_async(quarter + T_D + 64 + i, d1);
-                    tmem_ld8_async(quarter + T_D + 128 + i, d2);
-                    tmem_loaded(d0);
-                    tmem_loaded(d1);
-                    tmem_loaded(d2);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        h[i + e] = fmaf(dec, h[i + e],
-                                        __uint_as_float(d0[e]) +
-                                            (__uint_as_float(d1[e]) + __uint_as_float(d2[e])));
-                }
-                fence_before();
-                mbar_arrive(d_free);
-            }
-            if (ok && a.h_last && r < a.dk) {
-#pragma unroll
-                for (int i = 0; i < DV; i += 4)
-                    if (c0 + i < a.dv)
-                        *reinterpret_cast<float4 *>(a.h_last + at + i) =
-                            make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
-            }
+            if (it.len == 0 && r < a.dk)
+                for (int i = 0; i < DV && c0 + i < a.dv; ++i)
+                    a.h_last[at + i] = a.h0 ? a.h0[at + i] : 0.0f;
         }
     } else if (warp < 12) {
         // ---------------------------------------------------------------- P
@@ -531,10 +595,8 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             // e^{blocks between}: block b's columns for the rows of block w
             const float f0 = rowf * (w == 2 ? sc[s * 16 + SC_1] : w == 3 ? sc[s * 16 + SC_12] : 1.0f);
             const float f1 = rowf * (w == 3 ? sc[s * 16 + SC_2] : 1.0f);
-            if (!wait_warp(s_full, c & 1, 0x432)) break;
-            fence_after();
             // P of the chunk before has been read
-            if (!wait_warp(o_full, (c & 1) ^ 1, 0x433)) break;
+            if (!wait_warp(s_full, c & 1, 0x432) || !wait_warp(o_full, (c & 1) ^ 1, 0x433)) break;
             fence_after();
 #pragma unroll 1
             for (int n = 2 * odd; n < 2 * w + 2; n += (n & 1) ? 3 : 1) {   // 16 columns
@@ -575,90 +637,89 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             fence_before();
             mbar_arrive(p_full);
         }
-    } else {
-        // ------------------------------------------- V~ and the output rows
+    } else if (warp < 16) {
+        // --------------------------------------------------------------- V~
+        // the rows of V times e^{G_C - G_j}, in three bf16 parts
         const int w = warp & 3, r = 32 * w + lane;
-        const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
-        // iteration n: V~ of chunk n, the rows of V times e^{G_C - G_j} in three
-        // bf16 parts; then the outputs of chunk n - 1
+        uint8_t *const trow = smem + OFF_VT + r * 128;
         Walk k(a, tiles, items);
-        Item it = k.it;
-        int64_t t0 = 0;
-        for (uint32_t n = 0;; ++n) {
-          const bool more = k.valid();
-          if (more) {
-            const int s = n & 1;
-            const uint32_t ph2 = (n >> 1) & 1;
+        for (; k.valid(); k.next()) {
+            const uint32_t c = k.c, ph2 = (c >> 1) & 1;
+            const int s = c & 1;
             const int64_t left = k.it.len - k.t0;
             const int m = (int)(left < C ? left : C);
             if (!wait_warp(g_full(s), ph2, 0x441)) break;
             const float wj = colf[s * C + r] * sc[s * 16 + SC_AFTER + w];
             if (!wait_warp(full_v(s), ph2, 0x442)) break;
             if (m < C && !wait_warp(full_k(s), ph2, 0x443)) break;
-            if (!wait_warp(d_full, (n & 1) ^ 1, 0x444)) break;             // V~ (n - 1) read
+            if (!wait_warp(d_full, (c & 1) ^ 1, 0x444)) break;             // V~ (c - 1) read
             uint8_t *const vrow = smem + OFF_V + s * SUB + r * 128;
-            uint8_t *const trow = smem + OFF_VT + r * 128;
-            if (r < m) {
-#pragma unroll 2
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t off = (uint32_t)((i ^ (r & 7)) << 4);
-                    const uint4 x4 = *reinterpret_cast<const uint4 *>(vrow + off);
-                    const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
-                    uint32_t p0[4], p1[4], p2[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float lo = bf_lo(x[e]) * wj, hi = bf_hi(x[e]) * wj;
-                        p0[e] = pack_bf16(lo, hi);
-                        lo -= bf_lo(p0[e]);
-                        hi -= bf_hi(p0[e]);
-                        p1[e] = pack_bf16(lo, hi);
-                        p2[e] = pack_bf16(lo - bf_lo(p1[e]), hi - bf_hi(p1[e]));
-                    }
-                    *reinterpret_cast<uint4 *>(trow + off) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-                    *reinterpret_cast<uint4 *>(trow + SUB + off) =
-                        make_uint4(p1[0], p1[1], p1[2], p1[3]);
-                    *reinterpret_cast<uint4 *>(trow + 2 * SUB + off) =
-                        make_uint4(p2[0], p2[1], p2[2], p2[3]);
-                }
-            } else {
+            if (r >= m) {
                 // rows behind the sequence (another one's, or nothing): zero in
-                // V, V~ and K, whose values a product would otherwise meet
+                // V and K, whose values a product would otherwise meet
                 const uint4 z = make_uint4(0, 0, 0, 0);
                 uint8_t *const krow = smem + OFF_K + s * 2 * SUB + r * 128;
 #pragma unroll 1
                 for (int i = 0; i < 8; ++i) {
                     *reinterpret_cast<uint4 *>(vrow + i * 16) = z;
-                    *reinterpret_cast<uint4 *>(trow + i * 16) = z;
-                    *reinterpret_cast<uint4 *>(trow + SUB + i * 16) = z;
-                    *reinterpret_cast<uint4 *>(trow + 2 * SUB + i * 16) = z;
                     *reinterpret_cast<uint4 *>(krow + i * 16) = z;
                     *reinterpret_cast<uint4 *>(krow + SUB + i * 16) = z;
                 }
             }
+#pragma unroll 2
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t off = (uint32_t)((i ^ (r & 7)) << 4);   // free of bank conflicts
+                const uint4 x4 = *reinterpret_cast<const uint4 *>(vrow + off);
+                const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+                uint32_t p0[4], p1[4], p2[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float lo = bf_lo(x[e]) * wj, hi = bf_hi(x[e]) * wj;
+                    p0[e] = pack_bf16(lo, hi);
+                    lo -= bf_lo(p0[e]);
+                    hi -= bf_hi(p0[e]);
+                    p1[e] = pack_bf16(lo, hi);
+                    p2[e] = pack_bf16(lo - bf_lo(p1[e]), hi - bf_hi(p1[e]));
+                }
+                *reinterpret_cast<uint4 *>(trow + off) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+                *reinterpret_cast<uint4 *>(trow + SUB + off) =
+                    make_uint4(p1[0], p1[1], p1[2], p1[3]);
+                *reinterpret_cast<uint4 *>(trow + 2 * SUB + off) =
+                    make_uint4(p2[0], p2[1], p2[2], p2[3]);
+            }
             fence_async_smem();
             mbar_arrive(vt_full);
-          }
-          if (n > 0) {
-            const int s = (n - 1) & 1;
+        }
+    } else if (warp < 20) {
+        // -------------------------------------------------- the output rows
+        const int w = warp & 3, r = 32 * w + lane;
+        const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
+        Walk k(a, tiles, items);
+        for (; k.valid(); k.next()) {
+            const uint32_t c = k.c;
+            const int s = c & 1;
+            if (!wait_warp(g_full(s), (c >> 1) & 1, 0x446)) break;
             const float ei = ex2(g2[s * C + r]) * sc[s * 16 + SC_BEFORE + w] * a.scale;
-            if (!wait_warp(o_full, (n - 1) & 1, 0x445)) break;
-            mbar_arrive(g_free(s));                      // P (n - 1) has read them too
+            const int64_t bq = a.cu ? 0 : k.it.seq;
+            const int64_t t = k.t0 + r;
+            const int c0 = k.it.tile * DV;
+            __nv_bfloat16 *const row = static_cast<__nv_bfloat16 *>(a.o) + bq * a.os[0] +
+                                       (k.it.row0 + t) * a.os[1] + k.it.h * a.os[2] + c0;
+            if (!wait_warp(o_full, c & 1, 0x445)) break;
+            mbar_arrive(g_free(s));                      // P (c) has read them too
             fence_after();
-            const int64_t bq = a.cu ? 0 : it.seq;
-            const int64_t t = t0 + r;
 #pragma unroll 1
-            for (int part = 0; part < 4; ++part) {
-                const int col = it.tile * DV + 16 * part;
+            for (int i0 = 0; i0 < DV; i0 += 16) {
                 uint32_t pv[16], qh[16];
-                tmem_ld16_async(quarter + T_PV + 16 * part, pv);
-                tmem_ld16_async(quarter + T_QH + 16 * part, qh);
+                tmem_ld16_async(quarter + T_PV + i0, pv);
+                tmem_ld16_async(quarter + T_QH + i0, qh);
                 tmem_loaded(pv);
                 tmem_loaded(qh);
-                if (part == 3) {
+                if (i0 == DV - 16) {
                     fence_before();
                     mbar_arrive(o_free);
                 }
-                if (t < it.len) {
+                if (t < k.it.len) {
                     float y[16];
                     float bad = 0.0f;                     // 0, or NaN
 #pragma unroll
@@ -666,37 +727,30 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                         y[i] = __uint_as_float(pv[i]);
                         bad = fmaf(0.0f, y[i], bad);
                     }
-                    if (bad != 0.0f) masked_row(a, it, t0, t, col, y);
+                    if (bad != 0.0f) masked_row(a, k.it, k.t0, t, c0 + i0, y);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         y[i] = fmaf(y[i], a.scale, __uint_as_float(qh[i]) * ei);
-                    __nv_bfloat16 *const row = static_cast<__nv_bfloat16 *>(a.o) + bq * a.os[0] +
-                                               (it.row0 + t) * a.os[1] + it.h * a.os[2] + col;
 #pragma unroll
                     for (int i = 0; i < 16; i += 8)
-                        if (col + i < a.dv) {
+                        if (c0 + i0 + i < a.dv) {
                             uint4 x;
                             x.x = pack_bf16(y[i], y[i + 1]);
                             x.y = pack_bf16(y[i + 2], y[i + 3]);
                             x.z = pack_bf16(y[i + 4], y[i + 5]);
                             x.w = pack_bf16(y[i + 6], y[i + 7]);
-                            *reinterpret_cast<uint4 *>(row + i) = x;
+                            *reinterpret_cast<uint4 *>(row + i0 + i) = x;
                         }
                 }
                 __syncwarp();
             }
-          }
-          if (!more) break;
-          it = k.it;
-          t0 = k.t0;
-          k.next();
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 17) {
+    if (warp == 21) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
