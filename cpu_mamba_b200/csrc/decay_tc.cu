@@ -3,7 +3,7 @@
 // state S (Dk x 64) in fp32 in TMEM.  Within a chunk, with G_i the sum of the
 // log decays up to token i and S0 the state before it,
 //   P_ij = e^{G_i - G_j} (q_i . k_j)  for j <= i, else 0
-//   o_i  = scale (sum_j P_ij v_j + e^{G_i} q_i^T S0)
+//   o_i  = scale (sum_j P_ij v_j + e^{G_i} q_i^T S0)      (scale joins P's factors)
 //   S    = e^{G_C} S0 + sum_j k_j (e^{G_C - G_j} v_j)^T
 // so four products: Q K^T (128 x 128 x Dk), P V (128 x 64 x 128), Q S0
 // (128 x 64 x Dk) and K^T V~ (Dk x 64 x 128), V~ the decayed rows of V.
@@ -22,7 +22,7 @@
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone.
 //
-// Roles (23 warps): 0-3 the state, 4-11 P, 12-15 V~, 16-19 the output rows, 20 TMA
+// Roles (23 warps): 0-3 the state, 4-11 P, 12-15 the output rows, 16-19 V~, 20 TMA
 // loads, 21 MMA issue, 22 decays.  A chunk's products are issued as
 //   Q S0 (n), P V (n), Q K^T (n + 1), K^T V~ (n + 1)
 // so that P (n + 1) and the state update overlap the others' MMAs.  Every
@@ -48,7 +48,9 @@ using namespace tc;
 
 constexpr int C = 128;                       // tokens per chunk
 constexpr int DV = 64;                       // columns of v per CTA
-constexpr int THREADS = 736;
+// first warp of each role: the state, P (8 warps), output rows, V~, TMA, MMA, decays
+constexpr int W_P = 4, W_O = 12, W_V = 16, W_TMA = 20, W_MMA = 21, W_G = 22;
+constexpr int THREADS = 23 * 32;
 constexpr uint32_t SUB = 128 * 128;          // one 128-row x 128-byte operand tile
 // shared memory (bytes from a 1024-aligned base)
 constexpr uint32_t OFF_Q = 0;                            // [2][2 SUB]
@@ -59,7 +61,9 @@ constexpr uint32_t OFF_H = OFF_VT + 3 * SUB;             // [SUB]
 constexpr uint32_t OFF_COLF = OFF_H + SUB;               // float [2][128]
 constexpr uint32_t OFF_G2 = OFF_COLF + 2 * C * 4;        // float [2][128]
 constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
-constexpr uint32_t OFF_BARS = OFF_SC + 2 * 16 * 4;
+constexpr uint32_t OFF_DEC = OFF_SC + 2 * 16 * 4;        // float [4]
+constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // int4 [4][2]
+constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 2 * 16;
 constexpr int NBARS = 6 + 6 + 4 + 9 + 1;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
@@ -150,12 +154,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
           "r"(b)
         : "memory");
 }
-__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap *map, int32_t x, int32_t head,
-                                                int32_t tok, int32_t b) {
-    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(b)
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t src, int32_t x,
+                                             int32_t head, int32_t tok, int32_t b) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(head), "r"(tok), "r"(b)
                  : "memory");
 }
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;"); }
+__device__ __forceinline__ void bulk_wait_read0() {
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -167,8 +177,37 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+// two fp32 values in one register pair (packed FMA: half the instructions)
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair(float v) {
+    return pair(__float_as_uint(v), __float_as_uint(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t lo_of(uint64_t v) { return (uint32_t)v; }
+__device__ __forceinline__ uint32_t hi_of(uint64_t v) { return (uint32_t)(v >> 32); }
+__device__ __forceinline__ uint32_t pack_bf16(uint64_t v) {
+    return pack_bf16(__uint_as_float(lo_of(v)), __uint_as_float(hi_of(v)));
+}
+// a bf16 pair as two fp32 values
+__device__ __forceinline__ uint64_t unpack_bf16(uint32_t v) { return pair(v << 16, v & 0xffff0000u); }
 
 // e^x of a 64-bit sum, to fp32 precision
 __device__ __forceinline__ float exp_of(double x) {
@@ -191,6 +230,13 @@ __device__ __forceinline__ Item item_of(const Args &a, int tiles, uint32_t id) {
     bounds(a, it.seq, it.row0, it.len);
     return it;
 }
+// A chunk as the roles see it, in shared memory beside its decays: one warp walks
+// the items, the others read.
+struct Chunk {
+    int row, m;                          // first token (of the batch row), tokens; m 0: the end
+    int first, last;                     // of its sequence
+    int h, seq, tile, pad;
+};
 // the chunks of a CTA's items, in order
 struct Walk {
     const Args &a;
@@ -231,47 +277,65 @@ __device__ __forceinline__ float load_g(const Args &a, const Item &it, int64_t t
 // differences; NaN stays
 __device__ __forceinline__ float clamp_g(float g) { return g < -256.0f ? -256.0f : g; }
 
-// a bounded wait of a whole warp; every lane gets the same answer
+// Bounded waits: about 20 cycles a try, 2^27 tries.  (A try_wait with a time hint
+// sleeps instead of polling, but wakes late: 393 -> 445 us at 8 x 8192.)
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int where) {
+    uint32_t ok, tries = 0;
+    do {
+        ok = mbar_try(bar, parity);
+    } while (!ok && ++tries < (1u << 27));
+    if (!ok) atomicCAS(&g_mb2_device_error, 0, where);
+    return ok != 0;
+}
+// of a whole warp; every lane gets the same answer
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int where) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, where));
+    return __all_sync(0xffffffffu, wait_one(bar, parity, where));
 }
 
-// sum_j P_ij v_j of row t over its own tokens j <= t of the chunk, from global
+// scale sum_j P_ij v_j of row r over its own tokens j <= r of the chunk, from global
 // memory: for rows that met an infinity or a NaN, perhaps in a masked token
-__device__ __forceinline__ void masked_row(const Args &a, const Item &it, int64_t t0, int64_t t,
-                                           int col, float (&y)[16]) {
-    const int64_t bq = a.cu ? 0 : it.seq;
+__device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r, int col,
+                                           float (&y)[16]) {
+    const int64_t bq = a.cu ? 0 : k.seq;
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + bq * a.qs[0] +
-                             (it.row0 + t) * a.qs[1] + (it.h / a.q_rep) * a.qs[2];
+                             (k.row + r) * a.qs[1] + (k.h / a.q_rep) * a.qs[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) y[i] = 0.0f;
     double sum = 0.0;
-    for (int64_t j = t; j >= t0; --j) {
-        const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(a.k) + bq * a.ks[0] +
-                                 (it.row0 + j) * a.ks[1] + (it.h / a.k_rep) * a.ks[2];
+#pragma unroll 1
+    for (int64_t j = k.row + r; j >= k.row; --j) {
+        const __nv_bfloat16 *kj = static_cast<const __nv_bfloat16 *>(a.k) + bq * a.ks[0] +
+                                  j * a.ks[1] + (k.h / a.k_rep) * a.ks[2];
         const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(a.v) + bq * a.vs[0] +
-                                 (it.row0 + j) * a.vs[1] + (it.h / a.v_rep) * a.vs[2] + col;
+                                 j * a.vs[1] + (k.h / a.v_rep) * a.vs[2] + col;
         float d = 0.0f;
+#pragma unroll 1
         for (int e = 0; e < (int)a.dk; ++e)
-            d = fmaf(__bfloat162float(q[e]), __bfloat162float(k[e]), d);
-        const float p = io<__nv_bfloat16>::round(d * __expf((float)sum));
+            d = fmaf(__bfloat162float(q[e]), __bfloat162float(kj[e]), d);
+        const float p = io<__nv_bfloat16>::round(d * __expf((float)sum) * a.scale);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (col + i < a.dv) y[i] = fmaf(p, __bfloat162float(v[i]), y[i]);
-        sum += clamp_g(load_g(a, it, j));
+        sum += clamp_g(a.g[bq * a.gs[0] + j * a.gs[1] + k.h * a.gs[2]]);
     }
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
 decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k,
-                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a,
+                   const __grid_constant__ CUtensorMap map_v,
+                   const __grid_constant__ CUtensorMap map_o, const __grid_constant__ Args a,
                    int tiles, uint32_t items) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     float *const colf = reinterpret_cast<float *>(smem + OFF_COLF);
     float *const g2 = reinterpret_cast<float *>(smem + OFF_G2);
     float *const sc = reinterpret_cast<float *>(smem + OFF_SC);
+    // e^{G_C}, four deep: the state's warps read it after the outputs of their
+    // chunk may already have freed its other decays
+    float *const dec = reinterpret_cast<float *>(smem + OFF_DEC);
+    // the chunks, four deep for the same reason
+    Chunk *const chunks = reinterpret_cast<Chunk *>(smem + OFF_CHUNK);
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(smem + OFF_TMEM);
     auto bar = [&](int i) { return base + OFF_BARS + 8u * i; };
     auto full_q = [&](int s) { return bar(s); };
@@ -293,17 +357,19 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     const uint32_t o_free = bar(24);    // ... read
     const uint32_t drain = bar(25);     // every MMA complete (once, at the end)
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // through a shuffle, so that the compiler knows it to be one value a warp
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const bool wide = a.dk > 64;                         // two 64-column operand tiles
     if (threadIdx.x == 0) {
         for (int i = 0; i < NBARS; ++i) {
-            const int n = (i == 12 || i == 13) ? 32 : (i == 14 || i == 15) ? 256 :
-                          (i == 17 || i == 19 || i == 20 || i == 24) ? 128 : i == 22 ? 256 : 1;
+            const int n = (i == 10 || i == 11) ? 4 : (i == 12 || i == 13) ? 32 :
+                          i == 17 ? 128 : i == 22 ? 256 :
+                          (i == 14 || i == 15 || i == 19 || i == 20 || i == 24) ? 128 : 1;
             mbar_init(bar(i), n);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 21) {
+    if (warp == W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(base + OFF_TMEM), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -311,115 +377,112 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
 
-    if (warp == 20) {
+    if (warp == W_TMA) {
         // -------------------------------------------------------- TMA loads
         if (lane == 0) {
-            Walk k(a, tiles, items), ahead(a, tiles, items);
+            Walk k(a, tiles, items);
             const uint32_t qk = wide ? 2 * SUB : SUB;
-            if (ahead.valid()) ahead.next();
             for (; k.valid(); k.next()) {
                 const int s = k.c & 1;
                 const uint32_t ph = ((k.c >> 1) & 1) ^ 1;
                 const int tok = (int)(k.it.row0 + k.t0), bq = a.cu ? 0 : (int)k.it.seq;
                 const int hq = k.it.h / a.q_rep, hk = k.it.h / a.k_rep, hv = k.it.h / a.v_rep;
                 const uint32_t dk = base + OFF_K + s * 2 * SUB, dq = base + OFF_Q + s * 2 * SUB;
-                if (!mbar_wait(empty_k(s), ph, 0x401)) break;
+                if (!wait_one(empty_k(s), ph, 0x401)) break;
                 mbar_expect_tx(full_k(s), qk);
                 tma_load_4d(dk, &map_k, full_k(s), 0, hk, tok, bq);
                 if (wide) tma_load_4d(dk + SUB, &map_k, full_k(s), 64, hk, tok, bq);
-                if (!mbar_wait(empty_q(s), ph, 0x402)) break;
+                if (!wait_one(empty_q(s), ph, 0x402)) break;
                 mbar_expect_tx(full_q(s), qk);
                 tma_load_4d(dq, &map_q, full_q(s), 0, hq, tok, bq);
                 if (wide) tma_load_4d(dq + SUB, &map_q, full_q(s), 64, hq, tok, bq);
-                if (!mbar_wait(empty_v(s), ph, 0x403)) break;
+                if (!wait_one(empty_v(s), ph, 0x403)) break;
                 mbar_expect_tx(full_v(s), SUB);
                 tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
-                // the chunk that these stages take next comes from L2
-                if (ahead.valid()) ahead.next();
-                if (ahead.valid()) {
-                    const Item &it = ahead.it;
-                    const int tk = (int)(it.row0 + ahead.t0), b = a.cu ? 0 : (int)it.seq;
-                    tma_prefetch_4d(&map_k, 0, it.h / a.k_rep, tk, b);
-                    if (wide) tma_prefetch_4d(&map_k, 64, it.h / a.k_rep, tk, b);
-                    tma_prefetch_4d(&map_q, 0, it.h / a.q_rep, tk, b);
-                    if (wide) tma_prefetch_4d(&map_q, 64, it.h / a.q_rep, tk, b);
-                    tma_prefetch_4d(&map_v, it.tile * DV, it.h / a.v_rep, tk, b);
-                }
             }
             // no load is in flight when the CTA ends (its consumers may have given up)
             for (uint32_t n = k.c > 2 ? k.c - 2 : 0; n < k.c; ++n) {
-                mbar_wait(full_k(n & 1), (n >> 1) & 1, 0x404);
-                mbar_wait(full_q(n & 1), (n >> 1) & 1, 0x404);
-                mbar_wait(full_v(n & 1), (n >> 1) & 1, 0x404);
+                wait_one(full_k(n & 1), (n >> 1) & 1, 0x404);
+                wait_one(full_q(n & 1), (n >> 1) & 1, 0x404);
+                wait_one(full_v(n & 1), (n >> 1) & 1, 0x404);
             }
         }
         __syncwarp();
-    } else if (warp == 21) {
+    } else if (warp == W_MMA) {
         // -------------------------------------------------------- MMA issue
-        // the whole warp walks the chunks (descriptors stay uniform); one lane
-        // issues
-        const bool leader = elect_one();
+        // The whole warp walks the chunks and one lane issues: descriptors and loop
+        // are then provably one value a warp and stay in uniform registers, where
+        // an MMA wants them.
         uint32_t total = 0;
         for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
             total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
+        total = uniform(total);
         const uint64_t dq0 = smem_desc(base + OFF_Q), dk0 = smem_desc(base + OFF_K);
         const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
         const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
         constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
-        const int steps = wide ? 8 : 4;                  // of 16 columns of q and k
+        bool ok = true;
         // iteration n: Q S0 and P V of chunk n - 1, then Q K^T and K^T V~ of chunk n
-        for (uint32_t n = 0; n <= total; ++n) {
+        for (uint32_t n = 0; n <= total && ok; ++n) {
             if (n > 0) {
-                const uint32_t c = n - 1, ph = c & 1;
+                const uint32_t ph = (n - 1) & 1;
                 const uint64_t q = dq0 + ph * STAGE, v = v0 + ph * (SUB >> 4);
-                if (!wait_warp(h_full, ph, 0x415) || !wait_warp(o_free, ph ^ 1, 0x416)) break;
+                ok = wait_warp(h_full, ph, 0x415) && wait_warp(o_free, ph ^ 1, 0x416);
                 fence_after();
-                if (leader) {
-#pragma unroll 2
-                    for (int i = 0; i < steps; ++i)
-                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h0 + i * ROWS16,
-                               idesc(64, false, true), i != 0);
+                if (ok && elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma_ss(tmem + T_QH, q + i * 2, h0 + i * ROWS16, idesc(64, false, true), i != 0);
+                    if (wide) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mma_ss(tmem + T_QH, q + (SUB >> 4) + i * 2, h0 + (4 + i) * ROWS16,
+                                   idesc(64, false, true), 1);
+                    }
                     mma_commit(h_free);
                     mma_commit(empty_q(ph));
                 }
                 __syncwarp();
-                if (!wait_warp(p_full, ph, 0x417)) break;
+                ok = ok && wait_warp(p_full, ph, 0x417);
                 fence_after();
-                if (leader) {
-#pragma unroll 2
+                if (ok && elect_one()) {
+#pragma unroll
                     for (int i = 0; i < C / 16; ++i)
                         mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, v + i * ROWS16,
                                     idesc(64, false, true), i != 0);
                     mma_commit(o_full);
-                    mma_commit(empty_v(ph));
                 }
                 __syncwarp();
             }
             if (n < total) {
                 const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
                 const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE, kt = kt0 + s * STAGE;
-                if (!wait_warp(full_k(s), ph2, 0x411) || !wait_warp(full_q(s), ph2, 0x412)) break;
+                ok = ok && wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
                 fence_after();
-                if (leader) {
-#pragma unroll 2
-                    for (int i = 0; i < steps; ++i) {
-                        const uint64_t off = (i >> 2) * (SUB >> 4) + (i & 3) * 2;
-                        mma_ss(tmem + T_S, q + off, k + off, idesc(128, false, false), i != 0);
+                if (ok && elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma_ss(tmem + T_S, q + i * 2, k + i * 2, idesc(128, false, false), i != 0);
+                    if (wide) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mma_ss(tmem + T_S, q + (SUB >> 4) + i * 2, k + (SUB >> 4) + i * 2,
+                                   idesc(128, false, false), 1);
                     }
                     mma_commit(s_full);
                 }
                 __syncwarp();
-                if (!wait_warp(vt_full, s, 0x413) || !wait_warp(d_free, s ^ 1, 0x414)) break;
+                ok = ok && wait_warp(vt_full, s, 0x413) && wait_warp(d_free, s ^ 1, 0x414);
                 fence_after();
-                if (leader) {
+                if (ok && elect_one()) {
                     // V~'s first two parts side by side, the third added to the second's
-#pragma unroll 2
+#pragma unroll
                     for (int i = 0; i < C / 16; ++i)
                         mma_ss(tmem + T_D, kt + i * ROWS16, vt0 + i * ROWS16, idesc(128, true, true),
                                i != 0);
-#pragma unroll 2
+#pragma unroll
                     for (int i = 0; i < C / 16; ++i)
                         mma_ss(tmem + T_D + 64, kt + i * ROWS16, vt0 + (2 * SUB >> 4) + i * ROWS16,
                                idesc(64, true, true), 1);
@@ -429,12 +492,12 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 __syncwarp();
             }
         }
-        if (leader) {
+        if (elect_one()) {
             mma_commit(drain);                           // before TMEM is given back
-            mbar_wait(drain, 0, 0x418);
+            wait_one(drain, 0, 0x418);
         }
         __syncwarp();
-    } else if (warp == 22) {
+    } else if (warp == W_G) {
         // ----------------------------------------------------------- decays
         Walk k(a, tiles, items);
         float gn[4];
@@ -442,16 +505,31 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
             for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
         }
-        while (k.valid()) {
+        for (bool more = true; more;) {
             const uint32_t c = k.c;
             const int s = c & 1;
             double g[4], t[4];
+            more = k.valid();
+            Chunk now = {};                              // behind the last one: m = 0
+            if (more) {
+                const int64_t left = k.it.len - k.t0;
+                now.row = (int)(k.it.row0 + k.t0);
+                now.m = (int)(left < C ? left : C);
+                now.first = k.t0 == 0;
+                now.last = left <= C;
+                now.h = k.it.h;
+                now.seq = (int)k.it.seq;
+                now.tile = k.it.tile;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) g[b] = (double)clamp_g(gn[b]);
-            k.next();                                    // the next chunk's loads
-            if (k.valid()) {
+                for (int b = 0; b < 4; ++b) g[b] = (double)clamp_g(gn[b]);
+                k.next();                                // the next chunk's loads
+                if (k.valid()) {
 #pragma unroll
-                for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
+                    for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) g[b] = 0.0;
             }
 #pragma unroll 1
             for (int d = 1; d < 32; d <<= 1)
@@ -470,128 +548,126 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             for (int b = 0; b < 4; ++b)
                 if (set >> b & 1u) sum += t[b];
             const float mine = exp_of(sum);
+            float cf[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) cf[b] = exp_of(t[b] - g[b]);
             if (!wait_warp(g_free(s), ((c >> 1) & 1) ^ 1, 0x451)) break;
-            if (lane < 16) sc[s * 16 + lane] = mine;
+            if (lane < 12) sc[s * 16 + lane] = mine;
+            if (lane == SC_ALL) {
+                dec[c & 3] = mine;                       // chunk c - 4 is long done
+                chunks[c & 3] = now;
+            }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                colf[s * C + 32 * b + lane] = exp_of(t[b] - g[b]);
+                colf[s * C + 32 * b + lane] = cf[b];
                 g2[s * C + 32 * b + lane] = (float)(g[b] * 1.4426950408889634);
             }
             mbar_arrive(g_full(s));
         }
-    } else if (warp < 4) {
+    } else if (warp < W_P) {
         // -------------------------------------------------------- the state
-        // Row r of the state, 16 columns at a time: from h0 at an item's start, else
-        // e^{G_C} S0 + K^T V~ of the chunk just done; to TMEM and (bf16, for Q S0)
-        // to shared memory, or to h_last behind an item's last chunk.
+        // Row r of the state, 16 columns at a time: from h0 at a
+        // sequence's start (pass 0), and e^{G_C} S0 + K^T V~ behind each chunk
+        // (pass 1); to TMEM and (bf16, for Q S0) to shared memory, or to h_last
+        // behind the last chunk.
         const int w = warp & 3, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
         uint8_t *const hrow = smem + OFF_H + r * 128;
-        Walk k(a, tiles, items);
-        bool fresh = true;
-        while (k.valid()) {
-            const uint32_t c = k.c;                      // the chunk to start, or just done
-            const bool last = !fresh && k.t0 + C >= k.it.len;
-            float dec = 0.0f;
-            if (!fresh) {
-                if (!wait_warp(g_full(c & 1), (c >> 1) & 1, 0x424)) break;
-                dec = sc[(c & 1) * 16 + SC_ALL];
-                if (!wait_warp(d_full, c & 1, 0x425)) break;
-                fence_after();
-            }
-            // Q S0 of the chunk before the one this state is for
-            const uint32_t m = fresh ? c : c + 1;
-            if (!last && !wait_warp(h_free, (m & 1) ^ 1, 0x423)) break;
-            const int c0 = k.it.tile * DV;
-            const int64_t at = ((k.it.seq * a.heads + k.it.h) * a.dk + r) * a.dv + c0;
+        bool ok = true;
+        for (uint32_t c = 0; ok; ++c) {
+            if (!wait_warp(g_full(c & 1), (c >> 1) & 1, 0x424)) break;
+            const Chunk k = chunks[c & 3];
+            if (k.m == 0) break;
+            const uint64_t dec2 = pair(dec[c & 3]);
+            const int c0 = k.tile * DV;
+            const int64_t at = (((int64_t)k.seq * a.heads + k.h) * a.dk + r) * a.dv + c0;
             const bool row = r < a.dk;
 #pragma unroll 1
-            for (int i = 0; i < DV; i += 16) {
-                uint32_t h[16];
-                if (fresh) {
-#pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (a.h0 && row && c0 + i + j < a.dv)
-                            x = *reinterpret_cast<const uint4 *>(a.h0 + at + i + j);
-                        h[j] = x.x; h[j + 1] = x.y; h[j + 2] = x.z; h[j + 3] = x.w;
-                    }
-                } else {
-                    uint32_t d0[16], d1[16];
-                    tmem_ld16_async(quarter + T_H + i, h);
-                    tmem_ld16_async(quarter + T_D + i, d0);
-                    tmem_ld16_async(quarter + T_D + 64 + i, d1);
-                    tmem_loaded(h);
-                    tmem_loaded(d0);
-                    tmem_loaded(d1);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        h[j] = __float_as_uint(fmaf(dec, __uint_as_float(h[j]),
-                                                    __uint_as_float(d0[j]) + __uint_as_float(d1[j])));
+            for (int pass = k.first ? 0 : 1; pass < 2; ++pass) {
+                const bool store = pass == 1 && k.last;
+                if (pass == 1) {
+                    if (!(ok = wait_warp(d_full, c & 1, 0x425))) break;
+                    fence_after();
                 }
-                if (last) {
+                // Q S0 of the chunk before the one this state is for
+                if (!store && !(ok = wait_warp(h_free, (c + pass + 1) & 1, 0x423))) break;
+#pragma unroll 1
+                for (int i = 0; i < DV; i += 16) {
+                    uint32_t h[16];
+                    if (pass == 0) {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4)
-                        if (a.h_last && row && c0 + i + j < a.dv)
-                            *reinterpret_cast<uint4 *>(a.h_last + at + i + j) =
-                                make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
-                } else {
-                    tmem_st16(quarter + T_H + i, h);
+                        for (int j = 0; j < 16; j += 4) {
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (a.h0 && row && c0 + i + j < a.dv)
+                                x = *reinterpret_cast<const uint4 *>(a.h0 + at + i + j);
+                            h[j] = x.x; h[j + 1] = x.y; h[j + 2] = x.z; h[j + 3] = x.w;
+                        }
+                    } else {
+                        uint32_t d0[16], d1[16];
+                        tmem_ld16_async(quarter + T_H + i, h);
+                        tmem_ld16_async(quarter + T_D + i, d0);
+                        tmem_ld16_async(quarter + T_D + 64 + i, d1);
+                        tmem_loaded(h);
+                        tmem_loaded(d0);
+                        tmem_loaded(d1);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint4 x;
-                        x.x = pack_bf16(__uint_as_float(h[8 * j]), __uint_as_float(h[8 * j + 1]));
-                        x.y = pack_bf16(__uint_as_float(h[8 * j + 2]), __uint_as_float(h[8 * j + 3]));
-                        x.z = pack_bf16(__uint_as_float(h[8 * j + 4]), __uint_as_float(h[8 * j + 5]));
-                        x.w = pack_bf16(__uint_as_float(h[8 * j + 6]), __uint_as_float(h[8 * j + 7]));
-                        *reinterpret_cast<uint4 *>(hrow + (((i / 8 + j) ^ (r & 7)) << 4)) = x;
+                        for (int j = 0; j < 16; j += 2) {
+                            const uint64_t x =
+                                fma2(dec2, pair(h[j], h[j + 1]),
+                                     add2(pair(d0[j], d0[j + 1]), pair(d1[j], d1[j + 1])));
+                            h[j] = lo_of(x);
+                            h[j + 1] = hi_of(x);
+                        }
+                    }
+                    if (store) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            if (a.h_last && row && c0 + i + j < a.dv)
+                                *reinterpret_cast<uint4 *>(a.h_last + at + i + j) =
+                                    make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
+                    } else {
+                        tmem_st16(quarter + T_H + i, h);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint4 x;
+                            x.x = pack_bf16(pair(h[8 * j], h[8 * j + 1]));
+                            x.y = pack_bf16(pair(h[8 * j + 2], h[8 * j + 3]));
+                            x.z = pack_bf16(pair(h[8 * j + 4], h[8 * j + 5]));
+                            x.w = pack_bf16(pair(h[8 * j + 6], h[8 * j + 7]));
+                            *reinterpret_cast<uint4 *>(hrow + (((i / 8 + j) ^ (r & 7)) << 4)) = x;
+                        }
                     }
                 }
+                if (pass == 1) {
+                    fence_before();
+                    mbar_arrive(d_free);
+                }
+                if (!store) {
+                    tmem_wait_st();
+                    fence_async_smem();
+                    mbar_arrive(h_full);
+                }
             }
-            if (!fresh) {
-                fence_before();
-                mbar_arrive(d_free);
-                mbar_arrive(g_free(c & 1));              // V~ (c) has read its decays too
-                k.next();
-            }
-            if (!last) {
-                tmem_wait_st();
-                fence_async_smem();
-                mbar_arrive(h_full);
-            }
-            fresh = last;
         }
-        // items without tokens keep their state
-        for (uint32_t id = blockIdx.x; a.h_last && id < items; id += gridDim.x) {
-            const Item it = item_of(a, tiles, id);
-            const int c0 = it.tile * DV;
-            const int64_t at = ((it.seq * a.heads + it.h) * a.dk + r) * a.dv + c0;
-            if (it.len == 0 && r < a.dk)
-                for (int i = 0; i < DV && c0 + i < a.dv; ++i)
-                    a.h_last[at + i] = a.h0 ? a.h0[at + i] : 0.0f;
-        }
-    } else if (warp < 12) {
+    } else if (warp < W_O) {
         // ---------------------------------------------------------------- P
         // rows 32 w + lane; the first four warps take blocks 0 and 2, the others
         // 1 and 3.  Blocks above the diagonal stay the zeros written here.
-        const int w = warp & 3, odd = (warp - 4) >> 2, r = 32 * w + lane;
+        const int w = warp & 3, odd = (warp - W_P) >> 2, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
         {
             uint32_t z[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) z[i] = 0u;
-            tmem_st16(quarter + T_P + 16 * odd, z);
-            tmem_st16(quarter + T_P + 16 * (odd + 2), z);
+            for (int b = odd; b < 4; b += 2) tmem_st16(quarter + T_P + 16 * b, z);
             tmem_wait_st();
         }
-        uint32_t total = 0;
-        for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
-            total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
-        for (uint32_t c = 0; c < total; ++c) {
+        const uint64_t scale2 = pair(a.scale);
+        for (uint32_t c = 0;; ++c) {
             const int s = c & 1;
-            if (!wait_warp(g_full(s), (c >> 1) & 1, 0x431)) break;
+            if (!wait_warp(g_full(s), (c >> 1) & 1, 0x431) || chunks[c & 3].m == 0) break;
             const float gr = g2[s * C + r];
-            const float rowf = ex2(gr);
+            const float rowf = ex2(gr) * a.scale;
             // e^{blocks between}: block b's columns for the rows of block w
             const float f0 = rowf * (w == 2 ? sc[s * 16 + SC_1] : w == 3 ? sc[s * 16 + SC_12] : 1.0f);
             const float f1 = rowf * (w == 3 ? sc[s * 16 + SC_2] : 1.0f);
@@ -604,16 +680,14 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 tmem_ld16_async(quarter + T_S + 16 * n, x);
                 const int b = n >> 1;
                 if (b < w) {
-                    const float fb = b == 0 ? f0 : b == 1 ? f1 : rowf;
-                    const float4 *cf = reinterpret_cast<const float4 *>(colf + s * C + 16 * n);
+                    const uint64_t fb = pair(b == 0 ? f0 : b == 1 ? f1 : rowf);
+                    const ulonglong2 *cf = reinterpret_cast<const ulonglong2 *>(colf + s * C + 16 * n);
                     tmem_loaded(x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float4 y = cf[i];
-                        p[2 * i] = pack_bf16(__uint_as_float(x[4 * i]) * (y.x * fb),
-                                             __uint_as_float(x[4 * i + 1]) * (y.y * fb));
-                        p[2 * i + 1] = pack_bf16(__uint_as_float(x[4 * i + 2]) * (y.z * fb),
-                                                 __uint_as_float(x[4 * i + 3]) * (y.w * fb));
+                        const ulonglong2 y = cf[i];
+                        p[2 * i] = pack_bf16(mul2(pair(x[4 * i], x[4 * i + 1]), mul2(y.x, fb)));
+                        p[2 * i + 1] = pack_bf16(mul2(pair(x[4 * i + 2], x[4 * i + 3]), mul2(y.y, fb)));
                     }
                 } else {
                     const float4 *gj = reinterpret_cast<const float4 *>(g2 + s * C + 16 * n);
@@ -622,13 +696,16 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float4 y = gj[i];
-                        const float e0 = __uint_as_float(x[4 * i]) * ex2(gr - y.x);
-                        const float e1 = __uint_as_float(x[4 * i + 1]) * ex2(gr - y.y);
-                        const float e2 = __uint_as_float(x[4 * i + 2]) * ex2(gr - y.z);
-                        const float e3 = __uint_as_float(x[4 * i + 3]) * ex2(gr - y.w);
-                        p[2 * i] = pack_bf16(4 * i <= last ? e0 : 0.0f, 4 * i + 1 <= last ? e1 : 0.0f);
-                        p[2 * i + 1] =
-                            pack_bf16(4 * i + 2 <= last ? e2 : 0.0f, 4 * i + 3 <= last ? e3 : 0.0f);
+                        const uint64_t e0 = mul2(pair(x[4 * i], x[4 * i + 1]),
+                                                 mul2(scale2, pair(__float_as_uint(ex2(gr - y.x)),
+                                                                   __float_as_uint(ex2(gr - y.y)))));
+                        const uint64_t e1 = mul2(pair(x[4 * i + 2], x[4 * i + 3]),
+                                                 mul2(scale2, pair(__float_as_uint(ex2(gr - y.z)),
+                                                                   __float_as_uint(ex2(gr - y.w)))));
+                        p[2 * i] = pack_bf16(pair(4 * i <= last ? lo_of(e0) : 0u,
+                                                  4 * i + 1 <= last ? hi_of(e0) : 0u));
+                        p[2 * i + 1] = pack_bf16(pair(4 * i + 2 <= last ? lo_of(e1) : 0u,
+                                                      4 * i + 3 <= last ? hi_of(e1) : 0u));
                     }
                 }
                 tmem_st8(quarter + T_P + 8 * n, p);
@@ -637,19 +714,19 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             fence_before();
             mbar_arrive(p_full);
         }
-    } else if (warp < 16) {
+    } else if (warp >= W_V) {
         // --------------------------------------------------------------- V~
         // the rows of V times e^{G_C - G_j}, in three bf16 parts
         const int w = warp & 3, r = 32 * w + lane;
         uint8_t *const trow = smem + OFF_VT + r * 128;
-        Walk k(a, tiles, items);
-        for (; k.valid(); k.next()) {
-            const uint32_t c = k.c, ph2 = (c >> 1) & 1;
+        for (uint32_t c = 0;; ++c) {
+            const uint32_t ph2 = (c >> 1) & 1;
             const int s = c & 1;
-            const int64_t left = k.it.len - k.t0;
-            const int m = (int)(left < C ? left : C);
             if (!wait_warp(g_full(s), ph2, 0x441)) break;
-            const float wj = colf[s * C + r] * sc[s * 16 + SC_AFTER + w];
+            const int m = chunks[c & 3].m;
+            if (m == 0) break;
+            const uint64_t wj2 = pair(colf[s * C + r] * sc[s * 16 + SC_AFTER + w]);
+            const uint64_t minus1 = pair(-1.0f);
             if (!wait_warp(full_v(s), ph2, 0x442)) break;
             if (m < C && !wait_warp(full_k(s), ph2, 0x443)) break;
             if (!wait_warp(d_full, (c & 1) ^ 1, 0x444)) break;             // V~ (c - 1) read
@@ -674,12 +751,11 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float lo = bf_lo(x[e]) * wj, hi = bf_hi(x[e]) * wj;
-                    p0[e] = pack_bf16(lo, hi);
-                    lo -= bf_lo(p0[e]);
-                    hi -= bf_hi(p0[e]);
-                    p1[e] = pack_bf16(lo, hi);
-                    p2[e] = pack_bf16(lo - bf_lo(p1[e]), hi - bf_hi(p1[e]));
+                    uint64_t y = mul2(unpack_bf16(x[e]), wj2);
+                    p0[e] = pack_bf16(y);
+                    y = fma2(unpack_bf16(p0[e]), minus1, y);
+                    p1[e] = pack_bf16(y);
+                    p2[e] = pack_bf16(fma2(unpack_bf16(p1[e]), minus1, y));
                 }
                 *reinterpret_cast<uint4 *>(trow + off) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
                 *reinterpret_cast<uint4 *>(trow + SUB + off) =
@@ -690,67 +766,109 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             fence_async_smem();
             mbar_arrive(vt_full);
         }
-    } else if (warp < 20) {
+    } else {
         // -------------------------------------------------- the output rows
         const int w = warp & 3, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
-        Walk k(a, tiles, items);
-        for (; k.valid(); k.next()) {
-            const uint32_t c = k.c;
+        for (uint32_t c = 0;; ++c) {
             const int s = c & 1;
             if (!wait_warp(g_full(s), (c >> 1) & 1, 0x446)) break;
-            const float ei = ex2(g2[s * C + r]) * sc[s * 16 + SC_BEFORE + w] * a.scale;
-            const int64_t bq = a.cu ? 0 : k.it.seq;
-            const int64_t t = k.t0 + r;
-            const int c0 = k.it.tile * DV;
-            __nv_bfloat16 *const row = static_cast<__nv_bfloat16 *>(a.o) + bq * a.os[0] +
-                                       (k.it.row0 + t) * a.os[1] + k.it.h * a.os[2] + c0;
+            const Chunk k = chunks[c & 3];
+            if (k.m == 0) break;
+            const uint64_t ei2 = pair(ex2(g2[s * C + r]) * sc[s * 16 + SC_BEFORE + w] * a.scale);
+            const int c0 = k.tile * DV;
+            __nv_bfloat16 *const row = static_cast<__nv_bfloat16 *>(a.o) +
+                                       (a.cu ? 0 : k.seq) * a.os[0] +
+                                       (int64_t)(k.row + r) * a.os[1] + k.h * a.os[2] + c0;
             if (!wait_warp(o_full, c & 1, 0x445)) break;
             mbar_arrive(g_free(s));                      // P (c) has read them too
             fence_after();
-#pragma unroll 1
+            // all 64 columns first, so that the accumulators are free again before
+            // the stores
+            uint32_t y[DV / 2];
+            uint32_t bad = 0;                            // 0, or NaN
+#pragma unroll
             for (int i0 = 0; i0 < DV; i0 += 16) {
                 uint32_t pv[16], qh[16];
                 tmem_ld16_async(quarter + T_PV + i0, pv);
                 tmem_ld16_async(quarter + T_QH + i0, qh);
                 tmem_loaded(pv);
                 tmem_loaded(qh);
-                if (i0 == DV - 16) {
-                    fence_before();
-                    mbar_arrive(o_free);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    uint32_t &yi = y[(i0 + i) / 2];
+                    yi = pack_bf16(fma2(pair(qh[i], qh[i + 1]), ei2, pair(pv[i], pv[i + 1])));
+                    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(bad) : "r"(yi), "r"(0));
                 }
-                if (t < k.it.len) {
-                    float y[16];
-                    float bad = 0.0f;                     // 0, or NaN
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        y[i] = __uint_as_float(pv[i]);
-                        bad = fmaf(0.0f, y[i], bad);
-                    }
-                    if (bad != 0.0f) masked_row(a, k.it, k.t0, t, c0 + i0, y);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        y[i] = fmaf(y[i], a.scale, __uint_as_float(qh[i]) * ei);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 8)
-                        if (c0 + i0 + i < a.dv) {
-                            uint4 x;
-                            x.x = pack_bf16(y[i], y[i + 1]);
-                            x.y = pack_bf16(y[i + 2], y[i + 3]);
-                            x.z = pack_bf16(y[i + 4], y[i + 5]);
-                            x.w = pack_bf16(y[i + 6], y[i + 7]);
-                            *reinterpret_cast<uint4 *>(row + i0 + i) = x;
-                        }
-                }
-                __syncwarp();
             }
+            const bool redo = r < k.m && (bad & 0x7fff7fffu);
+            if (__any_sync(0xffffffffu, redo)) {
+                // infinities or NaN: these rows again, from their own tokens
+#pragma unroll 1
+                for (int i0 = 0; i0 < DV; i0 += 16) {
+                    uint32_t qh[16];
+                    tmem_ld16_async(quarter + T_QH + i0, qh);
+                    tmem_loaded(qh);
+                    if (redo) {
+                        float z[16];
+                        masked_row(a, k, r, c0 + i0, z);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (c0 + i0 + i < a.dv)
+                                row[i0 + i] = __float2bfloat16_rn(
+                                    fmaf(__uint_as_float(qh[i]), __uint_as_float(lo_of(ei2)), z[i]));
+                    }
+                    __syncwarp();
+                }
+            }
+            fence_before();
+            mbar_arrive(o_free);
+            // P V of the chunk has read its V: the stage takes the output rows
+            uint8_t *const orow = smem + OFF_V + s * SUB + r * 128;
+            if (k.m == C && !__any_sync(0xffffffffu, redo)) {
+#pragma unroll
+                for (int i = 0; i < DV / 8; ++i)
+                    *reinterpret_cast<uint4 *>(orow + ((i ^ (r & 7)) << 4)) =
+                        make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_4d(&map_o, base + OFF_V + s * SUB + w * 32 * 128, k.tile * DV, k.h,
+                                 k.row + 32 * w, a.cu ? 0 : k.seq);
+                    bulk_commit();
+                    bulk_wait_read0();
+                }
+            } else if (r < k.m && !redo) {
+                // the rows behind a sequence's end may be another one's
+#pragma unroll
+                for (int i = 0; i < DV / 8; ++i)
+                    if (c0 + 8 * i < a.dv)
+                        *reinterpret_cast<uint4 *>(row + 8 * i) =
+                            make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty_v(s));
+            __syncwarp();
         }
+        if (lane == 0) bulk_wait0();                     // the stores are complete
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 21) {
+    // items without tokens keep their state
+    for (uint32_t id = blockIdx.x; a.h_last && id < items; id += gridDim.x) {
+        const Item it = item_of(a, tiles, id);
+        if (it.len > 0) continue;
+        const int64_t at = (it.seq * a.heads + it.h) * a.dk * a.dv;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < a.dk * DV; i += THREADS) {
+            const int col = it.tile * DV + i % DV;
+            const int64_t e = at + (i / DV) * a.dv + col;
+            if (col < a.dv) a.h_last[e] = a.h0 ? a.h0[e] : 0.0f;
+        }
+    }
+    if (warp == W_MMA) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
@@ -769,10 +887,10 @@ static int get_encode() {
     return MB2_OK;
 }
 
-// (batch, tokens, heads, width) bf16 as a 4D map of 128-token x 64-column boxes;
+// (batch, tokens, heads, width) bf16 as a 4D map of `rows`-token x 64-column boxes;
 // *ok = false when TMA cannot address it
 static int token_map(CUtensorMap *map, const void *p, const int64_t (&s)[3], int64_t batch,
-                     int64_t tokens, int64_t heads, int64_t width, bool *ok) {
+                     int64_t tokens, int64_t heads, int64_t width, int rows, bool *ok) {
     const int64_t n[3] = {batch, tokens, heads};
     int64_t st[3];
     *ok = aligned(p, 16) && tokens < 0x7fffff00 && batch < 0x7fffffff;
@@ -783,7 +901,7 @@ static int token_map(CUtensorMap *map, const void *p, const int64_t (&s)[3], int
     if (!*ok) return MB2_OK;
     cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
     cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
-    cuuint32_t box[4] = {64, 1, (cuuint32_t)C, 1};
+    cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
     CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(p), dims,
                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -805,13 +923,14 @@ int chunked(const Args &a, cudaStream_t st, bool *used) {
     *used = false;
     if (!fits(a)) return MB2_OK;
     MB2_TRY(get_encode());
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo;
     const int64_t batch = a.cu ? 1 : a.seqs;
-    bool ok[3];
-    MB2_TRY(token_map(&mq, a.q, a.qs, batch, a.seqlen, a.heads / a.q_rep, a.dk, &ok[0]));
-    MB2_TRY(token_map(&mk, a.k, a.ks, batch, a.seqlen, a.heads / a.k_rep, a.dk, &ok[1]));
-    MB2_TRY(token_map(&mv, a.v, a.vs, batch, a.seqlen, a.heads / a.v_rep, a.dv, &ok[2]));
-    if (!ok[0] || !ok[1] || !ok[2]) return MB2_OK;
+    bool ok[4];
+    MB2_TRY(token_map(&mq, a.q, a.qs, batch, a.seqlen, a.heads / a.q_rep, a.dk, C, &ok[0]));
+    MB2_TRY(token_map(&mk, a.k, a.ks, batch, a.seqlen, a.heads / a.k_rep, a.dk, C, &ok[1]));
+    MB2_TRY(token_map(&mv, a.v, a.vs, batch, a.seqlen, a.heads / a.v_rep, a.dv, C, &ok[2]));
+    MB2_TRY(token_map(&mo, a.o, a.os, batch, a.seqlen, a.heads, a.dv, 32, &ok[3]));
+    if (!ok[0] || !ok[1] || !ok[2] || !ok[3]) return MB2_OK;
     *used = true;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -824,7 +943,7 @@ int chunked(const Args &a, cudaStream_t st, bool *used) {
     const int64_t items = (int64_t)tiles * a.heads * a.seqs;
     MB2_REQUIRE(items < (1ll << 31), MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
     const unsigned grid = (unsigned)(items < sms ? items : sms);
-    decay_chunk_kernel<<<grid, THREADS, SMEM_BYTES, st>>>(mq, mk, mv, a, tiles, (uint32_t)items);
+    decay_chunk_kernel<<<grid, THREADS, SMEM_BYTES, st>>>(mq, mk, mv, mo, a, tiles, (uint32_t)items);
     return check_launch("decay_chunk_kernel");
 }
 
