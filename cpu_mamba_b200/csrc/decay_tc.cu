@@ -295,12 +295,12 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int whe
 // scale sum_j P_ij v_j of row r over its own tokens j <= r of the chunk, from global
 // memory: for rows that met an infinity or a NaN, perhaps in a masked token
 __device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r, int col,
-                                           float (&y)[16]) {
+                                           uint32_t (&y)[16]) {
     const int64_t bq = a.cu ? 0 : k.seq;
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + bq * a.qs[0] +
                              (k.row + r) * a.qs[1] + (k.h / a.q_rep) * a.qs[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = 0.0f;
+    for (int i = 0; i < 16; ++i) y[i] = 0u;
     double sum = 0.0;
 #pragma unroll 1
     for (int64_t j = k.row + r; j >= k.row; --j) {
@@ -315,7 +315,8 @@ __device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r,
         const float p = io<__nv_bfloat16>::round(d * __expf((float)sum) * a.scale);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            if (col + i < a.dv) y[i] = fmaf(p, __bfloat162float(v[i]), y[i]);
+            if (col + i < a.dv)
+                y[i] = __float_as_uint(fmaf(p, __bfloat162float(v[i]), __uint_as_float(y[i])));
         sum += clamp_g(a.g[bq * a.gs[0] + j * a.gs[1] + k.h * a.gs[2]]);
     }
 }
@@ -362,7 +363,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     const bool wide = a.dk > 64;                         // two 64-column operand tiles
     if (threadIdx.x == 0) {
         for (int i = 0; i < NBARS; ++i) {
-            const int n = (i == 10 || i == 11) ? 4 : (i == 12 || i == 13) ? 32 :
+            const int n = (i == 6 || i == 7) ? 4 : (i == 12 || i == 13) ? 32 :
                           i == 17 ? 128 : i == 22 ? 256 :
                           (i == 14 || i == 15 || i == 19 || i == 20 || i == 24) ? 128 : 1;
             mbar_init(bar(i), n);
@@ -423,8 +424,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
         const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
         constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
+        const int steps = wide ? 8 : 4;                  // of 16 columns of q and k
         bool ok = true;
         // iteration n: Q S0 and P V of chunk n - 1, then Q K^T and K^T V~ of chunk n
+#pragma unroll 1
         for (uint32_t n = 0; n <= total && ok; ++n) {
             if (n > 0) {
                 const uint32_t ph = (n - 1) & 1;
@@ -432,27 +435,22 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 ok = wait_warp(h_full, ph, 0x415) && wait_warp(o_free, ph ^ 1, 0x416);
                 fence_after();
                 if (ok && elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + T_QH, q + i * 2, h0 + i * ROWS16, idesc(64, false, true), i != 0);
-                    if (wide) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma_ss(tmem + T_QH, q + (SUB >> 4) + i * 2, h0 + (4 + i) * ROWS16,
-                                   idesc(64, false, true), 1);
-                    }
+#pragma unroll 1
+                    for (int i = 0; i < steps; ++i)
+                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h0 + i * ROWS16,
+                               idesc(64, false, true), i != 0);
                     mma_commit(h_free);
-                    mma_commit(empty_q(ph));
                 }
                 __syncwarp();
                 ok = ok && wait_warp(p_full, ph, 0x417);
                 fence_after();
                 if (ok && elect_one()) {
-#pragma unroll
+#pragma unroll 1
                     for (int i = 0; i < C / 16; ++i)
                         mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, v + i * ROWS16,
                                     idesc(64, false, true), i != 0);
                     mma_commit(o_full);
+                    mma_commit(empty_v(ph));
                 }
                 __syncwarp();
             }
@@ -462,14 +460,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 ok = ok && wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
                 fence_after();
                 if (ok && elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + T_S, q + i * 2, k + i * 2, idesc(128, false, false), i != 0);
-                    if (wide) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma_ss(tmem + T_S, q + (SUB >> 4) + i * 2, k + (SUB >> 4) + i * 2,
-                                   idesc(128, false, false), 1);
+#pragma unroll 1
+                    for (int i = 0; i < steps; ++i) {
+                        const uint64_t off = (i >> 2) * (SUB >> 4) + (i & 3) * 2;
+                        mma_ss(tmem + T_S, q + off, k + off, idesc(128, false, false), i != 0);
                     }
                     mma_commit(s_full);
                 }
@@ -478,14 +472,13 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 fence_after();
                 if (ok && elect_one()) {
                     // V~'s first two parts side by side, the third added to the second's
-#pragma unroll
-                    for (int i = 0; i < C / 16; ++i)
+#pragma unroll 1
+                    for (int i = 0; i < C / 16; ++i) {
                         mma_ss(tmem + T_D, kt + i * ROWS16, vt0 + i * ROWS16, idesc(128, true, true),
                                i != 0);
-#pragma unroll
-                    for (int i = 0; i < C / 16; ++i)
                         mma_ss(tmem + T_D + 64, kt + i * ROWS16, vt0 + (2 * SUB >> 4) + i * ROWS16,
                                idesc(64, true, true), 1);
+                    }
                     mma_commit(d_full);
                     mma_commit(empty_k(s));
                 }
@@ -499,18 +492,22 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         __syncwarp();
     } else if (warp == W_G) {
         // ----------------------------------------------------------- decays
+        // lane l: tokens 4 l .. 4 l + 3; lanes 8 b .. 8 b + 7 are block b
         Walk k(a, tiles, items);
         float gn[4];
         if (k.valid()) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
+            for (int e = 0; e < 4; ++e) gn[e] = load_g(a, k.it, k.t0 + 4 * lane + e);
         }
+#pragma unroll 1
         for (bool more = true; more;) {
             const uint32_t c = k.c;
             const int s = c & 1;
-            double g[4], t[4];
+            double g[4];
             more = k.valid();
             Chunk now = {};                              // behind the last one: m = 0
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = more ? (double)clamp_g(gn[e]) : 0.0;
             if (more) {
                 const int64_t left = k.it.len - k.t0;
                 now.row = (int)(k.it.row0 + k.t0);
@@ -520,48 +517,48 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 now.h = k.it.h;
                 now.seq = (int)k.it.seq;
                 now.tile = k.it.tile;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) g[b] = (double)clamp_g(gn[b]);
                 k.next();                                // the next chunk's loads
                 if (k.valid()) {
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) gn[b] = load_g(a, k.it, k.t0 + 32 * b + lane);
+                    for (int e = 0; e < 4; ++e) gn[e] = load_g(a, k.it, k.t0 + 4 * lane + e);
                 }
-            } else {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) g[b] = 0.0;
             }
-#pragma unroll 1
-            for (int d = 1; d < 32; d <<= 1)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const double y = __shfl_up_sync(0xffffffffu, g[b], d);
-                    if (lane >= d) g[b] += y;
-                }
+            for (int e = 1; e < 4; ++e) g[e] += g[e - 1];
+            double sum = g[3];                           // of the block's lanes up to this one
 #pragma unroll
-            for (int b = 0; b < 4; ++b) t[b] = __shfl_sync(0xffffffffu, g[b], 31);
+            for (int d = 1; d < 8; d <<= 1) {
+                const double y = __shfl_up_sync(0xffffffffu, sum, d, 8);
+                if ((lane & 7) >= d) sum += y;
+            }
+            const double last = __shfl_up_sync(0xffffffffu, sum, 1, 8);
+            const double before = (lane & 7) ? last : 0.0;
+            const double block = __shfl_sync(0xffffffffu, sum, 7, 8);
             // lane l: the blocks whose decays scalar l of OFF_SC multiplies
             constexpr uint64_t sets = 0x462F08CE7310ull;
             const uint32_t set = lane < 12 ? (uint32_t)(sets >> (4 * lane)) & 15u : 0u;
-            double sum = 0.0;
+            double all = 0.0;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (set >> b & 1u) sum += t[b];
-            const float mine = exp_of(sum);
-            float cf[4];
+            for (int b = 0; b < 4; ++b) {
+                const double t = __shfl_sync(0xffffffffu, block, 8 * b);
+                if (set >> b & 1u) all += t;
+            }
+            float cf[4], gg[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) cf[b] = exp_of(t[b] - g[b]);
+            for (int e = 0; e < 4; ++e) {
+                const double x = before + g[e];
+                cf[e] = exp_of(block - x);
+                gg[e] = (float)(x * 1.4426950408889634);
+            }
+            const float mine = exp_of(all);
             if (!wait_warp(g_free(s), ((c >> 1) & 1) ^ 1, 0x451)) break;
             if (lane < 12) sc[s * 16 + lane] = mine;
             if (lane == SC_ALL) {
                 dec[c & 3] = mine;                       // chunk c - 4 is long done
                 chunks[c & 3] = now;
             }
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                colf[s * C + 32 * b + lane] = cf[b];
-                g2[s * C + 32 * b + lane] = (float)(g[b] * 1.4426950408889634);
-            }
+            *reinterpret_cast<float4 *>(colf + s * C + 4 * lane) = make_float4(cf[0], cf[1], cf[2], cf[3]);
+            *reinterpret_cast<float4 *>(g2 + s * C + 4 * lane) = make_float4(gg[0], gg[1], gg[2], gg[3]);
             mbar_arrive(g_full(s));
         }
     } else if (warp < W_P) {
@@ -783,71 +780,72 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             if (!wait_warp(o_full, c & 1, 0x445)) break;
             mbar_arrive(g_free(s));                      // P (c) has read them too
             fence_after();
-            // all 64 columns first, so that the accumulators are free again before
-            // the stores
-            uint32_t y[DV / 2];
+            // Q K^T and Q S0 have read the chunk's q: its stage takes the output rows
+            uint8_t *const orow = smem + OFF_Q + s * 2 * SUB + r * 128;
             uint32_t bad = 0;                            // 0, or NaN
-#pragma unroll
+#pragma unroll 1
             for (int i0 = 0; i0 < DV; i0 += 16) {
-                uint32_t pv[16], qh[16];
+                uint32_t pv[16], qh[16], y[8];
                 tmem_ld16_async(quarter + T_PV + i0, pv);
                 tmem_ld16_async(quarter + T_QH + i0, qh);
                 tmem_loaded(pv);
                 tmem_loaded(qh);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    uint32_t &yi = y[(i0 + i) / 2];
-                    yi = pack_bf16(fma2(pair(qh[i], qh[i + 1]), ei2, pair(pv[i], pv[i + 1])));
-                    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(bad) : "r"(yi), "r"(0));
+                for (int i = 0; i < 8; ++i) {
+                    y[i] = pack_bf16(fma2(pair(qh[2 * i], qh[2 * i + 1]), ei2,
+                                          pair(pv[2 * i], pv[2 * i + 1])));
+                    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(bad) : "r"(y[i]), "r"(0));
                 }
+                const int j = i0 / 8;
+                *reinterpret_cast<uint4 *>(orow + ((j ^ (r & 7)) << 4)) =
+                    make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4 *>(orow + (((j + 1) ^ (r & 7)) << 4)) =
+                    make_uint4(y[4], y[5], y[6], y[7]);
             }
             const bool redo = r < k.m && (bad & 0x7fff7fffu);
-            if (__any_sync(0xffffffffu, redo)) {
-                // infinities or NaN: these rows again, from their own tokens
-#pragma unroll 1
-                for (int i0 = 0; i0 < DV; i0 += 16) {
-                    uint32_t qh[16];
-                    tmem_ld16_async(quarter + T_QH + i0, qh);
-                    tmem_loaded(qh);
-                    if (redo) {
-                        float z[16];
-                        masked_row(a, k, r, c0 + i0, z);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (c0 + i0 + i < a.dv)
-                                row[i0 + i] = __float2bfloat16_rn(
-                                    fmaf(__uint_as_float(qh[i]), __uint_as_float(lo_of(ei2)), z[i]));
-                    }
-                    __syncwarp();
-                }
-            }
-            fence_before();
-            mbar_arrive(o_free);
-            // P V of the chunk has read its V: the stage takes the output rows
-            uint8_t *const orow = smem + OFF_V + s * SUB + r * 128;
-            if (k.m == C && !__any_sync(0xffffffffu, redo)) {
-#pragma unroll
-                for (int i = 0; i < DV / 8; ++i)
-                    *reinterpret_cast<uint4 *>(orow + ((i ^ (r & 7)) << 4)) =
-                        make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            const bool cold = __any_sync(0xffffffffu, redo);
+            if (!cold) {
+                fence_before();
+                mbar_arrive(o_free);
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) {
-                    tma_store_4d(&map_o, base + OFF_V + s * SUB + w * 32 * 128, k.tile * DV, k.h,
-                                 k.row + 32 * w, a.cu ? 0 : k.seq);
-                    bulk_commit();
-                    bulk_wait_read0();
-                }
-            } else if (r < k.m && !redo) {
-                // the rows behind a sequence's end may be another one's
-#pragma unroll
-                for (int i = 0; i < DV / 8; ++i)
-                    if (c0 + 8 * i < a.dv)
+                if (k.m == C) {
+                    if (lane == 0) {
+                        tma_store_4d(&map_o, base + OFF_Q + s * 2 * SUB + w * 32 * 128, k.tile * DV,
+                                     k.h, k.row + 32 * w, a.cu ? 0 : k.seq);
+                        bulk_commit();
+                        bulk_wait_read0();
+                    }
+                } else if (r < k.m) {
+                    // the rows behind a sequence's end may be another one's
+#pragma unroll 1
+                    for (int i = 0; i < DV / 8 && c0 + 8 * i < a.dv; ++i)
                         *reinterpret_cast<uint4 *>(row + 8 * i) =
-                            make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                            *reinterpret_cast<const uint4 *>(orow + ((i ^ (r & 7)) << 4));
+                }
+            } else {
+                // infinities or NaN: those rows again, from their own tokens
+#pragma unroll 1
+                for (int i0 = 0; i0 < DV; i0 += 16) {
+                    uint32_t z[16], qh[16];
+                    tmem_ld16_async(quarter + T_PV + i0, z);
+                    tmem_ld16_async(quarter + T_QH + i0, qh);
+                    tmem_loaded(z);
+                    tmem_loaded(qh);
+                    if (redo) masked_row(a, k, r, c0 + i0, z);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (r < k.m && c0 + i0 + i < a.dv)
+                            row[i0 + i] = __float2bfloat16_rn(fmaf(
+                                __uint_as_float(qh[i]), __uint_as_float(lo_of(ei2)),
+                                __uint_as_float(z[i])));
+                    __syncwarp();
+                }
+                fence_before();
+                mbar_arrive(o_free);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty_v(s));
+            if (lane == 0) mbar_arrive(empty_q(s));
             __syncwarp();
         }
         if (lane == 0) bulk_wait0();                     // the stores are complete
