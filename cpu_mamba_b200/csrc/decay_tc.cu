@@ -22,9 +22,9 @@
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone.
 //
-// Roles (23 warps): 0-3 the state, 4-11 P, 12-15 the output rows, 16-19 V~, 20 TMA
-// loads, 21 MMA issue, 22 decays.  A chunk's products are issued as
-//   Q S0 (n), P V (n), Q K^T (n + 1), K^T V~ (n + 1)
+// Roles (28 warps): 0-7 the state, 8-15 P, 16-19 the output rows, 20-23 V~, 24 and
+// 25 MMA issue, 26 TMA loads, 27 decays.  One MMA warp issues P V (n), Q K^T (n + 1),
+// the other K^T V~ (n), Q S0 (n), each as soon as its operands are there,
 // so that P (n + 1) and the state update overlap the others' MMAs.  Every
 // mbarrier completes once per chunk (staged ones once per two), so its phase
 // follows from the chunk count.  All waits are bounded; a wait that expires sets
@@ -48,9 +48,10 @@ using namespace tc;
 
 constexpr int C = 128;                       // tokens per chunk
 constexpr int DV = 64;                       // columns of v per CTA
-// first warp of each role: the state, P (8 warps), output rows, V~, TMA, MMA, decays
-constexpr int W_P = 4, W_O = 12, W_V = 16, W_TMA = 20, W_MMA = 21, W_G = 22;
-constexpr int THREADS = 23 * 32;
+// first warp of each role: the state (8 warps), P (8), output rows, V~, MMA (2), TMA,
+// decays
+constexpr int W_P = 8, W_O = 16, W_V = 20, W_MMA = 24, W_TMA = 26, W_G = 27;
+constexpr int THREADS = 28 * 32;
 constexpr uint32_t SUB = 128 * 128;          // one 128-row x 128-byte operand tile
 // shared memory (bytes from a 1024-aligned base)
 constexpr uint32_t OFF_Q = 0;                            // [2][2 SUB]
@@ -64,7 +65,7 @@ constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
 constexpr uint32_t OFF_DEC = OFF_SC + 2 * 16 * 4;        // float [4]
 constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // int4 [4][2]
 constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 2 * 16;
-constexpr int NBARS = 6 + 6 + 4 + 9 + 1;
+constexpr int NBARS = 6 + 6 + 4 + 9 + 2;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
 // scalars of a chunk (OFF_SC), all e^sums of whole blocks' decays
@@ -356,16 +357,18 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     const uint32_t p_full = bar(22);    // P in TMEM, S read
     const uint32_t o_full = bar(23);    // P V and Q S0 in TMEM, P read
     const uint32_t o_free = bar(24);    // ... read
-    const uint32_t drain = bar(25);     // every MMA complete (once, at the end)
+    const uint32_t drain = bar(25);     // [2] a warp's MMAs complete (once, at the end)
 
     // through a shuffle, so that the compiler knows it to be one value a warp
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const bool wide = a.dk > 64;                         // two 64-column operand tiles
     if (threadIdx.x == 0) {
         for (int i = 0; i < NBARS; ++i) {
-            const int n = (i == 6 || i == 7) ? 4 : (i == 12 || i == 13) ? 32 :
-                          i == 17 ? 128 : i == 22 ? 256 :
-                          (i == 14 || i == 15 || i == 19 || i == 20 || i == 24) ? 128 : 1;
+            const int n = (i == 6 || i == 7) ? 4 :       // empty_q
+                          (i == 8 || i == 9 || i == 23) ? 2 :    // empty_k, o_full
+                          (i == 12 || i == 13) ? 32 :    // g_full
+                          (i == 14 || i == 15 || i == 17 || i == 24) ? 128 :
+                          (i == 19 || i == 20 || i == 22) ? 256 : 1;   // d_free, h_full, p_full
             mbar_init(bar(i), n);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -395,13 +398,13 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 mbar_expect_tx(full_k(s), qk);
                 tma_load_4d(dk, &map_k, full_k(s), 0, hk, tok, bq);
                 if (wide) tma_load_4d(dk + SUB, &map_k, full_k(s), 64, hk, tok, bq);
+                if (!wait_one(empty_v(s), ph, 0x403)) break;
+                mbar_expect_tx(full_v(s), SUB);
+                tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
                 if (!wait_one(empty_q(s), ph, 0x402)) break;
                 mbar_expect_tx(full_q(s), qk);
                 tma_load_4d(dq, &map_q, full_q(s), 0, hq, tok, bq);
                 if (wide) tma_load_4d(dq + SUB, &map_q, full_q(s), 64, hq, tok, bq);
-                if (!wait_one(empty_v(s), ph, 0x403)) break;
-                mbar_expect_tx(full_v(s), SUB);
-                tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
             }
             // no load is in flight when the CTA ends (its consumers may have given up)
             for (uint32_t n = k.c > 2 ? k.c - 2 : 0; n < k.c; ++n) {
@@ -411,7 +414,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             }
         }
         __syncwarp();
-    } else if (warp == W_MMA) {
+    } else if (warp == W_MMA || warp == W_MMA + 1) {
         // -------------------------------------------------------- MMA issue
         // The whole warp walks the chunks and one lane issues: descriptors and loop
         // are then provably one value a warp and stay in uniform registers, where
@@ -426,49 +429,50 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
         const int steps = wide ? 8 : 4;                  // of 16 columns of q and k
         bool ok = true;
-        // iteration n: Q S0 and P V of chunk n - 1, then Q K^T and K^T V~ of chunk n
+        if (warp == W_MMA) {
+            // iteration n: P V of chunk n - 1, Q K^T of chunk n
 #pragma unroll 1
-        for (uint32_t n = 0; n <= total && ok; ++n) {
-            if (n > 0) {
-                const uint32_t ph = (n - 1) & 1;
-                const uint64_t q = dq0 + ph * STAGE, v = v0 + ph * (SUB >> 4);
-                ok = wait_warp(h_full, ph, 0x415) && wait_warp(o_free, ph ^ 1, 0x416);
-                fence_after();
-                if (ok && elect_one()) {
-#pragma unroll 1
-                    for (int i = 0; i < steps; ++i)
-                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h0 + i * ROWS16,
-                               idesc(64, false, true), i != 0);
-                    mma_commit(h_free);
-                }
-                __syncwarp();
-                ok = ok && wait_warp(p_full, ph, 0x417);
-                fence_after();
-                if (ok && elect_one()) {
-#pragma unroll 1
-                    for (int i = 0; i < C / 16; ++i)
-                        mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, v + i * ROWS16,
-                                    idesc(64, false, true), i != 0);
-                    mma_commit(o_full);
-                    mma_commit(empty_v(ph));
-                }
-                __syncwarp();
-            }
-            if (n < total) {
-                const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
-                const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE, kt = kt0 + s * STAGE;
-                ok = ok && wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
-                fence_after();
-                if (ok && elect_one()) {
-#pragma unroll 1
-                    for (int i = 0; i < steps; ++i) {
-                        const uint64_t off = (i >> 2) * (SUB >> 4) + (i & 3) * 2;
-                        mma_ss(tmem + T_S, q + off, k + off, idesc(128, false, false), i != 0);
+            for (uint32_t n = 0; n <= total && ok; ++n) {
+                if (n > 0) {
+                    const uint32_t ph = (n - 1) & 1;
+                    const uint64_t v = v0 + ph * (SUB >> 4);
+                    ok = wait_warp(o_free, ph ^ 1, 0x416) && wait_warp(p_full, ph, 0x417);
+                    fence_after();
+                    if (ok && elect_one()) {
+#pragma unroll 2
+                        for (int i = 0; i < C / 16; ++i)
+                            mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, v + i * ROWS16,
+                                        idesc(64, false, true), i != 0);
+                        mma_commit(o_full);
+                        mma_commit(empty_v(ph));
                     }
-                    mma_commit(s_full);
+                    __syncwarp();
                 }
-                __syncwarp();
-                ok = ok && wait_warp(vt_full, s, 0x413) && wait_warp(d_free, s ^ 1, 0x414);
+                if (n < total) {
+                    const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
+                    const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE;
+                    ok = ok && wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
+                    fence_after();
+                    if (ok && elect_one()) {
+#pragma unroll 2
+                        for (int i = 0; i < steps; ++i) {
+                            const uint64_t off = (i >> 2) * (SUB >> 4) + (i & 3) * 2;
+                            mma_ss(tmem + T_S, q + off, k + off, idesc(128, false, false), i != 0);
+                        }
+                        mma_commit(s_full);
+                        mma_commit(empty_k(s));
+                    }
+                    __syncwarp();
+                }
+            }
+        } else {
+            // K^T V~, then Q S0 of each chunk
+#pragma unroll 1
+            for (uint32_t n = 0; n < total && ok; ++n) {
+                const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
+                const uint64_t q = dq0 + s * STAGE, kt = kt0 + s * STAGE;
+                ok = wait_warp(vt_full, s, 0x413) && wait_warp(full_k(s), ph2, 0x414) &&
+                     wait_warp(d_free, s ^ 1, 0x414);
                 fence_after();
                 if (ok && elect_one()) {
                     // V~'s first two parts side by side, the third added to the second's
@@ -483,11 +487,24 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     mma_commit(empty_k(s));
                 }
                 __syncwarp();
+                ok = ok && wait_warp(h_full, s, 0x415) && wait_warp(full_q(s), ph2, 0x412) &&
+                     wait_warp(o_free, s ^ 1, 0x416);
+                fence_after();
+                if (ok && elect_one()) {
+#pragma unroll 2
+                    for (int i = 0; i < steps; ++i)
+                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h0 + i * ROWS16,
+                               idesc(64, false, true), i != 0);
+                    mma_commit(h_free);
+                    mma_commit(o_full);
+                }
+                __syncwarp();
             }
         }
         if (elect_one()) {
-            mma_commit(drain);                           // before TMEM is given back
-            wait_one(drain, 0, 0x418);
+            const uint32_t mine = drain + 8 * (warp - W_MMA);
+            mma_commit(mine);                            // before TMEM is given back
+            wait_one(mine, 0, 0x418);
         }
         __syncwarp();
     } else if (warp == W_G) {
@@ -563,11 +580,11 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         }
     } else if (warp < W_P) {
         // -------------------------------------------------------- the state
-        // Row r of the state, 16 columns at a time: from h0 at a
+        // Row r of the state, 32 columns a warp, 16 at a time: from h0 at a
         // sequence's start (pass 0), and e^{G_C} S0 + K^T V~ behind each chunk
         // (pass 1); to TMEM and (bf16, for Q S0) to shared memory, or to h_last
         // behind the last chunk.
-        const int w = warp & 3, r = 32 * w + lane;
+        const int w = warp & 3, half = warp >> 2, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
         uint8_t *const hrow = smem + OFF_H + r * 128;
         bool ok = true;
@@ -589,7 +606,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 // Q S0 of the chunk before the one this state is for
                 if (!store && !(ok = wait_warp(h_free, (c + pass + 1) & 1, 0x423))) break;
 #pragma unroll 1
-                for (int i = 0; i < DV; i += 16) {
+                for (int i = 32 * half; i < 32 * half + 32; i += 16) {
                     uint32_t h[16];
                     if (pass == 0) {
 #pragma unroll
