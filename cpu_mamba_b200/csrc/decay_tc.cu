@@ -433,10 +433,13 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             // iteration n: P V of chunk n - 1, Q K^T of chunk n
 #pragma unroll 1
             for (uint32_t n = 0; n <= total && ok; ++n) {
+                const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
+                if (n < total)
+                    ok = wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
                 if (n > 0) {
                     const uint32_t ph = (n - 1) & 1;
                     const uint64_t v = v0 + ph * (SUB >> 4);
-                    ok = wait_warp(o_free, ph ^ 1, 0x416) && wait_warp(p_full, ph, 0x417);
+                    ok = ok && wait_warp(o_free, ph ^ 1, 0x416) && wait_warp(p_full, ph, 0x417);
                     fence_after();
                     if (ok && elect_one()) {
 #pragma unroll 2
@@ -449,10 +452,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     __syncwarp();
                 }
                 if (n < total) {
-                    const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
                     const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE;
-                    ok = ok && wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
-                    fence_after();
                     if (ok && elect_one()) {
 #pragma unroll 2
                         for (int i = 0; i < steps; ++i) {
@@ -691,37 +691,37 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll 1
             for (int n = 2 * odd; n < 2 * w + 2; n += (n & 1) ? 3 : 1) {   // 16 columns
                 uint32_t x[16], p[8];
+                uint64_t f[8];
                 tmem_ld16_async(quarter + T_S + 16 * n, x);
                 const int b = n >> 1;
                 if (b < w) {
                     const uint64_t fb = pair(b == 0 ? f0 : b == 1 ? f1 : rowf);
                     const ulonglong2 *cf = reinterpret_cast<const ulonglong2 *>(colf + s * C + 16 * n);
-                    tmem_loaded(x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const ulonglong2 y = cf[i];
-                        p[2 * i] = pack_bf16(mul2(pair(x[4 * i], x[4 * i + 1]), mul2(y.x, fb)));
-                        p[2 * i + 1] = pack_bf16(mul2(pair(x[4 * i + 2], x[4 * i + 3]), mul2(y.y, fb)));
+                        f[2 * i] = mul2(y.x, fb);
+                        f[2 * i + 1] = mul2(y.y, fb);
                     }
                 } else {
+                    // 0 above the diagonal; times an infinity or NaN that makes a
+                    // NaN, and the row is done again below
                     const float4 *gj = reinterpret_cast<const float4 *>(g2 + s * C + 16 * n);
                     const int last = lane - 16 * (n & 1);            // the diagonal's column
-                    tmem_loaded(x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float4 y = gj[i];
-                        const uint64_t e0 = mul2(pair(x[4 * i], x[4 * i + 1]),
-                                                 mul2(scale2, pair(__float_as_uint(ex2(gr - y.x)),
-                                                                   __float_as_uint(ex2(gr - y.y)))));
-                        const uint64_t e1 = mul2(pair(x[4 * i + 2], x[4 * i + 3]),
-                                                 mul2(scale2, pair(__float_as_uint(ex2(gr - y.z)),
-                                                                   __float_as_uint(ex2(gr - y.w)))));
-                        p[2 * i] = pack_bf16(pair(4 * i <= last ? lo_of(e0) : 0u,
-                                                  4 * i + 1 <= last ? hi_of(e0) : 0u));
-                        p[2 * i + 1] = pack_bf16(pair(4 * i + 2 <= last ? lo_of(e1) : 0u,
-                                                      4 * i + 3 <= last ? hi_of(e1) : 0u));
+                        const float e0 = 4 * i <= last ? ex2(gr - y.x) : 0.0f;
+                        const float e1 = 4 * i + 1 <= last ? ex2(gr - y.y) : 0.0f;
+                        const float e2 = 4 * i + 2 <= last ? ex2(gr - y.z) : 0.0f;
+                        const float e3 = 4 * i + 3 <= last ? ex2(gr - y.w) : 0.0f;
+                        f[2 * i] = mul2(scale2, pair(__float_as_uint(e0), __float_as_uint(e1)));
+                        f[2 * i + 1] = mul2(scale2, pair(__float_as_uint(e2), __float_as_uint(e3)));
                     }
                 }
+                tmem_loaded(x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[i] = pack_bf16(mul2(pair(x[2 * i], x[2 * i + 1]), f[i]));
                 tmem_st8(quarter + T_P + 8 * n, p);
             }
             tmem_wait_st();
