@@ -79,7 +79,8 @@ __device__ __forceinline__ void stage(T *dst, int pitch, const T *src, int64_t l
     }
 }
 
-template <typename T, int KT, int VT>
+// STATE: the pass over segments that leaves their states; no q, no outputs
+template <typename T, int KT, int VT, bool STATE>
 __global__ void __launch_bounds__(128)
 decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec_v) {
     using R = Rec<T, KT, VT>;
@@ -96,10 +97,12 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     const int tile = (int)(id % tiles);
     id /= tiles;
     const int h = (int)(id % a.heads);
-    const int64_t seq = id / a.heads;
-    int64_t row0, len;
-    bounds(a, seq, row0, len);
-    const int64_t bq = a.cu ? 0 : seq;
+    const Span sp = span_of<STATE>(a, id / a.heads);
+    if (STATE && sp.out < 0) return;
+    const int64_t row0 = sp.row0, len = sp.len;
+    const int64_t bq = a.cu ? 0 : sp.seq;
+    const float *const hin = !STATE && a.seg ? a.seg_state : a.h0;
+    float *const hout = STATE ? a.seg_state : a.h_last;
     const T *q = static_cast<const T *>(a.q) + bq * a.qs[0] + row0 * a.qs[1] + (h / a.q_rep) * a.qs[2];
     const T *k = static_cast<const T *>(a.k) + bq * a.ks[0] + row0 * a.ks[1] + (h / a.k_rep) * a.ks[2];
     const int c0 = tile * vtile;
@@ -128,8 +131,8 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
             const int dk = 32 * i + 4 * kg + j;
 #pragma unroll
             for (int c = 0; c < VT; ++c)
-                u[i][j][c] = (a.h0 && dk < a.dk && col + c < cols)
-                                 ? a.h0[((seq * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c]
+                u[i][j][c] = (sp.in >= 0 && dk < a.dk && col + c < cols)
+                                 ? hin[((sp.in * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c]
                                  : 0.0f;
         }
     __syncthreads();
@@ -139,7 +142,8 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         const int b = n & 1;
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
-        stage<T>(qs + b * L * R::PK, R::PK, q + t0 * a.qs[1], a.qs[1], m, (int)a.dk, vec_q);
+        if (!STATE)
+            stage<T>(qs + b * L * R::PK, R::PK, q + t0 * a.qs[1], a.qs[1], m, (int)a.dk, vec_q);
         stage<T>(ks + b * L * R::PK, R::PK, k + t0 * a.ks[1], a.ks[1], m, (int)a.dk, vec_k);
         stage<T>(vs + b * L * pv, pv, v + t0 * a.vs[1], a.vs[1], m, cols, vec_v);
         cp_async_commit();
@@ -148,6 +152,7 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     // log A is a 64-bit sum: a head that forgets over thousands of tokens adds
     // as many equal decays, whose roundings in 32 bits all point one way.
     double run = 0.0;                 // log A after the chunk (warp 0)
+    double span_g = 0.0;              // STATE: the sum of all log decays
     auto factors = [&](int n) {
         const int b = n & 1;
         const int64_t t0 = (int64_t)n * L;
@@ -161,6 +166,7 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
             const double below = __shfl_up_sync(0xffffffffu, cum, s);
             if (lane >= s) cum += below;
         }
+        if (STATE) span_g += __shfl_sync(0xffffffffu, cum, L - 1);
         cum += run;
         // false for NaN and infinities too
         if (__all_sync(0xffffffffu, lane >= m || fabs(cum) <= kRun)) {
@@ -218,27 +224,30 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
             for (int i = 0; i < KI; ++i) {
                 float kv[4], qv[4];
                 ld4<T>(kb + t * R::PK + 32 * i, kv);
-                ld4<T>(qb + t * R::PK + 32 * i, qv);
+                if (!STATE) ld4<T>(qb + t * R::PK + 32 * i, qv);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int c = 0; c < VT; ++c) {
                         u[i][j][c] = fmaf(kv[j], w[c], u[i][j][c]);
-                        acc[c] = fmaf(qv[j], u[i][j][c], acc[c]);
+                        if (!STATE) acc[c] = fmaf(qv[j], u[i][j][c], acc[c]);
                     }
             }
+            if constexpr (!STATE) {
 #pragma unroll
-            for (int s = 1; s < 8; s <<= 1)
+                for (int s = 1; s < 8; s <<= 1)
 #pragma unroll
-                for (int c = 0; c < VT; ++c) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], s);
-            float r = acc[0];
+                    for (int c = 0; c < VT; ++c) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], s);
+                float r = acc[0];
 #pragma unroll
-            for (int c = 1; c < VT; ++c) r = kg == c ? acc[c] : r;
-            if (kg < VT && col + kg < cols)
-                o[(t0 + t) * a.os[1] + col + kg] = io<T>::from_f(r * s_out[b][t]);
+                for (int c = 1; c < VT; ++c) r = kg == c ? acc[c] : r;
+                if (kg < VT && col + kg < cols)
+                    o[(t0 + t) * a.os[1] + col + kg] = io<T>::from_f(r * s_out[b][t]);
+            }
         }
     }
-    if (a.h_last) {
+    if (STATE && threadIdx.x == 0 && tile == 0) a.seg_g[sp.out * a.heads + h] = span_g;
+    if (sp.out >= 0) {
         // the last run's decay: every thread needs log A of the last token
         __shared__ float s_last;
         if (threadIdx.x == 0) s_last = (float)exp(run);
@@ -252,7 +261,7 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
 #pragma unroll
                 for (int c = 0; c < VT; ++c)
                     if (dk < a.dk && col + c < cols)
-                        a.h_last[((seq * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c] =
+                        hout[((sp.out * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c] =
                             u[i][j][c] * f;
             }
     }
@@ -264,15 +273,15 @@ static bool vec16(const void *p, const int64_t (&s)[3], int64_t cols) {
     return aligned(p, 16) && s[0] % E == 0 && s[1] % E == 0 && s[2] % E == 0 && cols % E == 0;
 }
 
-template <typename T, int KT, int VT>
+template <typename T, int KT, int VT, bool STATE>
 static int launch_recurrent(const Args &a, cudaStream_t st) {
     using R = Rec<T, KT, VT>;
     const int warps = (int)(ceil_div(a.dv, R::WV) < R::MAXW ? ceil_div(a.dv, R::WV) : R::MAXW);
     const int vtile = warps * R::WV;
-    const int64_t grid = ceil_div(a.dv, vtile) * a.heads * a.seqs;
+    const int64_t grid = ceil_div(a.dv, vtile) * a.heads * spans(a);
     MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
     const size_t smem = sizeof(T) * 2 * L * (2 * R::PK + vtile + 16 / sizeof(T));
-    auto kern = decay_recurrent_kernel<T, KT, VT>;
+    auto kern = decay_recurrent_kernel<T, KT, VT, STATE>;
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)smem);
@@ -285,12 +294,126 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
     return check_launch("decay_recurrent_kernel");
 }
 
-template <typename T>
-static int recurrent(const Args &a, cudaStream_t st) {
-    if (a.dk <= 32) return launch_recurrent<T, 4, 4>(a, st);
-    if (a.dk <= 64) return launch_recurrent<T, 8, 4>(a, st);
-    if (a.dk <= 128) return launch_recurrent<T, 16, 4>(a, st);
-    return launch_recurrent<T, 32, 2>(a, st);
+template <typename T, bool STATE>
+static int recurrent_of(const Args &a, cudaStream_t st) {
+    if (a.dk <= 32) return launch_recurrent<T, 4, 4, STATE>(a, st);
+    if (a.dk <= 64) return launch_recurrent<T, 8, 4, STATE>(a, st);
+    if (a.dk <= 128) return launch_recurrent<T, 16, 4, STATE>(a, st);
+    return launch_recurrent<T, 32, 2, STATE>(a, st);
+}
+static int recurrent(const Args &a, bool state_only, cudaStream_t st) {
+    if (a.dtype == MB2_F32)
+        return state_only ? recurrent_of<float, true>(a, st) : recurrent_of<float, false>(a, st);
+    return state_only ? recurrent_of<__nv_bfloat16, true>(a, st)
+                      : recurrent_of<__nv_bfloat16, false>(a, st);
+}
+
+// --------------------------------------------------------------- segments
+// slot0[i]: the first slot of packed sequence i (one warp, a running sum)
+__global__ void slots_kernel(const Args a, int32_t *slot0) {
+    int64_t base = 0;
+    for (int64_t i0 = 0; i0 < a.seqs; i0 += 32) {
+        const int64_t i = i0 + threadIdx.x;
+        int64_t row0 = 0, len = 0, n = 0;
+        if (i < a.seqs) {
+            bounds(a, i, row0, len);
+            n = segments(len, a.seg);
+        }
+        int64_t sum = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, sum, d);
+            if ((int)threadIdx.x >= d) sum += y;
+        }
+        // (overlapping sequences can ask for more slots than there are)
+        const int64_t at = base + sum - n;
+        if (i < a.seqs) slot0[i] = (int32_t)(at < a.slots ? at : a.slots);
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) slot0[a.seqs] = (int32_t)(base < a.slots ? base : a.slots);
+}
+
+// The segments' states, each from 0, become their initial states, element by
+// element: S_{j+1} = e^{G_j} S_j + own_j, S_0 = h0.  A sequence's last slot takes
+// its initial state without having held one.
+__global__ void __launch_bounds__(256) seg_states_kernel(const Args a) {
+    const int64_t per = a.dk * a.dv;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t seq = blockIdx.z, h = blockIdx.y;
+    if (e >= per) return;
+    const int64_t n = a.cu ? a.slot0[seq + 1] - a.slot0[seq] : segments(a.seqlen, a.seg);
+    const int64_t first = a.cu ? a.slot0[seq] : seq * n;
+    float *s = a.seg_state + (first * a.heads + h) * per + e;
+    const double *g = a.seg_g + first * a.heads + h;
+    float run = a.h0 ? a.h0[(seq * a.heads + h) * per + e] : 0.0f;
+    // the chain is short; the loads of eight segments run ahead of it
+    for (int64_t j0 = 0; j0 < n; j0 += 8) {
+        float own[8];
+        double lg[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = j0 + i + 1 < n;
+            own[i] = in ? s[(j0 + i) * a.heads * per] : 0.0f;
+            lg[i] = in ? g[(j0 + i) * a.heads] : 0.0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (j0 + i < n) {
+                s[(j0 + i) * a.heads * per] = run;
+                run = fmaf(expf((float)lg[i]), run, own[i]);
+            }
+    }
+}
+
+// Tokens per segment, 0 for whole sequences.  A walk takes its steps of `unit`
+// tokens one after the other, and `lanes` walks run at a time: with fewer sequences
+// x heads x column tiles than that (or an uneven last round of them) segments
+// shorten the longest chain, at the price of a first pass that costs `first` of the
+// second's time a step, a step or so to fill each walk, and the states' traffic.
+// Measured, one sequence of 8192 tokens, 24 heads of 128 x 64 in bf16: 134 us whole,
+// 95 in segments (27 first pass, 42 second).
+static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64_t unit,
+                              double first) {
+    if (a.seqs == 0 || a.seqlen == 0) return 0;
+    // packed: the lengths are not known here; the longest sequence is taken as
+    // twice the mean
+    const int64_t units = ceil_div(a.cu ? ceil_div(a.seqlen, a.seqs) : a.seqlen, unit);
+    const double even = (double)walks * (double)units / (double)lanes;
+    const double whole = !a.cu ? (double)ceil_div(walks, lanes) * (double)units
+                               : (even > 2.0 * units ? even : 2.0 * units);
+    double best = whole * 0.9;            // segments have to save a tenth
+    int64_t seg = 0;
+    for (int64_t n = 2; n <= 256 && n * 4 <= 2 * units; ++n) {
+        const int64_t per = ceil_div(units, n);
+        const double t = (double)ceil_div(walks * n, lanes) * (per + 1.0) +
+                         (double)ceil_div(walks * (n - 1), lanes) * (first * per + 1.0) +
+                         0.1 * n + 4.0;
+        if (t < best) {
+            best = t;
+            seg = per * unit;
+        }
+    }
+    return seg;
+}
+
+struct Plan { size_t slot0, g, state, bytes; };
+// how a call runs: sets a.seg and a.slots; the parts of its workspace
+static Plan plan(Args &a) {
+    // tensor cores: one walk of 64 columns an SM, 128 tokens a step; recurrent: four
+    // walks of up to 64 columns an SM, compared by 32 tokens
+    const int sms = num_sms();
+    const bool tc = chunked_fits(a);
+    const int64_t walks = a.seqs * a.heads * ceil_div(a.dv, 64);
+    a.seg = segment_tokens(a, walks, tc ? sms : 4 * sms, tc ? 128 : 32, tc ? 0.65 : 0.35);
+    a.slots = 0;
+    Plan p = {};
+    if (a.seg == 0) return p;
+    a.slots = a.cu ? a.seqs + a.seqlen / a.seg : a.seqs * segments(a.seqlen, a.seg);
+    p.slot0 = 0;
+    p.g = (size_t)round_up((a.seqs + 1) * 4, 256);
+    p.state = p.g + (size_t)round_up(a.slots * a.heads * 8, 256);
+    p.bytes = p.state + (size_t)(a.slots * a.heads * a.dk * a.dv) * 4;
+    return p;
 }
 
 // rows of o behind the last packed sequence (a freshly allocated o)
@@ -413,6 +536,16 @@ static int step(const Args &a, float *state, cudaStream_t st) {
     return check_launch("decay_step_kernel");
 }
 
+int num_sms() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    return sms;
+}
+
 static int to_args(const mb2_decay_attn *d, bool one, Args &a) {
     const char *what = one ? "decay_attention_step" : "decay_attention";
     MB2_REQUIRE(d, MB2_ERR_ARG, "%s: null descriptor", what);
@@ -453,6 +586,10 @@ static int to_args(const mb2_decay_attn *d, bool one, Args &a) {
     a.h_last = d->h_last;
     a.cu = d->cu_seqlens;
     a.scale = d->scale;
+    a.seg = a.slots = 0;
+    a.slot0 = nullptr;
+    a.seg_state = nullptr;
+    a.seg_g = nullptr;
     return MB2_OK;
 }
 
@@ -462,19 +599,23 @@ static int to_args(const mb2_decay_attn *d, bool one, Args &a) {
 using namespace mb2;
 
 extern "C" size_t mb2_decay_attention_workspace_bytes(const mb2_decay_attn *d) {
-    (void)d;
-    return 0;
+    decay::Args a;
+    return decay::to_args(d, false, a) == MB2_OK ? decay::plan(a).bytes : 0;
 }
 
 extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, size_t workspace_bytes,
                                    mb2_stream_t stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     decay::Args a;
     MB2_TRY(decay::to_args(d, false, a));
-    if (a.seqs == 0) return MB2_OK;
+    if (a.seqs == 0 && !(a.cu && d->zero_tail)) return MB2_OK;
     MB2_REQUIRE((a.q && a.k && a.v && a.g && a.o) || a.seqlen == 0, MB2_ERR_ARG,
                 "decay_attention: null pointer");
+    const decay::Plan p = decay::plan(a);
+    MB2_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), MB2_ERR_WORKSPACE,
+                "decay_attention: workspace of %llu bytes, %llu needed",
+                (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
+    MB2_REQUIRE(p.bytes == 0 || aligned(workspace, 256), MB2_ERR_ALIGN,
+                "decay_attention: misaligned workspace");
     cudaStream_t st = (cudaStream_t)stream;
     if (a.cu && d->zero_tail && a.seqlen > 0) {
         if (a.dtype == MB2_F32)
@@ -483,11 +624,29 @@ extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, siz
             decay::zero_tail_kernel<__nv_bfloat16><<<64, 256, 0, st>>>(a);
         MB2_TRY(check_launch("zero_tail_kernel"));
     }
+    if (a.seqs == 0) return MB2_OK;
     bool used = false;
-    MB2_TRY(decay::chunked(a, st, &used));
-    if (used) return MB2_OK;
-    return a.dtype == MB2_F32 ? decay::recurrent<float>(a, st)
-                              : decay::recurrent<__nv_bfloat16>(a, st);
+    if (a.seg) {
+        uint8_t *ws = static_cast<uint8_t *>(workspace);
+        int32_t *slot0 = reinterpret_cast<int32_t *>(ws + p.slot0);
+        a.slot0 = slot0;
+        a.seg_g = reinterpret_cast<double *>(ws + p.g);
+        a.seg_state = reinterpret_cast<float *>(ws + p.state);
+        MB2_REQUIRE(a.seqs < 65536 && a.heads < 65536, MB2_ERR_SHAPE,
+                    "decay_attention: too many sequences or heads");
+        if (a.cu) {
+            decay::slots_kernel<<<1, 32, 0, st>>>(a, slot0);
+            MB2_TRY(check_launch("slots_kernel"));
+        }
+        MB2_TRY(decay::chunked(a, true, st, &used));
+        if (!used) MB2_TRY(decay::recurrent(a, true, st));
+        const dim3 grid((unsigned)ceil_div(a.dk * a.dv, (int64_t)256), (unsigned)a.heads,
+                        (unsigned)a.seqs);
+        decay::seg_states_kernel<<<grid, 256, 0, st>>>(a);
+        MB2_TRY(check_launch("seg_states_kernel"));
+    }
+    MB2_TRY(decay::chunked(a, false, st, &used));
+    return used ? MB2_OK : decay::recurrent(a, false, st);
 }
 
 extern "C" int mb2_decay_attention_step(const mb2_decay_attn *d, float *state, mb2_stream_t stream) {

@@ -63,8 +63,8 @@ constexpr uint32_t OFF_COLF = OFF_H + SUB;               // float [2][128]
 constexpr uint32_t OFF_G2 = OFF_COLF + 2 * C * 4;        // float [2][128]
 constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
 constexpr uint32_t OFF_DEC = OFF_SC + 2 * 16 * 4;        // float [4]
-constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // int4 [4][2]
-constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 2 * 16;
+constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // Chunk [4]
+constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 3 * 16;
 constexpr int NBARS = 6 + 6 + 4 + 9 + 2;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
@@ -218,61 +218,88 @@ __device__ __forceinline__ float exp_of(double x) {
     return e == 0.0f || hi != hi ? e : fmaf(e, lo, e);
 }
 
+// An item of work: a span (32-bit: tokens and spans are below 2^31) x head x tile.
 struct Item {
-    int tile, h;
-    int64_t seq, row0, len;
+    int tile, h, seq, row0, len, in, out;
 };
-__device__ __forceinline__ Item item_of(const Args &a, int tiles, uint32_t id) {
+template <bool STATE>
+__device__ __forceinline__ Item item_of(const Args &a, uint32_t tiles, uint32_t id) {
     Item it;
-    const uint32_t n = id / (uint32_t)tiles, heads = (uint32_t)a.heads;
-    it.tile = (int)(id - n * (uint32_t)tiles);
-    it.seq = n / heads;
-    it.h = (int)(n - (uint32_t)it.seq * heads);
-    bounds(a, it.seq, it.row0, it.len);
+    const uint32_t n = id / tiles, heads = (uint32_t)a.heads, span = n / heads;
+    it.tile = (int)(id - n * tiles);
+    it.h = (int)(n - span * heads);
+    const int len = (int)a.seqlen, seg = (int)a.seg;
+    int seq = (int)span, j = 0, segs = 1;
+    if (seg > 0) {
+        if (a.cu) {
+            int hi = (int)a.seqs;         // the last sequence whose first slot is <= span
+            seq = 0;
+            while (hi - seq > 1) {
+                const int mid = (seq + hi) >> 1;
+                if (a.slot0[mid] <= (int)span) seq = mid;
+                else hi = mid;
+            }
+            j = (int)span - a.slot0[seq];
+            segs = a.slot0[seq + 1] - a.slot0[seq];
+        } else {
+            segs = len > seg ? (int)((uint32_t)(len + seg - 1) / (uint32_t)seg) : 1;
+            seq = (int)(span / (uint32_t)segs);
+            j = (int)span - seq * segs;
+        }
+    }
+    it.seq = seq;
+    it.row0 = 0;
+    it.len = len;
+    if (a.cu) {
+        const int b = a.cu[seq], e = a.cu[seq + 1];
+        it.row0 = b < 0 ? 0 : b > len ? len : b;
+        it.len = (e > len ? len : e) - it.row0;
+        if (it.len < 0) it.len = 0;
+    }
+    it.in = a.h0 ? seq : -1;
+    it.out = a.h_last ? seq : -1;
+    if (seg > 0) {
+        const bool last = j == segs - 1, valid = j < segs && (!STATE || !last);
+        it.row0 += j * seg;
+        it.len = it.len - j * seg < seg ? it.len - j * seg : seg;
+        if (!valid || it.len < 0) it.len = 0;
+        it.in = STATE ? -1 : (int)span;
+        it.out = !valid ? -1 : STATE ? (int)span : last ? it.out : -1;
+    }
     return it;
 }
 // A chunk as the roles see it, in shared memory beside its decays: one warp walks
 // the items, the others read.
-struct Chunk {
+struct alignas(16) Chunk {
     int row, m;                          // first token (of the batch row), tokens; m 0: the end
-    int first, last;                     // of its sequence
-    int h, seq, tile, pad;
+    int first, last;                     // of its span
+    int h, batch, tile;
+    int in, out;                         // Span's
 };
-// the chunks of a CTA's items, in order
-struct Walk {
-    const Args &a;
-    const int tiles;
-    const uint32_t items;
-    uint32_t id;
-    int64_t t0;
+// the chunks of a CTA's items, in order; items without tokens go to `empty`
+template <bool STATE> struct Walk {
     Item it;
-    uint32_t c;                          // chunks before this one
-    __device__ __forceinline__ Walk(const Args &a_, int tiles_, uint32_t items_)
-        : a(a_), tiles(tiles_), items(items_), id(blockIdx.x), t0(0), c(0) {
-        find();
-    }
-    __device__ __forceinline__ bool valid() const { return id < items; }
-    __device__ __forceinline__ void find() {     // the next item with tokens
-        for (; id < items; id += gridDim.x) {
-            it = item_of(a, tiles, id);
-            if (it.len > 0) break;
-        }
-    }
-    __device__ __forceinline__ void next() {
-        ++c;
+    int t0 = 0;
+    uint32_t id = blockIdx.x - gridDim.x;
+    __device__ __forceinline__ Walk() { it.len = 0; }
+    template <typename F>
+    __device__ __forceinline__ bool next(const Args &a, uint32_t tiles, uint32_t items, F empty) {
         t0 += C;
-        if (t0 >= it.len) {
-            t0 = 0;
+        if (t0 < it.len) return true;
+        t0 = 0;
+        for (;;) {
             id += gridDim.x;
-            find();
+            if (id >= items) return false;
+            it = item_of<STATE>(a, tiles, id);
+            if (it.len > 0) return true;
+            empty();
         }
     }
 };
 // g of token t of an item (0 behind its end)
-__device__ __forceinline__ float load_g(const Args &a, const Item &it, int64_t t) {
+__device__ __forceinline__ float load_g(const Args &a, const Item &it, int t) {
     if (t >= it.len) return 0.0f;
-    const int64_t bq = a.cu ? 0 : it.seq;
-    return a.g[bq * a.gs[0] + (it.row0 + t) * a.gs[1] + it.h * a.gs[2]];
+    return a.g[(a.cu ? 0 : it.seq) * a.gs[0] + (int64_t)(it.row0 + t) * a.gs[1] + it.h * a.gs[2]];
 }
 // below -256, e^g is 0 for every fp32 product, and a finite sum keeps later
 // differences; NaN stays
@@ -297,7 +324,7 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int whe
 // memory: for rows that met an infinity or a NaN, perhaps in a masked token
 __device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r, int col,
                                            uint32_t (&y)[16]) {
-    const int64_t bq = a.cu ? 0 : k.seq;
+    const int64_t bq = k.batch;
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + bq * a.qs[0] +
                              (k.row + r) * a.qs[1] + (k.h / a.q_rep) * a.qs[2];
 #pragma unroll
@@ -322,12 +349,14 @@ __device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r,
     }
 }
 
+// STATE: the pass over segments that leaves their states; no Q, no outputs
+template <bool STATE>
 __global__ void __launch_bounds__(THREADS, 1)
 decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ CUtensorMap map_o, const __grid_constant__ Args a,
-                   int tiles, uint32_t items) {
+                   uint32_t tiles, uint32_t items) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     float *const colf = reinterpret_cast<float *>(smem + OFF_COLF);
@@ -365,9 +394,12 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     if (threadIdx.x == 0) {
         for (int i = 0; i < NBARS; ++i) {
             const int n = (i == 6 || i == 7) ? 4 :       // empty_q
-                          (i == 8 || i == 9 || i == 23) ? 2 :    // empty_k, o_full
+                          (i == 8 || i == 9) ? (STATE ? 1 : 2) :   // empty_k
+                          (i == 10 || i == 11) ? (STATE ? 128 : 1) :   // empty_v
                           (i == 12 || i == 13) ? 32 :    // g_full
-                          (i == 14 || i == 15 || i == 17 || i == 24) ? 128 :
+                          (i == 14 || i == 15) ? (STATE ? 256 : 128) :   // g_free
+                          i == 23 ? 2 :                  // o_full
+                          (i == 17 || i == 24) ? 128 :   // vt_full, o_free
                           (i == 19 || i == 20 || i == 22) ? 256 : 1;   // d_free, h_full, p_full
             mbar_init(bar(i), n);
         }
@@ -386,12 +418,14 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     if (warp == W_TMA) {
         // -------------------------------------------------------- TMA loads
         if (lane == 0) {
-            Walk k(a, tiles, items);
+            Walk<STATE> k;
             const uint32_t qk = wide ? 2 * SUB : SUB;
-            for (; k.valid(); k.next()) {
-                const int s = k.c & 1;
-                const uint32_t ph = ((k.c >> 1) & 1) ^ 1;
-                const int tok = (int)(k.it.row0 + k.t0), bq = a.cu ? 0 : (int)k.it.seq;
+            uint32_t c = 0;
+#pragma unroll 1
+            for (; k.next(a, tiles, items, [] {}); ++c) {
+                const int s = c & 1;
+                const uint32_t ph = ((c >> 1) & 1) ^ 1;
+                const int tok = k.it.row0 + k.t0, bq = a.cu ? 0 : k.it.seq;
                 const int hq = k.it.h / a.q_rep, hk = k.it.h / a.k_rep, hv = k.it.h / a.v_rep;
                 const uint32_t dk = base + OFF_K + s * 2 * SUB, dq = base + OFF_Q + s * 2 * SUB;
                 if (!wait_one(empty_k(s), ph, 0x401)) break;
@@ -401,15 +435,16 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (!wait_one(empty_v(s), ph, 0x403)) break;
                 mbar_expect_tx(full_v(s), SUB);
                 tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
+                if (STATE) continue;
                 if (!wait_one(empty_q(s), ph, 0x402)) break;
                 mbar_expect_tx(full_q(s), qk);
                 tma_load_4d(dq, &map_q, full_q(s), 0, hq, tok, bq);
                 if (wide) tma_load_4d(dq + SUB, &map_q, full_q(s), 64, hq, tok, bq);
             }
             // no load is in flight when the CTA ends (its consumers may have given up)
-            for (uint32_t n = k.c > 2 ? k.c - 2 : 0; n < k.c; ++n) {
+            for (uint32_t n = c > 2 ? c - 2 : 0; n < c; ++n) {
                 wait_one(full_k(n & 1), (n >> 1) & 1, 0x404);
-                wait_one(full_q(n & 1), (n >> 1) & 1, 0x404);
+                if (!STATE) wait_one(full_q(n & 1), (n >> 1) & 1, 0x404);
                 wait_one(full_v(n & 1), (n >> 1) & 1, 0x404);
             }
         }
@@ -419,22 +454,21 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         // The whole warp walks the chunks and one lane issues: descriptors and loop
         // are then provably one value a warp and stay in uniform registers, where
         // an MMA wants them.
-        uint32_t total = 0;
-        for (uint32_t id = blockIdx.x; id < items; id += gridDim.x)
-            total += (uint32_t)ceil_div(item_of(a, tiles, id).len, C);
-        total = uniform(total);
         const uint64_t dq0 = smem_desc(base + OFF_Q), dk0 = smem_desc(base + OFF_K);
         const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
         const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
         constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
         const int steps = wide ? 8 : 4;                  // of 16 columns of q and k
         bool ok = true;
-        if (warp == W_MMA) {
+        if (STATE && warp == W_MMA) {
+        } else if (warp == W_MMA) {
             // iteration n: P V of chunk n - 1, Q K^T of chunk n
 #pragma unroll 1
-            for (uint32_t n = 0; n <= total && ok; ++n) {
+            for (uint32_t n = 0, more = 1; more && ok; ++n) {
                 const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
-                if (n < total)
+                ok = wait_warp(g_full(s), ph2, 0x410);
+                more = ok ? uniform(chunks[n & 3].m) : 0;
+                if (more)
                     ok = wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
                 if (n > 0) {
                     const uint32_t ph = (n - 1) & 1;
@@ -451,7 +485,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     }
                     __syncwarp();
                 }
-                if (n < total) {
+                if (more) {
                     const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE;
                     if (ok && elect_one()) {
 #pragma unroll 2
@@ -468,8 +502,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         } else {
             // K^T V~, then Q S0 of each chunk
 #pragma unroll 1
-            for (uint32_t n = 0; n < total && ok; ++n) {
+            for (uint32_t n = 0; ok; ++n) {
                 const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
+                ok = wait_warp(g_full(s), ph2, 0x410);
+                if (!ok || !uniform(chunks[n & 3].m)) break;
                 const uint64_t q = dq0 + s * STAGE, kt = kt0 + s * STAGE;
                 ok = wait_warp(vt_full, s, 0x413) && wait_warp(full_k(s), ph2, 0x414) &&
                      wait_warp(d_free, s ^ 1, 0x414);
@@ -487,6 +523,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     mma_commit(empty_k(s));
                 }
                 __syncwarp();
+                if (STATE) continue;
                 ok = ok && wait_warp(h_full, s, 0x415) && wait_warp(full_q(s), ph2, 0x412) &&
                      wait_warp(o_free, s ^ 1, 0x416);
                 fence_after();
@@ -510,36 +547,56 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     } else if (warp == W_G) {
         // ----------------------------------------------------------- decays
         // lane l: tokens 4 l .. 4 l + 3; lanes 8 b .. 8 b + 7 are block b
-        Walk k(a, tiles, items);
-        float gn[4];
-        if (k.valid()) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) gn[e] = load_g(a, k.it, k.t0 + 4 * lane + e);
-        }
+        Walk<STATE> k;
+        Chunk now = {};
+        float gnow[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        double span_g = 0.0;                             // of the span so far
+        bool more = true;
+        // iteration c: chunk c's loads, then the decays of chunk c - 1; the end is a
+        // chunk without tokens
 #pragma unroll 1
-        for (bool more = true; more;) {
-            const uint32_t c = k.c;
+        for (uint32_t n = 0;; ++n) {
+            const uint32_t c = n - 1;
             const int s = c & 1;
-            double g[4];
-            more = k.valid();
-            Chunk now = {};                              // behind the last one: m = 0
-#pragma unroll
-            for (int e = 0; e < 4; ++e) g[e] = more ? (double)clamp_g(gn[e]) : 0.0;
+            Chunk next = {};
+            float gn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (more)
+                more = k.next(a, tiles, items, [&] {
+                    // a span without tokens keeps its state
+                    if (STATE || k.it.out < 0) return;
+                    const int64_t per = a.heads * a.dk * a.dv, at = k.it.h * a.dk * a.dv;
+                    const float *const hin = (a.seg ? a.seg_state : a.h0) + k.it.in * per + at;
+                    float *const hout = a.h_last + k.it.out * per + at;
+#pragma unroll 1
+                    for (int i = lane; i < (int)a.dk * DV; i += 32) {
+                        const int col = k.it.tile * DV + i % DV;
+                        const int64_t e = (i / DV) * a.dv + col;
+                        if (col < a.dv) hout[e] = k.it.in >= 0 ? hin[e] : 0.0f;
+                    }
+                });
             if (more) {
-                const int64_t left = k.it.len - k.t0;
-                now.row = (int)(k.it.row0 + k.t0);
-                now.m = (int)(left < C ? left : C);
-                now.first = k.t0 == 0;
-                now.last = left <= C;
-                now.h = k.it.h;
-                now.seq = (int)k.it.seq;
-                now.tile = k.it.tile;
-                k.next();                                // the next chunk's loads
-                if (k.valid()) {
+                const int left = k.it.len - k.t0;
+                next.row = k.it.row0 + k.t0;
+                next.m = left < C ? left : C;
+                next.first = k.t0 == 0;
+                next.last = left <= C;
+                next.h = k.it.h;
+                next.batch = a.cu ? 0 : k.it.seq;
+                next.tile = k.it.tile;
+                next.in = k.it.in;
+                next.out = k.it.out;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) gn[e] = load_g(a, k.it, k.t0 + 4 * lane + e);
-                }
+                for (int e = 0; e < 4; ++e) gn[e] = load_g(a, k.it, k.t0 + 4 * lane + e);
             }
+            if (n == 0) {
+                now = next;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) gnow[e] = gn[e];
+                continue;
+            }
+            double g[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = (double)clamp_g(gnow[e]);
 #pragma unroll
             for (int e = 1; e < 4; ++e) g[e] += g[e - 1];
             double sum = g[3];                           // of the block's lanes up to this one
@@ -568,6 +625,11 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 gg[e] = (float)(x * 1.4426950408889634);
             }
             const float mine = exp_of(all);
+            if (STATE) {
+                span_g = now.first ? all : span_g + all;
+                if (lane == SC_ALL && now.last && now.tile == 0 && now.out >= 0)
+                    a.seg_g[(int64_t)now.out * a.heads + now.h] = span_g;
+            }
             if (!wait_warp(g_free(s), ((c >> 1) & 1) ^ 1, 0x451)) break;
             if (lane < 12) sc[s * 16 + lane] = mine;
             if (lane == SC_ALL) {
@@ -577,6 +639,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             *reinterpret_cast<float4 *>(colf + s * C + 4 * lane) = make_float4(cf[0], cf[1], cf[2], cf[3]);
             *reinterpret_cast<float4 *>(g2 + s * C + 4 * lane) = make_float4(gg[0], gg[1], gg[2], gg[3]);
             mbar_arrive(g_full(s));
+            if (now.m == 0) break;
+            now = next;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) gnow[e] = gn[e];
         }
     } else if (warp < W_P) {
         // -------------------------------------------------------- the state
@@ -594,7 +660,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             if (k.m == 0) break;
             const uint64_t dec2 = pair(dec[c & 3]);
             const int c0 = k.tile * DV;
-            const int64_t at = (((int64_t)k.seq * a.heads + k.h) * a.dk + r) * a.dv + c0;
+            const int64_t at = ((int64_t)k.h * a.dk + r) * a.dv + c0;
+            const int64_t per = a.heads * a.dk * a.dv;
+            const float *const hin = (!STATE && a.seg ? a.seg_state : a.h0) + k.in * per + at;
+            float *const hout = (STATE ? a.seg_state : a.h_last) + k.out * per + at;
             const bool row = r < a.dk;
 #pragma unroll 1
             for (int pass = k.first ? 0 : 1; pass < 2; ++pass) {
@@ -604,7 +673,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     fence_after();
                 }
                 // Q S0 of the chunk before the one this state is for
-                if (!store && !(ok = wait_warp(h_free, (c + pass + 1) & 1, 0x423))) break;
+                if (!STATE && !store && !(ok = wait_warp(h_free, (c + pass + 1) & 1, 0x423))) break;
 #pragma unroll 1
                 for (int i = 32 * half; i < 32 * half + 32; i += 16) {
                     uint32_t h[16];
@@ -612,8 +681,8 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             uint4 x = make_uint4(0, 0, 0, 0);
-                            if (a.h0 && row && c0 + i + j < a.dv)
-                                x = *reinterpret_cast<const uint4 *>(a.h0 + at + i + j);
+                            if (k.in >= 0 && row && c0 + i + j < a.dv)
+                                x = *reinterpret_cast<const uint4 *>(hin + i + j);
                             h[j] = x.x; h[j + 1] = x.y; h[j + 2] = x.z; h[j + 3] = x.w;
                         }
                     } else {
@@ -636,13 +705,13 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     if (store) {
 #pragma unroll
                         for (int j = 0; j < 16; j += 4)
-                            if (a.h_last && row && c0 + i + j < a.dv)
-                                *reinterpret_cast<uint4 *>(a.h_last + at + i + j) =
+                            if (k.out >= 0 && row && c0 + i + j < a.dv)
+                                *reinterpret_cast<uint4 *>(hout + i + j) =
                                     make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
                     } else {
                         tmem_st16(quarter + T_H + i, h);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
+                        for (int j = 0; !STATE && j < 2; ++j) {
                             uint4 x;
                             x.x = pack_bf16(pair(h[8 * j], h[8 * j + 1]));
                             x.y = pack_bf16(pair(h[8 * j + 2], h[8 * j + 3]));
@@ -655,9 +724,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (pass == 1) {
                     fence_before();
                     mbar_arrive(d_free);
+                    if (STATE) mbar_arrive(g_free(c & 1));   // V~ (c) has read them too
                 }
-                if (!store) {
-                    tmem_wait_st();
+                if (!store) tmem_wait_st();
+                if (!STATE && !store) {
                     fence_async_smem();
                     mbar_arrive(h_full);
                 }
@@ -677,7 +747,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             tmem_wait_st();
         }
         const uint64_t scale2 = pair(a.scale);
-        for (uint32_t c = 0;; ++c) {
+        for (uint32_t c = 0; !STATE; ++c) {
             const int s = c & 1;
             if (!wait_warp(g_full(s), (c >> 1) & 1, 0x431) || chunks[c & 3].m == 0) break;
             const float gr = g2[s * C + r];
@@ -779,12 +849,13 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             fence_async_smem();
             mbar_arrive(vt_full);
+            if (STATE) mbar_arrive(empty_v(s));
         }
     } else {
         // -------------------------------------------------- the output rows
         const int w = warp & 3, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
-        for (uint32_t c = 0;; ++c) {
+        for (uint32_t c = 0; !STATE; ++c) {
             const int s = c & 1;
             if (!wait_warp(g_full(s), (c >> 1) & 1, 0x446)) break;
             const Chunk k = chunks[c & 3];
@@ -792,7 +863,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             const uint64_t ei2 = pair(ex2(g2[s * C + r]) * sc[s * 16 + SC_BEFORE + w] * a.scale);
             const int c0 = k.tile * DV;
             __nv_bfloat16 *const row = static_cast<__nv_bfloat16 *>(a.o) +
-                                       (a.cu ? 0 : k.seq) * a.os[0] +
+                                       k.batch * a.os[0] +
                                        (int64_t)(k.row + r) * a.os[1] + k.h * a.os[2] + c0;
             if (!wait_warp(o_full, c & 1, 0x445)) break;
             mbar_arrive(g_free(s));                      // P (c) has read them too
@@ -829,7 +900,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (k.m == C) {
                     if (lane == 0) {
                         tma_store_4d(&map_o, base + OFF_Q + s * 2 * SUB + w * 32 * 128, k.tile * DV,
-                                     k.h, k.row + 32 * w, a.cu ? 0 : k.seq);
+                                     k.h, k.row + 32 * w, k.batch);
                         bulk_commit();
                         bulk_wait_read0();
                     }
@@ -871,18 +942,6 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     fence_before();
     __syncthreads();
     fence_after();
-    // items without tokens keep their state
-    for (uint32_t id = blockIdx.x; a.h_last && id < items; id += gridDim.x) {
-        const Item it = item_of(a, tiles, id);
-        if (it.len > 0) continue;
-        const int64_t at = (it.seq * a.heads + it.h) * a.dk * a.dv;
-#pragma unroll 1
-        for (int i = threadIdx.x; i < a.dk * DV; i += THREADS) {
-            const int col = it.tile * DV + i % DV;
-            const int64_t e = at + (i / DV) * a.dv + col;
-            if (col < a.dv) a.h_last[e] = a.h0 ? a.h0[e] : 0.0f;
-        }
-    }
     if (warp == W_MMA) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
@@ -934,7 +993,9 @@ static bool fits(const Args &a) {
            (!a.h0 || aligned(a.h0, 16)) && (!a.h_last || aligned(a.h_last, 16));
 }
 
-int chunked(const Args &a, cudaStream_t st, bool *used) {
+bool chunked_fits(const Args &a) { return fits(a); }
+
+int chunked(const Args &a, bool state_only, cudaStream_t st, bool *used) {
     *used = false;
     if (!fits(a)) return MB2_OK;
     MB2_TRY(get_encode());
@@ -947,18 +1008,16 @@ int chunked(const Args &a, cudaStream_t st, bool *used) {
     MB2_TRY(token_map(&mo, a.o, a.os, batch, a.seqlen, a.heads, a.dv, 32, &ok[3]));
     if (!ok[0] || !ok[1] || !ok[2] || !ok[3]) return MB2_OK;
     *used = true;
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decay_chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)SMEM_BYTES);
+    const int sms = num_sms();
+    auto kern = state_only ? decay_chunk_kernel<true> : decay_chunk_kernel<false>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)SMEM_BYTES);
     if (e != cudaSuccess) return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
     const int tiles = (int)ceil_div(a.dv, DV);
-    const int64_t items = (int64_t)tiles * a.heads * a.seqs;
+    const int64_t items = (int64_t)tiles * a.heads * spans(a);
     MB2_REQUIRE(items < (1ll << 31), MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
     const unsigned grid = (unsigned)(items < sms ? items : sms);
-    decay_chunk_kernel<<<grid, THREADS, SMEM_BYTES, st>>>(mq, mk, mv, mo, a, tiles, (uint32_t)items);
+    kern<<<grid, THREADS, SMEM_BYTES, st>>>(mq, mk, mv, mo, a, (uint32_t)tiles, (uint32_t)items);
     return check_launch("decay_chunk_kernel");
 }
 

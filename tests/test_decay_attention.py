@@ -169,6 +169,60 @@ def test_packed_sequences(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 3000, 1, 1, 1, 1, 64, 64), (2, 1537, 2, 1, 1, 2, 32, 40),
+                                   (1, 2049, 1, 1, 1, 1, 128, 128)])
+def test_few_heads_run_in_segments(shape, dtype):
+    """Long prompts of few heads are cut along their tokens."""
+    B, T, H, _, _, _, dk, dv = shape
+    q, k, v, g, h0 = make(*shape, dtype, seed=T)
+    g *= 0.05
+    ref = reference(spread(q, H), spread(k, H), v, g, 1.0, h0)
+    args = [t.cuda() for t in (q, k, v, g)]
+    start = h0.cuda()
+    o, s = ops.decay_attention(*args, initial_state=start, return_final_state=True)
+    check(o, s, ref, dtype, T, dk)
+    # its workspace is its own call's: two captured calls replayed in turn
+    graphs = []
+    for scale in (1.0, 2.0):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            graphs.append((gr, ops.decay_attention(*args, scale=scale, initial_state=start)))
+    for gr, _ in graphs * 2:
+        gr.replay()
+    assert torch.equal(graphs[0][1], o)
+    ref2 = tuple(2 * t if i in (0, 2) else t for i, t in enumerate(ref))
+    check(graphs[1][1], None, ref2, dtype, T, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_packed_segments(dtype):
+    """Ragged packed sequences long enough to be cut; an empty one keeps its
+    state; overlapping offsets stay inside the tensors and the workspace."""
+    lens = [1300, 0, 2, 2300, 129]
+    H, dk, dv, T = 1, 64, 64, 3731 + 5
+    q, k, v, g, _ = make(1, T, H, 1, 1, 1, dk, dv, dtype, seed=21)
+    g *= 0.1
+    h0 = torch.randn(len(lens), H, dk, dv, generator=torch.Generator().manual_seed(2))
+    cu = torch.tensor([0] + lens).cumsum(0)
+    args = [t.cuda() for t in (q, k, v, g)]
+    o, s = ops.decay_attention(*args, initial_state=h0.cuda(), cu_seqlens=cu.cuda(),
+                               return_final_state=True)
+    assert bool((o[:, T - 5:] == 0).all())
+    for i, n in enumerate(lens):
+        a, b = int(cu[i]), int(cu[i + 1])
+        if n == 0:
+            assert torch.equal(s[i].cpu(), h0[i])
+            continue
+        ref = reference(q[:, a:b], k[:, a:b], v[:, a:b], g[:, a:b], 1.0, h0[i:i + 1])
+        check(o[:, a:b], s[i:i + 1], ref, dtype, n, dk)
+    bad = torch.tensor([0, T, 0, T, 0, T], device="cuda")
+    ops.decay_attention(*args, initial_state=h0.cuda(), cu_seqlens=bad, return_final_state=True)
+    torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_and_column_slices(dtype):
     """q, k, v as slices of one projection's rows, and transposed (heads before
     tokens) inputs, give the bits of contiguous ones."""
