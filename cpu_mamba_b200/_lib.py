@@ -147,10 +147,11 @@ _SIGS = {
                                           _vp]),
     "mb2_peer_status": (ctypes.c_int, [ctypes.POINTER(PeerGroup), ctypes.POINTER(ctypes.c_int),
                                        ctypes.c_int]),
-    "mb2_decay_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecayAttn)]),
-    "mb2_decay_attention": (ctypes.c_int, [ctypes.POINTER(DecayAttn), _vp, ctypes.c_size_t, _vp]),
-    "mb2_decay_attention_step": (ctypes.c_int, [ctypes.POINTER(DecayAttn), _vp, _vp]),
-    "mb2_gated_norm": (ctypes.c_int, [ctypes.POINTER(GatedNorm), _vp]),
+    # (descriptors of the calls below as packed bytes or ctypes structures)
+    "mb2_decay_attention_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "mb2_decay_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "mb2_decay_attention_step": (ctypes.c_int, [_vp, _vp, _vp]),
+    "mb2_gated_norm": (ctypes.c_int, [_vp, _vp]),
     "mb2_beam_select_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] + [_c_i64] * 4),
     "mb2_beam_select": (ctypes.c_int, [ctypes.c_int, _vp, _c_i64, _c_i64, _vp, _vp] + [_c_i64] * 5 +
                         [_vp] * 4 + [ctypes.c_size_t, _vp]),

@@ -44,13 +44,36 @@ struct RowArgs {
     uint64_t *part_list;                      // (rows, splits, num): key << 32 | ~token, 0: none
 };
 
+// a vector of logits: the values of its 32-bit words
+template <typename T> struct Word;
+template <> struct Word<float> {
+    static constexpr int N = 1;
+    static __device__ __forceinline__ float at(uint32_t w, int) { return __uint_as_float(w); }
+    static __device__ __forceinline__ uint32_t masked(uint32_t w, int, bool in) {
+        return in ? w : 0xff800000u;
+    }
+};
+template <> struct Word<__nv_bfloat16> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ float at(uint32_t w, int i) {
+        return __uint_as_float(i ? w & 0xffff0000u : w << 16);
+    }
+    static __device__ __forceinline__ uint32_t masked(uint32_t w, int i, bool in) {
+        return in ? w : i ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
+    }
+};
+
+// The slice is kept as it was loaded (16 or 32 registers a thread).  Measured at 512
+// rows of 50257 bf16 logits: TODO us.
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 4 : 3)
 beam_rows_kernel(const RowArgs a) {
-    constexpr int VEC = 16 / (int)sizeof(T), NV = EPT / VEC;
+    constexpr int VEC = 16 / (int)sizeof(T), NV = EPT / VEC, WARPS = ROW_THREADS / 32;
+    constexpr int WN = Word<T>::N;                // values per 32-bit word
     __shared__ uint64_t list[LIST];
-    __shared__ uint64_t best[ROW_THREADS / 32];
-    __shared__ float redf[2][ROW_THREADS / 32];
+    __shared__ uint64_t best[WARPS];
+    __shared__ float redf[2][WARPS];
+    __shared__ uint32_t reach_key[WARPS];
     __shared__ int count;
     const int split = blockIdx.x, row = blockIdx.y;
     if (a.finished && a.finished[row]) return;              // beam_merge writes its candidates
@@ -65,74 +88,111 @@ beam_rows_kernel(const RowArgs a) {
     const int v0 = split * (ROW_THREADS * NV) + tid;
     if (tid == 0) count = 0;
 
-    uint32_t key[EPT];
-    float tmax = -INFINITY;
-    uint32_t kmax = 0;
+    constexpr uint32_t kNone = Word<T>::N == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
+    uint32_t raw[NV][4];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int v = v0 + j * ROW_THREADS;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (v < nvec) raw = __ldcs(reinterpret_cast<const uint4 *>(base) + v);
-        const T *e = reinterpret_cast<const T *>(&raw);
+        uint4 x = make_uint4(kNone, kNone, kNone, kNone);
+        if (v < nvec) x = __ldcs(reinterpret_cast<const uint4 *>(base) + v);
+        raw[j][0] = x.x; raw[j][1] = x.y; raw[j][2] = x.z; raw[j][3] = x.w;
+    }
+    // token of value (j, w, i)
+    auto token = [&](int j, int w, int i) {
+        return (v0 + j * ROW_THREADS) * VEC + w * WN + i - lead;
+    };
+    float tmax = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int tok = v * VEC + i - lead;
-            const bool in = tok >= 0 && tok < a.vocab;
-            const float x = io<T>::to_f(e[i]);
-            // kept as the value; what is not a logit gets key 0 below
-            key[j * VEC + i] = in ? __float_as_uint(x) : 0xffffffffu;   // a NaN pattern
-            if (in) tmax = fmaxf(tmax, x);
+    for (int j = 0; j < NV; ++j) {
+        const int v = v0 + j * ROW_THREADS;
+        if (v == 0 || v == nvec - 1) {                       // the row's first and last 16 bytes
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int i = 0; i < WN; ++i) {
+                    const int t = token(j, w, i);
+                    raw[j][w] = Word<T>::masked(raw[j][w], i, t >= 0 && t < a.vocab);
+                }
         }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int i = 0; i < WN; ++i) tmax = fmaxf(tmax, Word<T>::at(raw[j][w], i));
     }
     float m = tmax;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) redf[0][wid] = m;
+
+    // A threshold that at least `num` threads reach by their largest value, so that
+    // the slice's best `num` are among the values at or above it: the least of the
+    // warps' ceil(num / 8)-th largest thread maxima.
+    const int quota = (a.num + WARPS - 1) / WARPS;
+    const uint32_t kmax = v0 < nvec ? order_key(tmax) : 0u;
+    {
+        uint32_t left = kmax, got = 0;
+        for (int r = 0; r < quota; ++r) {
+            got = __reduce_max_sync(0xffffffffu, left);
+            const uint32_t who = __ballot_sync(0xffffffffu, left == got);
+            if (lane == __ffs(who) - 1) left = 0;
+        }
+        if (lane == 0) reach_key[wid] = got;                 // 0: fewer threads than that
+    }
     __syncthreads();
-    m = redf[0][0];
+    uint32_t thr = 0xffffffffu;
+    int full = 0;
 #pragma unroll
-    for (int w = 1; w < ROW_THREADS / 32; ++w) m = fmaxf(m, redf[0][w]);
+    for (int w = 0; w < WARPS; ++w) {
+        m = fmaxf(m, redf[0][w]);
+        const uint32_t k = reach_key[w];
+        if (k) {
+            ++full;
+            thr = k < thr ? k : thr;
+        }
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int tok = (v0 + j * ROW_THREADS) * VEC + i - lead;
-            const bool in = tok >= 0 && tok < a.vocab;
-            const float x = __uint_as_float(key[j * VEC + i]);
-            // all masked: no term; a NaN or +inf makes the sum NaN
-            if (in) sum += x == -INFINITY ? 0.0f : __expf(x - m);
-            const uint32_t k = in ? order_key(x) : 0u;
-            key[j * VEC + i] = k;
-            kmax = k > kmax ? k : kmax;
-        }
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int i = 0; i < WN; ++i) {
+                // a NaN or +inf makes the sum NaN
+                const float x = Word<T>::at(raw[j][w], i);
+                sum += x == -INFINITY ? 0.0f : ex2((x - m) * kLog2e);
+            }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) redf[1][wid] = sum;
 
-    // A threshold that at least `num` threads reach (each by its largest key),
-    // so that the slice's best `num` are among the keys at or above it: bisection
-    // of the key's bits, stopped once few more threads than needed reach it.
-    uint32_t thr = 1;
-    const int reach = __syncthreads_count(kmax > 0);
-    if (reach > a.num) {
-        thr = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t t = thr | (1u << bit);
-            const int c = __syncthreads_count(kmax >= t);
-            if (c >= a.num) thr = t;
-            if (c >= a.num && c <= a.num + 8) break;
+    if (full * quota < a.num) {
+        // a row's last, short slice: bisection of the key's bits, stopped once few
+        // more threads than needed reach it
+        thr = 1;
+        const int reach = __syncthreads_count(kmax > 0);
+        if (reach > a.num) {
+            thr = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t t = thr | (1u << bit);
+                const int c = __syncthreads_count(kmax >= t);
+                if (c >= a.num) thr = t;
+                if (c >= a.num && c <= a.num + 8) break;
+            }
         }
     }
     if (kmax >= thr) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (key[j * VEC + i] >= thr) {
-                    const int at = atomicAdd(&count, 1);
-                    const uint32_t tok = (uint32_t)((v0 + j * ROW_THREADS) * VEC + i - lead);
-                    if (at < LIST) list[at] = (uint64_t)key[j * VEC + i] << 32 | (uint32_t)~tok;
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int i = 0; i < WN; ++i) {
+                    const uint32_t k = order_key(Word<T>::at(raw[j][w], i));
+                    const int t = token(j, w, i);
+                    if (k >= thr && t >= 0 && t < a.vocab) {
+                        const int at = atomicAdd(&count, 1);
+                        if (at < LIST) list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)t;
+                    }
                 }
     }
     __syncthreads();
@@ -163,11 +223,14 @@ beam_rows_kernel(const RowArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const uint32_t tok = (uint32_t)((v0 + j * ROW_THREADS) * VEC + i - lead);
-                const uint64_t e = (uint64_t)key[j * VEC + i] << 32 | (uint32_t)~tok;
-                if (key[j * VEC + i] && e < last && e > b) b = e;
-            }
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int i = 0; i < WN; ++i) {
+                    const int t = token(j, w, i);
+                    const uint64_t e = (uint64_t)order_key(Word<T>::at(raw[j][w], i)) << 32 |
+                                       (uint32_t)~(uint32_t)t;
+                    if (t >= 0 && t < a.vocab && e < last && e > b) b = e;
+                }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const uint64_t x = __shfl_xor_sync(0xffffffffu, b, o);
@@ -191,7 +254,9 @@ struct MergeArgs {
     const uint64_t *part_list;
     float *out_scores;
     int64_t *out_parents, *out_tokens;
+    int staged;                               // the lists' entries fit shared memory
 };
+struct Entry { double val; int64_t at; };     // at: flat index, -1: none
 
 // better: the larger value, then the lower flat index (NaN never reaches here)
 __device__ __forceinline__ bool better(double v, int64_t at, double v2, int64_t at2) {
@@ -200,7 +265,11 @@ __device__ __forceinline__ bool better(double v, int64_t at, double v2, int64_t 
 
 __global__ void __launch_bounds__(1024)
 beam_merge_kernel(const MergeArgs a) {
-    extern __shared__ int heads[];            // per list: entries taken
+    extern __shared__ __align__(16) uint8_t dyn[];
+    const int lists = a.beams * a.splits;
+    Entry *const stage = reinterpret_cast<Entry *>(dyn);     // [lists][num] when staged
+    int *const heads = reinterpret_cast<int *>(dyn + (a.staged ? sizeof(Entry) * lists * a.num : 0));
+    // heads: per list, entries taken
     // a beam's score, largest logit and log sum of exp(logit - largest): a large
     // common offset of the logits must cancel before the other terms join
     __shared__ double s_score[MAX_BEAMS], s_max[MAX_BEAMS], s_logsum[MAX_BEAMS];
@@ -209,7 +278,7 @@ beam_merge_kernel(const MergeArgs a) {
     __shared__ int64_t w_at[2][32];
     __shared__ int w_list[2][32];
     const int batch = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const int warps = blockDim.x >> 5, lists = a.beams * a.splits;
+    const int warps = blockDim.x >> 5;
 
     for (int l = tid; l < lists; l += blockDim.x) heads[l] = 0;
     for (int k = wid; k < a.beams; k += warps) {
@@ -263,6 +332,15 @@ beam_merge_kernel(const MergeArgs a) {
         at = flat + (uint32_t)~(uint32_t)e;
         return true;
     };
+    // all entries at once, so that the rounds below wait for no global load
+    if (a.staged) {
+        for (int i = tid; i < lists * a.num; i += blockDim.x) {
+            Entry e;
+            if (!entry(i / a.num, i % a.num, e.val, e.at)) e.at = -1;
+            stage[i] = e;
+        }
+        __syncthreads();
+    }
     // this thread's best head over its lists
     double val;
     int64_t at;
@@ -274,7 +352,17 @@ beam_merge_kernel(const MergeArgs a) {
         for (int l = tid; l < lists; l += blockDim.x) {
             double v;
             int64_t p;
-            if (entry(l, heads[l], v, p) && (which < 0 || better(v, p, val, at))) {
+            const int h = heads[l];
+            bool has;
+            if (a.staged) {
+                const Entry e = stage[l * a.num + (h < a.num ? h : 0)];
+                has = h < a.num && e.at >= 0;
+                v = e.val;
+                p = e.at;
+            } else {
+                has = entry(l, h, v, p);
+            }
+            if (has && (which < 0 || better(v, p, val, at))) {
                 val = v;
                 at = p;
                 which = l;
@@ -431,7 +519,9 @@ extern "C" int mb2_beam_select(int dtype, const void *logits, int64_t batch_stri
     g.out_scores = out_scores; g.out_parents = out_parents; g.out_tokens = out_tokens;
     const int lists = (int)beams * splits;
     const int threads = (int)(round_up(lists, 32) < 1024 ? round_up(lists, 32) : 1024);
-    beam_merge_kernel<<<(unsigned)batch, threads, sizeof(int) * lists, st>>>(g);
+    const size_t staged = (sizeof(Entry) * (size_t)num + sizeof(int)) * lists;
+    g.staged = staged <= 48 * 1024;
+    beam_merge_kernel<<<(unsigned)batch, threads, g.staged ? staged : sizeof(int) * lists, st>>>(g);
     return check_launch("beam_merge_kernel");
 }
 

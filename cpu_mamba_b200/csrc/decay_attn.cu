@@ -308,6 +308,10 @@ static int recurrent(const Args &a, bool state_only, cudaStream_t st) {
                       : recurrent_of<__nv_bfloat16, false>(a, st);
 }
 
+template <int VEC> struct vecf;
+template <> struct vecf<4> { using t = float4; };
+template <> struct vecf<1> { using t = float; };
+
 // --------------------------------------------------------------- segments
 // slot0[i]: the first slot of packed sequence i (one warp, a running sum)
 __global__ void slots_kernel(const Args a, int32_t *slot0) {
@@ -336,31 +340,41 @@ __global__ void slots_kernel(const Args a, int32_t *slot0) {
 // The segments' states, each from 0, become their initial states, element by
 // element: S_{j+1} = e^{G_j} S_j + own_j, S_0 = h0.  A sequence's last slot takes
 // its initial state without having held one.
-__global__ void __launch_bounds__(256) seg_states_kernel(const Args a) {
+template <int VEC>
+__global__ void __launch_bounds__(128) seg_states_kernel(const Args a) {
+    using V = typename vecf<VEC>::t;
     const int64_t per = a.dk * a.dv;
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t e = ((int64_t)blockIdx.x * 128 + threadIdx.x) * VEC;
     const int64_t seq = blockIdx.z, h = blockIdx.y;
     if (e >= per) return;
     const int64_t n = a.cu ? a.slot0[seq + 1] - a.slot0[seq] : segments(a.seqlen, a.seg);
     const int64_t first = a.cu ? a.slot0[seq] : seq * n;
+    const int64_t step = a.heads * per;
     float *s = a.seg_state + (first * a.heads + h) * per + e;
     const double *g = a.seg_g + first * a.heads + h;
-    float run = a.h0 ? a.h0[(seq * a.heads + h) * per + e] : 0.0f;
+    V run = {};
+    if (a.h0) run = *reinterpret_cast<const V *>(a.h0 + (seq * a.heads + h) * per + e);
     // the chain is short; the loads of eight segments run ahead of it
     for (int64_t j0 = 0; j0 < n; j0 += 8) {
-        float own[8];
-        double lg[8];
+        V own[8];
+        float dec[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool in = j0 + i + 1 < n;
-            own[i] = in ? s[(j0 + i) * a.heads * per] : 0.0f;
-            lg[i] = in ? g[(j0 + i) * a.heads] : 0.0;
+            own[i] = V{};
+            dec[i] = 0.0f;
+            if (j0 + i + 1 < n) {
+                own[i] = *reinterpret_cast<const V *>(s + (j0 + i) * step);
+                dec[i] = expf((float)g[(j0 + i) * a.heads]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (j0 + i < n) {
-                s[(j0 + i) * a.heads * per] = run;
-                run = fmaf(expf((float)lg[i]), run, own[i]);
+                *reinterpret_cast<V *>(s + (j0 + i) * step) = run;
+                float *r = reinterpret_cast<float *>(&run);
+                const float *o = reinterpret_cast<const float *>(&own[i]);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) r[v] = fmaf(dec[i], r[v], o[v]);
             }
     }
 }
@@ -369,24 +383,24 @@ __global__ void __launch_bounds__(256) seg_states_kernel(const Args a) {
 // tokens one after the other, and `lanes` walks run at a time: with fewer sequences
 // x heads x column tiles than that (or an uneven last round of them) segments
 // shorten the longest chain, at the price of a first pass that costs `first` of the
-// second's time a step, a step or so to fill each walk, and the states' traffic.
+// second's time a step, two steps to fill each walk, and the states' traffic.
 // Measured, one sequence of 8192 tokens, 24 heads of 128 x 64 in bf16: 134 us whole,
 // 95 in segments (27 first pass, 42 second).
 static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64_t unit,
                               double first) {
     if (a.seqs == 0 || a.seqlen == 0) return 0;
-    // packed: the lengths are not known here; the longest sequence is taken as
-    // twice the mean
+    // packed: the lengths are not known here; the longest sequence is taken as one
+    // and a half times the mean
     const int64_t units = ceil_div(a.cu ? ceil_div(a.seqlen, a.seqs) : a.seqlen, unit);
     const double even = (double)walks * (double)units / (double)lanes;
     const double whole = !a.cu ? (double)ceil_div(walks, lanes) * (double)units
-                               : (even > 2.0 * units ? even : 2.0 * units);
+                               : (even > 1.5 * units ? even : 1.5 * units);
     double best = whole * 0.9;            // segments have to save a tenth
     int64_t seg = 0;
-    for (int64_t n = 2; n <= 256 && n * 4 <= 2 * units; ++n) {
+    for (int64_t n = 2; n <= 256 && n * 2 <= units; ++n) {
         const int64_t per = ceil_div(units, n);
-        const double t = (double)ceil_div(walks * n, lanes) * (per + 1.0) +
-                         (double)ceil_div(walks * (n - 1), lanes) * (first * per + 1.0) +
+        const double t = (double)ceil_div(walks * n, lanes) * (per + 2.2) +
+                         (double)ceil_div(walks * (n - 1), lanes) * (first * per + 2.2) +
                          0.1 * n + 4.0;
         if (t < best) {
             best = t;
@@ -436,10 +450,6 @@ __global__ void zero_tail_kernel(const Args a) {
 // through the Dk rows with ROWS rows' loads in flight per thread.  Partial
 // sums of o over the row slots meet in shared memory, added in a fixed order.
 constexpr int STEP_THREADS = 256;
-template <int VEC> struct vecf;
-template <> struct vecf<4> { using t = float4; };
-template <> struct vecf<1> { using t = float; };
-
 template <typename T, int VEC>
 __global__ void __launch_bounds__(STEP_THREADS)
 decay_step_kernel(const Args a, float *__restrict__ state, int lanes) {
@@ -640,9 +650,11 @@ extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, siz
         }
         MB2_TRY(decay::chunked(a, true, st, &used));
         if (!used) MB2_TRY(decay::recurrent(a, true, st));
-        const dim3 grid((unsigned)ceil_div(a.dk * a.dv, (int64_t)256), (unsigned)a.heads,
-                        (unsigned)a.seqs);
-        decay::seg_states_kernel<<<grid, 256, 0, st>>>(a);
+        const bool vec = a.dk * a.dv % 4 == 0 && (!a.h0 || aligned(a.h0, 16));
+        const dim3 grid((unsigned)ceil_div(a.dk * a.dv, (int64_t)(vec ? 512 : 128)),
+                        (unsigned)a.heads, (unsigned)a.seqs);
+        if (vec) decay::seg_states_kernel<4><<<grid, 128, 0, st>>>(a);
+        else decay::seg_states_kernel<1><<<grid, 128, 0, st>>>(a);
         MB2_TRY(check_launch("seg_states_kernel"));
     }
     MB2_TRY(decay::chunked(a, false, st, &used));

@@ -155,6 +155,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
           "r"(b)
         : "memory");
 }
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap *map, int32_t x, int32_t head,
+                                                int32_t tok, int32_t b) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(b)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t src, int32_t x,
                                              int32_t head, int32_t tok, int32_t b) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
@@ -587,6 +593,14 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 next.out = k.it.out;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) gn[e] = load_g(a, k.it, k.t0 + 4 * lane + e);
+                // its tiles into L2, before their stages are free
+                if (lane < (wide ? 2 : 1)) {
+                    const int x = 64 * lane;
+                    tma_prefetch_4d(&map_k, x, k.it.h / a.k_rep, next.row, next.batch);
+                    if (!STATE) tma_prefetch_4d(&map_q, x, k.it.h / a.q_rep, next.row, next.batch);
+                    if (lane == 0)
+                        tma_prefetch_4d(&map_v, next.tile * DV, next.h / a.v_rep, next.row, next.batch);
+                }
             }
             if (n == 0) {
                 now = next;

@@ -8,13 +8,13 @@ stages of the block for tests and for callers composing their own pipeline.
 from __future__ import annotations
 
 import contextlib
-import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import DecayAttn, GatedNorm, check, dtype_code, lib, ptr, require_cuda, stream_of
+from ._lib import check, dtype_code, lib, ptr, require_cuda, stream_of
 
 
 def selective_scan(x, dt, A, B, C, D, h0: Optional[torch.Tensor] = None,
@@ -266,19 +266,29 @@ def qlinear(x: torch.Tensor, scheme: str, weight_q: torch.Tensor, scale: torch.T
     return y.reshape(*lead, N)
 
 
-# ------------------------------------------------------------ decay attention
-def _one_device(what: str, first: torch.Tensor, *others) -> None:
-    require_cuda(first, *others, what=what)
+# The operators below are called once per token or per layer, where the host's time
+# per call counts: their descriptors are packed in one go (the C structures of
+# mamba_b200.h, no padding but at the end) and device and stream are plain integers.
+def _device_of(what: str, first: torch.Tensor, *others) -> int:
+    i = first.get_device()
+    if i < 0:
+        require_cuda(first, what=what)
     for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.get_device() != i:
+            require_cuda(t, what=what)
+            raise RuntimeError(f"{what}: tensors on cuda:{i} and {t.device}")
+    return i
 
 
-def _on(t: torch.Tensor):
-    """The device of ``t`` as the current one for a launch."""
-    if t.device.index == torch.cuda.current_device():
+def _on(index: int):
+    """Device ``index`` as the current one for a launch."""
+    if index == torch._C._cuda_getDevice():
         return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return torch.cuda.device(index)
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -286,47 +296,53 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool) -> DecayAttn:
+def _addr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------ decay attention
+_DECAY = struct.Struct("=2i8q5Q15q3Qqf4x")
+
+
+def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool, state_in=0, state_out=0, cu=0,
+                      seqs=0, zero_tail=0) -> bytes:
     """Argument checks shared by the prompt and the one-token form, and the
-    descriptor.  ``tokens``: q, k, v and o carry a token index after the batch."""
+    descriptor (mb2_decay_attn).  ``tokens``: q, k, v and o carry a token index
+    after the batch."""
     lead = 2 if tokens else 1
+    qs, ks, vs, gs, os = q.shape, k.shape, v.shape, g.shape, o.shape
     names = "(batch, tokens, heads, width)" if tokens else "(batch, heads, width)"
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != lead + 2:
-            raise RuntimeError(f"{what}: {n} must be {names}, got {tuple(t.shape)}")
-        if t.dtype != v.dtype:
-            raise RuntimeError(f"{what}: q, k and v must share a dtype")
-    d = DecayAttn()
-    d.dtype = dtype_code(v.dtype)
+    if not len(qs) == len(ks) == len(vs) == lead + 2:
+        raise RuntimeError(f"{what}: q, k and v must be {names}, got {tuple(qs)}, {tuple(ks)}, "
+                           f"{tuple(vs)}")
+    dtype = v.dtype
+    if q.dtype != dtype or k.dtype != dtype:
+        raise RuntimeError(f"{what}: q, k and v must share a dtype")
+    code = dtype_code(dtype)
     if g.dtype != torch.float32:
         raise RuntimeError(f"{what}: g must be float32")
-    if q.shape[:lead] != v.shape[:lead] or k.shape[:lead] != v.shape[:lead] or (
-            q.shape[-1] != k.shape[-1]):
-        raise RuntimeError(f"{what}: shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, "
-                           f"v {tuple(v.shape)}")
-    H = g.shape[-1] if g.dim() else 0
-    if g.dim() != 1 and g.shape != v.shape[:lead] + (H,):
-        raise RuntimeError(f"{what}: g must be (heads,) or {names[:-8]}), got {tuple(g.shape)}")
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.shape[-2] == 0 or t.shape[-1] == 0 or H == 0 or H % t.shape[-2]:
-            raise RuntimeError(f"{what}: the {t.shape[-2]} heads of {n} (width {t.shape[-1]}) "
-                               f"must divide the {H} decays of g")
-    d.batch, d.seqlen = v.shape[0], v.shape[1] if tokens else 1
-    d.heads, d.q_heads, d.k_heads, d.v_heads = H, q.shape[-2], k.shape[-2], v.shape[-2]
-    d.dk, d.dv = q.shape[-1], v.shape[-1]
-    if o.shape != v.shape[:lead] + (H, d.dv) or o.dtype != v.dtype or (
-            o.stride(-1) != 1 and o.shape[-1] > 1):
-        raise RuntimeError(f"{what}: out must be {tuple(v.shape[:lead]) + (H, d.dv)} in "
-                           f"{v.dtype} with its last index contiguous")
-    for n, t in (("q", q), ("k", k), ("v", v), ("o", o)):
-        s = t.stride()
-        setattr(d, n, t.data_ptr())
-        setattr(d, n + "_stride", (s[0], s[1] if tokens else 0, s[-2]))
-    d.g = g.data_ptr()
-    s = g.stride()
-    d.g_stride = (0, 0, s[0]) if g.dim() == 1 else (s[0], s[1] if tokens else 0, s[-1])
-    d.scale = scale
-    return d
+    batch, dk, dv, H = vs[0], qs[-1], vs[-1], gs[-1]
+    if qs[:lead] != vs[:lead] or ks[:lead] != vs[:lead] or dk != ks[-1]:
+        raise RuntimeError(f"{what}: shape mismatch: q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)}")
+    if len(gs) != 1 and gs[:-1] != vs[:lead]:
+        raise RuntimeError(f"{what}: g must be (heads,) or {names[:-8]}), got {tuple(gs)}")
+    hq, hk, hv = qs[-2], ks[-2], vs[-2]
+    if not (H and hq and hk and hv and dk and dv) or H % hq or H % hk or H % hv:
+        raise RuntimeError(f"{what}: the heads of q, k and v ({hq}, {hk}, {hv}; widths {dk}, {dv}) "
+                           f"must divide the {H} decays of g")
+    if os != vs[:lead] + (H, dv) or o.dtype != dtype or (dv > 1 and o.stride(-1) != 1):
+        raise RuntimeError(f"{what}: out must be {tuple(vs[:lead]) + (H, dv)} in {dtype} with its "
+                           "last index contiguous")
+    qt, kt, vt, ot, gt = q.stride(), k.stride(), v.stride(), o.stride(), g.stride()
+    if tokens:
+        strides = (qt[0], qt[1], qt[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2],
+                   *((0, 0, gt[0]) if len(gt) == 1 else gt), ot[0], ot[1], ot[2])
+    else:
+        strides = (qt[0], 0, qt[1], kt[0], 0, kt[1], vt[0], 0, vt[1],
+                   *((0, 0, gt[0]) if len(gt) == 1 else (gt[0], 0, gt[1])), ot[0], 0, ot[1])
+    return _DECAY.pack(code, zero_tail, batch, vs[1] if tokens else 1, H, hq, hk, hv, dk, dv,
+                       q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), o.data_ptr(),
+                       *strides, state_in, state_out, cu, seqs, scale)
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
@@ -339,49 +355,49 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
 
     q: (B, T, Hq, Dk), k: (B, T, Hk, Dk), v: (B, T, Hv, Dv), float32 or bfloat16
     (any strides with a contiguous last index); g: float32 log decays (B, T, H)
-    or (H,); Hq, Hk and Hv divide H, and head h reads q head h // (H // Hq).
-    Dk <= 256.  initial_state: float32 (N, H, Dk, Dv), zeros when None.
+    or (H,), at most 0 (-inf forgets the state); Hq, Hk and Hv divide H, and head
+    h reads q head h // (H // Hq).  Dk <= 256.  initial_state: float32
+    (N, H, Dk, Dv), zeros when None.
 
     cu_seqlens (int, N + 1 offsets on the device) packs N sequences along T with
     B = 1; rows behind the last one are zero in a new output and untouched in
-    ``out``.  Otherwise N = B.
+    ``out``, which must not overlap the inputs.  Otherwise N = B.
 
     Returns o (B, T, H, Dv), with the final state (N, H, Dk, Dv) float32 when
-    ``return_final_state``.  An empty sequence's final state is its initial one;
-    g = -inf forgets the state.  Forward only."""
+    ``return_final_state``.  An empty sequence's final state is its initial one.
+    Forward only."""
     what = "decay_attention"
-    _one_device(what, q, k, v, g, initial_state, cu_seqlens, out)
+    dev = _device_of(what, q, k, v, g, initial_state, cu_seqlens, out)
+    if v.dim() != 4 or q.dim() != 4 or k.dim() != 4 or g.dim() not in (1, 3):
+        raise RuntimeError(f"{what}: q, k and v must be (batch, tokens, heads, width) and g "
+                           f"(heads,) or (batch, tokens, heads), got {tuple(q.shape)}, "
+                           f"{tuple(k.shape)}, {tuple(v.shape)} and {tuple(g.shape)}")
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if v.dim() != 4 or g.dim() not in (1, 3):
-        raise RuntimeError(f"{what}: v must be (batch, tokens, heads, width) and g (heads,) or "
-                           f"(batch, tokens, heads), got {tuple(v.shape)} and {tuple(g.shape)}")
-    H = g.shape[-1]
-    o = out if out is not None else torch.empty(*v.shape[:2], H, v.shape[3], device=v.device,
-                                                dtype=v.dtype)
-    d = _decay_descriptor(what, q, k, v, g, scale, o, True)
-    n = d.batch
+    B, T, _, dv = v.shape
+    H, dk = g.shape[-1], q.shape[-1]
+    n, cu = B, 0
     if cu_seqlens is not None:
-        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or d.batch != 1 or (
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or B != 1 or (
                 cu_seqlens.dtype not in (torch.int32, torch.int64)):
             raise RuntimeError(f"{what}: cu_seqlens must hold N + 1 integer offsets into a "
                                "batch of 1")
         cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
-        n = cu_seqlens.shape[0] - 1
-        d.cu_seqlens, d.n_seqs, d.zero_tail = cu_seqlens.data_ptr(), n, int(out is None)
-    shape = (n, H, d.dk, d.dv)
+        n, cu = cu_seqlens.shape[0] - 1, cu_seqlens.data_ptr()
     if initial_state is not None:
-        if initial_state.shape != shape or initial_state.dtype != torch.float32:
-            raise RuntimeError(f"{what}: initial_state must be float32 {shape}")
+        if initial_state.shape != (n, H, dk, dv) or initial_state.dtype != torch.float32:
+            raise RuntimeError(f"{what}: initial_state must be float32 {(n, H, dk, dv)}")
         initial_state = initial_state.contiguous()
-        d.h0 = initial_state.data_ptr()
-    h_last = None
-    if return_final_state:
-        h_last = torch.empty(shape, device=v.device, dtype=torch.float32)
-        d.h_last = h_last.data_ptr()
-    with _on(v):
-        nbytes = lib().mb2_decay_attention_workspace_bytes(ctypes.byref(d))
+    with _on(dev):
+        o = torch.empty((B, T, H, dv), device=v.device, dtype=v.dtype) if out is None else out
+        h_last = (torch.empty((n, H, dk, dv), device=v.device, dtype=torch.float32)
+                  if return_final_state else None)
+        d = _decay_descriptor(what, q, k, v, g, scale, o, True, _addr(initial_state),
+                              _addr(h_last), cu, n, int(out is None))
+        nbytes = lib().mb2_decay_attention_workspace_bytes(d)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=v.device) if nbytes else None
-        check(lib().mb2_decay_attention(ctypes.byref(d), ptr(ws), nbytes, stream_of(v)), what)
+        rc = lib().mb2_decay_attention(d, _addr(ws), nbytes, _raw_stream(dev))
+        if rc:
+            check(rc, what)
     return (o, h_last) if return_final_state else o
 
 
@@ -391,23 +407,43 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: t
     g (B, H) or (H,); ``state`` (B, H, Dk, Dv) float32 contiguous is advanced in
     place.  Returns o (B, H, Dv)."""
     what = "decay_attention_step"
-    _one_device(what, q, k, v, g, state)
+    dev = _device_of(what, q, k, v, g, state)
+    if v.dim() != 3 or q.dim() != 3 or k.dim() != 3 or g.dim() not in (1, 2):
+        raise RuntimeError(f"{what}: q, k and v must be (batch, heads, width) and g (heads,) or "
+                           f"(batch, heads), got {tuple(q.shape)}, {tuple(k.shape)}, "
+                           f"{tuple(v.shape)} and {tuple(g.shape)}")
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if v.dim() != 3 or g.dim() not in (1, 2):
-        raise RuntimeError(f"{what}: v must be (batch, heads, width) and g (heads,) or "
-                           f"(batch, heads), got {tuple(v.shape)} and {tuple(g.shape)}")
-    o = torch.empty(v.shape[0], g.shape[-1], v.shape[2], device=v.device, dtype=v.dtype)
-    d = _decay_descriptor(what, q, k, v, g, scale, o, False)
-    if (state.shape != (d.batch, d.heads, d.dk, d.dv) or state.dtype != torch.float32
+    B, _, dv = v.shape
+    H = g.shape[-1]
+    if (state.shape != (B, H, q.shape[-1], dv) or state.dtype != torch.float32
             or not state.is_contiguous()):
-        raise RuntimeError(f"{what}: state must be contiguous float32 "
-                           f"{(d.batch, d.heads, d.dk, d.dv)}")
-    with _on(v):
-        check(lib().mb2_decay_attention_step(ctypes.byref(d), ptr(state), stream_of(v)), what)
+        raise RuntimeError(f"{what}: state must be contiguous float32 {(B, H, q.shape[-1], dv)}")
+    with _on(dev):
+        o = torch.empty((B, H, dv), device=v.device, dtype=v.dtype)
+        d = _decay_descriptor(what, q, k, v, g, scale, o, False)
+        rc = lib().mb2_decay_attention_step(d, state.data_ptr(), _raw_stream(dev))
+        if rc:
+            check(rc, what)
     return o
 
 
 # ------------------------------------------------------- norms around a block
+_NORM = struct.Struct("=2i3q8Q5q2f4i")
+
+
+def _norm_rows(name: str, t: torch.Tensor, shape, W: int) -> torch.Tensor:
+    if t.shape != shape:
+        raise RuntimeError(f"gated_norm: {name} {tuple(t.shape)} does not match x {tuple(shape)}")
+    t = _rows(t)
+    return t if t.dim() == 2 else t.reshape(-1, W)
+
+
+def _norm_vector(name: str, t: torch.Tensor, W: int, dtype) -> torch.Tensor:
+    if t.shape != (W,) or t.dtype not in (dtype, torch.float32):
+        raise RuntimeError(f"gated_norm: {name} must be ({W},) in {dtype} or float32")
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def gated_norm(x: torch.Tensor, gate: Optional[torch.Tensor] = None,
                weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                residual_scale=None, next_weight: Optional[torch.Tensor] = None,
@@ -429,69 +465,58 @@ def gated_norm(x: torch.Tensor, gate: Optional[torch.Tensor] = None,
 
     Returns u without a residual, r with one, (r, n) with ``next_weight``; r in
     residual's dtype, u and n in x's, n computed from the unrounded r.  ``out``
-    receives the first result; it may be ``residual`` itself.  Forward only."""
+    receives the first result; it may be ``residual`` itself (and overlap no
+    other input).  Forward only."""
     what = "gated_norm"
-    vec_scale = isinstance(residual_scale, torch.Tensor)
-    _one_device(what, x, gate, weight, residual, residual_scale if vec_scale else None,
-                next_weight, out)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"{what}: x must be (..., width), got {tuple(x.shape)}")
-    W = x.shape[-1]
-    if residual is None and (residual_scale is not None or next_weight is not None):
-        raise RuntimeError(f"{what}: residual_scale and next_weight need a residual")
-    d = GatedNorm()
-    d.dtype = d.residual_dtype = dtype_code(x.dtype)
+    scale_t = residual_scale if isinstance(residual_scale, torch.Tensor) else None
+    dev = _device_of(what, x, gate, weight, residual, scale_t, next_weight, out)
+    shape, dtype = x.shape, x.dtype
+    if len(shape) < 1 or shape[-1] < 1:
+        raise RuntimeError(f"{what}: x must be (..., width), got {tuple(shape)}")
+    W = shape[-1]
+    code = dtype_code(dtype)
     if group_size is not None and (group_size < 1 or W % group_size):
         raise RuntimeError(f"{what}: group_size {group_size} does not divide width {W}")
-    d.rows, d.width, d.group = x.numel() // W, W, group_size or 0
-    d.eps, d.norm_before_gate, d.scale = eps, int(norm_before_gate), 1.0
-    keep = []
-
-    def rows_of(name, t):
-        if t.shape != x.shape:
-            raise RuntimeError(f"{what}: {name} {tuple(t.shape)} does not match x "
-                               f"{tuple(x.shape)}")
-        t2 = _rows(t).reshape(-1, W)
-        keep.append(t2)
-        return t2.data_ptr(), t2.stride(0)
-
-    def vector(name, t):
-        if t.shape != (W,) or t.dtype not in (x.dtype, torch.float32):
-            raise RuntimeError(f"{what}: {name} must be ({W},) in {x.dtype} or float32")
-        t = t.contiguous()
-        keep.append(t)
-        return t.data_ptr(), int(t.dtype == torch.float32)
-
-    d.x, d.ld_x = rows_of("x", x)
+    x2 = _norm_rows("x", x, shape, W)
+    z2 = r2 = None
+    first, rcode, scale = dtype, code, 1.0
     if gate is not None:
-        if gate.dtype != x.dtype:
-            raise RuntimeError(f"{what}: gate must be in {x.dtype}")
-        d.gate, d.ld_gate = rows_of("gate", gate)
+        if gate.dtype != dtype:
+            raise RuntimeError(f"{what}: gate must be in {dtype}")
+        z2 = _norm_rows("gate", gate, shape, W)
     if weight is not None:
-        d.weight, d.weight_f32 = vector("weight", weight)
-    first = x.dtype
+        weight = _norm_vector("weight", weight, W, dtype)
     if residual is not None:
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise RuntimeError(f"{what}: residual must be in {x.dtype} or float32")
         first = residual.dtype
-        d.residual_dtype = dtype_code(first)
-        d.residual, d.ld_residual = rows_of("residual", residual)
-        if vec_scale:
-            d.residual_scale, d.scale_f32 = vector("residual_scale", residual_scale)
+        if first not in (dtype, torch.float32):
+            raise RuntimeError(f"{what}: residual must be in {dtype} or float32")
+        rcode = dtype_code(first)
+        r2 = _norm_rows("residual", residual, shape, W)
+        if scale_t is not None:
+            scale_t = _norm_vector("residual_scale", scale_t, W, dtype)
         elif residual_scale is not None:
-            d.scale = residual_scale
-    if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=first)
-    elif out.shape != x.shape or out.dtype != first or not out.is_contiguous():
-        raise RuntimeError(f"{what}: out must be contiguous {tuple(x.shape)} in {first}")
-    d.out, d.ld_out = out.data_ptr(), W
-    n = None
-    if next_weight is not None:
-        d.next_weight, d.next_f32 = vector("next_weight", next_weight)
-        n = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        d.next_out, d.ld_next = n.data_ptr(), W
-    with _on(x):
-        check(lib().mb2_gated_norm(ctypes.byref(d), stream_of(x)), what)
+            scale = residual_scale
+        if next_weight is not None:
+            next_weight = _norm_vector("next_weight", next_weight, W, dtype)
+    elif residual_scale is not None or next_weight is not None:
+        raise RuntimeError(f"{what}: residual_scale and next_weight need a residual")
+    with _on(dev):
+        if out is None:
+            out = torch.empty(shape, device=x.device, dtype=first)
+        elif out.shape != shape or out.dtype != first or not out.is_contiguous():
+            raise RuntimeError(f"{what}: out must be contiguous {tuple(shape)} in {first}")
+        n = None if next_weight is None else torch.empty(shape, device=x.device, dtype=dtype)
+        f32 = torch.float32
+        d = _NORM.pack(code, rcode, x2.shape[0], W, group_size or 0, x2.data_ptr(), _addr(z2),
+                       _addr(weight), _addr(r2), _addr(scale_t), _addr(next_weight),
+                       out.data_ptr(), _addr(n), x2.stride(0), 0 if z2 is None else z2.stride(0),
+                       0 if r2 is None else r2.stride(0), W, W, scale, eps, norm_before_gate,
+                       weight is not None and weight.dtype == f32,
+                       scale_t is not None and scale_t.dtype == f32,
+                       next_weight is not None and next_weight.dtype == f32)
+        rc = lib().mb2_gated_norm(d, _raw_stream(dev))
+        if rc:
+            check(rc, what)
     return out if n is None else (out, n)
 
 
@@ -513,39 +538,43 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
     Returns (scores (B, num) float32, parents (B, num), tokens (B, num)), the
     last two int64, parents being beams 0 .. K-1."""
     what = "beam_select"
-    _one_device(what, logits, scores, finished)
-    if logits.dim() != 3 or logits.shape[1] == 0 or logits.shape[2] == 0:
-        raise RuntimeError(f"{what}: logits must be (batch, beams, vocab), got "
-                           f"{tuple(logits.shape)}")
-    B, K, V = logits.shape
+    dev = _device_of(what, logits, scores, finished)
+    shape = logits.shape
+    if len(shape) != 3 or shape[1] == 0 or shape[2] == 0:
+        raise RuntimeError(f"{what}: logits must be (batch, beams, vocab), got {tuple(shape)}")
+    B, K, V = shape
     if scores.shape != (B, K) or scores.dtype != torch.float32:
         raise RuntimeError(f"{what}: scores must be float32 {(B, K)}")
-    if finished is not None and (finished.shape != (B, K) or finished.dtype != torch.bool):
-        raise RuntimeError(f"{what}: finished must be bool {(B, K)}")
+    if finished is not None:
+        if finished.shape != (B, K) or finished.dtype != torch.bool:
+            raise RuntimeError(f"{what}: finished must be bool {(B, K)}")
+        finished = finished.contiguous()
     num = K if num is None else int(num)
     code = dtype_code(logits.dtype)
     logits, scores = _rows(logits), scores.contiguous()
-    finished = None if finished is None else finished.contiguous()
-    with _on(logits):
+    with _on(dev):
         n = max(num, 0)
-        best = torch.empty(B, n, device=logits.device, dtype=torch.float32)
-        parents = torch.empty(B, n, device=logits.device, dtype=torch.int64)
-        tokens = torch.empty_like(parents)
+        best = torch.empty((B, n), device=logits.device, dtype=torch.float32)
+        parents = torch.empty((B, n), device=logits.device, dtype=torch.int64)
+        tokens = torch.empty((B, n), device=logits.device, dtype=torch.int64)
         nbytes = lib().mb2_beam_select_workspace_bytes(code, B, K, V, num)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-        check(lib().mb2_beam_select(code, ptr(logits), logits.stride(0), logits.stride(1),
-                                    ptr(scores), ptr(finished), pad_token, B, K, V, num,
-                                    ptr(best), ptr(parents), ptr(tokens), ptr(ws), nbytes,
-                                    stream_of(logits)), what)
+        rc = lib().mb2_beam_select(code, logits.data_ptr(), logits.stride(0), logits.stride(1),
+                                   scores.data_ptr(), _addr(finished), pad_token, B, K, V, num,
+                                   best.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                                   ws.data_ptr(), nbytes, _raw_stream(dev))
+        if rc:
+            check(rc, what)
     return best, parents, tokens
 
 
-def _leaves(states):
+def _leaves(states, out: list) -> list:
     if isinstance(states, torch.Tensor):
-        yield states
+        out.append(states)
     else:
         for s in states.values() if isinstance(states, dict) else states:
-            yield from _leaves(s)
+            _leaves(s, out)
+    return out
 
 
 def reorder_states(states, parents: torch.Tensor):
@@ -563,18 +592,21 @@ def reorder_states(states, parents: torch.Tensor):
         raise RuntimeError(f"{what}: parents must be (batch, beams) int64 or int32, got "
                            f"{tuple(parents.shape)} {parents.dtype}")
     B, K = parents.shape
-    rows, dev = B * K, parents.device
-    tensors = list(_leaves(states))
-    require_cuda(parents, *tensors, what=what)
-    n = len(tensors)
-    ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
-    for i, t in enumerate(tensors):
-        if t.dim() < 1 or t.shape[0] != rows or not t.is_contiguous() or t.device != dev:
-            raise RuntimeError(f"{what}: states must be contiguous with {rows} rows on {dev}, got "
-                               f"{tuple(t.shape)} on {t.device}")
-        ptrs[i] = t.data_ptr()
-        sizes[i] = t.numel() * t.element_size() // rows if rows else 0
+    rows = B * K
+    tensors = _leaves(states, [])
+    dev = _device_of(what, parents, *tensors)
+    ptrs, sizes = [], []
+    for t in tensors:
+        if t.dim() < 1 or t.shape[0] != rows or not t.is_contiguous():
+            raise RuntimeError(f"{what}: states must be contiguous with {rows} rows, got "
+                               f"{tuple(t.shape)}")
+        ptrs.append(t.data_ptr())
+        sizes.append(t.nbytes // rows if rows else 0)
     parents = parents.to(torch.int64).contiguous()
-    with _on(parents):
-        check(lib().mb2_reorder_rows(ptrs, sizes, n, ptr(parents), B, K, stream_of(parents)), what)
+    n = len(ptrs)
+    with _on(dev):
+        rc = lib().mb2_reorder_rows(struct.pack(f"{n}Q", *ptrs), struct.pack(f"{n}q", *sizes), n,
+                                    parents.data_ptr(), B, K, _raw_stream(dev))
+        if rc:
+            check(rc, what)
     return states
