@@ -52,6 +52,15 @@ template <> struct Word<float> {
     static __device__ __forceinline__ uint32_t masked(uint32_t w, int, bool in) {
         return in ? w : 0xff800000u;
     }
+    // the larger values (a NaN loses), the largest, and whether one is >= t
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+    static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
+    static __device__ __forceinline__ bool reaches(uint32_t w, uint32_t t) {
+        return __uint_as_float(w) >= __uint_as_float(t);
+    }
+    static __device__ __forceinline__ uint32_t splat(float v) { return __float_as_uint(v); }
 };
 template <> struct Word<__nv_bfloat16> {
     static constexpr int N = 2;
@@ -60,6 +69,20 @@ template <> struct Word<__nv_bfloat16> {
     }
     static __device__ __forceinline__ uint32_t masked(uint32_t w, int i, bool in) {
         return in ? w : i ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
+    }
+    static __device__ __forceinline__ __nv_bfloat162 two(uint32_t w) {
+        return *reinterpret_cast<const __nv_bfloat162 *>(&w);
+    }
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 m = __hmax2(two(a), two(b));
+        return *reinterpret_cast<const uint32_t *>(&m);
+    }
+    static __device__ __forceinline__ float top(uint32_t w) { return fmaxf(at(w, 0), at(w, 1)); }
+    static __device__ __forceinline__ bool reaches(uint32_t w, uint32_t t) {
+        return __hge2_mask(two(w), two(t)) != 0;
+    }
+    static __device__ __forceinline__ uint32_t splat(float v) {
+        return (__float_as_uint(v) >> 16) * 0x10001u;        // v is a bf16 value
     }
 };
 
@@ -101,7 +124,7 @@ beam_rows_kernel(const RowArgs a) {
     auto token = [&](int j, int w, int i) {
         return (v0 + j * ROW_THREADS) * VEC + w * WN + i - lead;
     };
-    float tmax = -INFINITY;
+    uint32_t wmax = kNone;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int v = v0 + j * ROW_THREADS;
@@ -115,10 +138,9 @@ beam_rows_kernel(const RowArgs a) {
                 }
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int i = 0; i < WN; ++i) tmax = fmaxf(tmax, Word<T>::at(raw[j][w], i));
+        for (int w = 0; w < 4; ++w) wmax = Word<T>::max(wmax, raw[j][w]);
     }
+    const float tmax = fmaxf(Word<T>::top(wmax), -INFINITY);
     float m = tmax;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -150,17 +172,18 @@ beam_rows_kernel(const RowArgs a) {
             thr = k < thr ? k : thr;
         }
     }
-    float sum = 0.0f;
+    // x - m first: a large common offset has to cancel.  All masked: every term is
+    // e^-inf; a NaN or +inf makes the sum NaN
+    const float off = m == -INFINITY ? 0.0f : m;
+    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int i = 0; i < WN; ++i) {
-                // a NaN or +inf makes the sum NaN
-                const float x = Word<T>::at(raw[j][w], i);
-                sum += x == -INFINITY ? 0.0f : ex2((x - m) * kLog2e);
-            }
+            for (int i = 0; i < WN; ++i)
+                sums[w] += ex2((Word<T>::at(raw[j][w], i) - off) * kLog2e);
+    float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) redf[1][wid] = sum;
@@ -178,14 +201,26 @@ beam_rows_kernel(const RowArgs a) {
                 if (c >= a.num) thr = t;
                 if (c >= a.num && c <= a.num + 8) break;
             }
+            // the bits need not be a value of T: the least thread maximum that
+            // reaches them is, and the same threads reach it
+            __shared__ uint32_t least;
+            if (tid == 0) least = 0xffffffffu;
+            __syncthreads();
+            if (kmax >= thr) atomicMin(&least, kmax);
+            __syncthreads();
+            thr = least;
         }
     }
     if (kmax >= thr) {
+        // a word without a value at the threshold is passed over at once; NaN (worth
+        // -inf) only counts where the threshold is that low
+        const uint32_t tw = Word<T>::splat(key_value(thr));
+        const bool all = thr <= order_key(-INFINITY);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if (!all && !Word<T>::reaches(raw[j][w], tw)) continue;
                 for (int i = 0; i < WN; ++i) {
                     const uint32_t k = order_key(Word<T>::at(raw[j][w], i));
                     const int t = token(j, w, i);
@@ -194,6 +229,7 @@ beam_rows_kernel(const RowArgs a) {
                         if (at < LIST) list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)t;
                     }
                 }
+            }
     }
     __syncthreads();
     const int64_t part = (int64_t)row * a.splits + split;
@@ -247,7 +283,7 @@ beam_rows_kernel(const RowArgs a) {
 
 struct MergeArgs {
     int beams, vocab, num, splits;
-    int64_t pad;
+    int pad;
     const float *scores;
     const uint8_t *finished;
     const float *part_max, *part_sum;
@@ -256,10 +292,9 @@ struct MergeArgs {
     int64_t *out_parents, *out_tokens;
     int staged;                               // the lists' entries fit shared memory
 };
-struct Entry { double val; int64_t at; };     // at: flat index, -1: none
 
 // better: the larger value, then the lower flat index (NaN never reaches here)
-__device__ __forceinline__ bool better(double v, int64_t at, double v2, int64_t at2) {
+__device__ __forceinline__ bool better(double v, int at, double v2, int at2) {
     return v > v2 || (v == v2 && at < at2);
 }
 
@@ -267,16 +302,17 @@ __global__ void __launch_bounds__(1024)
 beam_merge_kernel(const MergeArgs a) {
     extern __shared__ __align__(16) uint8_t dyn[];
     const int lists = a.beams * a.splits;
-    Entry *const stage = reinterpret_cast<Entry *>(dyn);     // [lists][num] when staged
-    int *const heads = reinterpret_cast<int *>(dyn + (a.staged ? sizeof(Entry) * lists * a.num : 0));
-    // heads: per list, entries taken
+    // [lists][num] when staged: values and flat indices (-1: none); entries taken
+    const int stage = a.staged ? lists * a.num : 0;
+    double *const s_val = reinterpret_cast<double *>(dyn);
+    int *const s_at = reinterpret_cast<int *>(s_val + stage);
+    int *const heads = s_at + stage;
     // a beam's score, largest logit and log sum of exp(logit - largest): a large
     // common offset of the logits must cancel before the other terms join
     __shared__ double s_score[MAX_BEAMS], s_max[MAX_BEAMS], s_logsum[MAX_BEAMS];
     __shared__ int s_kind[MAX_BEAMS];         // 0 live, 1 finished, 2 no continuation
     __shared__ double w_val[2][32];
-    __shared__ int64_t w_at[2][32];
-    __shared__ int w_list[2][32];
+    __shared__ int w_at[2][32];
     const int batch = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int warps = blockDim.x >> 5;
 
@@ -312,15 +348,15 @@ beam_merge_kernel(const MergeArgs a) {
     __syncthreads();
 
     // entry `h` of a list: false when it has none
-    auto entry = [&](int l, int h, double &val, int64_t &at) {
+    auto entry = [&](int l, int h, double &val, int &at) {
         const int k = l / a.splits, sp = l - k * a.splits;
         const int kind = s_kind[k];
-        const int64_t flat = (int64_t)k * a.vocab;
+        const int flat = k * a.vocab;
         if (kind != 0) {
             // a finished beam continues with the pad token alone; every other
             // token, and all of a beam without continuation, are worth -inf
             if (sp != 0 || h >= a.vocab) return false;
-            const int64_t tok = kind == 2 ? h : (h == 0 ? a.pad : h - 1 + (h - 1 >= a.pad));
+            const int tok = kind == 2 ? h : (h == 0 ? a.pad : h - 1 + (h - 1 >= a.pad));
             val = kind == 1 && h == 0 ? s_score[k] : -INFINITY;
             at = flat + tok;
             return true;
@@ -329,36 +365,42 @@ beam_merge_kernel(const MergeArgs a) {
         const uint64_t e = a.part_list[((int64_t)(batch * a.beams + k) * a.splits + sp) * a.num + h];
         if (e == 0) return false;
         val = s_score[k] + (((double)key_value((uint32_t)(e >> 32)) - s_max[k]) - s_logsum[k]);
-        at = flat + (uint32_t)~(uint32_t)e;
+        at = flat + (int)~(uint32_t)e;
         return true;
     };
     // all entries at once, so that the rounds below wait for no global load
     if (a.staged) {
         for (int i = tid; i < lists * a.num; i += blockDim.x) {
-            Entry e;
-            if (!entry(i / a.num, i % a.num, e.val, e.at)) e.at = -1;
-            stage[i] = e;
+            double v = 0.0;
+            int at = -1;
+            if (!entry(i / a.num, i % a.num, v, at)) at = -1;
+            s_val[i] = v;
+            s_at[i] = at;
         }
         __syncthreads();
     }
+    // few lists: one warp merges, without barriers
+    const int active = lists <= 128 ? 1 : warps;
+    if (wid >= active) return;
     // this thread's best head over its lists
     double val;
-    int64_t at;
-    int which;
+    int at, which;
     auto refresh = [&]() {
         which = -1;
         val = -INFINITY;
-        at = INT64_MAX;
-        for (int l = tid; l < lists; l += blockDim.x) {
-            double v;
-            int64_t p;
+        at = INT32_MAX;
+        for (int l = tid; l < lists; l += active * 32) {
+            double v = 0.0;
+            int p = -1;
             const int h = heads[l];
             bool has;
             if (a.staged) {
-                const Entry e = stage[l * a.num + (h < a.num ? h : 0)];
-                has = h < a.num && e.at >= 0;
-                v = e.val;
-                p = e.at;
+                has = h < a.num;
+                if (has) {
+                    v = s_val[l * a.num + h];
+                    p = s_at[l * a.num + h];
+                    has = p >= 0;
+                }
             } else {
                 has = entry(l, h, v, p);
             }
@@ -372,33 +414,32 @@ beam_merge_kernel(const MergeArgs a) {
     refresh();
     for (int n = 0; n < a.num; ++n) {
         double bv = val;
-        int64_t ba = at;
-        int bl = which;
+        int ba = at;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const double v = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int64_t p = __shfl_xor_sync(0xffffffffu, ba, o);
-            const int l = __shfl_xor_sync(0xffffffffu, bl, o);
-            if (better(v, p, bv, ba)) { bv = v; ba = p; bl = l; }
+            const int p = __shfl_xor_sync(0xffffffffu, ba, o);
+            if (better(v, p, bv, ba)) { bv = v; ba = p; }
         }
-        if (warps > 1) {
-            if (lane == 0) { w_val[n & 1][wid] = bv; w_at[n & 1][wid] = ba; w_list[n & 1][wid] = bl; }
+        if (active > 1) {
+            if (lane == 0) { w_val[n & 1][wid] = bv; w_at[n & 1][wid] = ba; }
             __syncthreads();
-            bv = w_val[n & 1][0]; ba = w_at[n & 1][0]; bl = w_list[n & 1][0];
-            for (int w = 1; w < warps; ++w)
+            bv = w_val[n & 1][0]; ba = w_at[n & 1][0];
+            for (int w = 1; w < active; ++w)
                 if (better(w_val[n & 1][w], w_at[n & 1][w], bv, ba)) {
-                    bv = w_val[n & 1][w]; ba = w_at[n & 1][w]; bl = w_list[n & 1][w];
+                    bv = w_val[n & 1][w]; ba = w_at[n & 1][w];
                 }
         }
-        if (bl < 0) break;                    // num <= beams x vocab: not reached
-        if (which == bl) {                    // the thread that offered it
+        if (ba == INT32_MAX) break;           // num <= beams x vocab: not reached
+        if (at == ba) {                       // the thread that offered it
             const int64_t i = (int64_t)batch * a.num + n;
             a.out_scores[i] = (float)bv;
             a.out_parents[i] = ba / a.vocab;
             a.out_tokens[i] = ba % a.vocab;
-            ++heads[bl];
+            ++heads[which];
             refresh();
         }
+        __syncwarp();
     }
 }
 
@@ -512,14 +553,15 @@ extern "C" int mb2_beam_select(int dtype, const void *logits, int64_t batch_stri
     MB2_TRY(check_launch("beam_rows_kernel"));
     MergeArgs g;
     g.beams = r.beams; g.vocab = r.vocab; g.num = r.num; g.splits = splits;
-    g.pad = pad_token;
+    g.pad = (int)pad_token;
     g.scores = scores;
     g.finished = finished;
     g.part_max = r.part_max; g.part_sum = r.part_sum; g.part_list = r.part_list;
     g.out_scores = out_scores; g.out_parents = out_parents; g.out_tokens = out_tokens;
     const int lists = (int)beams * splits;
-    const int threads = (int)(round_up(lists, 32) < 1024 ? round_up(lists, 32) : 1024);
-    const size_t staged = (sizeof(Entry) * (size_t)num + sizeof(int)) * lists;
+    // at most 32 x 2^20 candidates a batch: flat indices are 32-bit
+    const int threads = lists <= 256 ? 256 : lists <= 512 ? 512 : 1024;
+    const size_t staged = (size_t)lists * num * 12 + sizeof(int) * (size_t)lists;
     g.staged = staged <= 48 * 1024;
     beam_merge_kernel<<<(unsigned)batch, threads, g.staged ? staged : sizeof(int) * lists, st>>>(g);
     return check_launch("beam_merge_kernel");
