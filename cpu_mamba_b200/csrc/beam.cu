@@ -293,9 +293,26 @@ struct MergeArgs {
     int staged;                               // the lists' entries fit shared memory
 };
 
-// better: the larger value, then the lower flat index (NaN never reaches here)
-__device__ __forceinline__ bool better(double v, int at, double v2, int at2) {
+// a 64-bit value (never NaN) ordered as unsigned, 0 below all; compares as integers,
+// and a warp's largest takes three reductions
+__device__ __forceinline__ uint64_t order_key64(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+    return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double key_value64(uint64_t k) {
+    return __longlong_as_double((long long)((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
+}
+// the larger value, then the lower flat index
+__device__ __forceinline__ bool better(uint64_t v, int at, uint64_t v2, int at2) {
     return v > v2 || (v == v2 && at < at2);
+}
+// a warp's best (value, flat index)
+__device__ __forceinline__ void warp_best(uint64_t &v, int &at) {
+    const uint32_t hi = (uint32_t)(v >> 32), lo = (uint32_t)v;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t low = __reduce_max_sync(0xffffffffu, hi == top ? lo : 0u);
+    at = __reduce_min_sync(0xffffffffu, hi == top && lo == low ? at : INT32_MAX);
+    v = (uint64_t)top << 32 | low;
 }
 
 __global__ void __launch_bounds__(1024)
@@ -304,14 +321,14 @@ beam_merge_kernel(const MergeArgs a) {
     const int lists = a.beams * a.splits;
     // [lists][num] when staged: values and flat indices (-1: none); entries taken
     const int stage = a.staged ? lists * a.num : 0;
-    double *const s_val = reinterpret_cast<double *>(dyn);
+    uint64_t *const s_val = reinterpret_cast<uint64_t *>(dyn);
     int *const s_at = reinterpret_cast<int *>(s_val + stage);
     int *const heads = s_at + stage;
     // a beam's score, largest logit and log sum of exp(logit - largest): a large
     // common offset of the logits must cancel before the other terms join
     __shared__ double s_score[MAX_BEAMS], s_max[MAX_BEAMS], s_logsum[MAX_BEAMS];
     __shared__ int s_kind[MAX_BEAMS];         // 0 live, 1 finished, 2 no continuation
-    __shared__ double w_val[2][32];
+    __shared__ uint64_t w_val[2][32];
     __shared__ int w_at[2][32];
     const int batch = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int warps = blockDim.x >> 5;
@@ -348,7 +365,7 @@ beam_merge_kernel(const MergeArgs a) {
     __syncthreads();
 
     // entry `h` of a list: false when it has none
-    auto entry = [&](int l, int h, double &val, int &at) {
+    auto entry = [&](int l, int h, uint64_t &val, int &at) {
         const int k = l / a.splits, sp = l - k * a.splits;
         const int kind = s_kind[k];
         const int flat = k * a.vocab;
@@ -357,21 +374,22 @@ beam_merge_kernel(const MergeArgs a) {
             // token, and all of a beam without continuation, are worth -inf
             if (sp != 0 || h >= a.vocab) return false;
             const int tok = kind == 2 ? h : (h == 0 ? a.pad : h - 1 + (h - 1 >= a.pad));
-            val = kind == 1 && h == 0 ? s_score[k] : -INFINITY;
+            val = order_key64(kind == 1 && h == 0 ? s_score[k] : -INFINITY);
             at = flat + tok;
             return true;
         }
         if (h >= a.num) return false;
         const uint64_t e = a.part_list[((int64_t)(batch * a.beams + k) * a.splits + sp) * a.num + h];
         if (e == 0) return false;
-        val = s_score[k] + (((double)key_value((uint32_t)(e >> 32)) - s_max[k]) - s_logsum[k]);
+        val = order_key64(s_score[k] +
+                          (((double)key_value((uint32_t)(e >> 32)) - s_max[k]) - s_logsum[k]));
         at = flat + (int)~(uint32_t)e;
         return true;
     };
     // all entries at once, so that the rounds below wait for no global load
     if (a.staged) {
         for (int i = tid; i < lists * a.num; i += blockDim.x) {
-            double v = 0.0;
+            uint64_t v = 0;
             int at = -1;
             if (!entry(i / a.num, i % a.num, v, at)) at = -1;
             s_val[i] = v;
@@ -383,14 +401,14 @@ beam_merge_kernel(const MergeArgs a) {
     const int active = lists <= 128 ? 1 : warps;
     if (wid >= active) return;
     // this thread's best head over its lists
-    double val;
+    uint64_t val;
     int at, which;
     auto refresh = [&]() {
         which = -1;
-        val = -INFINITY;
+        val = 0;
         at = INT32_MAX;
         for (int l = tid; l < lists; l += active * 32) {
-            double v = 0.0;
+            uint64_t v = 0;
             int p = -1;
             const int h = heads[l];
             bool has;
@@ -413,14 +431,9 @@ beam_merge_kernel(const MergeArgs a) {
     };
     refresh();
     for (int n = 0; n < a.num; ++n) {
-        double bv = val;
+        uint64_t bv = val;
         int ba = at;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double v = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int p = __shfl_xor_sync(0xffffffffu, ba, o);
-            if (better(v, p, bv, ba)) { bv = v; ba = p; }
-        }
+        warp_best(bv, ba);
         if (active > 1) {
             if (lane == 0) { w_val[n & 1][wid] = bv; w_at[n & 1][wid] = ba; }
             __syncthreads();
@@ -433,7 +446,7 @@ beam_merge_kernel(const MergeArgs a) {
         if (ba == INT32_MAX) break;           // num <= beams x vocab: not reached
         if (at == ba) {                       // the thread that offered it
             const int64_t i = (int64_t)batch * a.num + n;
-            a.out_scores[i] = (float)bv;
+            a.out_scores[i] = (float)key_value64(bv);
             a.out_parents[i] = ba / a.vocab;
             a.out_tokens[i] = ba % a.vocab;
             ++heads[which];
