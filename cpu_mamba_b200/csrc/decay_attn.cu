@@ -14,82 +14,65 @@ namespace mb2 {
 namespace decay {
 
 // ------------------------------------------------------- recurrent prompt
-// One CTA walks one (sequence, head, column tile) token by token, the state in
-// registers: thread (kg, vg) of a warp owns VT columns and the KT rows
-// dk = 32 i + 4 kg + (0..3), so the eight row groups of a warp read 128
-// consecutive bytes of k and q per shared-memory load.
+// One CTA walks one (sequence or segment, head, column tile) token by token, the
+// state in registers: KG neighbouring lanes share two columns, each holding R rows
+// of them (rows 4 KG i + 4 kg .. + 3, so a group's k and q loads are neighbours and
+// all other lanes' are broadcasts).  With R <= 32 rows a lane, widths up to 32 need
+// no sum over lanes at all.
 //
 // Deferred decay: the registers hold u_t = S_t / A_t, A_t the product of the
 // decays since the last renormalisation.  Then u += k (v / A_t)^T and
-// o = (scale A_t) u^T q: two FMAs per state element and token instead of
-// three operations.  A run ends (u *= A, A = 1) when log A leaves
-// [-5.5, 5.5], so v / A grows by 2^8 at most (|v| > 1e36 would overflow) and
-// every product has the relative precision it has without the factor.
+// o = (scale A_t) u^T q: two FMAs per state element and token instead of three
+// operations, done for two rows at a time (fma.rn.f32x2).  A run ends (u *= A,
+// A = 1) when log A leaves [-5.5, 5.5], so v / A grows by 2^8 at most (|v| > 1e36
+// would overflow) and every product has the relative precision it has without the
+// factor.
 //
-// Bound: the FP32 pipe, 2 Dk Dv FMAs per token and head.
+// Bound: the FP32 pipe, 2 Dk Dv FMAs per token and head, and the shared-memory
+// loads of k and q (two 16-byte loads per 8 packed FMAs).  One warp per head of 64
+// columns instead of four with eight lanes a column: TODO us at 151 x 180.
 constexpr int L = 16;                 // tokens staged at a time
 constexpr float kRun = 5.5f;          // bound on |log A| within a run
 
-template <typename T, int KT, int VT> struct Rec {
-    static constexpr int DK = 8 * KT;       // padded rows
-    static constexpr int WV = 4 * VT;       // columns per warp
-    static constexpr int MAXW = 4;          // warps per CTA
-    static constexpr int PK = DK + 16 / (int)sizeof(T);   // row pitch of q and k in shared memory
-};
-
+// rows [0, n) x cols of a strided matrix into shared memory as fp32 (pitch
+// `pitch`): 16-byte asynchronous copies of fp32 rows that allow them, else through
+// registers
 template <typename T>
-__device__ __forceinline__ void ld4(const T *p, float (&r)[4]);
-template <> __device__ __forceinline__ void ld4<float>(const float *p, float (&r)[4]) {
-    const float4 v = *reinterpret_cast<const float4 *>(p);
-    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
-}
-template <> __device__ __forceinline__ void ld4<__nv_bfloat16>(const __nv_bfloat16 *p, float (&r)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    r[0] = __uint_as_float(v.x << 16); r[1] = __uint_as_float(v.x & 0xffff0000u);
-    r[2] = __uint_as_float(v.y << 16); r[3] = __uint_as_float(v.y & 0xffff0000u);
-}
-// p aligned to VT elements
-template <typename T, int VT>
-__device__ __forceinline__ void ldv(const T *p, float (&r)[VT]) {
-    if constexpr (VT == 4) {
-        ld4<T>(p, r);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VT; ++i) r[i] = io<T>::to_f(p[i]);
-    }
-}
-
-// rows [0, n) x cols of a strided matrix into shared memory (pitch `pitch`):
-// 16-byte asynchronous copies where the rows allow them, else element copies
-template <typename T>
-__device__ __forceinline__ void stage(T *dst, int pitch, const T *src, int64_t ld, int n, int cols,
-                                      bool vec) {
+__device__ __forceinline__ void stage(float *dst, int pitch, const T *src, int64_t ld, int n,
+                                      int cols, bool vec) {
     if (vec) {
         constexpr int E = 16 / (int)sizeof(T);
         const int per = cols / E;
         for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
             const int r = i / per, c = (i - r * per) * E;
-            cp_async16(dst + r * pitch + c, src + r * ld + c);
+            if constexpr (sizeof(T) == 4) {
+                cp_async16(dst + r * pitch + c, src + r * ld + c);
+            } else {
+                const uint4 x = *reinterpret_cast<const uint4 *>(src + r * ld + c);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<float2 *>(dst + r * pitch + c + 2 * e) =
+                        make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+            }
         }
     } else {
         for (int i = threadIdx.x; i < n * cols; i += blockDim.x) {
             const int r = i / cols, c = i - r * cols;
-            dst[r * pitch + c] = src[r * ld + c];
+            dst[r * pitch + c] = io<T>::to_f(src[r * ld + c]);
         }
     }
 }
 
 // STATE: the pass over segments that leaves their states; no q, no outputs
-template <typename T, int KT, int VT, bool STATE>
+template <typename T, int KG, int R, bool STATE>
 __global__ void __launch_bounds__(128)
 decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec_v) {
-    using R = Rec<T, KT, VT>;
-    constexpr int KI = KT / 4;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    const int pv = vtile + 16 / (int)sizeof(T);
-    T *const qs = reinterpret_cast<T *>(smem_raw);         // [2][L][PK]
-    T *const ks = qs + 2 * L * R::PK;                      // [2][L][PK]
-    T *const vs = ks + 2 * L * R::PK;                      // [2][L][pv]
+    constexpr int DK = KG * R, QUADS = R / 4;              // padded rows
+    extern __shared__ __align__(16) float smem_f[];
+    float *const ks = smem_f;                              // [2][L][DK]
+    float *const vs = ks + 2 * L * DK;                     // [2][L][vtile]
+    float *const qs = vs + 2 * L * vtile;                  // [2][L][DK]
     __shared__ float s_ren[2][L], s_inv[2][L], s_out[2][L];
 
     const int tiles = (int)ceil_div(a.dv, vtile);
@@ -113,27 +96,28 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     T *o = static_cast<T *>(a.o) + bq * a.os[0] + row0 * a.os[1] + h * a.os[2] + c0;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int kg = lane & 7, vg = lane >> 3;
-    const int col = warp * R::WV + vg * VT;
+    const int kg = lane & (KG - 1);
+    const int col = 2 * ((int)threadIdx.x / KG);           // this lane's two columns
 
     // columns past Dk and Dv are zero for the whole walk
-    for (int i = threadIdx.x; i < 2 * L * R::PK; i += blockDim.x) {
-        qs[i] = io<T>::from_f(0.0f);
-        ks[i] = io<T>::from_f(0.0f);
-    }
-    for (int i = threadIdx.x; i < 2 * L * pv; i += blockDim.x) vs[i] = io<T>::from_f(0.0f);
+    const int words = 2 * L * (vtile + (STATE ? 1 : 2) * DK);
+    for (int i = threadIdx.x; i < words; i += blockDim.x) smem_f[i] = 0.0f;
 
-    float u[KI][4][VT];
+    uint64_t u[2 * QUADS][2];                              // row pairs x columns
+    auto row_of = [&](int i) { return 4 * KG * (i >> 1) + 4 * kg + 2 * (i & 1); };
 #pragma unroll
-    for (int i = 0; i < KI; ++i)
+    for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int dk = 32 * i + 4 * kg + j;
+        for (int c = 0; c < 2; ++c) {
+            float e[2];
 #pragma unroll
-            for (int c = 0; c < VT; ++c)
-                u[i][j][c] = (sp.in >= 0 && dk < a.dk && col + c < cols)
-                                 ? hin[((sp.in * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c]
-                                 : 0.0f;
+            for (int j = 0; j < 2; ++j) {
+                const int dk = row_of(i) + j;
+                e[j] = (sp.in >= 0 && dk < a.dk && col + c < cols)
+                           ? hin[((sp.in * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c]
+                           : 0.0f;
+            }
+            u[i][c] = pair(__float_as_uint(e[0]), __float_as_uint(e[1]));
         }
     __syncthreads();
 
@@ -143,9 +127,9 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
         if (!STATE)
-            stage<T>(qs + b * L * R::PK, R::PK, q + t0 * a.qs[1], a.qs[1], m, (int)a.dk, vec_q);
-        stage<T>(ks + b * L * R::PK, R::PK, k + t0 * a.ks[1], a.ks[1], m, (int)a.dk, vec_k);
-        stage<T>(vs + b * L * pv, pv, v + t0 * a.vs[1], a.vs[1], m, cols, vec_v);
+            stage<T>(qs + b * L * DK, DK, q + t0 * a.qs[1], a.qs[1], m, (int)a.dk, vec_q);
+        stage<T>(ks + b * L * DK, DK, k + t0 * a.ks[1], a.ks[1], m, (int)a.dk, vec_k);
+        stage<T>(vs + b * L * vtile, vtile, v + t0 * a.vs[1], a.vs[1], m, cols, vec_v);
         cp_async_commit();
     };
     // Per token: the factor on u before it (1: none), 1 / A and scale * A.
@@ -202,47 +186,52 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         }
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
-        const T *qb = qs + b * L * R::PK + 4 * kg;
-        const T *kb = ks + b * L * R::PK + 4 * kg;
-        const T *vb = vs + b * L * pv + col;
+        const float *qb = qs + b * L * DK + 4 * kg;
+        const float *kb = ks + b * L * DK + 4 * kg;
+        const float *vb = vs + b * L * vtile + col;
         for (int t = 0; t < m; ++t) {
             const float ren = s_ren[b][t];
             if (ren != 1.0f) {
+                const uint64_t r2 = pair(ren);
 #pragma unroll
-                for (int i = 0; i < KI; ++i)
+                for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int c = 0; c < VT; ++c) u[i][j][c] *= ren;
+                    for (int c = 0; c < 2; ++c) u[i][c] = mul2(u[i][c], r2);
             }
-            float w[VT], acc[VT];
-            ldv<T, VT>(vb + t * pv, w);
+            const float2 vv = *reinterpret_cast<const float2 *>(vb + t * vtile);
             const float inv = s_inv[b][t];
+            const uint64_t w0 = pair(vv.x * inv), w1 = pair(vv.y * inv);
+            uint64_t acc0 = 0, acc1 = 0;
 #pragma unroll
-            for (int c = 0; c < VT; ++c) { w[c] *= inv; acc[c] = 0.0f; }
-#pragma unroll
-            for (int i = 0; i < KI; ++i) {
-                float kv[4], qv[4];
-                ld4<T>(kb + t * R::PK + 32 * i, kv);
-                if (!STATE) ld4<T>(qb + t * R::PK + 32 * i, qv);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int c = 0; c < VT; ++c) {
-                        u[i][j][c] = fmaf(kv[j], w[c], u[i][j][c]);
-                        if (!STATE) acc[c] = fmaf(qv[j], u[i][j][c], acc[c]);
-                    }
+            for (int i = 0; i < QUADS; ++i) {
+                const ulonglong2 kk = *reinterpret_cast<const ulonglong2 *>(kb + t * DK + 4 * KG * i);
+                u[2 * i][0] = fma2(kk.x, w0, u[2 * i][0]);
+                u[2 * i][1] = fma2(kk.x, w1, u[2 * i][1]);
+                u[2 * i + 1][0] = fma2(kk.y, w0, u[2 * i + 1][0]);
+                u[2 * i + 1][1] = fma2(kk.y, w1, u[2 * i + 1][1]);
+                if constexpr (!STATE) {
+                    const ulonglong2 qq =
+                        *reinterpret_cast<const ulonglong2 *>(qb + t * DK + 4 * KG * i);
+                    acc0 = fma2(qq.x, u[2 * i][0], acc0);
+                    acc1 = fma2(qq.x, u[2 * i][1], acc1);
+                    acc0 = fma2(qq.y, u[2 * i + 1][0], acc0);
+                    acc1 = fma2(qq.y, u[2 * i + 1][1], acc1);
+                }
             }
             if constexpr (!STATE) {
+                float r0 = __uint_as_float(lo_of(acc0)) + __uint_as_float(hi_of(acc0));
+                float r1 = __uint_as_float(lo_of(acc1)) + __uint_as_float(hi_of(acc1));
 #pragma unroll
-                for (int s = 1; s < 8; s <<= 1)
-#pragma unroll
-                    for (int c = 0; c < VT; ++c) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], s);
-                float r = acc[0];
-#pragma unroll
-                for (int c = 1; c < VT; ++c) r = kg == c ? acc[c] : r;
-                if (kg < VT && col + kg < cols)
-                    o[(t0 + t) * a.os[1] + col + kg] = io<T>::from_f(r * s_out[b][t]);
+                for (int s = 1; s < KG; s <<= 1) {
+                    r0 += __shfl_xor_sync(0xffffffffu, r0, s);
+                    r1 += __shfl_xor_sync(0xffffffffu, r1, s);
+                }
+                const float f = s_out[b][t];
+                T *const to = o + (t0 + t) * a.os[1] + col;
+                if (kg == 0 && col < cols) {
+                    to[0] = io<T>::from_f(r0 * f);
+                    if (col + 1 < cols) to[1] = io<T>::from_f(r1 * f);
+                }
             }
         }
     }
@@ -254,16 +243,16 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         __syncthreads();
         const float f = s_last;
 #pragma unroll
-        for (int i = 0; i < KI; ++i)
+        for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int dk = 32 * i + 4 * kg + j;
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int c = 0; c < VT; ++c)
+                for (int j = 0; j < 2; ++j) {
+                    const int dk = row_of(i) + j;
+                    const float x = __uint_as_float(j ? hi_of(u[i][c]) : lo_of(u[i][c]));
                     if (dk < a.dk && col + c < cols)
-                        hout[((sp.out * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c] =
-                            u[i][j][c] * f;
-            }
+                        hout[((sp.out * a.heads + h) * a.dk + dk) * a.dv + c0 + col + c] = x * f;
+                }
     }
 }
 
@@ -273,15 +262,15 @@ static bool vec16(const void *p, const int64_t (&s)[3], int64_t cols) {
     return aligned(p, 16) && s[0] % E == 0 && s[1] % E == 0 && s[2] % E == 0 && cols % E == 0;
 }
 
-template <typename T, int KT, int VT, bool STATE>
+template <typename T, int KG, int R, bool STATE>
 static int launch_recurrent(const Args &a, cudaStream_t st) {
-    using R = Rec<T, KT, VT>;
-    const int warps = (int)(ceil_div(a.dv, R::WV) < R::MAXW ? ceil_div(a.dv, R::WV) : R::MAXW);
-    const int vtile = warps * R::WV;
+    constexpr int WV = 64 / KG;                            // columns of a warp
+    const int warps = (int)(ceil_div(a.dv, WV) < 4 ? ceil_div(a.dv, WV) : 4);
+    const int vtile = warps * WV;
     const int64_t grid = ceil_div(a.dv, vtile) * a.heads * spans(a);
     MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
-    const size_t smem = sizeof(T) * 2 * L * (2 * R::PK + vtile + 16 / sizeof(T));
-    auto kern = decay_recurrent_kernel<T, KT, VT, STATE>;
+    const size_t smem = sizeof(float) * 2 * L * ((STATE ? 1 : 2) * KG * R + vtile);
+    auto kern = decay_recurrent_kernel<T, KG, R, STATE>;
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)smem);
@@ -296,10 +285,12 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
 
 template <typename T, bool STATE>
 static int recurrent_of(const Args &a, cudaStream_t st) {
-    if (a.dk <= 32) return launch_recurrent<T, 4, 4, STATE>(a, st);
-    if (a.dk <= 64) return launch_recurrent<T, 8, 4, STATE>(a, st);
-    if (a.dk <= 128) return launch_recurrent<T, 16, 4, STATE>(a, st);
-    return launch_recurrent<T, 32, 2, STATE>(a, st);
+    if (a.dk <= 16) return launch_recurrent<T, 1, 16, STATE>(a, st);
+    if (a.dk <= 24) return launch_recurrent<T, 1, 24, STATE>(a, st);
+    if (a.dk <= 32) return launch_recurrent<T, 1, 32, STATE>(a, st);
+    if (a.dk <= 64) return launch_recurrent<T, 2, 32, STATE>(a, st);
+    if (a.dk <= 128) return launch_recurrent<T, 4, 32, STATE>(a, st);
+    return launch_recurrent<T, 8, 32, STATE>(a, st);
 }
 static int recurrent(const Args &a, bool state_only, cudaStream_t st) {
     if (a.dtype == MB2_F32)

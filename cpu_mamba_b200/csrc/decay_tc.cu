@@ -184,32 +184,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// two fp32 values in one register pair (packed FMA: half the instructions)
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ uint64_t pair(float v) {
-    return pair(__float_as_uint(v), __float_as_uint(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t lo_of(uint64_t v) { return (uint32_t)v; }
-__device__ __forceinline__ uint32_t hi_of(uint64_t v) { return (uint32_t)(v >> 32); }
 __device__ __forceinline__ uint32_t pack_bf16(uint64_t v) {
     return pack_bf16(__uint_as_float(lo_of(v)), __uint_as_float(hi_of(v)));
 }
