@@ -34,35 +34,49 @@ namespace decay {
 constexpr int L = 16;                 // tokens staged at a time
 constexpr float kRun = 5.5f;          // bound on |log A| within a run
 
-// rows [0, n) x cols of a strided matrix into shared memory as fp32 (pitch
+// Copies rows [0, n) of a strided matrix into shared memory as fp32 (pitch
 // `pitch`): 16-byte asynchronous copies of fp32 rows that allow them, else through
-// registers
-template <typename T>
-__device__ __forceinline__ void stage(float *dst, int pitch, const T *src, int64_t ld, int n,
-                                      int cols, bool vec) {
-    if (vec) {
+// registers.  A thread's place in a row and its step are divided out once.
+template <typename T> struct Stager {
+    int per, r, c, dr, dc;                // pieces a row; first piece; step
+    bool vec;
+    __device__ __forceinline__ Stager(int cols, bool vec_) : vec(vec_) {
+        per = vec ? cols / (16 / (int)sizeof(T)) : cols;
+        r = (int)threadIdx.x / per;
+        c = (int)threadIdx.x - r * per;
+        dr = (int)blockDim.x / per;
+        dc = (int)blockDim.x - dr * per;
+    }
+    __device__ __forceinline__ void operator()(float *dst, int pitch, const T *src, int64_t ld,
+                                               int n) const {
         constexpr int E = 16 / (int)sizeof(T);
-        const int per = cols / E;
-        for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
-            const int r = i / per, c = (i - r * per) * E;
-            if constexpr (sizeof(T) == 4) {
-                cp_async16(dst + r * pitch + c, src + r * ld + c);
-            } else {
-                const uint4 x = *reinterpret_cast<const uint4 *>(src + r * ld + c);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        int y = r, x = c;
+        while (y < n) {
+            if (vec) {
+                float *to = dst + y * pitch + x * E;
+                const T *from = src + y * ld + x * E;
+                if constexpr (sizeof(T) == 4) {
+                    cp_async16(to, from);
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(from);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    *reinterpret_cast<float2 *>(dst + r * pitch + c + 2 * e) =
-                        make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<float2 *>(to + 2 * e) = make_float2(
+                            __uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+                }
+            } else {
+                dst[y * pitch + x] = io<T>::to_f(src[y * ld + x]);
+            }
+            y += dr;
+            x += dc;
+            if (x >= per) {
+                x -= per;
+                ++y;
             }
         }
-    } else {
-        for (int i = threadIdx.x; i < n * cols; i += blockDim.x) {
-            const int r = i / cols, c = i - r * cols;
-            dst[r * pitch + c] = io<T>::to_f(src[r * ld + c]);
-        }
     }
-}
+};
 
 // STATE: the pass over segments that leaves their states; no q, no outputs
 template <typename T, int KG, int R, bool STATE>
@@ -100,8 +114,9 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     const int col = 2 * ((int)threadIdx.x / KG);           // this lane's two columns
 
     // columns past Dk and Dv are zero for the whole walk
-    const int words = 2 * L * (vtile + (STATE ? 1 : 2) * DK);
-    for (int i = threadIdx.x; i < words; i += blockDim.x) smem_f[i] = 0.0f;
+    const int words = 2 * L * (vtile + (STATE ? 1 : 2) * DK);      // a multiple of 4
+    for (int i = threadIdx.x; i < words / 4; i += blockDim.x)
+        reinterpret_cast<float4 *>(smem_f)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
     uint64_t u[2 * QUADS][2];                              // row pairs x columns
     auto row_of = [&](int i) { return 4 * KG * (i >> 1) + 4 * kg + 2 * (i & 1); };
@@ -122,19 +137,20 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     __syncthreads();
 
     const int nchunks = (int)ceil_div(len, (int64_t)L);
+    const Stager<T> get_q((int)a.dk, vec_q), get_k((int)a.dk, vec_k), get_v(cols, vec_v);
     auto load = [&](int n) {
         const int b = n & 1;
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
-        if (!STATE)
-            stage<T>(qs + b * L * DK, DK, q + t0 * a.qs[1], a.qs[1], m, (int)a.dk, vec_q);
-        stage<T>(ks + b * L * DK, DK, k + t0 * a.ks[1], a.ks[1], m, (int)a.dk, vec_k);
-        stage<T>(vs + b * L * vtile, vtile, v + t0 * a.vs[1], a.vs[1], m, cols, vec_v);
+        if (!STATE) get_q(qs + b * L * DK, DK, q + t0 * a.qs[1], a.qs[1], m);
+        get_k(ks + b * L * DK, DK, k + t0 * a.ks[1], a.ks[1], m);
+        get_v(vs + b * L * vtile, vtile, v + t0 * a.vs[1], a.vs[1], m);
         cp_async_commit();
     };
     // Per token: the factor on u before it (1: none), 1 / A and scale * A.
-    // log A is a 64-bit sum: a head that forgets over thousands of tokens adds
-    // as many equal decays, whose roundings in 32 bits all point one way.
+    // log A is carried in 64 bits (the 16 decays of a chunk are added in 32): a head
+    // that forgets over thousands of tokens adds as many equal decays, whose
+    // roundings in 32 bits would all point one way.
     double run = 0.0;                 // log A after the chunk (warp 0)
     double span_g = 0.0;              // STATE: the sum of all log decays
     auto factors = [&](int n) {
@@ -142,16 +158,15 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
         const float gt = lane < m ? g[(t0 + lane) * a.gs[1]] : 0.0f;
-        double cum = gt;
-        float ren = 0.0f;
+        float pre = gt, ren = 0.0f;
         bool r = false;
 #pragma unroll
         for (int s = 1; s < L; s <<= 1) {
-            const double below = __shfl_up_sync(0xffffffffu, cum, s);
-            if (lane >= s) cum += below;
+            const float below = __shfl_up_sync(0xffffffffu, pre, s);
+            if (lane >= s) pre += below;
         }
-        if (STATE) span_g += __shfl_sync(0xffffffffu, cum, L - 1);
-        cum += run;
+        if (STATE) span_g += (double)__shfl_sync(0xffffffffu, pre, L - 1);
+        double cum = run + (double)pre;
         // false for NaN and infinities too
         if (__all_sync(0xffffffffu, lane >= m || fabs(cum) <= kRun)) {
             run = __shfl_sync(0xffffffffu, cum, m - 1);
@@ -166,7 +181,9 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         if (lane < L) {
             const float hi = (float)cum, lo = (float)(cum - (double)hi);
             const float dn = expf(-hi), up = expf(hi);
-            s_ren[b][lane] = r ? expf(ren) : 1.0f;
+            float again = 1.0f;
+            if (r) again = expf(ren);
+            s_ren[b][lane] = again;
             s_inv[b][lane] = fmaf(dn, -lo, dn);
             s_out[b][lane] = fmaf(up, lo, up) * a.scale;
         }
@@ -189,7 +206,9 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         const float *qb = qs + b * L * DK + 4 * kg;
         const float *kb = ks + b * L * DK + 4 * kg;
         const float *vb = vs + b * L * vtile + col;
-        for (int t = 0; t < m; ++t) {
+        T *to = o + t0 * a.os[1] + col;
+#pragma unroll 1
+        for (int t = 0; t < m; ++t, to += a.os[1]) {
             const float ren = s_ren[b][t];
             if (ren != 1.0f) {
                 const uint64_t r2 = pair(ren);
@@ -227,7 +246,6 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
                     r1 += __shfl_xor_sync(0xffffffffu, r1, s);
                 }
                 const float f = s_out[b][t];
-                T *const to = o + (t0 + t) * a.os[1] + col;
                 if (kg == 0 && col < cols) {
                     to[0] = io<T>::from_f(r0 * f);
                     if (col + 1 < cols) to[1] = io<T>::from_f(r1 * f);
@@ -409,7 +427,7 @@ static Plan plan(Args &a) {
     const int sms = num_sms();
     const bool tc = chunked_fits(a);
     const int64_t walks = a.seqs * a.heads * ceil_div(a.dv, 64);
-    a.seg = segment_tokens(a, walks, tc ? sms : 4 * sms, tc ? 128 : 32, tc ? 0.65 : 0.35);
+    a.seg = segment_tokens(a, walks, tc ? sms : 4 * sms, tc ? 128 : 32, tc ? 0.65 : 0.6);
     a.slots = 0;
     Plan p = {};
     if (a.seg == 0) return p;
