@@ -80,7 +80,7 @@ template <typename T> struct Stager {
 
 // STATE: the pass over segments that leaves their states; no q, no outputs
 template <typename T, int KG, int R, bool STATE>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(KG == 1 ? 32 : 128, KG == 1 ? 14 : 3)
 decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec_v) {
     constexpr int DK = KG * R, QUADS = R / 4;              // padded rows
     extern __shared__ __align__(16) float smem_f[];
@@ -283,18 +283,18 @@ static bool vec16(const void *p, const int64_t (&s)[3], int64_t cols) {
 template <typename T, int KG, int R, bool STATE>
 static int launch_recurrent(const Args &a, cudaStream_t st) {
     constexpr int WV = 64 / KG;                            // columns of a warp
-    const int warps = (int)(ceil_div(a.dv, WV) < 4 ? ceil_div(a.dv, WV) : 4);
+    const int most = KG == 1 ? 1 : 4;
+    const int warps = (int)(ceil_div(a.dv, WV) < most ? ceil_div(a.dv, WV) : most);
     const int vtile = warps * WV;
     const int64_t grid = ceil_div(a.dv, vtile) * a.heads * spans(a);
     MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
     const size_t smem = sizeof(float) * 2 * L * ((STATE ? 1 : 2) * KG * R + vtile);
     auto kern = decay_recurrent_kernel<T, KG, R, STATE>;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem);
-        if (e != cudaSuccess)
-            return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
-    }
+    // all of the SM's shared memory: the walks resident at once are what hides latency
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e == cudaSuccess && smem > 48 * 1024)
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
     kern<<<(unsigned)grid, warps * 32, smem, st>>>(a, vtile, vec16<T>(a.q, a.qs, a.dk),
                                                    vec16<T>(a.k, a.ks, a.dk),
                                                    vec16<T>(a.v, a.vs, a.dv));
@@ -422,12 +422,14 @@ static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64
 struct Plan { size_t slot0, g, state, bytes; };
 // how a call runs: sets a.seg and a.slots; the parts of its workspace
 static Plan plan(Args &a) {
-    // tensor cores: one walk of 64 columns an SM, 128 tokens a step; recurrent: four
-    // walks of up to 64 columns an SM, compared by 32 tokens
+    // tensor cores: one walk of 64 columns an SM, 128 tokens a step; recurrent: 14
+    // (up to 32 rows, one warp) or about 3 walks (four warps), compared by 32 tokens
     const int sms = num_sms();
     const bool tc = chunked_fits(a);
-    const int64_t walks = a.seqs * a.heads * ceil_div(a.dv, 64);
-    a.seg = segment_tokens(a, walks, tc ? sms : 4 * sms, tc ? 128 : 32, tc ? 0.65 : 0.6);
+    const int64_t cols = tc || a.dk <= 32 ? 64 : a.dk <= 64 ? 128 : a.dk <= 128 ? 64 : 32;
+    const int64_t walks = a.seqs * a.heads * ceil_div(a.dv, cols);
+    a.seg = segment_tokens(a, walks, tc ? sms : a.dk <= 32 ? 14 * sms : 3 * sms, tc ? 128 : 32,
+                           tc ? 0.65 : 0.6);
     a.slots = 0;
     Plan p = {};
     if (a.seg == 0) return p;
