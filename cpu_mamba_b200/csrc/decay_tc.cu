@@ -15,26 +15,35 @@
 // scans, so strong decays earlier in a chunk cost later differences nothing; g
 // below -256 counts as -256, whose e^g is below every fp32 product's reach.
 //
-// Roundings to bf16: P and S0 as MMA operands (the products of a flash-attention
-// style kernel; outputs are bf16 anyway).  V~ is held as three bf16 parts
-// (24 bits), because the state is an fp32 output and lives for many chunks.
+// Roundings to bf16: P and S0 as MMA operands; each costs an output about as much
+// as its own rounding (2.3e-3 relative in all, 1.7e-3 for the output's alone).  V~
+// is held as three bf16 parts (24 bits), because the state is an fp32 output and
+// lives for many chunks.
 //
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone.
 //
 // Roles (28 warps): 0-7 the state, 8-15 P, 16-19 the output rows, 20-23 V~, 24 and
 // 25 MMA issue, 26 TMA loads, 27 decays.  One MMA warp issues P V (n), Q K^T (n + 1),
-// the other K^T V~ (n), Q S0 (n), each as soon as its operands are there,
-// so that P (n + 1) and the state update overlap the others' MMAs.  Every
+// the other K^T V~ (n), Q S0 (n), each as soon as its operands are there.  Every
 // mbarrier completes once per chunk (staged ones once per two), so its phase
 // follows from the chunk count.  All waits are bounded; a wait that expires sets
 // the device status.
 //
-// Instruction supply is what this layout is built around: five roles' warps
-// share each scheduler's small instruction cache, and with straight-line bodies
-// (the state in registers, 500 instructions a role) a chunk took 11,000 cycles,
-// half of them stalled for instructions.  So each role's chunk is a short loop
-// over 16-column pieces, and the state lives in TMEM.
+// Bound: neither bytes nor MMAs (2100 cycles a chunk) but the chain of hand-overs
+// between the roles, about 4300 cycles = 2.3 us a chunk with 128-wide q and k, one
+// CTA an SM (shared memory and TMEM are full).  What brought it there, at 8
+// sequences of 8192 tokens, 24 heads of 128 x 64 (1.5 us of HBM time a chunk):
+//   733 us  one role after the other, the state in registers
+//   411     a short loop over 16-column pieces per role instead of straight-line
+//           code, the state in TMEM: five roles share each scheduler's instruction
+//           cache, and half of all issue slots waited for instructions
+//   336     output rows through shared memory and TMA: 32 rows a store instruction
+//           blocked the load/store unit for everyone
+//   327     MMA descriptors provably uniform (else every MMA moves six operands
+//           into uniform registers first)
+//   303     two MMA warps, eight warps for the state, P's factors before its scores,
+//           tiles fetched into L2 a chunk ahead
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -286,7 +295,8 @@ __device__ __forceinline__ float load_g(const Args &a, const Item &it, int t) {
 __device__ __forceinline__ float clamp_g(float g) { return g < -256.0f ? -256.0f : g; }
 
 // Bounded waits: about 20 cycles a try, 2^27 tries.  (A try_wait with a time hint
-// sleeps instead of polling, but wakes late: 393 -> 445 us at 8 x 8192.)
+// sleeps instead of polling, but wakes later; polling by one lane takes 400 cycles a
+// hand-over instead of 170.)
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int where) {
     uint32_t ok, tries = 0;
     do {
@@ -917,6 +927,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                                 __uint_as_float(z[i])));
                     __syncwarp();
                 }
+                fence_async_smem();                      // the stage is a TMA load's next
                 fence_before();
                 mbar_arrive(o_free);
             }
