@@ -315,6 +315,9 @@ __device__ __forceinline__ void warp_best(uint64_t &v, int &at) {
     v = (uint64_t)top << 32 | low;
 }
 
+// a launch has 48 KB of shared memory, the kernel's own arrays (1.6 KB) among them
+constexpr size_t MERGE_STAGE = 46 * 1024;
+
 __global__ void __launch_bounds__(1024)
 beam_merge_kernel(const MergeArgs a) {
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -575,7 +578,7 @@ extern "C" int mb2_beam_select(int dtype, const void *logits, int64_t batch_stri
     // at most 32 x 2^20 candidates a batch: flat indices are 32-bit
     const int threads = lists <= 256 ? 256 : lists <= 512 ? 512 : 1024;
     const size_t staged = (size_t)lists * num * 12 + sizeof(int) * (size_t)lists;
-    g.staged = staged <= 48 * 1024;
+    g.staged = staged <= MERGE_STAGE;
     beam_merge_kernel<<<(unsigned)batch, threads, g.staged ? staged : sizeof(int) * lists, st>>>(g);
     return check_launch("beam_merge_kernel");
 }

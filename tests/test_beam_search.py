@@ -79,6 +79,14 @@ def test_select(B, K, V, num, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("K,V", [(29, 9000), (31, 9000), (32, 9000)])
+def test_select_lists_around_the_shared_memory_limit(K, V):
+    """58, 62 and 64 lists of 64 entries: 44776, 47864 and 49408 bytes staged."""
+    g = torch.Generator().manual_seed(K)
+    check(torch.randn(1, K, V, generator=g) * 3, torch.zeros(1, K), 64)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_select_ties_go_to_the_lowest_index(dtype):
     """All logits equal; logits on a coarse grid; equal beams."""
