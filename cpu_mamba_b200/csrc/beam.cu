@@ -5,22 +5,24 @@
 //   scores[k] + logits[k, v] - log sum_v' exp(logits[k, v'])
 // and the best `num` of all K V candidates come out in order, ties to the
 // lowest beam, then the lowest token.  Two kernels:
-//   beam_rows   one CTA per (row, slice of 8192 logits or so): the slice stays
-//               in registers, so the logits are read once; its maximum, its sum
+//   beam_rows   one CTA per (row, slice of up to 32 KB): the slice stays in
+//               registers, so the logits are read once; its maximum, its sum
 //               of exponentials and its best `num` (value, token) pairs
 //   beam_merge  one CTA per batch: the rows' normalisers (64-bit sums of the
 //               slices') and a merge of the slices' sorted lists, comparing the
 //               candidates' 64-bit values
-// Bound: the logits' read (HBM).
+// The logits have to be read once; what bounds each kernel instead stands there.
 #include "common.cuh"
+#include "pair.cuh"
 
 namespace mb2 {
 namespace {
 
 constexpr int ROW_THREADS = 256;
-constexpr int EPT = 32;                       // logits per thread
-constexpr int SLICE = ROW_THREADS * EPT;
+constexpr int NV = 8;                         // 16-byte vectors of logits per thread, at most
+constexpr int SLICE = ROW_THREADS * NV;       // vectors of a slice, at most
 constexpr int LIST = 1024;                    // candidates above a slice's threshold
+constexpr int HELD = 256;                     // vectors with a value at the threshold
 constexpr int MAX_NUM = 64;
 constexpr int MAX_BEAMS = 32;
 constexpr int MAX_VOCAB = 1 << 20;
@@ -39,6 +41,7 @@ struct RowArgs {
     const void *logits;
     int64_t s_batch, s_beam;                  // strides
     int beams, vocab, num, splits;
+    int per;                                  // 16-byte vectors of a slice
     const uint8_t *finished;
     float *part_max, *part_sum;               // (rows, splits)
     uint64_t *part_list;                      // (rows, splits, num): key << 32 | ~token, 0: none
@@ -86,18 +89,26 @@ template <> struct Word<__nv_bfloat16> {
     }
 };
 
-// The slice is kept as it was loaded (16 or 32 registers a thread; as fp32 keys it
-// was 60 us at 512 rows of 50257 bf16 logits, so 33 us = 1.6 TB/s).
+// The slice is kept as it was loaded (32 registers a thread), four CTAs to an SM.
+// 512 rows of 50257 bf16 logits, 25 us = 2.1 TB/s: issue slots bound it, half of
+// them the search for the best, whose cost per slice does not shrink with it.
+//   as fp32 keys                                     60 us
+//   as loaded, slices of 16 KB                       33
+//   slices of 32 KB, three CTAs to an SM             28
+//   four                                             25   (64 KB, two: 27)
+// Loads and maxima alone take 7 us, the exponentials 4 more.
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 4 : 3)
+__global__ void __launch_bounds__(ROW_THREADS, 4)
 beam_rows_kernel(const RowArgs a) {
-    constexpr int VEC = 16 / (int)sizeof(T), NV = EPT / VEC, WARPS = ROW_THREADS / 32;
+    constexpr int VEC = 16 / (int)sizeof(T), WARPS = ROW_THREADS / 32;
     constexpr int WN = Word<T>::N;                // values per 32-bit word
     __shared__ uint64_t list[LIST];
     __shared__ uint64_t best[WARPS];
     __shared__ float redf[2][WARPS];
     __shared__ uint32_t reach_key[WARPS];
-    __shared__ int count;
+    __shared__ uint4 held_vec[HELD];
+    __shared__ int held_at[HELD];
+    __shared__ int count, held;
     const int split = blockIdx.x, row = blockIdx.y;
     if (a.finished && a.finished[row]) return;              // beam_merge writes its candidates
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -108,8 +119,8 @@ beam_rows_kernel(const RowArgs a) {
     const int lead = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
     const T *base = p - lead;
     const int nvec = (a.vocab + lead + VEC - 1) / VEC;
-    const int v0 = split * (ROW_THREADS * NV) + tid;
-    if (tid == 0) count = 0;
+    const int v0 = split * a.per + tid, end = min(nvec, (split + 1) * a.per);
+    if (tid == 0) count = held = 0;
 
     constexpr uint32_t kNone = Word<T>::N == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
     uint32_t raw[NV][4];
@@ -117,14 +128,14 @@ beam_rows_kernel(const RowArgs a) {
     for (int j = 0; j < NV; ++j) {
         const int v = v0 + j * ROW_THREADS;
         uint4 x = make_uint4(kNone, kNone, kNone, kNone);
-        if (v < nvec) x = __ldcs(reinterpret_cast<const uint4 *>(base) + v);
+        if (v < end) x = __ldcs(reinterpret_cast<const uint4 *>(base) + v);
         raw[j][0] = x.x; raw[j][1] = x.y; raw[j][2] = x.z; raw[j][3] = x.w;
     }
     // token of value (j, w, i)
     auto token = [&](int j, int w, int i) {
         return (v0 + j * ROW_THREADS) * VEC + w * WN + i - lead;
     };
-    uint32_t wmax = kNone;
+    uint32_t vmax[NV], wmax = kNone;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int v = v0 + j * ROW_THREADS;
@@ -137,30 +148,29 @@ beam_rows_kernel(const RowArgs a) {
                     raw[j][w] = Word<T>::masked(raw[j][w], i, t >= 0 && t < a.vocab);
                 }
         }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) wmax = Word<T>::max(wmax, raw[j][w]);
+        vmax[j] = Word<T>::max(Word<T>::max(raw[j][0], raw[j][1]),
+                               Word<T>::max(raw[j][2], raw[j][3]));
+        wmax = Word<T>::max(wmax, vmax[j]);
     }
     const float tmax = fmaxf(Word<T>::top(wmax), -INFINITY);
-    float m = tmax;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) redf[0][wid] = m;
 
     // A threshold that at least `num` threads reach by their largest value, so that
     // the slice's best `num` are among the values at or above it: the least of the
     // warps' ceil(num / 8)-th largest thread maxima.
     const int quota = (a.num + WARPS - 1) / WARPS;
-    const uint32_t kmax = v0 < nvec ? order_key(tmax) : 0u;
+    const uint32_t kmax = v0 < end ? order_key(tmax) : 0u;
     {
         uint32_t left = kmax, got = 0;
         for (int r = 0; r < quota; ++r) {
             got = __reduce_max_sync(0xffffffffu, left);
+            if (r == 0 && lane == 0) redf[0][wid] = got ? key_value(got) : -INFINITY;
             const uint32_t who = __ballot_sync(0xffffffffu, left == got);
             if (lane == __ffs(who) - 1) left = 0;
         }
         if (lane == 0) reach_key[wid] = got;                 // 0: fewer threads than that
     }
     __syncthreads();
+    float m = -INFINITY;
     uint32_t thr = 0xffffffffu;
     int full = 0;
 #pragma unroll
@@ -175,21 +185,30 @@ beam_rows_kernel(const RowArgs a) {
     // x - m first: a large common offset has to cancel.  All masked: every term is
     // e^-inf; a NaN or +inf makes the sum NaN
     const float off = m == -INFINITY ? 0.0f : m;
-    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint64_t noff = pair(-off), log2e = pair(kLog2e);
+    uint64_t sums[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        if (v0 - lane + j * ROW_THREADS >= end) break;       // behind the slice, for the whole warp
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int i = 0; i < WN; ++i)
-                sums[w] += ex2((Word<T>::at(raw[j][w], i) - off) * kLog2e);
-    float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        for (int n = 0; n < VEC; n += 2) {
+            const uint64_t y = mul2(add2(pair(__float_as_uint(Word<T>::at(raw[j][n / WN], n % WN)),
+                                              __float_as_uint(Word<T>::at(raw[j][(n + 1) / WN],
+                                                                          (n + 1) % WN))),
+                                         noff), log2e);
+            sums[n / 2 % 2] = add2(sums[n / 2 % 2],
+                                   pair(__float_as_uint(ex2(__uint_as_float(lo_of(y)))),
+                                        __float_as_uint(ex2(__uint_as_float(hi_of(y))))));
+        }
+    }
+    sums[0] = add2(sums[0], sums[1]);
+    float sum = __uint_as_float(lo_of(sums[0])) + __uint_as_float(hi_of(sums[0]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) redf[1][wid] = sum;
 
     if (full * quota < a.num) {
-        // a row's last, short slice: bisection of the key's bits, stopped once few
+        // a short slice or a large `num`: bisection of the key's bits, stopped once few
         // more threads than needed reach it
         thr = 1;
         const int reach = __syncthreads_count(kmax > 0);
@@ -211,25 +230,33 @@ beam_rows_kernel(const RowArgs a) {
             thr = least;
         }
     }
-    if (kmax >= thr) {
-        // a word without a value at the threshold is passed over at once; NaN (worth
-        // -inf) only counts where the threshold is that low
+    // The vectors with a value at the threshold (NaN, worth -inf, only counts where
+    // the threshold is that low) go through shared memory, so that their values are
+    // looked at by as many threads: taken from the registers, that is 1000 instructions
+    // of which a few are used.
+    {
         const uint32_t tw = Word<T>::splat(key_value(thr));
         const bool all = thr <= order_key(-INFINITY);
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if (!all && !Word<T>::reaches(raw[j][w], tw)) continue;
-                for (int i = 0; i < WN; ++i) {
-                    const uint32_t k = order_key(Word<T>::at(raw[j][w], i));
-                    const int t = token(j, w, i);
-                    if (k >= thr && t >= 0 && t < a.vocab) {
-                        const int at = atomicAdd(&count, 1);
-                        if (at < LIST) list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)t;
-                    }
+        for (int j = 0; j < NV; ++j) {
+            if (v0 + j * ROW_THREADS < end && (all || Word<T>::reaches(vmax[j], tw))) {
+                const int at = atomicAdd(&held, 1);
+                if (at < HELD) {
+                    held_vec[at] = make_uint4(raw[j][0], raw[j][1], raw[j][2], raw[j][3]);
+                    held_at[at] = v0 + j * ROW_THREADS;
                 }
             }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < min(held, HELD) * VEC; i += ROW_THREADS) {
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(held_vec);
+        const uint32_t k = order_key(Word<T>::at(words[i / WN], i % WN));
+        const int t = held_at[i / VEC] * VEC + i % VEC - lead;
+        if (k >= thr && t >= 0 && t < a.vocab) {
+            const int at = atomicAdd(&count, 1);
+            if (at < LIST) list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)t;
+        }
     }
     __syncthreads();
     const int64_t part = (int64_t)row * a.splits + split;
@@ -241,32 +268,37 @@ beam_rows_kernel(const RowArgs a) {
         a.part_sum[part] = s;
     }
     const int c = count;
-    if (c <= LIST) {
+    if (held <= HELD && c <= LIST) {
         // distinct entries: each one's rank is the number of larger ones
-        for (int i = tid; i < c; i += ROW_THREADS) {
+        for (int i = wid; i < c; i += WARPS) {
             const uint64_t mine = list[i];
             int rank = 0;
-            for (int j = 0; j < c; ++j) rank += list[j] > mine;
-            if (rank < a.num) out[rank] = mine;
+            for (int j = 0; j < c; j += 32)
+                rank += __popc(__ballot_sync(0xffffffffu, j + lane < c && list[j + lane] > mine));
+            if (lane == 0 && rank < a.num) out[rank] = mine;
         }
         for (int i = c + tid; i < a.num; i += ROW_THREADS) out[i] = 0;
         return;
     }
-    // many equal logits at the threshold: pick one after the other
+    // many equal logits at the threshold: pick one after the other, from memory again
+    // (the values kept in registers for this would cost every call its occupancy)
     uint64_t last = ~0ull;
     for (int n = 0; n < a.num; ++n) {
         uint64_t b = 0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
+#pragma unroll 1
+        for (int v = v0; v < end; v += ROW_THREADS) {
+            const uint4 x = reinterpret_cast<const uint4 *>(base)[v];
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int i = 0; i < WN; ++i) {
-                    const int t = token(j, w, i);
-                    const uint64_t e = (uint64_t)order_key(Word<T>::at(raw[j][w], i)) << 32 |
+                    const int t = v * VEC + w * WN + i - lead;
+                    const uint64_t e = (uint64_t)order_key(Word<T>::at(words[w], i)) << 32 |
                                        (uint32_t)~(uint32_t)t;
                     if (t >= 0 && t < a.vocab && e < last && e > b) b = e;
                 }
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const uint64_t x = __shfl_xor_sync(0xffffffffu, b, o);
@@ -318,6 +350,9 @@ __device__ __forceinline__ void warp_best(uint64_t &v, int &at) {
 // a launch has 48 KB of shared memory, the kernel's own arrays (1.6 KB) among them
 constexpr size_t MERGE_STAGE = 46 * 1024;
 
+// Bound: latency, a chain of `num` warp reductions behind three dependent reads (64
+// batches of 32 lists of 16: 9.1 us, of which 16 rounds 4; with the outputs written
+// inside the rounds 10.2; lists of 16 KB slices, 56 of them, 13).
 __global__ void __launch_bounds__(1024)
 beam_merge_kernel(const MergeArgs a) {
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -433,6 +468,10 @@ beam_merge_kernel(const MergeArgs a) {
         }
     };
     refresh();
+    // the n-th best stays with lane n % 32 of the first warp, written when all are known
+    uint64_t kept[2] = {0, 0};
+    int kept_at[2] = {INT32_MAX, INT32_MAX};
+#pragma unroll 1
     for (int n = 0; n < a.num; ++n) {
         uint64_t bv = val;
         int ba = at;
@@ -440,22 +479,30 @@ beam_merge_kernel(const MergeArgs a) {
         if (active > 1) {
             if (lane == 0) { w_val[n & 1][wid] = bv; w_at[n & 1][wid] = ba; }
             __syncthreads();
-            bv = w_val[n & 1][0]; ba = w_at[n & 1][0];
-            for (int w = 1; w < active; ++w)
-                if (better(w_val[n & 1][w], w_at[n & 1][w], bv, ba)) {
-                    bv = w_val[n & 1][w]; ba = w_at[n & 1][w];
-                }
+            bv = lane < active ? w_val[n & 1][lane] : 0;
+            ba = lane < active ? w_at[n & 1][lane] : INT32_MAX;
+            warp_best(bv, ba);
         }
         if (ba == INT32_MAX) break;           // num <= beams x vocab: not reached
+        if (lane == (n & 31)) {
+            if (n < 32) { kept[0] = bv; kept_at[0] = ba; }
+            else { kept[1] = bv; kept_at[1] = ba; }
+        }
         if (at == ba) {                       // the thread that offered it
-            const int64_t i = (int64_t)batch * a.num + n;
-            a.out_scores[i] = (float)key_value64(bv);
-            a.out_parents[i] = ba / a.vocab;
-            a.out_tokens[i] = ba % a.vocab;
             ++heads[which];
             refresh();
         }
         __syncwarp();
+    }
+    if (wid != 0) return;
+#pragma unroll
+    for (int r = 0; r < MAX_NUM / 32; ++r) {
+        const int n = r * 32 + lane;
+        if (n >= a.num || kept_at[r] == INT32_MAX) continue;
+        const int64_t i = (int64_t)batch * a.num + n;
+        a.out_scores[i] = (float)key_value64(kept[r]);
+        a.out_parents[i] = kept_at[r] / a.vocab;
+        a.out_tokens[i] = kept_at[r] % a.vocab;
     }
 }
 
@@ -508,11 +555,19 @@ reorder_kernel(const __grid_constant__ Reorder r) {
     else move_rows<uint8_t, KMAX>(p, row_bytes, i, K, src);
 }
 
-// slices of a row; one more element vector where the row may start off a
-// 16-byte boundary
-int beam_splits(int64_t vocab, size_t e) {
+// a row's 16-byte vectors (one more where it may start off a 16-byte boundary) and
+// its slices, which share them evenly: a short last slice has no `num` threads of
+// its own at a threshold and would have to search for one.  Few rows are cut in
+// slices of 16 KB, for more of the SMs (16 rows of 32000 fp32 logits: 4.7 us, in
+// slices of up to 64 KB 5.5).
+int64_t beam_vecs(int64_t vocab, size_t e) {
     const int64_t vec = 16 / (int64_t)e;
-    return (int)ceil_div(ceil_div(vocab + vec - 1, vec), SLICE / vec);
+    return ceil_div(vocab + vec - 1, vec);
+}
+int beam_splits(int64_t rows, int64_t vocab, size_t e) {
+    const int64_t n = beam_vecs(vocab, e), fill = 4 * 148;
+    const int64_t most = ceil_div(n, SLICE / 2), least = ceil_div(n, SLICE);
+    return (int)std::max(least, std::min(most, ceil_div(fill, rows)));
 }
 
 }  // namespace
@@ -523,7 +578,7 @@ using namespace mb2;
 extern "C" size_t mb2_beam_select_workspace_bytes(int dtype, int64_t batch, int64_t beams,
                                                   int64_t vocab, int64_t num) {
     if (batch <= 0 || beams <= 0 || vocab <= 0 || num <= 0 || vocab > MAX_VOCAB) return 0;
-    const size_t lists = (size_t)(batch * beams) * beam_splits(vocab, dtype_size(dtype));
+    const size_t lists = (size_t)(batch * beams) * beam_splits(batch * beams, vocab, dtype_size(dtype));
     return lists * ((size_t)num * 8 + 8);
 }
 
@@ -551,13 +606,14 @@ extern "C" int mb2_beam_select(int dtype, const void *logits, int64_t batch_stri
                     workspace,
                 MB2_ERR_WORKSPACE, "beam_select: workspace too small");
     MB2_REQUIRE(aligned(workspace, 8), MB2_ERR_ALIGN, "beam_select: misaligned workspace");
-    const int splits = beam_splits(vocab, dtype_size(dtype));
+    const int splits = beam_splits(batch * beams, vocab, dtype_size(dtype));
     const int64_t rows = batch * beams;
     RowArgs r;
     r.logits = logits;
     r.s_batch = batch_stride;
     r.s_beam = beam_stride;
     r.beams = (int)beams; r.vocab = (int)vocab; r.num = (int)num; r.splits = splits;
+    r.per = (int)ceil_div(beam_vecs(vocab, dtype_size(dtype)), splits);
     r.finished = finished;
     r.part_list = static_cast<uint64_t *>(workspace);
     r.part_max = reinterpret_cast<float *>(r.part_list + rows * splits * num);

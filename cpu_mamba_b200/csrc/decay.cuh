@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "pair.cuh"
 
 namespace mb2 {
 namespace decay {
@@ -36,33 +37,6 @@ struct Span {
     int64_t seq, row0, len;
     int64_t in, out;                      // state to start from (-1: 0) and to leave (-1: none)
 };
-
-// two fp32 values in one register pair (packed FMA: half the instructions)
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ uint64_t pair(float v) {
-    return pair(__float_as_uint(v), __float_as_uint(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t lo_of(uint64_t v) { return (uint32_t)v; }
-__device__ __forceinline__ uint32_t hi_of(uint64_t v) { return (uint32_t)(v >> 32); }
 
 __device__ __forceinline__ int64_t clamp_row(int64_t r, int64_t n) {
     return r < 0 ? 0 : (r > n ? n : r);

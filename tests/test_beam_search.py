@@ -68,7 +68,8 @@ def check(logits, scores, num, finished=None, pad=0, exact=False):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("B,K,V,num", [(1, 1, 1, 1), (2, 3, 5, 15), (1, 2, 7, 4), (3, 4, 100, 8),
                                        (2, 5, 8191, 5), (2, 4, 8192, 8), (1, 3, 8200, 6),
-                                       (2, 8, 50257, 16), (1, 32, 16400, 64), (1, 2, 131073, 33)])
+                                       (2, 8, 50257, 16), (1, 32, 16400, 64), (1, 2, 131073, 33),
+                                       (149, 4, 9001, 3), (150, 4, 17000, 12)])
 def test_select(B, K, V, num, dtype):
     g = torch.Generator().manual_seed(V + K)
     logits = (torch.randn(B, K, V, generator=g) * 3).to(dtype)
