@@ -21,6 +21,8 @@ struct Args {
     float *h_last;                        // same, or null
     const int32_t *cu;                    // seqs + 1 offsets of packed sequences, or null
     float scale;
+    int recurrent;                        // not for the tensor cores
+    int narrow;                           // recurrent: a state spread over more lanes
     // A sequence may be walked in segments of `seg` tokens (0: whole) side by side:
     // a first pass leaves every segment's own final state (from 0) and the sum of
     // its log decays, seg_states turns them into the segments' initial states, and

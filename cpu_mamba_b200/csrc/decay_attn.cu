@@ -10,6 +10,8 @@
 // kernel.
 #include "decay.cuh"
 
+#include <type_traits>
+
 namespace mb2 {
 namespace decay {
 
@@ -32,21 +34,22 @@ namespace decay {
 // loads of k and q (two 16-byte loads per 8 packed FMAs).  One warp per head of 64
 // columns instead of four with eight lanes a column: 425 -> 192 us at 151 sequences
 // of 180 tokens, 24 heads of 24 x 64 (the FMAs alone take about 80).
-constexpr int L = 16;                 // tokens staged at a time
+// tokens staged at a time: more where few walks wait for each step's latency
+template <int R> __host__ __device__ constexpr int stage_tokens() { return R == 8 ? 32 : 16; }
 constexpr float kRun = 5.5f;          // bound on |log A| within a run
 
 // Copies rows [0, n) of a strided matrix into shared memory as fp32 (pitch
-// `pitch`): 16-byte asynchronous copies of fp32 rows that allow them, else through
-// registers.  A thread's place in a row and its step are divided out once.
+// `pitch`): asynchronous copies of fp32 rows, 16 bytes each where they allow it;
+// bf16 rows through registers.  A thread's place in a row and its step are divided out once.
 template <typename T> struct Stager {
     int per, r, c, dr, dc;                // pieces a row; first piece; step
     bool vec;
-    __device__ __forceinline__ Stager(int cols, bool vec_) : vec(vec_) {
+    __device__ __forceinline__ Stager(int cols, bool vec_, int tid, int threads) : vec(vec_) {
         per = vec ? cols / (16 / (int)sizeof(T)) : cols;
-        r = (int)threadIdx.x / per;
-        c = (int)threadIdx.x - r * per;
-        dr = (int)blockDim.x / per;
-        dc = (int)blockDim.x - dr * per;
+        r = tid / per;
+        c = tid - r * per;
+        dr = threads / per;
+        dc = threads - dr * per;
     }
     __device__ __forceinline__ void operator()(float *dst, int pitch, const T *src, int64_t ld,
                                                int n) const {
@@ -67,7 +70,8 @@ template <typename T> struct Stager {
                             __uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
                 }
             } else {
-                dst[y * pitch + x] = io<T>::to_f(src[y * ld + x]);
+                if constexpr (sizeof(T) == 4) cp_async4(dst + y * pitch + x, src + y * ld + x);
+                else dst[y * pitch + x] = io<T>::to_f(src[y * ld + x]);
             }
             y += dr;
             x += dc;
@@ -79,17 +83,24 @@ template <typename T> struct Stager {
     }
 };
 
+// R rows and two columns of the state a lane, KG lanes a column pair.  R 16 to 32 is for
+// calls that fill the machine.  R 8 is for few walks, where the step's latency is the
+// call's time: eight tokens at once unless a run starts among them (one after the other
+// 0.24 us a token, four 0.22), and other warps stage what comes next (beside the walk
+// 0.20; with eight tokens 0.12; R 32 without any of it 0.36).
 // STATE: the pass over segments that leaves their states; no q, no outputs
 template <typename T, int KG, int R, bool STATE>
-__global__ void __launch_bounds__(KG == 1 ? 32 : 128, KG == 1 ? 14 : 3)
+__global__ void __launch_bounds__(KG == 1 ? 32 : R == 8 ? 256 : 128, KG == 1 ? 14 : R == 8 ? 2 : 3)
 decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec_v, bool pair_o) {
     constexpr int DK = KG * R, QUADS = R / 4;              // padded rows
+    constexpr int L = stage_tokens<R>();
     extern __shared__ __align__(16) float smem_f[];
     float *const ks = smem_f;                              // [2][L][DK]
     float *const vs = ks + 2 * L * DK;                     // [2][L][vtile]
     float *const qs = vs + 2 * L * vtile;                  // [2][L][DK]
     // per token: the factor on u before it (1: none), 1 / A, scale * A
     __shared__ float4 s_f[2][L];
+    __shared__ uint32_t s_again[2];   // the chunk's tokens that start a run
 
     const int tiles = (int)ceil_div(a.dv, vtile);
     int64_t id = blockIdx.x;
@@ -112,6 +123,13 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     T *o = static_cast<T *>(a.o) + bq * a.os[0] + row0 * a.os[1] + h * a.os[2] + c0;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // R 8: three warps stage the next chunk and a fourth takes its factors, beside the
+    // warps that walk
+    const int walkers = (int)blockDim.x - (R == 8 ? 128 : 0);
+    const int loader = (int)threadIdx.x - (R == 8 ? walkers : 0);
+    const int loaders = R == 8 ? 96 : (int)blockDim.x;
+    const bool loads = loader >= 0 && loader < loaders;
+    const bool first = R == 8 ? loader >= 96 : warp == 0;
     const int kg = lane & (KG - 1);
     const int col = 2 * ((int)threadIdx.x / KG);           // this lane's two columns
 
@@ -139,7 +157,8 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     __syncthreads();
 
     const int nchunks = (int)ceil_div(len, (int64_t)L);
-    const Stager<T> get_q((int)a.dk, vec_q), get_k((int)a.dk, vec_k), get_v(cols, vec_v);
+    const Stager<T> get_q((int)a.dk, vec_q, loader, loaders), get_k((int)a.dk, vec_k, loader, loaders),
+        get_v(cols, vec_v, loader, loaders);
     auto load = [&](int n) {
         const int b = n & 1;
         const int64_t t0 = (int64_t)n * L;
@@ -152,13 +171,20 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     // log A is carried in 64 bits (the 16 decays of a chunk are added in 32): a head
     // that forgets over thousands of tokens adds as many equal decays, whose
     // roundings in 32 bits would all point one way.
-    double run = 0.0;                 // log A after the chunk (warp 0)
+    double run = 0.0;                 // log A after the chunk (the first warp)
     double span_g = 0.0;              // STATE: the sum of all log decays
+    // the next chunk's decay of this lane's token, loaded a chunk ahead
+    auto load_g = [&](int n) {
+        const int64_t t = (int64_t)n * L + lane;
+        return lane < L && t < len ? g[t * a.gs[1]] : 0.0f;
+    };
+    float gt_next = first ? load_g(0) : 0.0f;
     auto factors = [&](int n) {
         const int b = n & 1;
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
-        const float gt = lane < m ? g[(t0 + lane) * a.gs[1]] : 0.0f;
+        const float gt = gt_next;
+        gt_next = load_g(n + 1);
         float pre = gt, ren = 0.0f;
         bool r = false;
 #pragma unroll
@@ -179,6 +205,8 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
                 if (lane == t) { cum = run; ren = (float)next; r = !keep; }
             }
         }
+        const uint32_t again_mask = __ballot_sync(0xffffffffu, r);
+        if (lane == 0) s_again[b] = again_mask;
         if (lane < L) {
             const float hi = (float)cum, lo = (float)(cum - (double)hi);
             const float dn = expf(-hi), up = expf(hi);
@@ -189,82 +217,122 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     };
 
     if (nchunks > 0) {
-        load(0);
-        if (warp == 0) factors(0);
+        if (loads) load(0);
+        if (first) factors(0);
     }
     for (int n = 0; n < nchunks; ++n) {
         const int b = n & 1;
         cp_async_wait<0>();
         __syncthreads();              // chunk n staged; chunk n - 1 read by every warp
         if (n + 1 < nchunks) {
-            load(n + 1);
-            if (warp == 0) factors(n + 1);
+            if (loads) load(n + 1);
+            if (first) factors(n + 1);
         }
+        if (R == 8 && loader >= 0) continue;
         const int64_t t0 = (int64_t)n * L;
         const int m = (int)(len - t0 < L ? len - t0 : L);
         const float *qb = qs + b * L * DK + 4 * kg;
         const float *kb = ks + b * L * DK + 4 * kg;
         const float *vb = vs + b * L * vtile + col;
         T *to = o + t0 * a.os[1] + col;
-        constexpr int UNROLL = KG == 1 ? 2 : 1;            // more spills the wider states
-#pragma unroll UNROLL
-        for (int t = 0; t < m; ++t, to += a.os[1]) {
-            const float4 f = s_f[b][t];
-            if (f.x != 1.0f) {
-                const uint64_t r2 = pair(f.x);
+        // the start of a run
+        auto again = [&](int t) {
+            const float x = s_f[b][t].x;
+            if (x == 1.0f) return;
+            const uint64_t x2 = pair(x);
 #pragma unroll
-                for (int i = 0; i < 2 * QUADS; ++i)
+            for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) u[i][c] = mul2(u[i][c], r2);
+                for (int c = 0; c < 2; ++c) u[i][c] = mul2(u[i][c], x2);
+        };
+        // N tokens behind one another: their loads, sums over the lanes and stores overlap
+        auto tokens = [&](auto count, int t) {
+            constexpr int N = decltype(count)::value;
+            float4 f[N];
+            float2 vv[N];
+            float r0[N], r1[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                f[j] = s_f[b][t + j];
+                vv[j] = *reinterpret_cast<const float2 *>(vb + (t + j) * vtile);
             }
-            const float2 vv = *reinterpret_cast<const float2 *>(vb + t * vtile);
-            const uint64_t w0 = pair(vv.x * f.y), w1 = pair(vv.y * f.y);
-            uint64_t acc0 = 0, acc1 = 0;
 #pragma unroll
-            for (int i = 0; i < QUADS; ++i) {
-                const ulonglong2 kk = *reinterpret_cast<const ulonglong2 *>(kb + t * DK + 4 * KG * i);
-                u[2 * i][0] = fma2(kk.x, w0, u[2 * i][0]);
-                u[2 * i][1] = fma2(kk.x, w1, u[2 * i][1]);
-                u[2 * i + 1][0] = fma2(kk.y, w0, u[2 * i + 1][0]);
-                u[2 * i + 1][1] = fma2(kk.y, w1, u[2 * i + 1][1]);
-                if constexpr (!STATE) {
-                    const ulonglong2 qq =
-                        *reinterpret_cast<const ulonglong2 *>(qb + t * DK + 4 * KG * i);
-                    acc0 = fma2(qq.x, u[2 * i][0], acc0);
-                    acc1 = fma2(qq.x, u[2 * i][1], acc1);
-                    acc0 = fma2(qq.y, u[2 * i + 1][0], acc0);
-                    acc1 = fma2(qq.y, u[2 * i + 1][1], acc1);
-                }
-            }
-            if constexpr (!STATE) {
-                float r0 = __uint_as_float(lo_of(acc0)) + __uint_as_float(hi_of(acc0));
-                float r1 = __uint_as_float(lo_of(acc1)) + __uint_as_float(hi_of(acc1));
+            for (int j = 0; j < N; ++j) {
+                if (R != 8) again(t + j);
+                const uint64_t w0 = pair(vv[j].x * f[j].y), w1 = pair(vv[j].y * f[j].y);
+                uint64_t acc0 = 0, acc1 = 0;
 #pragma unroll
-                for (int s = 1; s < KG; s <<= 1) {
-                    r0 += __shfl_xor_sync(0xffffffffu, r0, s);
-                    r1 += __shfl_xor_sync(0xffffffffu, r1, s);
-                }
-                r0 *= f.z;
-                r1 *= f.z;
-                if (kg == 0 && col < cols) {
-                    if (pair_o) {
-                        if constexpr (sizeof(T) == 4)
-                            *reinterpret_cast<float2 *>(to) = make_float2(r0, r1);
-                        else
-                            *reinterpret_cast<__nv_bfloat162 *>(to) = __floats2bfloat162_rn(r0, r1);
-                    } else {
-                        to[0] = io<T>::from_f(r0);
-                        if (col + 1 < cols) to[1] = io<T>::from_f(r1);
+                for (int i = 0; i < QUADS; ++i) {
+                    const ulonglong2 kk =
+                        *reinterpret_cast<const ulonglong2 *>(kb + (t + j) * DK + 4 * KG * i);
+                    u[2 * i][0] = fma2(kk.x, w0, u[2 * i][0]);
+                    u[2 * i][1] = fma2(kk.x, w1, u[2 * i][1]);
+                    u[2 * i + 1][0] = fma2(kk.y, w0, u[2 * i + 1][0]);
+                    u[2 * i + 1][1] = fma2(kk.y, w1, u[2 * i + 1][1]);
+                    if constexpr (!STATE) {
+                        const ulonglong2 qq =
+                            *reinterpret_cast<const ulonglong2 *>(qb + (t + j) * DK + 4 * KG * i);
+                        acc0 = fma2(qq.x, u[2 * i][0], acc0);
+                        acc1 = fma2(qq.x, u[2 * i][1], acc1);
+                        acc0 = fma2(qq.y, u[2 * i + 1][0], acc0);
+                        acc1 = fma2(qq.y, u[2 * i + 1][1], acc1);
                     }
                 }
+                r0[j] = __uint_as_float(lo_of(acc0)) + __uint_as_float(hi_of(acc0));
+                r1[j] = __uint_as_float(lo_of(acc1)) + __uint_as_float(hi_of(acc1));
             }
+            if constexpr (!STATE) {
+#pragma unroll
+                for (int s = 1; s < KG; s <<= 1)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        r0[j] += __shfl_xor_sync(0xffffffffu, r0[j], s);
+                        r1[j] += __shfl_xor_sync(0xffffffffu, r1[j], s);
+                    }
+                if (kg == 0 && col < cols) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        T *const at = to + j * a.os[1];
+                        const float x0 = r0[j] * f[j].z, x1 = r1[j] * f[j].z;
+                        if (pair_o) {
+                            if constexpr (sizeof(T) == 4)
+                                *reinterpret_cast<float2 *>(at) = make_float2(x0, x1);
+                            else
+                                *reinterpret_cast<__nv_bfloat162 *>(at) = __floats2bfloat162_rn(x0, x1);
+                        } else {
+                            at[0] = io<T>::from_f(x0);
+                            if (col + 1 < cols) at[1] = io<T>::from_f(x1);
+                        }
+                    }
+                }
+                to += N * a.os[1];
+            }
+        };
+        if constexpr (R == 8) {
+            const uint32_t starts = s_again[b];
+#pragma unroll 1
+            for (int t = 0; t < m;) {
+                if (t + 8 <= m && !(starts >> t & 0xfeu)) {
+                    again(t);
+                    tokens(std::integral_constant<int, 8>{}, t);
+                    t += 8;
+                } else {
+                    again(t);
+                    tokens(std::integral_constant<int, 1>{}, t);
+                    ++t;
+                }
+            }
+        } else {
+            constexpr int UNROLL = KG == 1 ? 2 : 1;        // more spills the wider states
+#pragma unroll UNROLL
+            for (int t = 0; t < m; ++t) tokens(std::integral_constant<int, 1>{}, t);
         }
     }
-    if (STATE && threadIdx.x == 0 && tile == 0) a.seg_g[sp.out * a.heads + h] = span_g;
+    if (STATE && first && lane == 0 && tile == 0) a.seg_g[sp.out * a.heads + h] = span_g;
     if (sp.out >= 0) {
         // the last run's decay: every thread needs log A of the last token
         __shared__ float s_last;
-        if (threadIdx.x == 0) s_last = (float)exp(run);
+        if (first && lane == 0) s_last = (float)exp(run);
         __syncthreads();
         const float f = s_last;
 #pragma unroll
@@ -295,6 +363,7 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
     const int vtile = warps * WV;
     const int64_t grid = ceil_div(a.dv, vtile) * a.heads * spans(a);
     MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
+    constexpr int L = stage_tokens<R>();
     const size_t smem = sizeof(float) * 2 * L * ((STATE ? 1 : 2) * KG * R + vtile);
     auto kern = decay_recurrent_kernel<T, KG, R, STATE>;
     const bool pairs = a.dv % 2 == 0 && aligned(a.o, 2 * sizeof(T)) && a.os[0] % 2 == 0 &&
@@ -304,7 +373,7 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
     if (e == cudaSuccess && smem > 48 * 1024)
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
-    kern<<<(unsigned)grid, warps * 32, smem, st>>>(a, vtile, vec16<T>(a.q, a.qs, a.dk),
+    kern<<<(unsigned)grid, warps * 32 + (R == 8 ? 128 : 0), smem, st>>>(a, vtile, vec16<T>(a.q, a.qs, a.dk),
                                                    vec16<T>(a.k, a.ks, a.dk),
                                                    vec16<T>(a.v, a.vs, a.dv), pairs);
     return check_launch("decay_recurrent_kernel");
@@ -312,6 +381,13 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
 
 template <typename T, bool STATE>
 static int recurrent_of(const Args &a, cudaStream_t st) {
+    if (a.narrow) {
+        if (a.dk <= 16) return launch_recurrent<T, 2, 8, STATE>(a, st);
+        if (a.dk <= 32) return launch_recurrent<T, 4, 8, STATE>(a, st);
+        if (a.dk <= 64) return launch_recurrent<T, 8, 8, STATE>(a, st);
+        if (a.dk <= 128) return launch_recurrent<T, 16, 8, STATE>(a, st);
+        return launch_recurrent<T, 32, 8, STATE>(a, st);
+    }
     if (a.dk <= 16) return launch_recurrent<T, 1, 16, STATE>(a, st);
     if (a.dk <= 24) return launch_recurrent<T, 1, 24, STATE>(a, st);
     if (a.dk <= 32) return launch_recurrent<T, 1, 32, STATE>(a, st);
@@ -405,7 +481,8 @@ __global__ void __launch_bounds__(128) seg_states_kernel(const Args a) {
 // Measured, one sequence of 8192 tokens, 24 heads of 128 x 64 in bf16: 134 us whole,
 // 95 in segments (27 first pass, 42 second).
 static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64_t unit,
-                              double first) {
+                              double first, double &time) {
+    time = 0.0;
     if (a.seqs == 0 || a.seqlen == 0) return 0;
     // packed: the lengths are not known here; the longest sequence is taken as one
     // and a half times the mean
@@ -415,36 +492,248 @@ static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64
                                : (even > 1.5 * units ? even : 1.5 * units);
     double best = whole * 0.9;            // segments have to save a tenth
     int64_t seg = 0;
+    time = whole;
     for (int64_t n = 2; n <= 256 && n * 2 <= units; ++n) {
         const int64_t per = ceil_div(units, n);
         const double t = (double)ceil_div(walks * n, lanes) * (per + 2.2) +
                          (double)ceil_div(walks * (n - 1), lanes) * (first * per + 2.2) +
                          0.1 * n + 4.0;
         if (t < best) {
-            best = t;
+            best = time = t;
             seg = per * unit;
         }
     }
     return seg;
 }
 
+// --------------------------------------------------------- relaid tensors
+// The tensor-core kernel wants rows of 16-byte groups (TMA).  bf16 prompts whose
+// widths or strides are others are laid out for it first, zeros behind Dk and Dv,
+// and o and h_last copied back: two launches and their traffic, where the recurrent
+// kernel took (us, both ways)
+//   8 x 379 tokens, 12 heads of 87 x 64                   247 -> 23
+//   15 x 2560, 6 heads of 64 x 14                         528 -> 66
+//   51221 in 23 sequences, 1 head of 89 x 104             330 -> 86
+//   40 x 568, 24 heads of 10 x 64                         355 -> 104
+struct Relay {
+    struct Item {
+        const void *src;
+        void *dst;
+        int64_t s[3];                     // the caller's strides
+        uint32_t n[3], rows;              // (batch, token, head); rows of n[2] that the caller has
+        uint32_t width, padded;           // of a row: the caller's, ours
+        int bytes;                        // an element's
+    } item[4];
+    int n;
+    const int32_t *cu;                    // o: rows outside the sequences stay as they are
+    int64_t seqs, seqlen;
+};
+constexpr int RELAY_THREADS = 256;
+
+// a thread's 16 bytes of our rows: from the caller's (IN) or back
+template <typename E, bool IN>
+__device__ __forceinline__ void relay_rows(const Relay::Item &it, int64_t lo, int64_t hi) {
+    constexpr uint32_t V = 16 / sizeof(E);
+    const uint32_t groups = it.padded / V;
+    const uint64_t total = (uint64_t)it.n[0] * it.n[1] * it.n[2] * groups;
+    for (uint64_t i = (uint64_t)blockIdx.x * RELAY_THREADS + threadIdx.x; i < total;
+         i += (uint64_t)gridDim.x * RELAY_THREADS) {
+        // 32-bit divisions where the numbers allow them
+        const uint64_t row = i >> 32 ? i / groups : (uint32_t)i / groups;
+        const uint32_t c = (uint32_t)(i - row * groups) * V;
+        const uint64_t bt = row >> 32 ? row / it.n[2] : (uint32_t)row / it.n[2];
+        const uint32_t h = (uint32_t)(row - bt * it.n[2]);
+        const uint64_t b = bt >> 32 ? bt / it.n[1] : (uint32_t)bt / it.n[1];
+        const int64_t t = (int64_t)(bt - b * it.n[1]);
+        const int64_t at = (int64_t)b * it.s[0] + t * it.s[1] + (int64_t)h * it.s[2] + c;
+        E x[V];
+        if (IN) {
+            const E *const src = static_cast<const E *>(it.src) + at;
+#pragma unroll
+            for (uint32_t e = 0; e < V; ++e) {
+                x[e] = 0;
+                if (h < it.rows && c + e < it.width) x[e] = src[e];
+            }
+            *reinterpret_cast<uint4 *>(static_cast<E *>(it.dst) + i * V) =
+                *reinterpret_cast<const uint4 *>(x);
+        } else {
+            if (h >= it.rows || t < lo || t >= hi) continue;
+            *reinterpret_cast<uint4 *>(x) =
+                *reinterpret_cast<const uint4 *>(static_cast<const E *>(it.src) + i * V);
+            E *const dst = static_cast<E *>(it.dst) + at;
+#pragma unroll
+            for (uint32_t e = 0; e < V; ++e)
+                if (c + e < it.width) dst[e] = x[e];
+        }
+    }
+}
+
+template <bool IN>
+__global__ void __launch_bounds__(RELAY_THREADS)
+relay_kernel(const __grid_constant__ Relay r) {
+    const Relay::Item &it = r.item[blockIdx.y];
+    if (it.bytes == 4) {
+        relay_rows<uint32_t, IN>(it, 0, INT64_MAX);
+        return;
+    }
+    int64_t lo = 0, hi = INT64_MAX;
+    if (!IN && r.cu) {
+        lo = clamp_row(r.cu[0], r.seqlen);
+        hi = clamp_row(r.cu[r.seqs], r.seqlen);
+    }
+    relay_rows<uint16_t, IN>(it, lo, hi);
+}
+
+static int relay(const Relay &r, bool in, cudaStream_t st) {
+    if (r.n == 0) return MB2_OK;
+    uint64_t most = 1;
+    for (int i = 0; i < r.n; ++i) {
+        const Relay::Item &it = r.item[i];
+        const uint64_t groups = (uint64_t)it.n[0] * it.n[1] * it.n[2] * (it.padded * it.bytes / 16);
+        if (groups > most) most = groups;
+    }
+    const uint64_t blocks = (most + RELAY_THREADS - 1) / RELAY_THREADS;
+    const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192), (unsigned)r.n);
+    if (in) relay_kernel<true><<<grid, RELAY_THREADS, 0, st>>>(r);
+    else relay_kernel<false><<<grid, RELAY_THREADS, 0, st>>>(r);
+    return check_launch("relay_kernel");
+}
+
+static bool tma_rows(const void *p, const int64_t (&s)[3], int64_t batch, int64_t tokens,
+                     int64_t heads) {
+    const int64_t n[3] = {batch, tokens, heads};
+    bool ok = aligned(p, 16);
+    for (int i = 0; i < 3; ++i) ok = ok && s[i] % 8 == 0 && (s[i] > 0 || n[i] <= 1);
+    return ok;
+}
+
+// Points `a` to rows in the workspace (from byte `at` on) where the caller's do not
+// suit the tensor cores; what to copy before and after.  Returns the workspace's end.
+static size_t relaid(Args &a, uint8_t *ws, size_t at, Relay &in, Relay &out) {
+    in.n = out.n = 0;
+    in.cu = out.cu = a.cu;
+    in.seqs = out.seqs = a.seqs;
+    in.seqlen = out.seqlen = a.seqlen;
+    const int64_t batch = a.cu ? 1 : a.seqs;
+    if (a.recurrent || batch >= (1ll << 31) || a.seqlen >= (1ll << 31)) return at;
+    const int64_t dk = round_up(a.dk, 8), dv = round_up(a.dv, 8);
+    const int64_t hq = a.heads / a.q_rep, hk = a.heads / a.k_rep, hv = a.heads / a.v_rep;
+    auto take = [&](size_t bytes) {
+        uint8_t *p = ws + at;
+        at += (size_t)round_up((int64_t)bytes, 256);
+        return p;
+    };
+    auto tokens = [&](Relay &r, const void *src, void *dst, int64_t (&s)[3], int64_t heads,
+                      int64_t width, int64_t padded) {
+        Relay::Item &it = r.item[r.n++];
+        it = {src, dst, {s[0], s[1], s[2]}, {(uint32_t)batch, (uint32_t)a.seqlen, (uint32_t)heads},
+              (uint32_t)heads, (uint32_t)width, (uint32_t)padded, 2};
+        s[0] = a.seqlen * heads * padded;
+        s[1] = heads * padded;
+        s[2] = padded;
+    };
+    auto bytes = [&](int64_t heads, int64_t width) {
+        return (size_t)(batch * a.seqlen * heads * width) * 2;
+    };
+    if (dk != a.dk || !tma_rows(a.q, a.qs, batch, a.seqlen, hq)) {
+        void *p = take(bytes(hq, dk));
+        tokens(in, a.q, p, a.qs, hq, a.dk, dk);
+        a.q = p;
+    }
+    if (dk != a.dk || !tma_rows(a.k, a.ks, batch, a.seqlen, hk)) {
+        void *p = take(bytes(hk, dk));
+        tokens(in, a.k, p, a.ks, hk, a.dk, dk);
+        a.k = p;
+    }
+    if (dv != a.dv || !tma_rows(a.v, a.vs, batch, a.seqlen, hv)) {
+        void *p = take(bytes(hv, dv));
+        tokens(in, a.v, p, a.vs, hv, a.dv, dv);
+        a.v = p;
+    }
+    if (dv != a.dv || !tma_rows(a.o, a.os, batch, a.seqlen, a.heads)) {
+        void *p = take(bytes(a.heads, dv));
+        tokens(out, p, a.o, a.os, a.heads, a.dv, dv);
+        a.o = p;
+    }
+    const bool pad = dk != a.dk || dv != a.dv;
+    auto states = [&](Relay &r, const void *src, void *dst) {
+        r.item[r.n++] = {src, dst, {a.heads * a.dk * a.dv, a.dk * a.dv, a.dv},
+                         {(uint32_t)a.seqs, (uint32_t)a.heads, (uint32_t)dk},
+                         (uint32_t)a.dk, (uint32_t)a.dv, (uint32_t)dv, 4};
+    };
+    const size_t state = (size_t)(a.seqs * a.heads * dk * dv) * 4;
+    if (a.h0 && (pad || !aligned(a.h0, 16))) {
+        float *p = reinterpret_cast<float *>(take(state));
+        states(in, a.h0, p);
+        a.h0 = p;
+    }
+    if (a.h_last && (pad || !aligned(a.h_last, 16))) {
+        float *p = reinterpret_cast<float *>(take(state));
+        states(out, p, a.h_last);
+        a.h_last = p;
+    }
+    a.dk = dk;
+    a.dv = dv;
+    return at;
+}
+
+// The recurrent kernel's walks: 14 (up to 32 rows, one warp) or 3 (four warps) on an
+// SM at a time, narrow ones 2.
+struct Walks { int64_t n, lanes; };
+static Walks walks_of(const Args &a, bool narrow) {
+    const int64_t sms = num_sms();
+    int64_t cols = a.dk <= 32 ? 64 : a.dk <= 64 ? 128 : a.dk <= 128 ? 64 : 32;
+    if (narrow) cols = a.dk <= 16 ? 128 : a.dk <= 32 ? 64 : a.dk <= 64 ? 32 : a.dk <= 128 ? 16 : 8;
+    return {a.seqs * a.heads * ceil_div(a.dv, cols),
+            narrow ? 2 * sms : a.dk <= 32 ? 14 * sms : 3 * sms};
+}
+
+// Short bf16 prompts the recurrent kernel does sooner: a walk of the tensor cores
+// takes its 128 tokens whole.  In us, 64 heads of 64 x 64: 1 token 4.0 against 8.7, 16
+// tokens 5.6 against 8.6, 32 tokens 7.8 against 8.4; 1024 heads of 16 x 120: 1 token 5.6
+// against 65, 64 tokens 32 against 55.
+static bool short_prompt(const Args &a) {
+    if (a.seqs == 0) return true;
+    const double tokens = (double)(a.cu ? ceil_div(a.seqlen, a.seqs) : a.seqlen);
+    if (tokens > 128) return false;
+    const Walks n = walks_of(a, true), w = walks_of(a, false);
+    const double load = (double)w.n / (double)w.lanes, idle = a.dk <= 32 ? 0.27 : 0.36;
+    const double recurrent = 3.5 + tokens * (n.n <= n.lanes ? 0.13
+                                             : load <= 1.0 ? idle + (0.6 - idle) * load
+                                                           : 0.6 * load);
+    return recurrent < 4.5 + 4.0 * (double)ceil_div(a.seqs * a.heads * ceil_div(a.dv, 64), num_sms());
+}
+
 struct Plan { size_t slot0, g, state, bytes; };
-// how a call runs: sets a.seg and a.slots; the parts of its workspace
-static Plan plan(Args &a) {
-    // tensor cores: one walk of 64 columns an SM, 128 tokens a step; recurrent: 14
-    // (up to 32 rows, one warp) or about 3 walks (four warps), compared by 32 tokens
-    const int sms = num_sms();
-    const bool tc = chunked_fits(a);
-    const int64_t cols = tc || a.dk <= 32 ? 64 : a.dk <= 64 ? 128 : a.dk <= 128 ? 64 : 32;
-    const int64_t walks = a.seqs * a.heads * ceil_div(a.dv, cols);
-    a.seg = segment_tokens(a, walks, tc ? sms : a.dk <= 32 ? 14 * sms : 3 * sms, tc ? 128 : 32,
-                           tc ? 0.65 : 0.6);
+// how a call runs, in a workspace at ws: sets a.seg and a.slots, and points a to the
+// relaid tensors; the parts of the workspace
+static Plan plan(Args &a, uint8_t *ws, Relay &in, Relay &out) {
+    a.recurrent = a.dtype != MB2_BF16 || a.dk > 128 || short_prompt(a);
+    // the workspace's first bytes stay empty: a tensor at a null workspace (only its
+    // size is asked for) is none
+    const size_t begin = relaid(a, ws, 256, in, out);
+    // tensor cores: one walk of 64 columns an SM, 128 tokens a step; recurrent: compared
+    // by 32 tokens, which a narrow walk takes in 4.2 us, others in 2.3 times that (above
+    // 64 rows 1.6: in segments, 2048 tokens, 8 heads of 128 x 128, 136 us narrow, 103
+    // else).  Narrow ones lose once they share an SM by more than two (192 tokens of fp32, heads of
+    // 64 x 64: 8 heads 25 us, others 66; 128 heads 35 and 67; 512 heads 126 and 87).
+    double time, narrow_time;
+    if (chunked_fits(a)) {
+        a.seg = segment_tokens(a, a.seqs * a.heads * ceil_div(a.dv, 64), num_sms(), 128, 0.65, time);
+    } else {
+        const Walks w = walks_of(a, false), n = walks_of(a, true);
+        const int64_t wide = segment_tokens(a, w.n, w.lanes, 32, 0.6, time);
+        const int64_t narrow = segment_tokens(a, n.n, n.lanes, 32, 0.6, narrow_time);
+        a.narrow = n.n <= n.lanes && narrow_time <= (a.dk <= 64 ? 2.3 : 1.6) * time;
+        a.seg = a.narrow ? narrow : wide;
+    }
     a.slots = 0;
     Plan p = {};
+    p.bytes = in.n + out.n ? begin : 0;
     if (a.seg == 0) return p;
     a.slots = a.cu ? a.seqs + a.seqlen / a.seg : a.seqs * segments(a.seqlen, a.seg);
-    p.slot0 = 0;
-    p.g = (size_t)round_up((a.seqs + 1) * 4, 256);
+    p.slot0 = begin;
+    p.g = begin + (size_t)round_up((a.seqs + 1) * 4, 256);
     p.state = p.g + (size_t)round_up(a.slots * a.heads * 8, 256);
     p.bytes = p.state + (size_t)(a.slots * a.heads * a.dk * a.dv) * 4;
     return p;
@@ -616,6 +905,7 @@ static int to_args(const mb2_decay_attn *d, bool one, Args &a) {
     a.h_last = d->h_last;
     a.cu = d->cu_seqlens;
     a.scale = d->scale;
+    a.narrow = a.recurrent = 0;
     a.seg = a.slots = 0;
     a.slot0 = nullptr;
     a.seg_state = nullptr;
@@ -630,7 +920,8 @@ using namespace mb2;
 
 extern "C" size_t mb2_decay_attention_workspace_bytes(const mb2_decay_attn *d) {
     decay::Args a;
-    return decay::to_args(d, false, a) == MB2_OK ? decay::plan(a).bytes : 0;
+    decay::Relay in, out;
+    return decay::to_args(d, false, a) == MB2_OK ? decay::plan(a, nullptr, in, out).bytes : 0;
 }
 
 extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, size_t workspace_bytes,
@@ -640,7 +931,9 @@ extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, siz
     if (a.seqs == 0 && !(a.cu && d->zero_tail)) return MB2_OK;
     MB2_REQUIRE((a.q && a.k && a.v && a.g && a.o) || a.seqlen == 0, MB2_ERR_ARG,
                 "decay_attention: null pointer");
-    const decay::Plan p = decay::plan(a);
+    const decay::Args given = a;
+    decay::Relay in, out;
+    const decay::Plan p = decay::plan(a, static_cast<uint8_t *>(workspace), in, out);
     MB2_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), MB2_ERR_WORKSPACE,
                 "decay_attention: workspace of %llu bytes, %llu needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
@@ -649,12 +942,13 @@ extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, siz
     cudaStream_t st = (cudaStream_t)stream;
     if (a.cu && d->zero_tail && a.seqlen > 0) {
         if (a.dtype == MB2_F32)
-            decay::zero_tail_kernel<float><<<64, 256, 0, st>>>(a);
+            decay::zero_tail_kernel<float><<<64, 256, 0, st>>>(given);
         else
-            decay::zero_tail_kernel<__nv_bfloat16><<<64, 256, 0, st>>>(a);
+            decay::zero_tail_kernel<__nv_bfloat16><<<64, 256, 0, st>>>(given);
         MB2_TRY(check_launch("zero_tail_kernel"));
     }
     if (a.seqs == 0) return MB2_OK;
+    MB2_TRY(decay::relay(in, true, st));
     bool used = false;
     if (a.seg) {
         uint8_t *ws = static_cast<uint8_t *>(workspace);
@@ -678,7 +972,8 @@ extern "C" int mb2_decay_attention(const mb2_decay_attn *d, void *workspace, siz
         MB2_TRY(check_launch("seg_states_kernel"));
     }
     MB2_TRY(decay::chunked(a, false, st, &used));
-    return used ? MB2_OK : decay::recurrent(a, false, st);
+    if (!used) MB2_TRY(decay::recurrent(a, false, st));
+    return decay::relay(out, false, st);
 }
 
 extern "C" int mb2_decay_attention_step(const mb2_decay_attn *d, float *state, mb2_stream_t stream) {

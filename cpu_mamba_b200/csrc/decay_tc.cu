@@ -987,8 +987,8 @@ static int token_map(CUtensorMap *map, const void *p, const int64_t (&s)[3], int
 
 // bf16 prompts with widths in whole 16-byte groups, at rows TMA can address
 static bool fits(const Args &a) {
-    return a.dtype == MB2_BF16 && a.dk <= 128 && a.dk % 8 == 0 && a.dv % 8 == 0 && a.seqlen > 0 &&
-           aligned(a.o, 16) && a.os[0] % 8 == 0 && a.os[1] % 8 == 0 && a.os[2] % 8 == 0 &&
+    return !a.recurrent && a.dtype == MB2_BF16 && a.dk <= 128 && a.dk % 8 == 0 && a.dv % 8 == 0 &&
+           a.seqlen > 0 && aligned(a.o, 16) && a.os[0] % 8 == 0 && a.os[1] % 8 == 0 && a.os[2] % 8 == 0 &&
            (!a.h0 || aligned(a.h0, 16)) && (!a.h_last || aligned(a.h_last, 16));
 }
 

@@ -432,3 +432,91 @@ def test_refusals():
     wide = torch.zeros(1, 3, 1, 257, device="cuda")
     with pytest.raises(RuntimeError, match="257"):
         f(wide, wide, wide, torch.zeros(1, device="cuda"))
+
+
+# ---------------------------------------- widths and rows off 16-byte groups
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 200, 4, 2, 1, 4, 87, 64), (1, 260, 3, 1, 3, 1, 64, 14),
+                                   (3, 129, 2, 2, 2, 2, 10, 51), (40, 70, 8, 1, 2, 8, 33, 67),
+                                   (1, 1100, 1, 1, 1, 1, 127, 121)])
+def test_odd_widths(shape, dtype):
+    """States in and out, at an address off 16 bytes."""
+    B, T, H, Hq, Hk, Hv, dk, dv = shape
+    q, k, v, g, h0 = make(*shape, dtype, seed=T + dv)
+    ref = reference(spread(q, H), spread(k, H), spread(v, H), g.expand(B, T, H), 0.7, h0)
+    o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), scale=0.7,
+                               initial_state=h0.cuda(), return_final_state=True)
+    check(o, s, ref, dtype, T, dk)
+    shifted = torch.empty(h0.numel() + 1, device="cuda")[1:].view(h0.shape).copy_(h0)
+    o2, s2 = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), scale=0.7,
+                                 initial_state=shifted, return_final_state=True)
+    check(o2, s2, ref, dtype, T, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dv", [64, 61])
+def test_odd_packed_rows_outside_the_sequences_stay(dv):
+    """An `out` with other strides: rows behind the last sequence and columns
+    between its rows keep what they held; broadcast q, one sequence empty."""
+    T, H, dk, dtype = 700, 3, 45, torch.bfloat16
+    q, k, v, g, h0 = make(1, T, H, 1, 1, H, dk, dv, dtype, seed=dv)
+    cu = torch.tensor([0, 250, 250, 640], dtype=torch.int32)
+    h0 = torch.randn(3, H, dk, dv, generator=torch.Generator().manual_seed(2))
+    hold = torch.full((1, T, H, dv + 5), 7.0, dtype=dtype, device="cuda")
+    out = hold[..., 3:3 + dv]
+    o, s = ops.decay_attention(q.cuda().expand(1, T, H, dk), k.cuda(), v.cuda(), g.cuda(),
+                               cu_seqlens=cu.cuda(), initial_state=h0.cuda(),
+                               return_final_state=True, out=out)
+    assert o.data_ptr() == out.data_ptr()
+    assert bool((hold[:, 640:] == 7).all())
+    assert bool((hold[..., :3] == 7).all() and (hold[..., 3 + dv:] == 7).all())
+    for i in range(3):
+        a, b = cu[i].item(), cu[i + 1].item()
+        if a == b:
+            assert torch.equal(s[i].cpu(), h0[i])
+            continue
+        w = slice(a, b)
+        ref = reference(spread(q[:, w], H), spread(k[:, w], H), v[:, w], g[:, w], 1.0, h0[i:i + 1])
+        check(o[:, w], s[i:i + 1], ref, dtype, b - a, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_odd_widths_in_a_graph_and_on_two_streams(dtype):
+    q, k, v, g, h0 = (t.cuda() for t in make(2, 333, 4, 1, 1, 4, 50, 39, dtype, seed=3))
+    want = ops.decay_attention(q, k, v, g, initial_state=h0)
+    other = ops.decay_attention(k, q, v, g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.decay_attention(q, k, v, g, initial_state=h0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        y.fill_(3)
+        torch.cuda.synchronize()
+        got = []
+        for i in range(6):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append(ops.decay_attention(*((q, k) if i % 2 == 0 else (k, q)), v, g,
+                                               initial_state=h0 if i % 2 == 0 else None))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        assert all(torch.equal(x, other if i % 2 else want) for i, x in enumerate(got))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,T", [(1, 9), (8, 31), (148, 33), (300, 40), (2100, 20)])
+def test_few_and_many_walks(heads, T, dtype):
+    """Both spreads of a state over lanes, with decays that end a run inside a
+    group of tokens, at every place in it."""
+    for dk, dv in ((16, 24), (30, 64), (64, 32), (120, 8), (180, 4)):
+        q, k, v, g, h0 = make(1, T, heads, 1, 1, heads, dk, dv, dtype, seed=heads + dk)
+        g = g.clone()
+        g[0, ::7, ::2] = -6.0
+        g[0, 3::5, 1::3] = -3.5
+        ref = reference(spread(q, heads), spread(k, heads), v, g, 1.0, h0)
+        o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(),
+                                   initial_state=h0.cuda(), return_final_state=True)
+        check(o, s, ref, dtype, T, dk)
