@@ -266,7 +266,14 @@ static int dispatch(const NormArgs &a, bool vec, cudaStream_t st) {
         return launch<T, RT, V, 16 / V, false, 1024>(a, st);   // width <= 16384
     }
     if (many && a.width <= 128) return launch<T, RT, 1, 4, true, 128>(a, st);
+    // odd rows, an element at a time; few elements a thread, since 16 of three operands
+    // spill (8000 rows of 3501 in fp32, all parts: 230 us with 16, 167 with 4; 4000 of
+    // 7001: 241 and 200 with 8; 21 rows of 3501 in bf16: 11.3 and 5.4)
+    if (many && a.width <= 256) return launch<T, RT, 1, 8, true, 128>(a, st);
     if (a.width <= 1024) return launch<T, RT, 1, 4, false, 256>(a, st);
+    if (a.width <= 2048) return launch<T, RT, 1, 8, false, 256>(a, st);
+    if (a.width <= 4096) return launch<T, RT, 1, 4, false, 1024>(a, st);
+    if (a.width <= 8192) return launch<T, RT, 1, 8, false, 1024>(a, st);
     return launch<T, RT, 1, 16, false, 1024>(a, st);
 }
 
