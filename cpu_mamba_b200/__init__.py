@@ -4,7 +4,9 @@ Same public API as the reference package (src/cpu_mamba/__init__.py:22-34):
 CPUMamba, assert_state_dict_compatible, QuantConfig, QuantizedLinear,
 quantize_block, memory_footprint -- plus the scan ops of the reference's
 backends (selective_scan for the C++ op, selective_scan_assoc[_chunked] for
-the associative scans).  Every op runs in the CUDA library libmamba_b200.so
+the associative scans).  Beside the block, ``ops`` has linear attention with a decay
+per head, the norms around a block and beam selection, ``generate.beam_search`` the
+search over recurrent states.  Every op runs in the CUDA library libmamba_b200.so
 (C ABI: include/mamba_b200.h); there is no CPU fallback.
 """
 from .module import CPUMamba, StepGraph, assert_state_dict_compatible

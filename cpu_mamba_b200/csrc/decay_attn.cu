@@ -739,15 +739,17 @@ static Plan plan(Args &a, uint8_t *ws, Relay &in, Relay &out) {
     return p;
 }
 
-// rows of o behind the last packed sequence (a freshly allocated o)
+// rows of o before the first and behind the last packed sequence (a new o)
 template <typename T>
 __global__ void zero_tail_kernel(const Args a) {
     const int64_t end = clamp_row(a.cu[a.seqs], a.seqlen);
+    int64_t begin = clamp_row(a.cu[0], a.seqlen);
+    if (begin > end) begin = end;
     const int64_t per = a.heads * a.dv;
     T *o = static_cast<T *>(a.o);
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (a.seqlen - end) * per;
-         i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t t = end + i / per, r = i % per;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+         i < (begin + a.seqlen - end) * per; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t at = i / per, t = at < begin ? at : end - begin + at, r = i % per;
         o[t * a.os[1] + (r / a.dv) * a.os[2] + r % a.dv] = io<T>::from_f(0.0f);
     }
 }

@@ -360,8 +360,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
     (N, H, Dk, Dv), zeros when None.
 
     cu_seqlens (int, N + 1 offsets on the device) packs N sequences along T with
-    B = 1; rows behind the last one are zero in a new output and untouched in
-    ``out``, which must not overlap the inputs.  Otherwise N = B.
+    B = 1; rows before the first and behind the last one are zero in a new output
+    and untouched in ``out``, which must not overlap the inputs.  Otherwise N = B.
 
     Returns o (B, T, H, Dv), with the final state (N, H, Dk, Dv) float32 when
     ``return_final_state``.  An empty sequence's final state is its initial one.

@@ -424,12 +424,17 @@ int mb2_block_step_static(const mb2_block *blk, const void *x, void *out, float 
  * g_stride repeats a decay.  heads is a multiple of q_heads, k_heads and
  * v_heads; head h reads q head h / (heads / q_heads).  dk <= 256.
  * h0 (or NULL: zeros) and h_last (or NULL): (sequences, heads, dk, dv) fp32
- * contiguous.  A g of -inf resets the state.
+ * contiguous.  g is at most 0; -inf resets the state.  o overlaps no input.
  * cu_seqlens (device, n_seqs + 1 offsets): batch must be 1 and sequence i is
- * rows cu[i] .. cu[i+1]-1 of the seqlen rows; rows behind the last sequence
- * are zeroed when zero_tail is set and left alone otherwise.  Offsets are
+ * rows cu[i] .. cu[i+1]-1 of the seqlen rows; rows before the first and behind
+ * the last sequence are zeroed when zero_tail is set and left alone otherwise.  Offsets are
  * clamped to 0 .. seqlen; a sequence whose end is not behind its start is
- * empty (its h_last is its h0). */
+ * empty (its h_last is its h0).
+ * The workspace (256-byte aligned; MB2_ERR_WORKSPACE when smaller than asked
+ * for) holds the states of sequences that are cut along their tokens and
+ * tensors whose rows the tensor cores cannot read; ask for its size with the
+ * descriptor of the call, pointers and strides included, on its device.  Calls
+ * that may overlap need one each. */
 typedef struct mb2_decay_attn {
     int dtype;
     int zero_tail;

@@ -520,3 +520,23 @@ def test_few_and_many_walks(heads, T, dtype):
         o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(),
                                    initial_state=h0.cuda(), return_final_state=True)
         check(o, s, ref, dtype, T, dk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,dv", [(200, 64), (200, 37), (40, 16)])
+def test_rows_outside_the_packed_sequences(T, dv, dtype):
+    """Rows before the first sequence, too: zero in a new output, kept in `out`."""
+    q, k, v, g, _ = make(1, T, 2, 1, 1, 2, 32, dv, dtype, seed=T)
+    cu = torch.tensor([7, 20, T - 9], device="cuda")
+    args = [t.cuda() for t in (q, k, v, g)]
+    torch.full((1, T, 2, dv), float("nan"), dtype=dtype, device="cuda")    # freed: its bytes stay
+    new = ops.decay_attention(*args, cu_seqlens=cu)
+    assert bool((new[:, :7] == 0).all() and (new[:, T - 9:] == 0).all())
+    out = torch.full((1, T, 2, dv), 7.0, dtype=dtype, device="cuda")
+    ops.decay_attention(*args, cu_seqlens=cu, out=out)
+    assert bool((out[:, :7] == 7).all() and (out[:, T - 9:] == 7).all())
+    assert torch.equal(out[:, 7:T - 9], new[:, 7:T - 9])
+    for a, b in ((7, 20), (20, T - 9)):
+        ref = reference(spread(q[:, a:b], 2), spread(k[:, a:b], 2), v[:, a:b], g[:, a:b], 1.0)
+        check(new[:, a:b], None, ref, dtype, b - a, 32)
