@@ -15,6 +15,10 @@
 #include "common.cuh"
 #include "pair.cuh"
 
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 namespace mb2 {
 namespace {
 
@@ -650,6 +654,19 @@ extern "C" int mb2_reorder_rows(void *const *tensors, const int64_t *row_bytes, 
     for (int64_t i = 0; i < n_tensors; ++i)
         MB2_REQUIRE(row_bytes[i] >= 0 && (tensors[i] || row_bytes[i] == 0), MB2_ERR_ARG,
                     "reorder_rows: bad tensor %lld", (long long)i);
+    {
+        // moved in place side by side: no byte may belong to two tensors
+        std::vector<std::pair<const uint8_t *, int64_t>> spans;
+        spans.reserve((size_t)n_tensors);
+        for (int64_t i = 0; i < n_tensors; ++i)
+            if (row_bytes[i])
+                spans.emplace_back(static_cast<const uint8_t *>(tensors[i]),
+                                   row_bytes[i] * batch * beams);
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            MB2_REQUIRE(spans[i].first - spans[i - 1].first >= spans[i - 1].second, MB2_ERR_ARG,
+                        "reorder_rows: tensors overlap");
+    }
     for (int64_t t0 = 0; t0 < n_tensors; t0 += MAX_TENSORS) {
         Reorder r;
         r.n = 0;

@@ -168,7 +168,7 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
         get_v(vs + b * L * vtile, vtile, v + t0 * a.vs[1], a.vs[1], m);
         cp_async_commit();
     };
-    // log A is carried in 64 bits (the 16 decays of a chunk are added in 32): a head
+    // log A is carried in 64 bits (the 16 or 32 decays of a chunk are added in 32): a head
     // that forgets over thousands of tokens adds as many equal decays, whose
     // roundings in 32 bits would all point one way.
     double run = 0.0;                 // log A after the chunk (the first warp)

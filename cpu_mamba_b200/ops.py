@@ -584,8 +584,8 @@ def reorder_states(states, parents: torch.Tensor):
 
     Each tensor is contiguous with B * K rows (its first index) of any dtype;
     parents: (B, K) int64 or int32 beams, K <= 32; a parent outside 0 .. K-1
-    leaves its row as it is.  Tensors that overlap one another are not
-    supported.  Returns ``states``."""
+    leaves its row as it is.  Tensors that overlap, the same one twice among them,
+    are refused.  Returns ``states``."""
     what = "reorder_states"
     if parents.dim() != 2 or parents.shape[1] == 0 or (
             parents.dtype not in (torch.int64, torch.int32)):

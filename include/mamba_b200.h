@@ -502,7 +502,7 @@ int mb2_gated_norm(const mb2_gated_norm_desc *d, mb2_stream_t stream);
  * (batch x beams rows of row_bytes[i] bytes) becomes row b beams +
  * parents[b, j], in place, in one launch per 64 tensors.  tensors and
  * row_bytes are host arrays, parents a device one; a parent outside 0 ..
- * beams-1 leaves its row as it is.  The tensors do not overlap. */
+ * beams-1 leaves its row as it is.  Tensors that overlap are refused. */
 size_t mb2_beam_select_workspace_bytes(int dtype, int64_t batch, int64_t beams, int64_t vocab,
                                        int64_t num);
 int mb2_beam_select(int dtype, const void *logits, int64_t batch_stride, int64_t beam_stride,

@@ -353,3 +353,23 @@ def test_refusals():
             call()
     with pytest.raises(TypeError):
         f(x.double(), s)
+
+
+@pytest.mark.parametrize("bases", [(4096, 4096), (4096, 4096 + 47), (4096 + 47, 4096)])
+def test_reorder_c_entry_refuses_overlap(bases):
+    """Two tensors of 2 x 3 rows of 8 bytes."""
+    ptrs, sizes = (ctypes.c_void_p * 2)(*bases), (ctypes.c_int64 * 2)(8, 8)
+    assert _lib.lib().mb2_reorder_rows(ptrs, sizes, 2, 4096, 2, 3, None) == 1
+    assert b"overlap" in _lib.lib().mb2_last_error()
+
+
+@gpu
+def test_reorder_refuses_the_same_tensor_twice():
+    x = torch.randn(6, 5, device="cuda")
+    keep = x.clone()
+    parents = torch.tensor([[1, 1, 0], [2, 0, 1]], device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.reorder_states([x, {"h": x}], parents)
+    assert torch.equal(x, keep)
+    a, b = x[:, :0], torch.randn(12, 4, device="cuda")
+    ops.reorder_states([a.contiguous(), b[:6], b[6:]], parents)      # neighbours in one buffer
