@@ -17,7 +17,7 @@ namespace decay {
 
 // ------------------------------------------------------- recurrent prompt
 // One CTA walks one (sequence or segment, head, column tile) token by token, the
-// state in registers: KG neighbouring lanes share two columns, each holding R rows
+// state in registers: KG neighbouring lanes share C columns, each holding R rows
 // of them (rows 4 KG i + 4 kg .. + 3, so a group's k and q loads are neighbours and
 // all other lanes' are broadcasts).  With R <= 32 rows a lane, widths up to 32 need
 // no sum over lanes at all.
@@ -31,7 +31,12 @@ namespace decay {
 // factor.
 //
 // Bound: the FP32 pipe, 2 Dk Dv FMAs per token and head, and the shared-memory
-// loads of k and q (two 16-byte loads per 8 packed FMAs).  One warp per head of 64
+// loads of k and q (two 16-byte loads per 4 C packed FMAs; a warp's 16-byte load
+// takes four cycles of its SM's path to the registers even where all lanes read the
+// same).  Above 32 rows, four columns of 16 rows a lane instead of two of 32 halve
+// those loads for one more exchange between lanes: 1083 -> 890 us at 192 tokens, 2048
+// heads of 128 x 128; 278 -> 246 with heads of 64 x 64.  Up to 32 rows they lose (24 x
+// 64: 181 us two columns of all rows, 193 four of half).  One warp per head of 64
 // columns instead of four with eight lanes a column: 425 -> 192 us at 151 sequences
 // of 180 tokens, 24 heads of 24 x 64 (the FMAs alone take about 80).
 // tokens staged at a time: more where few walks wait for each step's latency
@@ -83,13 +88,13 @@ template <typename T> struct Stager {
     }
 };
 
-// R rows and two columns of the state a lane, KG lanes a column pair.  R 16 to 32 is for
-// calls that fill the machine.  R 8 is for few walks, where the step's latency is the
+// R rows and C columns of the state a lane, KG lanes the same columns.  R 16 to 32 is for
+// calls that fill the machine.  R 8 (two columns) is for few walks, where the step's latency is the
 // call's time: eight tokens at once unless a run starts among them (one after the other
 // 0.24 us a token, four 0.22), and other warps stage what comes next (beside the walk
 // 0.20; with eight tokens 0.12; R 32 without any of it 0.36).
 // STATE: the pass over segments that leaves their states; no q, no outputs
-template <typename T, int KG, int R, bool STATE>
+template <typename T, int KG, int R, int C, bool STATE>
 __global__ void __launch_bounds__(KG == 1 ? 32 : R == 8 ? 256 : 128, KG == 1 ? 14 : R == 8 ? 2 : 3)
 decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec_v, bool pair_o) {
     constexpr int DK = KG * R, QUADS = R / 4;              // padded rows
@@ -131,19 +136,19 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
     const bool loads = loader >= 0 && loader < loaders;
     const bool first = R == 8 ? loader >= 96 : warp == 0;
     const int kg = lane & (KG - 1);
-    const int col = 2 * ((int)threadIdx.x / KG);           // this lane's two columns
+    const int col = C * ((int)threadIdx.x / KG);           // this lane's first column
 
     // columns past Dk and Dv are zero for the whole walk
     const int words = 2 * L * (vtile + (STATE ? 1 : 2) * DK);      // a multiple of 4
     for (int i = threadIdx.x; i < words / 4; i += blockDim.x)
         reinterpret_cast<float4 *>(smem_f)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
-    uint64_t u[2 * QUADS][2];                              // row pairs x columns
+    uint64_t u[2 * QUADS][C];                              // row pairs x columns
     auto row_of = [&](int i) { return 4 * KG * (i >> 1) + 4 * kg + 2 * (i & 1); };
 #pragma unroll
     for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < C; ++c) {
             float e[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -243,65 +248,99 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
 #pragma unroll
             for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) u[i][c] = mul2(u[i][c], x2);
+                for (int c = 0; c < C; ++c) u[i][c] = mul2(u[i][c], x2);
         };
         // N tokens behind one another: their loads, sums over the lanes and stores overlap
         auto tokens = [&](auto count, int t) {
             constexpr int N = decltype(count)::value;
             float4 f[N];
-            float2 vv[N];
-            float r0[N], r1[N];
+            float vv[N][C], r[N][C];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 f[j] = s_f[b][t + j];
-                vv[j] = *reinterpret_cast<const float2 *>(vb + (t + j) * vtile);
+                const float *const from = vb + (t + j) * vtile;
+                if constexpr (C == 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(from);
+                    vv[j][0] = x.x; vv[j][1] = x.y; vv[j][2] = x.z; vv[j][3] = x.w;
+                } else {
+                    const float2 x = *reinterpret_cast<const float2 *>(from);
+                    vv[j][0] = x.x; vv[j][1] = x.y;
+                }
             }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 if (R != 8) again(t + j);
-                const uint64_t w0 = pair(vv[j].x * f[j].y), w1 = pair(vv[j].y * f[j].y);
-                uint64_t acc0 = 0, acc1 = 0;
+                uint64_t w[C], acc[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    w[c] = pair(vv[j][c] * f[j].y);
+                    acc[c] = 0;
+                }
 #pragma unroll
                 for (int i = 0; i < QUADS; ++i) {
                     const ulonglong2 kk =
                         *reinterpret_cast<const ulonglong2 *>(kb + (t + j) * DK + 4 * KG * i);
-                    u[2 * i][0] = fma2(kk.x, w0, u[2 * i][0]);
-                    u[2 * i][1] = fma2(kk.x, w1, u[2 * i][1]);
-                    u[2 * i + 1][0] = fma2(kk.y, w0, u[2 * i + 1][0]);
-                    u[2 * i + 1][1] = fma2(kk.y, w1, u[2 * i + 1][1]);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        u[2 * i][c] = fma2(kk.x, w[c], u[2 * i][c]);
+                        u[2 * i + 1][c] = fma2(kk.y, w[c], u[2 * i + 1][c]);
+                    }
                     if constexpr (!STATE) {
                         const ulonglong2 qq =
                             *reinterpret_cast<const ulonglong2 *>(qb + (t + j) * DK + 4 * KG * i);
-                        acc0 = fma2(qq.x, u[2 * i][0], acc0);
-                        acc1 = fma2(qq.x, u[2 * i][1], acc1);
-                        acc0 = fma2(qq.y, u[2 * i + 1][0], acc0);
-                        acc1 = fma2(qq.y, u[2 * i + 1][1], acc1);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) acc[c] = fma2(qq.x, u[2 * i][c], acc[c]);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) acc[c] = fma2(qq.y, u[2 * i + 1][c], acc[c]);
                     }
                 }
-                r0[j] = __uint_as_float(lo_of(acc0)) + __uint_as_float(hi_of(acc0));
-                r1[j] = __uint_as_float(lo_of(acc1)) + __uint_as_float(hi_of(acc1));
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    r[j][c] = __uint_as_float(lo_of(acc[c])) + __uint_as_float(hi_of(acc[c]));
             }
             if constexpr (!STATE) {
-#pragma unroll
-                for (int s = 1; s < KG; s <<= 1)
+                // the sum over the KG lanes; four columns are shared out between them
+                int mine = col;                            // this lane's first sum
+                if constexpr (C == 4) {
+                    const bool odd = kg & 1, up = kg & 2;
+                    mine += odd ? 2 : 0;
+                    if (KG > 2) mine += up ? 1 : 0;
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        r0[j] += __shfl_xor_sync(0xffffffffu, r0[j], s);
-                        r1[j] += __shfl_xor_sync(0xffffffffu, r1[j], s);
+                        const float g0 = odd ? r[j][0] : r[j][2], g1 = odd ? r[j][1] : r[j][3];
+                        r[j][0] = (odd ? r[j][2] : r[j][0]) + __shfl_xor_sync(0xffffffffu, g0, 1);
+                        r[j][1] = (odd ? r[j][3] : r[j][1]) + __shfl_xor_sync(0xffffffffu, g1, 1);
+                        if constexpr (KG > 2) {
+                            const float g2 = up ? r[j][0] : r[j][1];
+                            r[j][0] = (up ? r[j][1] : r[j][0]) + __shfl_xor_sync(0xffffffffu, g2, 2);
+#pragma unroll
+                            for (int s = 4; s < KG; s <<= 1)
+                                r[j][0] += __shfl_xor_sync(0xffffffffu, r[j][0], s);
+                        }
                     }
-                if (kg == 0 && col < cols) {
+                } else {
+#pragma unroll
+                    for (int s = 1; s < KG; s <<= 1)
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+#pragma unroll
+                            for (int c = 0; c < C; ++c)
+                                r[j][c] += __shfl_xor_sync(0xffffffffu, r[j][c], s);
+                }
+                constexpr bool TWO = C == 2 || KG == 2;    // sums a lane stores
+                if (kg < (C == 2 ? 1 : 4) && mine < cols) {
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        T *const at = to + j * a.os[1];
-                        const float x0 = r0[j] * f[j].z, x1 = r1[j] * f[j].z;
-                        if (pair_o) {
+                        T *const at = to + j * a.os[1] + (mine - col);
+                        const float x0 = r[j][0] * f[j].z, x1 = TWO ? r[j][1] * f[j].z : 0.0f;
+                        if (TWO && pair_o) {
                             if constexpr (sizeof(T) == 4)
                                 *reinterpret_cast<float2 *>(at) = make_float2(x0, x1);
                             else
                                 *reinterpret_cast<__nv_bfloat162 *>(at) = __floats2bfloat162_rn(x0, x1);
                         } else {
                             at[0] = io<T>::from_f(x0);
-                            if (col + 1 < cols) at[1] = io<T>::from_f(x1);
+                            if (TWO && mine + 1 < cols) at[1] = io<T>::from_f(x1);
                         }
                     }
                 }
@@ -338,7 +377,7 @@ decay_recurrent_kernel(const Args a, int vtile, bool vec_q, bool vec_k, bool vec
 #pragma unroll
         for (int i = 0; i < 2 * QUADS; ++i)
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int dk = row_of(i) + j;
@@ -355,9 +394,9 @@ static bool vec16(const void *p, const int64_t (&s)[3], int64_t cols) {
     return aligned(p, 16) && s[0] % E == 0 && s[1] % E == 0 && s[2] % E == 0 && cols % E == 0;
 }
 
-template <typename T, int KG, int R, bool STATE>
+template <typename T, int KG, int R, int C, bool STATE>
 static int launch_recurrent(const Args &a, cudaStream_t st) {
-    constexpr int WV = 64 / KG;                            // columns of a warp
+    constexpr int WV = 32 / KG * C;                        // columns of a warp
     const int most = KG == 1 ? 1 : 4;
     const int warps = (int)(ceil_div(a.dv, WV) < most ? ceil_div(a.dv, WV) : most);
     const int vtile = warps * WV;
@@ -365,7 +404,7 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
     MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention: too many sequences x heads");
     constexpr int L = stage_tokens<R>();
     const size_t smem = sizeof(float) * 2 * L * ((STATE ? 1 : 2) * KG * R + vtile);
-    auto kern = decay_recurrent_kernel<T, KG, R, STATE>;
+    auto kern = decay_recurrent_kernel<T, KG, R, C, STATE>;
     const bool pairs = a.dv % 2 == 0 && aligned(a.o, 2 * sizeof(T)) && a.os[0] % 2 == 0 &&
                        a.os[1] % 2 == 0 && a.os[2] % 2 == 0;
     // all of the SM's shared memory: the walks resident at once are what hides latency
@@ -373,27 +412,27 @@ static int launch_recurrent(const Args &a, cudaStream_t st) {
     if (e == cudaSuccess && smem > 48 * 1024)
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(MB2_ERR_CUDA, "decay_attention: %s", cudaGetErrorString(e));
-    kern<<<(unsigned)grid, warps * 32 + (R == 8 ? 128 : 0), smem, st>>>(a, vtile, vec16<T>(a.q, a.qs, a.dk),
-                                                   vec16<T>(a.k, a.ks, a.dk),
-                                                   vec16<T>(a.v, a.vs, a.dv), pairs);
+    kern<<<(unsigned)grid, warps * 32 + (R == 8 ? 128 : 0), smem, st>>>(
+        a, vtile, vec16<T>(a.q, a.qs, a.dk), vec16<T>(a.k, a.ks, a.dk), vec16<T>(a.v, a.vs, a.dv),
+        pairs);
     return check_launch("decay_recurrent_kernel");
 }
 
 template <typename T, bool STATE>
 static int recurrent_of(const Args &a, cudaStream_t st) {
     if (a.narrow) {
-        if (a.dk <= 16) return launch_recurrent<T, 2, 8, STATE>(a, st);
-        if (a.dk <= 32) return launch_recurrent<T, 4, 8, STATE>(a, st);
-        if (a.dk <= 64) return launch_recurrent<T, 8, 8, STATE>(a, st);
-        if (a.dk <= 128) return launch_recurrent<T, 16, 8, STATE>(a, st);
-        return launch_recurrent<T, 32, 8, STATE>(a, st);
+        if (a.dk <= 16) return launch_recurrent<T, 2, 8, 2, STATE>(a, st);
+        if (a.dk <= 32) return launch_recurrent<T, 4, 8, 2, STATE>(a, st);
+        if (a.dk <= 64) return launch_recurrent<T, 8, 8, 2, STATE>(a, st);
+        if (a.dk <= 128) return launch_recurrent<T, 16, 8, 2, STATE>(a, st);
+        return launch_recurrent<T, 32, 8, 2, STATE>(a, st);
     }
-    if (a.dk <= 16) return launch_recurrent<T, 1, 16, STATE>(a, st);
-    if (a.dk <= 24) return launch_recurrent<T, 1, 24, STATE>(a, st);
-    if (a.dk <= 32) return launch_recurrent<T, 1, 32, STATE>(a, st);
-    if (a.dk <= 64) return launch_recurrent<T, 2, 32, STATE>(a, st);
-    if (a.dk <= 128) return launch_recurrent<T, 4, 32, STATE>(a, st);
-    return launch_recurrent<T, 8, 32, STATE>(a, st);
+    if (a.dk <= 16) return launch_recurrent<T, 1, 16, 2, STATE>(a, st);
+    if (a.dk <= 24) return launch_recurrent<T, 1, 24, 2, STATE>(a, st);
+    if (a.dk <= 32) return launch_recurrent<T, 1, 32, 2, STATE>(a, st);
+    if (a.dk <= 64) return launch_recurrent<T, 4, 16, 4, STATE>(a, st);
+    if (a.dk <= 128) return launch_recurrent<T, 8, 16, 4, STATE>(a, st);
+    return launch_recurrent<T, 16, 16, 4, STATE>(a, st);
 }
 static int recurrent(const Args &a, bool state_only, cudaStream_t st) {
     if (a.dtype == MB2_F32)

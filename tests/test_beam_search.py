@@ -373,3 +373,18 @@ def test_reorder_refuses_the_same_tensor_twice():
     assert torch.equal(x, keep)
     a, b = x[:, :0], torch.randn(12, 4, device="cuda")
     ops.reorder_states([a.contiguous(), b[:6], b[6:]], parents)      # neighbours in one buffer
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [7, 2047, 2049, 16383, 16384, 16385, 16391, 40000])
+def test_select_around_the_slices(V, dtype):
+    """Rows off 16 bytes; two tokens left of a row; rising logits, whose best all
+    stand in the last slice."""
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(1, 2, V + 3, generator=g) * 3).to(dtype)[..., 3:]
+    check(x, torch.zeros(1, 2), min(64, 2 * V))
+    check(x.sort(-1).values, torch.zeros(1, 2), min(64, 2 * V))
+    few = torch.full((1, 2, V), -torch.inf, dtype=dtype)
+    few[..., V // 2], few[..., V - 1] = 1.0, 0.5
+    check(few, torch.tensor([[-1.0, -2.0]]), 3)
