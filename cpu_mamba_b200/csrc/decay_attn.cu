@@ -516,11 +516,12 @@ __global__ void __launch_bounds__(128) seg_states_kernel(const Args a) {
 // tokens one after the other, and `lanes` walks run at a time: with fewer sequences
 // x heads x column tiles than that (or an uneven last round of them) segments
 // shorten the longest chain, at the price of a first pass that costs `first` of the
-// second's time a step, two steps to fill each walk, and the states' traffic.
+// second's time a step, `fill` steps to start each walk, and the states' traffic
+// (`join` steps and a tenth for each segment).
 // Measured, one sequence of 8192 tokens, 24 heads of 128 x 64 in bf16: 134 us whole,
 // 95 in segments (27 first pass, 42 second).
 static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64_t unit,
-                              double first, double &time) {
+                              double first, double fill, double join, double &time) {
     time = 0.0;
     if (a.seqs == 0 || a.seqlen == 0) return 0;
     // packed: the lengths are not known here; the longest sequence is taken as one
@@ -534,9 +535,9 @@ static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64
     time = whole;
     for (int64_t n = 2; n <= 256 && n * 2 <= units; ++n) {
         const int64_t per = ceil_div(units, n);
-        const double t = (double)ceil_div(walks * n, lanes) * (per + 2.2) +
-                         (double)ceil_div(walks * (n - 1), lanes) * (first * per + 2.2) +
-                         0.1 * n + 4.0;
+        const double t = (double)ceil_div(walks * n, lanes) * (per + fill) +
+                         (double)ceil_div(walks * (n - 1), lanes) * (first * per + fill) +
+                         0.1 * n + join;
         if (t < best) {
             best = time = t;
             seg = per * unit;
@@ -758,11 +759,12 @@ static Plan plan(Args &a, uint8_t *ws, Relay &in, Relay &out) {
     // 64 x 64: 8 heads 25 us, others 66; 128 heads 35 and 67; 512 heads 126 and 87).
     double time, narrow_time;
     if (chunked_fits(a)) {
-        a.seg = segment_tokens(a, a.seqs * a.heads * ceil_div(a.dv, 64), num_sms(), 128, 0.65, time);
+        a.seg = segment_tokens(a, a.seqs * a.heads * ceil_div(a.dv, 64), num_sms(), 128, 0.65, 2.2,
+                               4.0, time);
     } else {
         const Walks w = walks_of(a, false), n = walks_of(a, true);
-        const int64_t wide = segment_tokens(a, w.n, w.lanes, 32, 0.6, time);
-        const int64_t narrow = segment_tokens(a, n.n, n.lanes, 32, 0.6, narrow_time);
+        const int64_t wide = segment_tokens(a, w.n, w.lanes, 32, 0.6, 2.2, 4.0, time);
+        const int64_t narrow = segment_tokens(a, n.n, n.lanes, 32, 0.6, 0.9, 1.3, narrow_time);
         a.narrow = n.n <= n.lanes && narrow_time <= (a.dk <= 64 ? 2.3 : 1.6) * time;
         a.seg = a.narrow ? narrow : wide;
     }
