@@ -717,15 +717,16 @@ static size_t relaid(Args &a, uint8_t *ws, size_t at, Relay &in, Relay &out) {
     return at;
 }
 
-// The recurrent kernel's walks: 14 (up to 32 rows, one warp) or 3 (four warps) on an
-// SM at a time, narrow ones 2.
+// The recurrent kernel's walks: 14 (up to 32 rows, one warp) or 12 warps' worth of them
+// (up to four each) on an SM at a time, narrow ones 2.
 struct Walks { int64_t n, lanes; };
 static Walks walks_of(const Args &a, bool narrow) {
     const int64_t sms = num_sms();
     int64_t cols = a.dk <= 32 ? 64 : a.dk <= 64 ? 128 : a.dk <= 128 ? 64 : 32;
     if (narrow) cols = a.dk <= 16 ? 128 : a.dk <= 32 ? 64 : a.dk <= 64 ? 32 : a.dk <= 128 ? 16 : 8;
+    const int64_t warps = ceil_div(a.dv < cols ? a.dv : cols, cols / 4);
     return {a.seqs * a.heads * ceil_div(a.dv, cols),
-            narrow ? 2 * sms : a.dk <= 32 ? 14 * sms : 3 * sms};
+            narrow ? 2 * sms : a.dk <= 32 ? 14 * sms : 12 / warps * sms};
 }
 
 // Short bf16 prompts the recurrent kernel does sooner: a walk of the tensor cores
