@@ -305,12 +305,12 @@ _DECAY = struct.Struct("=2i8q5Q15q3Qqf4x")
 
 
 def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool, state_in=0, state_out=0, cu=0,
-                      seqs=0, zero_tail=0) -> bytes:
+                      seqs=0, new=True) -> bytes:
     """Argument checks shared by the prompt and the one-token form, and the
     descriptor (mb2_decay_attn).  ``tokens``: q, k, v and o carry a token index
-    after the batch."""
+    after the batch.  ``new``: o was made for this call."""
     lead = 2 if tokens else 1
-    qs, ks, vs, gs, os = q.shape, k.shape, v.shape, g.shape, o.shape
+    qs, ks, vs, gs = q.shape, k.shape, v.shape, g.shape
     names = "(batch, tokens, heads, width)" if tokens else "(batch, heads, width)"
     if not len(qs) == len(ks) == len(vs) == lead + 2:
         raise RuntimeError(f"{what}: q, k and v must be {names}, got {tuple(qs)}, {tuple(ks)}, "
@@ -322,7 +322,8 @@ def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool, state_in=0, stat
     if g.dtype != torch.float32:
         raise RuntimeError(f"{what}: g must be float32")
     batch, dk, dv, H = vs[0], qs[-1], vs[-1], gs[-1]
-    if qs[:lead] != vs[:lead] or ks[:lead] != vs[:lead] or dk != ks[-1]:
+    if (qs[0] != batch or ks[0] != batch or dk != ks[-1]
+            or (tokens and (qs[1] != vs[1] or ks[1] != vs[1]))):
         raise RuntimeError(f"{what}: shape mismatch: q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)}")
     if len(gs) != 1 and gs[:-1] != vs[:lead]:
         raise RuntimeError(f"{what}: g must be (heads,) or {names[:-8]}), got {tuple(gs)}")
@@ -330,7 +331,8 @@ def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool, state_in=0, stat
     if not (H and hq and hk and hv and dk and dv) or H % hq or H % hk or H % hv:
         raise RuntimeError(f"{what}: the heads of q, k and v ({hq}, {hk}, {hv}; widths {dk}, {dv}) "
                            f"must divide the {H} decays of g")
-    if os != vs[:lead] + (H, dv) or o.dtype != dtype or (dv > 1 and o.stride(-1) != 1):
+    if not new and (o.shape != vs[:lead] + (H, dv) or o.dtype != dtype
+                    or (dv > 1 and o.stride(-1) != 1)):
         raise RuntimeError(f"{what}: out must be {tuple(vs[:lead]) + (H, dv)} in {dtype} with its "
                            "last index contiguous")
     qt, kt, vt, ot, gt = q.stride(), k.stride(), v.stride(), o.stride(), g.stride()
@@ -340,7 +342,7 @@ def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool, state_in=0, stat
     else:
         strides = (qt[0], 0, qt[1], kt[0], 0, kt[1], vt[0], 0, vt[1],
                    *((0, 0, gt[0]) if len(gt) == 1 else (gt[0], 0, gt[1])), ot[0], 0, ot[1])
-    return _DECAY.pack(code, zero_tail, batch, vs[1] if tokens else 1, H, hq, hk, hv, dk, dv,
+    return _DECAY.pack(code, tokens and new, batch, vs[1] if tokens else 1, H, hq, hk, hv, dk, dv,
                        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), o.data_ptr(),
                        *strides, state_in, state_out, cu, seqs, scale)
 
@@ -388,11 +390,11 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
             raise RuntimeError(f"{what}: initial_state must be float32 {(n, H, dk, dv)}")
         initial_state = initial_state.contiguous()
     with _on(dev):
-        o = torch.empty((B, T, H, dv), device=v.device, dtype=v.dtype) if out is None else out
+        o = v.new_empty((B, T, H, dv)) if out is None else out
         h_last = (torch.empty((n, H, dk, dv), device=v.device, dtype=torch.float32)
                   if return_final_state else None)
         d = _decay_descriptor(what, q, k, v, g, scale, o, True, _addr(initial_state),
-                              _addr(h_last), cu, n, int(out is None))
+                              _addr(h_last), cu, n, out is None)
         nbytes = lib().mb2_decay_attention_workspace_bytes(d)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=v.device) if nbytes else None
         rc = lib().mb2_decay_attention(d, _addr(ws), nbytes, _raw_stream(dev))
@@ -419,7 +421,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: t
             or not state.is_contiguous()):
         raise RuntimeError(f"{what}: state must be contiguous float32 {(B, H, q.shape[-1], dv)}")
     with _on(dev):
-        o = torch.empty((B, H, dv), device=v.device, dtype=v.dtype)
+        o = v.new_empty((B, H, dv))
         d = _decay_descriptor(what, q, k, v, g, scale, o, False)
         rc = lib().mb2_decay_attention_step(d, state.data_ptr(), _raw_stream(dev))
         if rc:
@@ -502,10 +504,10 @@ def gated_norm(x: torch.Tensor, gate: Optional[torch.Tensor] = None,
         raise RuntimeError(f"{what}: residual_scale and next_weight need a residual")
     with _on(dev):
         if out is None:
-            out = torch.empty(shape, device=x.device, dtype=first)
+            out = (x if first == dtype else residual).new_empty(shape)
         elif out.shape != shape or out.dtype != first or not out.is_contiguous():
             raise RuntimeError(f"{what}: out must be contiguous {tuple(shape)} in {first}")
-        n = None if next_weight is None else torch.empty(shape, device=x.device, dtype=dtype)
+        n = None if next_weight is None else x.new_empty(shape)
         f32 = torch.float32
         d = _NORM.pack(code, rcode, x2.shape[0], W, group_size or 0, x2.data_ptr(), _addr(z2),
                        _addr(weight), _addr(r2), _addr(scale_t), _addr(next_weight),
@@ -554,9 +556,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
     logits, scores = _rows(logits), scores.contiguous()
     with _on(dev):
         n = max(num, 0)
-        best = torch.empty((B, n), device=logits.device, dtype=torch.float32)
+        best = scores.new_empty((B, n))
         parents = torch.empty((B, n), device=logits.device, dtype=torch.int64)
-        tokens = torch.empty((B, n), device=logits.device, dtype=torch.int64)
+        tokens = torch.empty_like(parents)
         nbytes = lib().mb2_beam_select_workspace_bytes(code, B, K, V, num)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
         rc = lib().mb2_beam_select(code, logits.data_ptr(), logits.stride(0), logits.stride(1),
@@ -571,8 +573,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
 def _leaves(states, out: list) -> list:
     if isinstance(states, torch.Tensor):
         out.append(states)
-    else:
-        for s in states.values() if isinstance(states, dict) else states:
+        return out
+    for s in states.values() if isinstance(states, dict) else states:
+        if isinstance(s, torch.Tensor):
+            out.append(s)
+        else:
             _leaves(s, out)
     return out
 
@@ -595,13 +600,12 @@ def reorder_states(states, parents: torch.Tensor):
     rows = B * K
     tensors = _leaves(states, [])
     dev = _device_of(what, parents, *tensors)
-    ptrs, sizes = [], []
     for t in tensors:
         if t.dim() < 1 or t.shape[0] != rows or not t.is_contiguous():
             raise RuntimeError(f"{what}: states must be contiguous with {rows} rows, got "
                                f"{tuple(t.shape)}")
-        ptrs.append(t.data_ptr())
-        sizes.append(t.nbytes // rows if rows else 0)
+    ptrs = [t.data_ptr() for t in tensors]
+    sizes = [t.nbytes // (rows or 1) for t in tensors]
     parents = parents.to(torch.int64).contiguous()
     n = len(ptrs)
     with _on(dev):
