@@ -802,8 +802,7 @@ __global__ void zero_tail_kernel(const Args a) {
 // threads per state row of VEC columns each, the CTA's row slots stepping
 // through the Dk rows with ROWS rows' loads in flight per thread.  Partial
 // sums of o over the row slots meet in shared memory, added in a fixed order.
-constexpr int STEP_THREADS = 256;
-template <typename T, int VEC>
+template <typename T, int VEC, int STEP_THREADS>
 __global__ void __launch_bounds__(STEP_THREADS)
 decay_step_kernel(const Args a, float *__restrict__ state, int lanes) {
     constexpr int ROWS = 8;
@@ -892,10 +891,22 @@ static int step(const Args &a, float *state, cudaStream_t st) {
     int lanes = (int)(ceil_div(a.dv, per) < 64 ? ceil_div(a.dv, per) : 64);
     const int64_t grid = ceil_div(a.dv, lanes * per) * a.heads * a.seqs;
     MB2_REQUIRE(grid <= 0x7fffffff, MB2_ERR_SHAPE, "decay_attention_step: batch x heads too large");
-    if (vec)
-        decay_step_kernel<T, 4><<<(unsigned)grid, STEP_THREADS, 0, st>>>(a, state, lanes);
-    else
-        decay_step_kernel<T, 1><<<(unsigned)grid, STEP_THREADS, 0, st>>>(a, state, lanes);
+    // about 12 rows of 16 bytes a thread, or 64 of 4: small states want small CTAs, so that
+    // more of them hide one another's start (us; 64, 128, 256 threads):
+    //   334 x 12 heads of 24 x 64       8.7   13.2   22.4
+    //   800 x 8 of 128 x 40            45.7   44.5   53.3
+    //   512 x 24 of 128 x 64            127    122    121
+    //   500 x 12 of 18 x 63            17.5   23.0   32.7
+    //   561 x 24 of 115 x 46            138    134    145
+    const int64_t need = a.dk * lanes / (vec ? 12 : 64);
+    const int threads = need <= 64 ? 64 : need <= 128 ? 128 : 256;
+    auto kern = vec ? threads == 64    ? decay_step_kernel<T, 4, 64>
+                      : threads == 128 ? decay_step_kernel<T, 4, 128>
+                                       : decay_step_kernel<T, 4, 256>
+                    : threads == 64    ? decay_step_kernel<T, 1, 64>
+                      : threads == 128 ? decay_step_kernel<T, 1, 128>
+                                       : decay_step_kernel<T, 1, 256>;
+    kern<<<(unsigned)grid, threads, 0, st>>>(a, state, lanes);
     return check_launch("decay_step_kernel");
 }
 

@@ -540,3 +540,17 @@ def test_rows_outside_the_packed_sequences(T, dv, dtype):
     for a, b in ((7, 20), (20, T - 9)):
         ref = reference(spread(q[:, a:b], 2), spread(k[:, a:b], 2), v[:, a:b], g[:, a:b], 1.0)
         check(new[:, a:b], None, ref, dtype, b - a, 32)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dk,dv", [(18, 63), (65, 62), (66, 63), (129, 64), (250, 129), (24, 64),
+                                   (48, 64), (49, 64), (97, 64), (3, 4), (256, 256)])
+def test_one_token_by_every_size_of_block(dk, dv, dtype):
+    """Few and many threads, by rows of 16 and of 4 bytes; an address off 16 bytes."""
+    q, k, v, g, h0 = make(3, 1, 4, 2, 1, 4, dk, dv, dtype, seed=dk + dv)
+    ref = reference(spread(q, 4), spread(k, 4), v, g, 1.0, h0)
+    one = [t[:, 0].cuda() for t in (q, k, v, g)]
+    for s in (h0.cuda(), torch.empty(h0.numel() + 1, device="cuda")[1:].view(h0.shape).copy_(h0)):
+        o = ops.decay_attention_step(*one, s)
+        check(o.unsqueeze(1), s, ref, dtype, 1, dk)
