@@ -74,7 +74,7 @@ constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
 constexpr uint32_t OFF_DEC = OFF_SC + 2 * 16 * 4;        // float [4]
 constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // Chunk [4]
 constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 3 * 16;
-constexpr int NBARS = 6 + 6 + 4 + 9 + 2;
+constexpr int NBARS = 6 + 6 + 4 + 9 + 2 + 2;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
 // scalars of a chunk (OFF_SC), all e^sums of whole blocks' decays
@@ -377,6 +377,9 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     const uint32_t o_full = bar(23);    // P V and Q S0 in TMEM, P read
     const uint32_t o_free = bar(24);    // ... read
     const uint32_t drain = bar(25);     // [2] a warp's MMAs complete (once, at the end)
+    // V in shared memory with its tail zeroed, V~ made; by stage, since V~ may be a chunk
+    // ahead of P V (vt_full would then be in its next phase)
+    auto v_full = [&](int s) { return bar(27 + s); };
 
     // through a shuffle, so that the compiler knows it to be one value a warp
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -389,7 +392,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                           (i == 12 || i == 13) ? 32 :    // g_full
                           (i == 14 || i == 15) ? (STATE ? 256 : 128) :   // g_free
                           i == 23 ? 2 :                  // o_full
-                          (i == 17 || i == 24) ? 128 :   // vt_full, o_free
+                          (i == 17 || i == 24 || i >= 27) ? 128 :   // vt_full, o_free, v_full
                           (i == 19 || i == 20 || i == 22) ? 256 : 1;   // d_free, h_full, p_full
             mbar_init(bar(i), n);
         }
@@ -463,7 +466,9 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (n > 0) {
                     const uint32_t ph = (n - 1) & 1;
                     const uint64_t v = v0 + ph * (SUB >> 4);
-                    ok = ok && wait_warp(o_free, ph ^ 1, 0x416) && wait_warp(p_full, ph, 0x417);
+                    ok = ok && wait_warp(o_free, ph ^ 1, 0x416) &&
+                         wait_warp(v_full(ph), ((n - 1) >> 1) & 1, 0x419) &&
+                         wait_warp(p_full, ph, 0x417);
                     fence_after();
                     if (ok && elect_one()) {
 #pragma unroll 2
@@ -847,7 +852,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             fence_async_smem();
             mbar_arrive(vt_full);
-            if (STATE) mbar_arrive(empty_v(s));
+            mbar_arrive(STATE ? empty_v(s) : v_full(s));
         }
     } else {
         // -------------------------------------------------- the output rows

@@ -554,3 +554,39 @@ def test_one_token_by_every_size_of_block(dk, dv, dtype):
     for s in (h0.cuda(), torch.empty(h0.numel() + 1, device="cuda")[1:].view(h0.shape).copy_(h0)):
         o = ops.decay_attention_step(*one, s)
         check(o.unsqueeze(1), s, ref, dtype, 1, dk)
+
+
+# ------------------------------------------------- hand-overs between the roles
+def beside_copies(call, times):
+    """The results of ``call`` on one stream while another one copies: loads then
+    come late and out of order."""
+    a = torch.zeros(1 << 26, device="cuda")
+    b = torch.empty_like(a)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(times):
+        with torch.cuda.stream(side):
+            b.copy_(a)
+        got.append(call())
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    return got
+
+
+@gpu
+def test_v_has_arrived_before_it_is_multiplied():
+    """The same bits whenever the loads of v come; each sequence ends inside a chunk,
+    before one whose first token holds infinities."""
+    lens = [300, 129, 1, 500, 77, 640, 255]
+    H, dk, dv, dtype = 40, 128, 64, torch.bfloat16
+    q, k, v, g, _ = make(1, sum(lens), H, 1, 1, H, dk, dv, dtype, seed=31)
+    cu = torch.tensor([0] + lens).cumsum(0)
+    clean = v.clone()
+    v[:, cu[1:-1], :, ::3] = float("-inf")
+    args = [t.cuda() for t in (q, k, v, g)]
+    got = beside_copies(lambda: ops.decay_attention(*args, cu_seqlens=cu.cuda()), 30)
+    assert all(torch.equal(o.view(torch.int16), got[0].view(torch.int16)) for o in got)
+    w = slice(0, lens[0])                                # the sequence without them
+    ref = reference(spread(q[:, w], H), spread(k[:, w], H), clean[:, w], g[:, w], 1.0)
+    check(got[0][:, w], None, ref, dtype, lens[0], dk)
