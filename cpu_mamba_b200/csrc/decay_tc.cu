@@ -390,7 +390,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                           (i == 8 || i == 9) ? (STATE ? 1 : 2) :   // empty_k
                           (i == 10 || i == 11) ? (STATE ? 128 : 1) :   // empty_v
                           (i == 12 || i == 13) ? 32 :    // g_full
-                          (i == 14 || i == 15) ? (STATE ? 256 : 128) :   // g_free
+                          (i == 14 || i == 15) ? (STATE ? 256 : 384) :   // g_free
                           i == 23 ? 2 :                  // o_full
                           (i == 17 || i == 24 || i >= 27) ? 128 :   // vt_full, o_free, v_full
                           (i == 19 || i == 20 || i == 22) ? 256 : 1;   // d_free, h_full, p_full
@@ -661,6 +661,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             if (!wait_warp(g_full(c & 1), (c >> 1) & 1, 0x424)) break;
             const Chunk k = chunks[c & 3];
             if (k.m == 0) break;
+            // g_full's next phase of this stage has to wait for this one to be seen here,
+            // too: the state of chunk c is handed over a chunk earlier, so that all other
+            // roles can be done with the chunk before these warps have looked
+            if (!STATE) mbar_arrive(g_free(c & 1));
             const uint64_t dec2 = pair(dec[c & 3]);
             const int c0 = k.tile * DV;
             const int64_t at = ((int64_t)k.h * a.dk + r) * a.dv + c0;

@@ -590,3 +590,22 @@ def test_v_has_arrived_before_it_is_multiplied():
     w = slice(0, lens[0])                                # the sequence without them
     ref = reference(spread(q[:, w], H), spread(k[:, w], H), clean[:, w], g[:, w], 1.0)
     check(got[0][:, w], None, ref, dtype, lens[0], dk)
+
+
+@gpu
+def test_many_short_spans_and_long_ones_keep_their_hand_overs():
+    """Sequences of one chunk and of many, side by side, several items a CTA."""
+    r = torch.Generator().manual_seed(5)
+    lens = [int(n) for n in torch.randint(1, 3, (40,), generator=r) * 127] + [2000, 1, 128, 129, 0]
+    H, dk, dv, dtype = 32, 64, 64, torch.bfloat16
+    q, k, v, g, _ = make(1, sum(lens), H, 1, 1, H, dk, dv, dtype, seed=32)
+    h0 = torch.randn(len(lens), H, dk, dv, generator=r)
+    cu = torch.tensor([0] + lens).cumsum(0)
+    args = [t.cuda() for t in (q, k, v, g)]
+    got = beside_copies(lambda: ops.decay_attention(*args, cu_seqlens=cu.cuda(), return_final_state=True,
+                                                    initial_state=h0.cuda()), 20)
+    assert all(torch.equal(x, y) for pair in got for x, y in zip(pair, got[0]))
+    for i in (0, 7, 40, 42, 43):
+        w = slice(int(cu[i]), int(cu[i + 1]))
+        ref = reference(spread(q[:, w], H), spread(k[:, w], H), v[:, w], g[:, w], 1.0, h0[i:i + 1])
+        check(got[0][0][:, w], got[0][1][i:i + 1], ref, dtype, lens[i], dk)
