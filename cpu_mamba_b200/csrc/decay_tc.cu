@@ -74,7 +74,7 @@ constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
 constexpr uint32_t OFF_DEC = OFF_SC + 2 * 16 * 4;        // float [4]
 constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // Chunk [4]
 constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 3 * 16;
-constexpr int NBARS = 6 + 6 + 4 + 9 + 2 + 2;
+constexpr int NBARS = 6 + 6 + 4 + 9 + 2 + 4;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
 // scalars of a chunk (OFF_SC), all e^sums of whole blocks' decays
@@ -310,6 +310,13 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int whe
     return __all_sync(0xffffffffu, wait_one(bar, parity, where));
 }
 
+// a row of `tiles` operand tiles
+__device__ __forceinline__ void zero_row(uint8_t *row, int tiles) {
+#pragma unroll 1
+    for (int i = 0; i < 8 * tiles; ++i)
+        *reinterpret_cast<uint4 *>(row + (i >> 3) * SUB + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+}
+
 // scale sum_j P_ij v_j of row r over its own tokens j <= r of the chunk, from global
 // memory: for rows that met an infinity or a NaN, perhaps in a masked token
 __device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r, int col,
@@ -380,6 +387,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     // V in shared memory with its tail zeroed, V~ made; by stage, since V~ may be a chunk
     // ahead of P V (vt_full would then be in its next phase)
     auto v_full = [&](int s) { return bar(27 + s); };
+    auto k_tail = [&](int s) { return bar(29 + s); };    // K's rows behind the end zeroed
 
     // through a shuffle, so that the compiler knows it to be one value a warp
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -392,7 +400,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                           (i == 12 || i == 13) ? 32 :    // g_full
                           (i == 14 || i == 15) ? (STATE ? 256 : 384) :   // g_free
                           i == 23 ? 2 :                  // o_full
-                          (i == 17 || i == 24 || i >= 27) ? 128 :   // vt_full, o_free, v_full
+                          (i == 17 || i == 24 || i >= 27) ? 128 :   // vt_full, o_free, v_full, k_tail
                           (i == 19 || i == 20 || i == 22) ? 256 : 1;   // d_free, h_full, p_full
             mbar_init(bar(i), n);
         }
@@ -461,8 +469,10 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 const uint32_t s = n & 1, ph2 = (n >> 1) & 1;
                 ok = wait_warp(g_full(s), ph2, 0x410);
                 more = ok ? uniform(chunks[n & 3].m) : 0;
-                if (more)
+                if (more) {
                     ok = wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
+                    if (more < C) ok = ok && wait_warp(k_tail(s), ph2, 0x41a);
+                }
                 if (n > 0) {
                     const uint32_t ph = (n - 1) & 1;
                     const uint64_t v = v0 + ph * (SUB >> 4);
@@ -816,24 +826,20 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             if (!wait_warp(g_full(s), ph2, 0x441)) break;
             const int m = chunks[c & 3].m;
             if (m == 0) break;
+            if (m < C) {
+                // rows behind the sequence (another one's, or nothing): zero in V and K,
+                // whose values a product would otherwise meet; in K before Q K^T
+                if (!wait_warp(full_k(s), ph2, 0x443)) break;
+                if (r >= m) zero_row(smem + OFF_K + s * 2 * SUB + r * 128, 2);
+                fence_async_smem();
+            }
+            if (!STATE) mbar_arrive(k_tail(s));
             const uint64_t wj2 = pair(colf[s * C + r] * sc[s * 16 + SC_AFTER + w]);
             const uint64_t minus1 = pair(-1.0f);
             if (!wait_warp(full_v(s), ph2, 0x442)) break;
-            if (m < C && !wait_warp(full_k(s), ph2, 0x443)) break;
             if (!wait_warp(d_full, (c & 1) ^ 1, 0x444)) break;             // V~ (c - 1) read
             uint8_t *const vrow = smem + OFF_V + s * SUB + r * 128;
-            if (r >= m) {
-                // rows behind the sequence (another one's, or nothing): zero in
-                // V and K, whose values a product would otherwise meet
-                const uint4 z = make_uint4(0, 0, 0, 0);
-                uint8_t *const krow = smem + OFF_K + s * 2 * SUB + r * 128;
-#pragma unroll 1
-                for (int i = 0; i < 8; ++i) {
-                    *reinterpret_cast<uint4 *>(vrow + i * 16) = z;
-                    *reinterpret_cast<uint4 *>(krow + i * 16) = z;
-                    *reinterpret_cast<uint4 *>(krow + SUB + i * 16) = z;
-                }
-            }
+            if (r >= m) zero_row(vrow, 1);
 #pragma unroll 2
             for (int i = 0; i < 8; ++i) {
                 const uint32_t off = (uint32_t)((i ^ (r & 7)) << 4);   // free of bank conflicts

@@ -609,3 +609,25 @@ def test_many_short_spans_and_long_ones_keep_their_hand_overs():
         w = slice(int(cu[i]), int(cu[i + 1]))
         ref = reference(spread(q[:, w], H), spread(k[:, w], H), v[:, w], g[:, w], 1.0, h0[i:i + 1])
         check(got[0][0][:, w], got[0][1][i:i + 1], ref, dtype, lens[i], dk)
+
+
+@gpu
+def test_keys_behind_a_sequence_do_not_reach_it():
+    """The bits of a call without them, whatever keys follow a sequence's last token."""
+    lens = [300, 129, 1, 500, 77, 640, 255]
+    H, dk, dv, dtype = 40, 128, 64, torch.bfloat16
+    q, k, v, g, _ = make(1, sum(lens), H, 1, 1, H, dk, dv, dtype, seed=33)
+    cu = torch.tensor([0] + lens).cumsum(0)
+    args = [t.cuda() for t in (q, k, v, g)]
+    want = ops.decay_attention(*args, cu_seqlens=cu.cuda())
+    bad = args[1].clone()                     # every second sequence without a finite key
+    keep = torch.zeros(sum(lens), dtype=torch.bool, device="cuda")
+    for i in range(len(lens)):
+        w = slice(int(cu[i]), int(cu[i + 1]))
+        keep[w] = i % 2 == 0
+        if i % 2:
+            bad[:, w] = float("nan") if i % 4 == 1 else float("inf")
+    got = beside_copies(lambda: ops.decay_attention(args[0], bad, *args[2:], cu_seqlens=cu.cuda()), 30)
+    for o in got:
+        assert torch.equal(o[:, keep], want[:, keep])
+        assert not bool(torch.isfinite(o[:, ~keep]).any())
