@@ -15,25 +15,34 @@
 // scans, so strong decays earlier in a chunk cost later differences nothing; g
 // below -256 counts as -256, whose e^g is below every fp32 product's reach.
 //
-// Roundings to bf16: P and S0 as MMA operands; each costs an output about as much
-// as its own rounding (2.3e-3 relative in all, 1.7e-3 for the output's alone).  V~
-// is held as three bf16 parts (24 bits), because the state is an fp32 output and
-// lives for many chunks.
+// Operands: P and S0 are two bf16 parts each (16 bits: 2^-16 of a term, so an output's
+// error is that of its own rounding, 1.66e-3 rms of 1.66e-3; with one part each it was
+// 2.3e-3, and 8 sequences of 8192 tokens took 306 us instead of 363).  V~ is three
+// (24 bits), because the state is an fp32 output and lives for many chunks.  An
+// infinity stands in the first part alone.
+//
+// Room: S0's second part lies in the second half of the q stage of the chunk before,
+// which Q K^T and Q S0 have read and the output rows leave free; the next q waits for
+// the Q S0 that reads it.  (In the k stage or the v stage the next chunk's K^T V~ waits
+// for it too: 412 and 478 us.)  P replaces its scores in TMEM.
 //
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone.
 //
-// Roles (28 warps): 0-7 the state, 8-15 P, 16-19 the output rows, 20-23 V~, 24 and
-// 25 MMA issue, 26 TMA loads, 27 decays.  One MMA warp issues P V (n), Q K^T (n + 1),
-// the other K^T V~ (n), Q S0 (n), each as soon as its operands are there.  Every
+// Roles (28 warps): 0-7 the state, 8-15 P, 16-19 the output rows, 20-23 V~, 24
+// decays (its scheduler has the least of P's triangle), 25 TMA loads, 26 and 27 MMA
+// issue.  One MMA warp issues P V (n), Q K^T (n + 1), the other K^T V~ (n), Q S0 (n),
+// each as soon as its operands are there.  Every
 // mbarrier completes once per chunk (staged ones once per two), so its phase
 // follows from the chunk count.  All waits are bounded; a wait that expires sets
 // the device status.
 //
-// Bound: neither bytes nor MMAs (2100 cycles a chunk) but the chain of hand-overs
-// between the roles, about 4300 cycles = 2.3 us a chunk with 128-wide q and k, one
-// CTA an SM (shared memory and TMEM are full).  What brought it there, at 8
-// sequences of 8192 tokens, 24 heads of 128 x 64 (1.5 us of HBM time a chunk):
+// Bound: neither bytes nor MMAs (2700 cycles a chunk) but the chain of hand-overs
+// between the roles, about 4800 cycles = 2.6 us a chunk with 128-wide q and k, one
+// CTA an SM (shared memory and TMEM are full): Q K^T 1100, P 2400 (its scheduler's FMA
+// and ALU pipes, shared with V~ and the state), P V 700.  What brought it there, at 8
+// sequences of 8192 tokens, 24 heads of 128 x 64 (1.5 us of HBM time a chunk), with
+// P and S0 in one part:
 //   733 us  one role after the other, the state in registers
 //   411     a short loop over 16-column pieces per role instead of straight-line
 //           code, the state in TMEM: five roles share each scheduler's instruction
@@ -59,7 +68,7 @@ constexpr int C = 128;                       // tokens per chunk
 constexpr int DV = 64;                       // columns of v per CTA
 // first warp of each role: the state (8 warps), P (8), output rows, V~, MMA (2), TMA,
 // decays
-constexpr int W_P = 8, W_O = 16, W_V = 20, W_MMA = 24, W_TMA = 26, W_G = 27;
+constexpr int W_P = 8, W_O = 16, W_V = 20, W_MMA = 26, W_TMA = 25, W_G = 24;
 constexpr int THREADS = 28 * 32;
 constexpr uint32_t SUB = 128 * 128;          // one 128-row x 128-byte operand tile
 // shared memory (bytes from a 1024-aligned base)
@@ -67,14 +76,16 @@ constexpr uint32_t OFF_Q = 0;                            // [2][2 SUB]
 constexpr uint32_t OFF_K = OFF_Q + 4 * SUB;              // [2][2 SUB]
 constexpr uint32_t OFF_V = OFF_K + 4 * SUB;              // [2][SUB]
 constexpr uint32_t OFF_VT = OFF_V + 2 * SUB;             // [3][SUB]
-constexpr uint32_t OFF_H = OFF_VT + 3 * SUB;             // [SUB]
+constexpr uint32_t OFF_H = OFF_VT + 3 * SUB;             // [SUB]: S0's first part
+// S0's second part, of chunk c: where the second half of q of chunk c - 1 was
+__device__ __forceinline__ uint32_t off_h2(uint32_t c) { return OFF_Q + ((c & 1) ^ 1) * 2 * SUB + SUB; }
 constexpr uint32_t OFF_COLF = OFF_H + SUB;               // float [2][128]
 constexpr uint32_t OFF_G2 = OFF_COLF + 2 * C * 4;        // float [2][128]
 constexpr uint32_t OFF_SC = OFF_G2 + 2 * C * 4;          // float [2][16]
 constexpr uint32_t OFF_DEC = OFF_SC + 2 * 16 * 4;        // float [4]
 constexpr uint32_t OFF_CHUNK = OFF_DEC + 4 * 4;          // Chunk [4]
 constexpr uint32_t OFF_BARS = OFF_CHUNK + 4 * 3 * 16;
-constexpr int NBARS = 6 + 6 + 4 + 9 + 2 + 4;
+constexpr int NBARS = 6 + 6 + 4 + 9 + 2 + 6;
 constexpr uint32_t OFF_TMEM = OFF_BARS + NBARS * 8;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16;
 // scalars of a chunk (OFF_SC), all e^sums of whole blocks' decays
@@ -84,14 +95,16 @@ constexpr int SC_ALL = 8;        // the chunk
 constexpr int SC_1 = 9, SC_12 = 10, SC_2 = 11;   // block 1; blocks 1 and 2; block 2
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 // TMEM columns
-// (T_D: K^T V~ of V~'s first part, then of the other two)
-constexpr uint32_t T_S = 0, T_P = 128, T_PV = 192, T_QH = 256, T_D = 320, T_H = 448;
+// (P takes the place of the scores: of every 16 tokens 8 columns of its first part, 8
+// of its second.  T_QH: Q times S0's second part, then its first; T_D: K^T V~ of V~'s
+// first part, then of the other two)
+constexpr uint32_t T_S = 0, T_PV = 128, T_QH = 192, T_D = 320, T_H = 448;
 
 // UMMA descriptor of an MN-major operand, 128-byte swizzle: rows are the
 // contraction index (128 bytes of 64 MN elements each), 8-row groups 1024 B
-// apart, further 64-element MN atoms SUB apart.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(SUB >> 4) << 16) |
+// apart, further 64-element MN atoms `next` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t next = SUB) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(next >> 4) << 16) |
            ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // D fp32, A and B bf16, M = 128
@@ -121,12 +134,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
           "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
           "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
-                   "r"(r[6]), "r"(r[7])
-                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld8_async(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -198,6 +205,20 @@ __device__ __forceinline__ uint32_t pack_bf16(uint64_t v) {
 }
 // a bf16 pair as two fp32 values
 __device__ __forceinline__ uint64_t unpack_bf16(uint32_t v) { return pair(v << 16, v & 0xffff0000u); }
+// what a rounding to bf16 left behind (exact)
+__device__ __forceinline__ uint64_t rest(uint64_t x, uint32_t rounded) {
+    return fma2(unpack_bf16(rounded), pair(-1.0f), x);
+}
+// bad becomes NaN where v holds an infinity or NaN, else stays 0
+__device__ __forceinline__ void poison(uint32_t &bad, uint32_t v) {
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(bad) : "r"(v), "r"(0));
+}
+// 0 for infinities and NaN
+__device__ __forceinline__ uint32_t finite(uint32_t v) {
+    if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
+    if ((v & 0x7f800000u) == 0x7f800000u) v &= 0xffffu;
+    return v;
+}
 
 // e^x of a 64-bit sum, to fp32 precision
 __device__ __forceinline__ float exp_of(double x) {
@@ -337,7 +358,7 @@ __device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r,
 #pragma unroll 1
         for (int e = 0; e < (int)a.dk; ++e)
             d = fmaf(__bfloat162float(q[e]), __bfloat162float(kj[e]), d);
-        const float p = io<__nv_bfloat16>::round(d * __expf((float)sum) * a.scale);
+        const float p = d * expf((float)sum) * a.scale;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (col + i < a.dv)
@@ -388,6 +409,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
     // ahead of P V (vt_full would then be in its next phase)
     auto v_full = [&](int s) { return bar(27 + s); };
     auto k_tail = [&](int s) { return bar(29 + s); };    // K's rows behind the end zeroed
+    auto q_read = [&](int s) { return bar(31 + s); };    // Q K^T has read Q
 
     // through a shuffle, so that the compiler knows it to be one value a warp
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -400,7 +422,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                           (i == 12 || i == 13) ? 32 :    // g_full
                           (i == 14 || i == 15) ? (STATE ? 256 : 384) :   // g_free
                           i == 23 ? 2 :                  // o_full
-                          (i == 17 || i == 24 || i >= 27) ? 128 :   // vt_full, o_free, v_full, k_tail
+                          (i == 17 || i == 24 || (i >= 27 && i < 31)) ? 128 :   // vt_full, o_free, v_full, k_tail
                           (i == 19 || i == 20 || i == 22) ? 256 : 1;   // d_free, h_full, p_full
             mbar_init(bar(i), n);
         }
@@ -421,9 +443,9 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         if (lane == 0) {
             Walk<STATE> k;
             const uint32_t qk = wide ? 2 * SUB : SUB;
-            uint32_t c = 0;
+            uint32_t nk = 0, nq = 0, nv = 0;             // loads issued
 #pragma unroll 1
-            for (; k.next(a, tiles, items, [] {}); ++c) {
+            for (uint32_t c = 0; k.next(a, tiles, items, [] {}); ++c) {
                 const int s = c & 1;
                 const uint32_t ph = ((c >> 1) & 1) ^ 1;
                 const int tok = k.it.row0 + k.t0, bq = a.cu ? 0 : k.it.seq;
@@ -433,21 +455,26 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 mbar_expect_tx(full_k(s), qk);
                 tma_load_4d(dk, &map_k, full_k(s), 0, hk, tok, bq);
                 if (wide) tma_load_4d(dk + SUB, &map_k, full_k(s), 64, hk, tok, bq);
+                ++nk;
                 if (!wait_one(empty_v(s), ph, 0x403)) break;
                 mbar_expect_tx(full_v(s), SUB);
                 tma_load_4d(base + OFF_V + s * SUB, &map_v, full_v(s), k.it.tile * DV, hv, tok, bq);
+                ++nv;
                 if (STATE) continue;
-                if (!wait_one(empty_q(s), ph, 0x402)) break;
+                // the stage held output rows (c - 2) and S0 (c - 1)'s second part
+                if (!wait_one(empty_q(s), ph, 0x402) || !wait_one(h_free, s ^ 1, 0x402)) break;
                 mbar_expect_tx(full_q(s), qk);
                 tma_load_4d(dq, &map_q, full_q(s), 0, hq, tok, bq);
                 if (wide) tma_load_4d(dq + SUB, &map_q, full_q(s), 64, hq, tok, bq);
+                ++nq;
             }
             // no load is in flight when the CTA ends (its consumers may have given up)
-            for (uint32_t n = c > 2 ? c - 2 : 0; n < c; ++n) {
-                wait_one(full_k(n & 1), (n >> 1) & 1, 0x404);
-                if (!STATE) wait_one(full_q(n & 1), (n >> 1) & 1, 0x404);
-                wait_one(full_v(n & 1), (n >> 1) & 1, 0x404);
-            }
+            auto land = [&](auto full, uint32_t n) {
+                for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) wait_one(full(i & 1), (i >> 1) & 1, 0x404);
+            };
+            land(full_k, nk);
+            land(full_q, nq);
+            land(full_v, nv);
         }
         __syncwarp();
     } else if (warp == W_MMA || warp == W_MMA + 1) {
@@ -457,7 +484,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
         // an MMA wants them.
         const uint64_t dq0 = smem_desc(base + OFF_Q), dk0 = smem_desc(base + OFF_K);
         const uint64_t kt0 = smem_desc_mn(base + OFF_K), v0 = smem_desc_mn(base + OFF_V);
-        const uint64_t vt0 = smem_desc_mn(base + OFF_VT), h0 = smem_desc_mn(base + OFF_H);
+        const uint64_t vt0 = smem_desc_mn(base + OFF_VT);
         constexpr uint64_t STAGE = 2 * SUB >> 4, ROWS16 = 2048 >> 4;
         const int steps = wide ? 8 : 4;                  // of 16 columns of q and k
         bool ok = true;
@@ -470,7 +497,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 ok = wait_warp(g_full(s), ph2, 0x410);
                 more = ok ? uniform(chunks[n & 3].m) : 0;
                 if (more) {
-                    ok = wait_warp(full_k(s), ph2, 0x411) && wait_warp(full_q(s), ph2, 0x412);
+                    ok = ok && wait_warp(full_k(s), ph2, 0x411);
                     if (more < C) ok = ok && wait_warp(k_tail(s), ph2, 0x41a);
                 }
                 if (n > 0) {
@@ -482,9 +509,12 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     fence_after();
                     if (ok && elect_one()) {
 #pragma unroll 2
-                        for (int i = 0; i < C / 16; ++i)
-                            mma_ts_bf16(tmem + T_PV, tmem + T_P + i * 8, v + i * ROWS16,
+                        for (int i = 0; i < C / 16; ++i) {
+                            mma_ts_bf16(tmem + T_PV, tmem + T_S + i * 16 + 8, v + i * ROWS16,
                                         idesc(64, false, true), i != 0);
+                            mma_ts_bf16(tmem + T_PV, tmem + T_S + i * 16, v + i * ROWS16,
+                                        idesc(64, false, true), 1);
+                        }
                         mma_commit(o_full);
                         mma_commit(empty_v(ph));
                     }
@@ -492,6 +522,8 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
                 if (more) {
                     const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE;
+                    ok = ok && wait_warp(full_q(s), ph2, 0x412);
+                    fence_after();
                     if (ok && elect_one()) {
 #pragma unroll 2
                         for (int i = 0; i < steps; ++i) {
@@ -500,6 +532,7 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                         }
                         mma_commit(s_full);
                         mma_commit(empty_k(s));
+                        mma_commit(q_read(s));
                     }
                     __syncwarp();
                 }
@@ -512,6 +545,8 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 ok = wait_warp(g_full(s), ph2, 0x410);
                 if (!ok || !uniform(chunks[n & 3].m)) break;
                 const uint64_t q = dq0 + s * STAGE, kt = kt0 + s * STAGE;
+                // S0's second part and, behind it, its first
+                const uint64_t h = smem_desc_mn(base + off_h2(s), OFF_H - off_h2(s));
                 ok = wait_warp(vt_full, s, 0x413) && wait_warp(full_k(s), ph2, 0x414) &&
                      wait_warp(d_free, s ^ 1, 0x414);
                 fence_after();
@@ -535,8 +570,8 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (ok && elect_one()) {
 #pragma unroll 2
                     for (int i = 0; i < steps; ++i)
-                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h0 + i * ROWS16,
-                               idesc(64, false, true), i != 0);
+                        mma_ss(tmem + T_QH, q + (i >> 2) * (SUB >> 4) + (i & 3) * 2, h + i * ROWS16,
+                               idesc(128, false, true), i != 0);
                     mma_commit(h_free);
                     mma_commit(o_full);
                 }
@@ -689,8 +724,6 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     if (!(ok = wait_warp(d_full, c & 1, 0x425))) break;
                     fence_after();
                 }
-                // Q S0 of the chunk before the one this state is for
-                if (!STATE && !store && !(ok = wait_warp(h_free, (c + pass + 1) & 1, 0x423))) break;
 #pragma unroll 1
                 for (int i = 32 * half; i < 32 * half + 32; i += 16) {
                     uint32_t h[16];
@@ -727,15 +760,6 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                                     make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
                     } else {
                         tmem_st16(quarter + T_H + i, h);
-#pragma unroll
-                        for (int j = 0; !STATE && j < 2; ++j) {
-                            uint4 x;
-                            x.x = pack_bf16(pair(h[8 * j], h[8 * j + 1]));
-                            x.y = pack_bf16(pair(h[8 * j + 2], h[8 * j + 3]));
-                            x.z = pack_bf16(pair(h[8 * j + 4], h[8 * j + 5]));
-                            x.w = pack_bf16(pair(h[8 * j + 6], h[8 * j + 7]));
-                            *reinterpret_cast<uint4 *>(hrow + (((i / 8 + j) ^ (r & 7)) << 4)) = x;
-                        }
                     }
                 }
                 if (pass == 1) {
@@ -744,25 +768,50 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                     if (STATE) mbar_arrive(g_free(c & 1));   // V~ (c) has read them too
                 }
                 if (!store) tmem_wait_st();
-                if (!STATE && !store) {
-                    fence_async_smem();
-                    mbar_arrive(h_full);
+                if (STATE || store) continue;
+                // Q S0 of the chunk before the one this state is for, and all else that
+                // reads that chunk's q, where the second part goes
+                const uint32_t prev = c + pass - 1;
+                if (!(ok = wait_warp(h_free, prev & 1, 0x423) &&
+                           wait_warp(q_read(prev & 1), (prev >> 1) & 1, 0x426)))
+                    break;
+                uint8_t *const hrow2 = smem + off_h2(c + pass) + r * 128;
+#pragma unroll 1
+                for (int i = 32 * half; i < 32 * half + 32; i += 16) {
+                    uint32_t h[16], p[8], p2[8], bad = 0;
+                    tmem_ld16_async(quarter + T_H + i, h);
+                    tmem_loaded(h);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint64_t x = pair(h[2 * j], h[2 * j + 1]);
+                        p[j] = pack_bf16(x);
+                        p2[j] = pack_bf16(rest(x, p[j]));
+                        poison(bad, p2[j]);
+                    }
+                    if (__any_sync(0xffffffffu, row && (bad & 0x7fff7fffu))) {
+                        // infinities stand in the first part alone
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) p2[j] = finite(p2[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t off = ((i / 8 + j) ^ (r & 7)) << 4;
+                        *reinterpret_cast<uint4 *>(hrow + off) =
+                            make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+                        *reinterpret_cast<uint4 *>(hrow2 + off) =
+                            make_uint4(p2[4 * j], p2[4 * j + 1], p2[4 * j + 2], p2[4 * j + 3]);
+                    }
                 }
+                fence_async_smem();
+                mbar_arrive(h_full);
             }
         }
     } else if (warp < W_O) {
         // ---------------------------------------------------------------- P
         // rows 32 w + lane; the first four warps take blocks 0 and 2, the others
-        // 1 and 3.  Blocks above the diagonal stay the zeros written here.
+        // 1 and 3, each in place of its scores; zeros above the diagonal.
         const int w = warp & 3, odd = (warp - W_P) >> 2, r = 32 * w + lane;
         const uint32_t quarter = tmem + ((uint32_t)(32 * w) << 16);
-        {
-            uint32_t z[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = 0u;
-            for (int b = odd; b < 4; b += 2) tmem_st16(quarter + T_P + 16 * b, z);
-            tmem_wait_st();
-        }
         const uint64_t scale2 = pair(a.scale);
         for (uint32_t c = 0; !STATE; ++c) {
             const int s = c & 1;
@@ -772,13 +821,18 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             // e^{blocks between}: block b's columns for the rows of block w
             const float f0 = rowf * (w == 2 ? sc[s * 16 + SC_1] : w == 3 ? sc[s * 16 + SC_12] : 1.0f);
             const float f1 = rowf * (w == 3 ? sc[s * 16 + SC_2] : 1.0f);
-            // P of the chunk before has been read
-            if (!wait_warp(s_full, c & 1, 0x432) || !wait_warp(o_full, (c & 1) ^ 1, 0x433)) break;
+            if (!wait_warp(s_full, c & 1, 0x432)) break;
             fence_after();
 #pragma unroll 1
-            for (int n = 2 * odd; n < 2 * w + 2; n += (n & 1) ? 3 : 1) {   // 16 columns
-                uint32_t x[16], p[8];
+            for (int n = 2 * odd; n < C / 16; n += (n & 1) ? 3 : 1) {      // 16 columns
+                uint32_t x[16], p[16];
                 uint64_t f[8];
+                if (n >= 2 * w + 2) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[i] = 0u;
+                    tmem_st16(quarter + T_S + 16 * n, p);
+                    continue;
+                }
                 tmem_ld16_async(quarter + T_S + 16 * n, x);
                 const int b = n >> 1;
                 if (b < w) {
@@ -808,8 +862,12 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
                 tmem_loaded(x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) p[i] = pack_bf16(mul2(pair(x[2 * i], x[2 * i + 1]), f[i]));
-                tmem_st8(quarter + T_P + 8 * n, p);
+                for (int i = 0; i < 8; ++i) {
+                    const uint64_t y = mul2(pair(x[2 * i], x[2 * i + 1]), f[i]);
+                    p[i] = pack_bf16(y);
+                    p[8 + i] = pack_bf16(rest(y, p[i]));
+                }
+                tmem_st16(quarter + T_S + 16 * n, p);
             }
             tmem_wait_st();
             fence_before();
@@ -835,7 +893,6 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             if (!STATE) mbar_arrive(k_tail(s));
             const uint64_t wj2 = pair(colf[s * C + r] * sc[s * 16 + SC_AFTER + w]);
-            const uint64_t minus1 = pair(-1.0f);
             if (!wait_warp(full_v(s), ph2, 0x442)) break;
             if (!wait_warp(d_full, (c & 1) ^ 1, 0x444)) break;             // V~ (c - 1) read
             uint8_t *const vrow = smem + OFF_V + s * SUB + r * 128;
@@ -850,9 +907,9 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 for (int e = 0; e < 4; ++e) {
                     uint64_t y = mul2(unpack_bf16(x[e]), wj2);
                     p0[e] = pack_bf16(y);
-                    y = fma2(unpack_bf16(p0[e]), minus1, y);
+                    y = rest(y, p0[e]);
                     p1[e] = pack_bf16(y);
-                    p2[e] = pack_bf16(fma2(unpack_bf16(p1[e]), minus1, y));
+                    p2[e] = pack_bf16(rest(y, p1[e]));
                 }
                 *reinterpret_cast<uint4 *>(trow + off) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
                 *reinterpret_cast<uint4 *>(trow + SUB + off) =
@@ -886,16 +943,19 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
             uint32_t bad = 0;                            // 0, or NaN
 #pragma unroll 1
             for (int i0 = 0; i0 < DV; i0 += 16) {
-                uint32_t pv[16], qh[16], y[8];
+                uint32_t pv[16], q2[16], qh[16], y[8];
                 tmem_ld16_async(quarter + T_PV + i0, pv);
-                tmem_ld16_async(quarter + T_QH + i0, qh);
+                tmem_ld16_async(quarter + T_QH + i0, q2);
+                tmem_ld16_async(quarter + T_QH + 64 + i0, qh);
                 tmem_loaded(pv);
+                tmem_loaded(q2);
                 tmem_loaded(qh);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    y[i] = pack_bf16(fma2(pair(qh[2 * i], qh[2 * i + 1]), ei2,
-                                          pair(pv[2 * i], pv[2 * i + 1])));
-                    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(bad) : "r"(y[i]), "r"(0));
+                    y[i] = pack_bf16(fma2(add2(pair(q2[2 * i], q2[2 * i + 1]),
+                                               pair(qh[2 * i], qh[2 * i + 1])),
+                                          ei2, pair(pv[2 * i], pv[2 * i + 1])));
+                    poison(bad, y[i]);
                 }
                 const int j = i0 / 8;
                 *reinterpret_cast<uint4 *>(orow + ((j ^ (r & 7)) << 4)) =
@@ -928,12 +988,21 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 // infinities or NaN: those rows again, from their own tokens
 #pragma unroll 1
                 for (int i0 = 0; i0 < DV; i0 += 16) {
-                    uint32_t z[16], qh[16];
+                    uint32_t z[16], q2[16], qh[16];
                     tmem_ld16_async(quarter + T_PV + i0, z);
-                    tmem_ld16_async(quarter + T_QH + i0, qh);
                     tmem_loaded(z);
-                    tmem_loaded(qh);
                     if (redo) masked_row(a, k, r, c0 + i0, z);
+                    __syncwarp();
+                    tmem_ld16_async(quarter + T_QH + i0, q2);
+                    tmem_ld16_async(quarter + T_QH + 64 + i0, qh);
+                    tmem_loaded(q2);
+                    tmem_loaded(qh);
+                    // an infinite q meets S0's first part alone: the second's sign is its own
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = __uint_as_float(qh[i]);
+                        if (x - x == 0.0f) qh[i] = __float_as_uint(x + __uint_as_float(q2[i]));
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (r < k.m && c0 + i0 + i < a.dv)

@@ -631,3 +631,24 @@ def test_keys_behind_a_sequence_do_not_reach_it():
     for o in got:
         assert torch.equal(o[:, keep], want[:, keep])
         assert not bool(torch.isfinite(o[:, ~keep]).any())
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1, 128, 3, 1, 1, 3, 128, 64), (2, 129, 2, 1, 1, 2, 64, 72),
+                                   (1, 300, 2, 2, 1, 2, 24, 64), (2, 515, 4, 1, 2, 4, 128, 128),
+                                   (1, 2049, 1, 1, 1, 1, 128, 64), (3, 200, 4, 2, 1, 4, 87, 50),
+                                   (148, 20, 1, 1, 1, 1, 16, 8)])
+def test_bf16_outputs_are_rounded_once(shape):
+    """A bf16 prompt's output is the formula's, rounded to bf16 (2^-8 of it): scores and
+    carried states enter their products in two bf16 parts, which lose 2^-8 2^-8 of a term."""
+    B, T, H, _, _, _, dk, dv = shape
+    q, k, v, g, h0 = make(*shape, torch.bfloat16, seed=T + dv)
+    ro, rs, ob, m = reference(spread(q, H), spread(k, H), spread(v, H), g, 0.7, h0)
+    o, s = ops.decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), scale=0.7,
+                               initial_state=h0.cuda(), return_final_state=True)
+    terms = (2.0 ** -16 + (3 * T + dk + 32) * 2.0 ** -24) * ob
+    tol = 2.0 ** -8 * (ro.abs() + terms) + terms + 1e-30
+    d = (o.double().cpu() - ro).abs()
+    assert bool((d <= tol).all()), (d / tol).max().item()
+    d = (s.double().cpu() - rs).abs()
+    assert bool((d <= state_tolerance(T, m)).all()), (d / state_tolerance(T, m)).max().item()
