@@ -27,7 +27,8 @@
 // for it too: 412 and 478 us.)  P replaces its scores in TMEM.
 //
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
-// row whose P V comes out non-finite is computed again from its own tokens alone.
+// row whose P V comes out non-finite is computed again from its own tokens alone (in
+// the chunk that holds them; a state that is not finite costs later chunks nothing).
 //
 // Roles (28 warps): 0-7 the state, 8-15 P, 16-19 the output rows, 20-23 V~, 24
 // decays (its scheduler has the least of P's triangle), 25 TMA loads, 26 and 27 MMA
@@ -338,32 +339,86 @@ __device__ __forceinline__ void zero_row(uint8_t *row, int tiles) {
         *reinterpret_cast<uint4 *>(row + (i >> 3) * SUB + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// scale sum_j P_ij v_j of row r over its own tokens j <= r of the chunk, from global
-// memory: for rows that met an infinity or a NaN, perhaps in a masked token
-__device__ __forceinline__ void masked_row(const Args &a, const Chunk &k, int r, int col,
-                                           uint32_t (&y)[16]) {
+// The output rows of a warp (`row0` .. row0 + 31 of the chunk) whose P V met an infinity
+// or a NaN, perhaps in a later token's v: their own tokens' share again, from global
+// memory.  The whole warp takes one row after the other: a lane the scores of four
+// tokens, then two columns of v.  `base`: 16 rows of 64 fp32, what P V is added to; redo:
+// the rows (a bit each) that get it.
+__device__ __forceinline__ double prefix_sum(double x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+__device__ __noinline__ void masked_rows(const Args &a, const Chunk &k, int row0, uint32_t redo,
+                                         const float *base) {
+    const int lane = threadIdx.x & 31;
     const int64_t bq = k.batch;
-    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + bq * a.qs[0] +
-                             (k.row + r) * a.qs[1] + (k.h / a.q_rep) * a.qs[2];
+    const __nv_bfloat16 *const q = static_cast<const __nv_bfloat16 *>(a.q) + bq * a.qs[0] +
+                                   (k.h / a.q_rep) * a.qs[2];
+    const __nv_bfloat16 *const kk = static_cast<const __nv_bfloat16 *>(a.k) + bq * a.ks[0] +
+                                    (int64_t)k.row * a.ks[1] + (k.h / a.k_rep) * a.ks[2];
+    const __nv_bfloat16 *const v = static_cast<const __nv_bfloat16 *>(a.v) + bq * a.vs[0] +
+                                   (int64_t)k.row * a.vs[1] + (k.h / a.v_rep) * a.vs[2] + k.tile * DV;
+    const float *const g = a.g + bq * a.gs[0] + (int64_t)k.row * a.gs[1] + k.h * a.gs[2];
+    __nv_bfloat16 *const o = static_cast<__nv_bfloat16 *>(a.o) + bq * a.os[0] + k.h * a.os[2] + k.tile * DV;
+    const int cols = (int)(a.dv - k.tile * DV < DV ? a.dv - k.tile * DV : DV);
+    double sum[4];                       // of g up to token 32 t + lane
+    double before = 0.0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = 0u;
-    double sum = 0.0;
+    for (int t = 0; t < 4; ++t) {
+        const int j = 32 * t + lane;
+        sum[t] = before + prefix_sum(j < k.m ? (double)clamp_g(g[j * a.gs[1]]) : 0.0, lane);
+        before = __shfl_sync(0xffffffffu, sum[t], 31);
+    }
 #pragma unroll 1
-    for (int64_t j = k.row + r; j >= k.row; --j) {
-        const __nv_bfloat16 *kj = static_cast<const __nv_bfloat16 *>(a.k) + bq * a.ks[0] +
-                                  j * a.ks[1] + (k.h / a.k_rep) * a.ks[2];
-        const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(a.v) + bq * a.vs[0] +
-                                 j * a.vs[1] + (k.h / a.v_rep) * a.vs[2] + col;
-        float d = 0.0f;
-#pragma unroll 1
-        for (int e = 0; e < (int)a.dk; ++e)
-            d = fmaf(__bfloat162float(q[e]), __bfloat162float(kj[e]), d);
-        const float p = d * expf((float)sum) * a.scale;
+    for (int n = 0; n < 16 && row0 + n < k.m; ++n) {
+        const int r = row0 + n;
+        float y0 = base[64 * n + lane], y1 = base[64 * n + 32 + lane];
+        if (redo >> n & 1) {
+            double at = 0.0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (col + i < a.dv)
-                y[i] = __float_as_uint(fmaf(p, __bfloat162float(v[i]), __uint_as_float(y[i])));
-        sum += clamp_g(a.g[bq * a.gs[0] + j * a.gs[1] + k.h * a.gs[2]]);
+            for (int t = 0; t < 4; ++t) {
+                const double x = __shfl_sync(0xffffffffu, sum[t], r & 31);
+                if (t == r >> 5) at = x;
+            }
+            const uint4 *const qr = reinterpret_cast<const uint4 *>(q + (int64_t)(k.row + r) * a.qs[1]);
+            float add0 = 0.0f, add1 = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int j = 32 * t + lane;
+                float p = 0.0f;
+                if (j <= r) {
+                    const uint4 *const kr = reinterpret_cast<const uint4 *>(kk + j * a.ks[1]);
+#pragma unroll 1
+                    for (int e = 0; e < (int)a.dk / 8; ++e) {
+                        const uint4 x = qr[e], y = kr[e];
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), p);
+                            p = fmaf(__uint_as_float(xs[i] & 0xffff0000u),
+                                     __uint_as_float(ys[i] & 0xffff0000u), p);
+                        }
+                    }
+                    p *= expf((float)(at - sum[t])) * a.scale;
+                }
+#pragma unroll 1
+                for (int i = 0; i < 32 && 32 * t + i <= r; ++i) {
+                    const float pj = __shfl_sync(0xffffffffu, p, i);
+                    const __nv_bfloat16 *const vj = v + (32 * t + i) * a.vs[1];
+                    if (lane < cols) add0 = fmaf(pj, __bfloat162float(vj[lane]), add0);
+                    if (32 + lane < cols) add1 = fmaf(pj, __bfloat162float(vj[32 + lane]), add1);
+                }
+            }
+            y0 += add0;
+            y1 += add1;
+        }
+        __nv_bfloat16 *const to = o + (int64_t)(k.row + r) * a.os[1];
+        if (lane < cols) to[lane] = __float2bfloat16_rn(y0);
+        if (32 + lane < cols) to[32 + lane] = __float2bfloat16_rn(y1);
     }
 }
 
@@ -963,8 +1018,21 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 *reinterpret_cast<uint4 *>(orow + (((j + 1) ^ (r & 7)) << 4)) =
                     make_uint4(y[4], y[5], y[6], y[7]);
             }
-            const bool redo = r < k.m && (bad & 0x7fff7fffu);
-            const bool cold = __any_sync(0xffffffffu, redo);
+            // what P V alone has met (a state that is not finite stays so: its rows are right)
+            uint32_t redo = 0;
+            if (__any_sync(0xffffffffu, r < k.m && (bad & 0x7fff7fffu))) {
+                uint64_t nan = 0;                        // 0, or NaN
+#pragma unroll 1
+                for (int i0 = 0; i0 < DV; i0 += 16) {
+                    uint32_t pv[16];
+                    tmem_ld16_async(quarter + T_PV + i0, pv);
+                    tmem_loaded(pv);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) nan = fma2(pair(pv[2 * i], pv[2 * i + 1]), 0, nan);
+                }
+                redo = __ballot_sync(0xffffffffu, r < k.m && ((lo_of(nan) | hi_of(nan)) & 0x7fffffffu));
+            }
+            const bool cold = redo != 0;
             if (!cold) {
                 fence_before();
                 mbar_arrive(o_free);
@@ -985,30 +1053,35 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                             *reinterpret_cast<const uint4 *>(orow + ((i ^ (r & 7)) << 4));
                 }
             } else {
-                // infinities or NaN: those rows again, from their own tokens
+                // infinities or NaN: those rows again, from their own tokens; 16 rows at a
+                // time through the warp's part of the stage
+                float *const part = reinterpret_cast<float *>(smem + OFF_Q + s * 2 * SUB + w * 32 * 128);
 #pragma unroll 1
-                for (int i0 = 0; i0 < DV; i0 += 16) {
-                    uint32_t z[16], q2[16], qh[16];
-                    tmem_ld16_async(quarter + T_PV + i0, z);
-                    tmem_loaded(z);
-                    if (redo) masked_row(a, k, r, c0 + i0, z);
-                    __syncwarp();
-                    tmem_ld16_async(quarter + T_QH + i0, q2);
-                    tmem_ld16_async(quarter + T_QH + 64 + i0, qh);
-                    tmem_loaded(q2);
-                    tmem_loaded(qh);
-                    // an infinite q meets S0's first part alone: the second's sign is its own
+                for (int n = 0; n < 2; ++n) {
+#pragma unroll 1
+                    for (int i0 = 0; i0 < DV; i0 += 16) {
+                        uint32_t z[16], q2[16], qh[16];
+                        tmem_ld16_async(quarter + T_PV + i0, z);
+                        tmem_ld16_async(quarter + T_QH + i0, q2);
+                        tmem_ld16_async(quarter + T_QH + 64 + i0, qh);
+                        tmem_loaded(z);
+                        tmem_loaded(q2);
+                        tmem_loaded(qh);
+                        if (lane >> 4 == n) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x = __uint_as_float(qh[i]);
-                        if (x - x == 0.0f) qh[i] = __float_as_uint(x + __uint_as_float(q2[i]));
+                            for (int i = 0; i < 16; ++i) {
+                                // an infinite q meets S0's first part alone: the second's
+                                // sign is its own
+                                float x = __uint_as_float(qh[i]);
+                                if (x - x == 0.0f) x += __uint_as_float(q2[i]);
+                                x *= __uint_as_float(lo_of(ei2));
+                                part[64 * (lane & 15) + i0 + i] =
+                                    redo >> lane & 1 ? x : x + __uint_as_float(z[i]);
+                            }
+                        }
+                        __syncwarp();
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (r < k.m && c0 + i0 + i < a.dv)
-                            row[i0 + i] = __float2bfloat16_rn(fmaf(
-                                __uint_as_float(qh[i]), __uint_as_float(lo_of(ei2)),
-                                __uint_as_float(z[i])));
+                    masked_rows(a, chunks[c & 3], 32 * w + 16 * n, redo >> 16 * n, part);
                     __syncwarp();
                 }
                 fence_async_smem();                      // the stage is a TMA load's next

@@ -652,3 +652,60 @@ def test_bf16_outputs_are_rounded_once(shape):
     assert bool((d <= tol).all()), (d / tol).max().item()
     d = (s.double().cpu() - rs).abs()
     assert bool((d <= state_tolerance(T, m)).all()), (d / state_tolerance(T, m)).max().item()
+
+
+def fastest(call, times=5):
+    best = float("inf")
+    for _ in range(times):
+        a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@gpu
+def test_a_state_that_is_not_finite_costs_its_own_columns_only():
+    """One NaN in h0: its column is NaN, every other output keeps its bits, and the call
+    takes no longer (a row that is computed again costs hundreds of times a chunk; a
+    call next to it on the stream and the clocks stay within a factor of 4)."""
+    B, T, H, dk, dv = 2, 1024, 8, 128, 64
+    q, k, v, g, h0 = (t.cuda() for t in make(B, T, H, 1, 1, H, dk, dv, torch.bfloat16, seed=41))
+    bad = h0.clone()
+    bad[:, :, 17, 5] = float("nan")
+    clean = ops.decay_attention(q, k, v, g, initial_state=h0)
+    got = ops.decay_attention(q, k, v, g, initial_state=bad)
+    keep = torch.arange(dv, device="cuda") != 5
+    assert torch.equal(got[..., keep], clean[..., keep])
+    assert bool(torch.isnan(got[..., 5]).all())
+    for x in (float("inf"), float("-inf")):
+        bad[:, :, 17, 5] = x
+        got = ops.decay_attention(q, k, v, g, initial_state=bad)
+        assert torch.equal(got[..., keep], clean[..., keep])
+        want = torch.sign(q[..., 17].float()).expand(B, T, H) * x
+        assert torch.equal(got[..., 5].float(), want)
+    # (no segments: their states carry it from one to the next)
+    wide = [t.repeat_interleave(24, 0) for t in (q, k, v, g, h0, bad)]
+    plain = fastest(lambda: ops.decay_attention(*wide[:4], initial_state=wide[4]))
+    assert fastest(lambda: ops.decay_attention(*wide[:4], initial_state=wide[5])) <= 4 * plain
+
+
+@gpu
+@pytest.mark.parametrize("dv", [64, 40])
+def test_rows_before_an_infinity_are_rounded_once(dv):
+    """Rows that share a chunk with a later infinity are computed again, to the same
+    accuracy as all others."""
+    B, T, H, dk = 2, 300, 3, 128
+    q, k, v, g, h0 = make(B, T, H, 1, 1, H, dk, dv, torch.bfloat16, seed=42)
+    ro, _, ob, _ = reference(spread(q, H), spread(k, H), v, g, 1.0, h0)
+    v[:, 200] = float("inf")
+    v[1, 37, 1, 3] = float("nan")
+    o = ops.decay_attention(*(t.cuda() for t in (q, k, v, g)), initial_state=h0.cuda())
+    terms = (2.0 ** -16 + (3 * T + dk + 32) * 2.0 ** -24) * ob
+    d = (o.double().cpu() - ro).abs()
+    ok = d <= 2.0 ** -8 * (ro.abs() + terms) + terms + 1e-30
+    ok[1, 37:, 1, 3] = True
+    assert bool(ok[:, :200].all()) and not bool(torch.isfinite(o[:, 200:]).any())
+    assert bool(torch.isnan(o[1, 37:, 1, 3]).all())
