@@ -29,6 +29,11 @@
 // Causality with infinities and NaN: a masked P_ij is 0, but 0 * inf = NaN, so a
 // row whose P V comes out non-finite is computed again from its own tokens alone (in
 // the chunk that holds them; a state that is not finite costs later chunks nothing).
+// K^T V~ splits an infinity into an infinity and NaN: such a chunk's state is taken
+// token by token.  So states are those of the recurrence, infinities with their signs
+// (until decays that sum below -104 in a chunk: 0 * inf), and so are the outputs that
+// meet them, but for a q or a v that is infinite itself (its terms have both signs, or
+// a padded row's 0: infinite or NaN).
 //
 // Roles (28 warps): 0-7 the state, 8-15 P, 16-19 the output rows, 20-23 V~, 24
 // decays (its scheduler has the least of P's triangle), 25 TMA loads, 26 and 27 MMA
@@ -422,6 +427,35 @@ __device__ __noinline__ void masked_rows(const Args &a, const Chunk &k, int row0
     }
 }
 
+// 16 columns from `col` of row r of the state (at `taddr`) over a chunk's tokens, by the
+// recurrence
+__device__ __forceinline__ void walk_state(const Args &a, const Chunk &k, int r, int col, uint32_t taddr) {
+    uint32_t h[16];
+    tmem_ld16_async(taddr, h);
+    tmem_loaded(h);
+    const int64_t bq = k.batch;
+    const __nv_bfloat16 *kk = static_cast<const __nv_bfloat16 *>(a.k) + bq * a.ks[0] +
+                              (int64_t)k.row * a.ks[1] + (k.h / a.k_rep) * a.ks[2] + r;
+    const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(a.v) + bq * a.vs[0] +
+                             (int64_t)k.row * a.vs[1] + (k.h / a.v_rep) * a.vs[2] + k.tile * DV + col;
+    const float *g = a.g + bq * a.gs[0] + (int64_t)k.row * a.gs[1] + k.h * a.gs[2];
+    const int cols = (int)(a.dv - k.tile * DV - col);
+#pragma unroll 1
+    for (int t = 0; t < k.m; ++t) {
+        const float f = expf(*g), x = r < a.dk ? __bfloat162float(*kk) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < cols)
+                h[j] = __float_as_uint(fmaf(f, __uint_as_float(h[j]), x * __bfloat162float(v[j])));
+        kk += a.ks[1];
+        v += a.vs[1];
+        g += a.gs[1];
+    }
+    __syncwarp();
+    tmem_st16(taddr, h);
+    tmem_wait_st();
+}
+
 // STATE: the pass over segments that leaves their states; no Q, no outputs
 template <bool STATE>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -798,13 +832,21 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                         tmem_loaded(h);
                         tmem_loaded(d0);
                         tmem_loaded(d1);
+                        uint64_t nan = 0;                // 0, or NaN
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            const uint64_t x =
-                                fma2(dec2, pair(h[j], h[j + 1]),
-                                     add2(pair(d0[j], d0[j + 1]), pair(d1[j], d1[j + 1])));
+                            const uint64_t own = add2(pair(d0[j], d0[j + 1]), pair(d1[j], d1[j + 1]));
+                            const uint64_t x = fma2(dec2, pair(h[j], h[j + 1]), own);
+                            nan = fma2(own, 0, nan);
                             h[j] = lo_of(x);
                             h[j + 1] = hi_of(x);
+                        }
+                        if (__any_sync(0xffffffffu, row && ((lo_of(nan) | hi_of(nan)) & 0x7fffffffu))) {
+                            // an infinity times V~'s parts makes NaN: the chunk's tokens one
+                            // by one
+                            walk_state(a, chunks[c & 3], r, i, quarter + T_H + i);
+                            tmem_ld16_async(quarter + T_H + i, h);
+                            tmem_loaded(h);
                         }
                     }
                     if (store) {

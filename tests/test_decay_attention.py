@@ -709,3 +709,37 @@ def test_rows_before_an_infinity_are_rounded_once(dv):
     ok[1, 37:, 1, 3] = True
     assert bool(ok[:, :200].all()) and not bool(torch.isfinite(o[:, 200:]).any())
     assert bool(torch.isnan(o[1, 37:, 1, 3]).all())
+
+
+def kinds(x):
+    """0 finite, 1 +inf, -1 -inf, 2 NaN"""
+    k = torch.where(x.isnan(), 2.0, 0.0)
+    return torch.where(x.isinf(), x.sign().double(), k.double())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,B", [(400, 3), (100, 3), (20, 40), (2049, 1)])
+def test_infinities_stay_infinities_in_the_state(T, B, dtype):
+    """An infinite v or k leaves the infinities of the recurrence in the final state (and
+    in the outputs behind an infinite k), on both paths and in segments; every other
+    element is finite and right."""
+    H, dk, dv = 3, 64, 40
+    q, k, v, g, h0 = make(B, T, H, H, H, H, dk, dv, dtype, seed=T)
+    g *= min(1.0, 200 / T)
+    inf = float("inf")
+    v[:, T // 3, 0, 7] = inf
+    v[:, T // 2, 0, 11] = -inf
+    k[:, T // 4, 1, 30] = inf
+    k[:, T - 1, 1, 33] = -inf
+    ref = reference(q, k, v, g, 1.0, h0)
+    o, s = ops.decay_attention(*(t.cuda() for t in (q, k, v, g)), initial_state=h0.cuda(),
+                               return_final_state=True)
+    s, o = s.double().cpu(), o.double().cpu()
+    assert torch.equal(kinds(s), kinds(ref[1]))
+    fine = kinds(ref[1]) == 0
+    assert bool(((s - ref[1]).abs() <= state_tolerance(T, ref[3]))[fine].all())
+    assert torch.equal(kinds(o[:, :, 1:]), kinds(ref[0][:, :, 1:]))
+    cols = [c for c in range(dv) if c not in (7, 11)]
+    assert bool(o[:, :, 0, cols].isfinite().all())
+    assert not bool(o[:, T // 3:, 0, 7].isfinite().any())
