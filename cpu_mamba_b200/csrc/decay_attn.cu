@@ -570,9 +570,11 @@ struct Relay {
 };
 constexpr int RELAY_THREADS = 256;
 
-// a thread's 16 bytes of our rows: from the caller's (IN) or back
+// a thread's 16 bytes of our rows: from the caller's (IN) or back (rows lo .. hi - 1, or
+// those of any sequence of r where it is given)
 template <typename E, bool IN>
-__device__ __forceinline__ void relay_rows(const Relay::Item &it, int64_t lo, int64_t hi) {
+__device__ __forceinline__ void relay_rows(const Relay::Item &it, int64_t lo, int64_t hi,
+                                           const Relay *r = nullptr) {
     constexpr uint32_t V = 16 / sizeof(E);
     const uint32_t groups = it.padded / V;
     const uint64_t total = (uint64_t)it.n[0] * it.n[1] * it.n[2] * groups;
@@ -598,6 +600,12 @@ __device__ __forceinline__ void relay_rows(const Relay::Item &it, int64_t lo, in
                 *reinterpret_cast<const uint4 *>(x);
         } else {
             if (h >= it.rows || t < lo || t >= hi) continue;
+            if (r) {
+                bool any = false;
+                for (int64_t i = 0; i < r->seqs && !any; ++i)
+                    any = t >= clamp_row(r->cu[i], r->seqlen) && t < clamp_row(r->cu[i + 1], r->seqlen);
+                if (!any) continue;
+            }
             *reinterpret_cast<uint4 *>(x) =
                 *reinterpret_cast<const uint4 *>(static_cast<const E *>(it.src) + i * V);
             E *const dst = static_cast<E *>(it.dst) + at;
@@ -618,6 +626,14 @@ relay_kernel(const __grid_constant__ Relay r) {
     }
     int64_t lo = 0, hi = INT64_MAX;
     if (!IN && r.cu) {
+        // offsets that rise cover all rows between the first and the last; others do not
+        bool falls = false;
+        for (int64_t i = threadIdx.x; i < r.seqs; i += RELAY_THREADS)
+            falls = falls || clamp_row(r.cu[i + 1], r.seqlen) < clamp_row(r.cu[i], r.seqlen);
+        if (__syncthreads_or(falls)) {
+            relay_rows<uint16_t, IN>(it, lo, hi, &r);
+            return;
+        }
         lo = clamp_row(r.cu[0], r.seqlen);
         hi = clamp_row(r.cu[r.seqs], r.seqlen);
     }

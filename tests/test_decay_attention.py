@@ -743,3 +743,34 @@ def test_infinities_stay_infinities_in_the_state(T, B, dtype):
     cols = [c for c in range(dv) if c not in (7, 11)]
     assert bool(o[:, :, 0, cols].isfinite().all())
     assert not bool(o[:, T // 3:, 0, 7].isfinite().any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dv", [64, 61])
+def test_offsets_that_fall(dv, dtype):
+    """A sequence whose end is not behind its start is empty, and the others are computed
+    wherever they stand: with rows as they are and with rows that are laid out again."""
+    T, H, dk = 400, 2, 64
+    q, k, v, g, _ = make(1, T, H, 1, 1, H, dk, dv, dtype, seed=dv)
+    h0 = torch.randn(4, H, dk, dv, generator=torch.Generator().manual_seed(2))
+    args = [t.cuda() for t in (q, k, v, g)]
+    for cu in ([150, 390, 20, 140, 10], [300, 399, 0, 0, 250], [0, 100, 90, 90, 90]):
+        out = torch.full((1, T, H, dv), 7.0, dtype=dtype, device="cuda")
+        held = torch.zeros(T, dtype=torch.bool)
+        n = len(cu) - 1
+        kw = dict(cu_seqlens=torch.tensor(cu, device="cuda"), initial_state=h0.cuda(),
+                  return_final_state=True)
+        new, s = ops.decay_attention(*args, **kw)
+        ops.decay_attention(*args, out=out, **kw)
+        for i in range(n):
+            w = slice(cu[i], cu[i + 1])
+            if cu[i + 1] <= cu[i]:
+                assert torch.equal(s[i].cpu(), h0[i])
+                continue
+            held[w] = True
+            ref = reference(spread(q[:, w], H), spread(k[:, w], H), v[:, w], g[:, w], 1.0, h0[i:i + 1])
+            check(new[:, w], s[i:i + 1], ref, dtype, cu[i + 1] - cu[i], dk)
+        assert torch.equal(out[:, held.cuda()], new[:, held.cuda()])
+        assert bool((out[:, ~held.cuda()] == 7).all())
+        assert bool((new[:, ~held.cuda()] == 0).all())
