@@ -250,7 +250,8 @@ def beam_search(model, sampler, prompt: torch.Tensor, max_new_tokens: int, beams
         raise ValueError(f"eos_token {eos_token} outside the vocabulary of {V}")
     if beams > V:
         raise ValueError(f"{beams} beams from a vocabulary of {V}")
-    scores, _, tokens = ops.beam_select(logits.unsqueeze(1), logits.new_zeros(B, 1), num=beams)
+    start = torch.zeros(B, 1, device=logits.device)
+    scores, _, tokens = ops.beam_select(logits.unsqueeze(1), start, num=beams)
     rest = max_new_tokens - 1
     loop = BeamLoop(model, sampler, _repeat_state(state, beams), tokens, scores, eos_token,
                     max(1, min(steps_per_graph, rest)), prompt.dtype)

@@ -388,3 +388,27 @@ def test_select_around_the_slices(V, dtype):
     few = torch.full((1, 2, V), -torch.inf, dtype=dtype)
     few[..., V // 2], few[..., V - 1] = 1.0, 0.5
     check(few, torch.tensor([[-1.0, -2.0]]), 3)
+
+
+class Bf16Sampler(TiedEmbeddingSampler):
+    """A sampler whose logits are bf16 (a head that is not widened)."""
+
+    def logits(self, y):
+        return super().logits(y).to(BF16)
+
+
+@gpu
+def test_search_over_bf16_logits():
+    model = _stack(F32)
+    g = torch.Generator().manual_seed(12)
+    E = torch.randn(40, 64, generator=g).cuda()
+    prompt = torch.randn(2, 4, 64, generator=g).cuda()
+    tok, sc = beam_search(model, Bf16Sampler(E), prompt, 5, 3)
+    assert tok.shape == (2, 3, 5) and sc.dtype == F32 and bool(torch.isfinite(sc).all())
+    with torch.no_grad():
+        y, _ = model.forward_with_final_state(prompt)
+        first = torch.log_softmax(Bf16Sampler(E).logits(y[:, -1]).double(), -1)
+    one, s1 = beam_search(model, Bf16Sampler(E), prompt, 1, 3)
+    want = first.sort(dim=-1, descending=True, stable=True)
+    assert torch.equal(one[..., 0], want.indices[:, :3])
+    assert ((s1.double() - want.values[:, :3]).abs() <= LSE + 2.0 ** -24 * want.values[:, :3].abs()).all()
