@@ -412,3 +412,29 @@ def test_search_over_bf16_logits():
     want = first.sort(dim=-1, descending=True, stable=True)
     assert torch.equal(one[..., 0], want.indices[:, :3])
     assert ((s1.double() - want.values[:, :3]).abs() <= LSE + 2.0 ** -24 * want.values[:, :3].abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [1008, 9000, 20000])
+def test_select_reads_an_expanded_beam_index(V, dtype):
+    """Logits shared by a batch's beams (stride 0), each row at a 16-byte boundary as in
+    the copy it is compared with: the same bits; and with logits on a coarse grid and
+    equal scores, ties by beam and token as in 64 bits."""
+    B, K, num = 2, 3, 12
+    g = torch.Generator().manual_seed(V)
+    row = torch.randn(B, 1, V, generator=g).to(dtype).cuda()
+    s = torch.tensor([[0.0, -1.0, -0.3], [-2.0, -2.5, 0.0]]).cuda()
+    wide = row.expand(B, K, V)
+    assert wide.stride(1) == 0
+    got, want = ops.beam_select(wide, s, num=num), ops.beam_select(wide.contiguous(), s, num=num)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    c, at = reference(wide.cpu(), s.cpu(), num)
+    assert torch.equal((got[1] * V + got[2]).cpu(), at)
+    assert bool(((got[0].double().cpu() - c.gather(1, at)).abs()
+                 <= LSE + 2.0 ** -24 * c.gather(1, at).abs()).all())
+    grid = torch.randint(-3, 4, (B, 1, V), generator=g).to(dtype).cuda().expand(B, K, V)
+    same = torch.full((B, K), -2.0, device="cuda")
+    got = ops.beam_select(grid, same, num=40)
+    _, at = reference(grid.cpu(), same.cpu(), 40)
+    assert torch.equal((got[1] * V + got[2]).cpu(), at)
