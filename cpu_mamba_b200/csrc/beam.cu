@@ -16,6 +16,7 @@
 #include "pair.cuh"
 
 #include <algorithm>
+#include <exception>
 #include <utility>
 #include <vector>
 
@@ -654,7 +655,7 @@ extern "C" int mb2_reorder_rows(void *const *tensors, const int64_t *row_bytes, 
     for (int64_t i = 0; i < n_tensors; ++i)
         MB2_REQUIRE(row_bytes[i] >= 0 && (tensors[i] || row_bytes[i] == 0), MB2_ERR_ARG,
                     "reorder_rows: bad tensor %lld", (long long)i);
-    {
+    try {
         // moved in place side by side: no byte may belong to two tensors
         std::vector<std::pair<const uint8_t *, int64_t>> spans;
         spans.reserve((size_t)n_tensors);
@@ -666,6 +667,9 @@ extern "C" int mb2_reorder_rows(void *const *tensors, const int64_t *row_bytes, 
         for (size_t i = 1; i < spans.size(); ++i)
             MB2_REQUIRE(spans[i].first - spans[i - 1].first >= spans[i - 1].second, MB2_ERR_ARG,
                         "reorder_rows: tensors overlap");
+    } catch (const std::exception &e) {           // no exception leaves a C entry
+        return fail(MB2_ERR_UNSUPPORTED, "reorder_rows: %lld tensors: %s", (long long)n_tensors,
+                    e.what());
     }
     for (int64_t t0 = 0; t0 < n_tensors; t0 += MAX_TENSORS) {
         Reorder r;

@@ -438,3 +438,25 @@ def test_select_reads_an_expanded_beam_index(V, dtype):
     got = ops.beam_select(grid, same, num=40)
     _, at = reference(grid.cpu(), same.cpu(), 40)
     assert torch.equal((got[1] * V + got[2]).cpu(), at)
+
+
+def test_reorder_c_entry_without_memory_returns_an_error():
+    """Four million empty tensors in a process without room for the list of them."""
+    import pathlib
+    import subprocess
+    import sys
+    code = """
+import ctypes, resource
+from cpu_mamba_b200 import _lib
+f, n = _lib.lib().mb2_reorder_rows, 1 << 22
+ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (8 << 20), resource.RLIM_INFINITY))
+rc = f(ptrs, sizes, n, 256, 1, 2, None)
+resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))
+print(rc, _lib.lib().mb2_last_error())
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=str(pathlib.Path(__file__).resolve().parent.parent))
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.startswith("4 b'reorder_rows"), r.stdout
