@@ -336,6 +336,8 @@ def _decay_descriptor(what, q, k, v, g, scale, o, tokens: bool, state_in=0, stat
         raise RuntimeError(f"{what}: out must be {tuple(vs[:lead]) + (H, dv)} in {dtype} with its "
                            "last index contiguous")
     qt, kt, vt, ot, gt = q.stride(), k.stride(), v.stride(), o.stride(), g.stride()
+    if not new and any(st == 0 and n > 1 for st, n in zip(ot, o.shape)):
+        raise RuntimeError(f"{what}: out holds several of its elements in one place")
     if tokens:
         strides = (qt[0], qt[1], qt[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2],
                    *((0, 0, gt[0]) if len(gt) == 1 else gt), ot[0], ot[1], ot[2])

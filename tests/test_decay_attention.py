@@ -774,3 +774,15 @@ def test_offsets_that_fall(dv, dtype):
         assert torch.equal(out[:, held.cuda()], new[:, held.cuda()])
         assert bool((out[:, ~held.cuda()] == 7).all())
         assert bool((new[:, ~held.cuda()] == 0).all())
+
+
+@gpu
+def test_an_expanded_out_is_refused():
+    """Rows, heads or sequences that would be written to one place."""
+    q, k, v, g, _ = (t.cuda() for t in make(2, 6, 4, 1, 2, 4, 8, 8, torch.float32, seed=1))
+    for i in range(3):
+        shape = [1 if j == i else n for j, n in enumerate(v.shape)]
+        with pytest.raises(RuntimeError, match="one place"):
+            ops.decay_attention(q, k, v, g, out=torch.empty(shape, device="cuda").expand(v.shape))
+    one = torch.empty_like(v[:1]).expand(1, 6, 4, 8)
+    assert ops.decay_attention(q[:1], k[:1], v[:1], g[:1], out=one).data_ptr() == one.data_ptr()
