@@ -733,8 +733,9 @@ static size_t relaid(Args &a, uint8_t *ws, size_t at, Relay &in, Relay &out) {
     return at;
 }
 
-// The recurrent kernel's walks: 14 (up to 32 rows, one warp) or 12 warps' worth of them
-// (up to four each) on an SM at a time, narrow ones 2.
+// The recurrent kernel's walks: 14 of one warp (up to 24 rows; 12 up to 32) or 12 warps'
+// worth of them (up to four each) on an SM at a time; narrow ones 2 (1 above 128 rows):
+// what registers and shared memory leave room for.
 struct Walks { int64_t n, lanes; };
 static Walks walks_of(const Args &a, bool narrow) {
     const int64_t sms = num_sms();
@@ -742,7 +743,10 @@ static Walks walks_of(const Args &a, bool narrow) {
     if (narrow) cols = a.dk <= 16 ? 128 : a.dk <= 32 ? 64 : a.dk <= 64 ? 32 : a.dk <= 128 ? 16 : 8;
     const int64_t warps = ceil_div(a.dv < cols ? a.dv : cols, cols / 4);
     return {a.seqs * a.heads * ceil_div(a.dv, cols),
-            narrow ? 2 * sms : a.dk <= 32 ? 14 * sms : 12 / warps * sms};
+            narrow         ? (a.dk <= 128 ? 2 : 1) * sms
+            : a.dk <= 24   ? 14 * sms
+            : a.dk <= 32   ? 12 * sms
+                           : 12 / warps * sms};
 }
 
 // Short bf16 prompts the recurrent kernel does sooner: a walk of the tensor cores
@@ -772,8 +776,11 @@ static Plan plan(Args &a, uint8_t *ws, Relay &in, Relay &out) {
     // tensor cores: one walk of 64 columns an SM, 128 tokens a step; recurrent: compared
     // by 32 tokens, which a narrow walk takes in 4.2 us, others in 2.3 times that (above
     // 64 rows 1.6: in segments, 2048 tokens, 8 heads of 128 x 128, 136 us narrow, 103
-    // else).  Narrow ones lose once they share an SM by more than two (192 tokens of fp32, heads of
-    // 64 x 64: 8 heads 25 us, others 66; 128 heads 35 and 67; 512 heads 126 and 87).
+    // else; above 128 rows 1.8, 3 up to 8 columns, whose wide walk is a single warp: 600
+    // tokens, 296 heads of 200 x 8, 171 us narrow, 297 else; 500 tokens, 60 heads of 256 x
+    // 32, 144 and 107).  Narrow ones lose once they share an SM by more than two (192 tokens of
+    // fp32, heads of 64 x 64: 8 heads 25 us, others 66; 128 heads 35 and 67; 512 heads 126
+    // and 87).
     double time, narrow_time;
     if (chunked_fits(a)) {
         a.seg = segment_tokens(a, a.seqs * a.heads * ceil_div(a.dv, 64), num_sms(), 128, 0.65, 2.2,
@@ -782,7 +789,8 @@ static Plan plan(Args &a, uint8_t *ws, Relay &in, Relay &out) {
         const Walks w = walks_of(a, false), n = walks_of(a, true);
         const int64_t wide = segment_tokens(a, w.n, w.lanes, 32, 0.6, 2.2, 4.0, time);
         const int64_t narrow = segment_tokens(a, n.n, n.lanes, 32, 0.6, 0.9, 1.3, narrow_time);
-        a.narrow = n.n <= n.lanes && narrow_time <= (a.dk <= 64 ? 2.3 : 1.6) * time;
+        const double wider = a.dk <= 64 ? 2.3 : a.dk <= 128 ? 1.6 : a.dv <= 8 ? 3.0 : 1.8;
+        a.narrow = n.n <= 2 * num_sms() && narrow_time <= wider * time;
         a.seg = a.narrow ? narrow : wide;
     }
     a.slots = 0;

@@ -786,3 +786,13 @@ def test_an_expanded_out_is_refused():
             ops.decay_attention(q, k, v, g, out=torch.empty(shape, device="cuda").expand(v.shape))
     one = torch.empty_like(v[:1]).expand(1, 6, 4, 8)
     assert ops.decay_attention(q[:1], k[:1], v[:1], g[:1], out=one).data_ptr() == one.data_ptr()
+
+
+@pytest.mark.parametrize("heads,tokens,dk,dv", [(1900, 32768, 32, 64), (20, 600, 250, 64)])
+def test_segments_are_planned_for_the_walks_that_fit(heads, tokens, dk, dv):
+    """12 one-warp walks of 32 rows share an SM, and one narrow walk of more than 128 rows
+    has it for itself: these calls (two uneven rounds) are cut along their tokens, which
+    shows in their workspace."""
+    import ctypes
+    d = desc(heads=heads, v_heads=1, seqlen=tokens, dk=dk, dv=dv)
+    assert _lib.lib().mb2_decay_attention_workspace_bytes(ctypes.byref(d)) >= 2 * heads * dk * dv * 4
