@@ -612,6 +612,8 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (more) {
                     const uint64_t q = dq0 + s * STAGE, k = dk0 + s * STAGE;
                     ok = ok && wait_warp(full_q(s), ph2, 0x412);
+                    // the scores' columns hold P until P V has read it
+                    if (n > 0) ok = ok && wait_warp(empty_v(s ^ 1), ((n - 1) >> 1) & 1, 0x41c);
                     fence_after();
                     if (ok && elect_one()) {
 #pragma unroll 2
