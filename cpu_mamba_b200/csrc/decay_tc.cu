@@ -638,8 +638,9 @@ decay_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
                 const uint64_t q = dq0 + s * STAGE, kt = kt0 + s * STAGE;
                 // S0's second part and, behind it, its first
                 const uint64_t h = smem_desc_mn(base + off_h2(s), OFF_H - off_h2(s));
-                ok = wait_warp(vt_full, s, 0x413) && wait_warp(full_k(s), ph2, 0x414) &&
-                     wait_warp(d_free, s ^ 1, 0x414);
+                // (behind Q K^T, which P is waiting for: side by side they take twice as long)
+                ok = (STATE || wait_warp(q_read(s), ph2, 0x41d)) && wait_warp(vt_full, s, 0x413) &&
+                     wait_warp(full_k(s), ph2, 0x414) && wait_warp(d_free, s ^ 1, 0x414);
                 fence_after();
                 if (ok && elect_one()) {
                     // V~'s first two parts side by side, the third added to the second's
