@@ -38,7 +38,7 @@ namespace decay {
 // heads of 128 x 128; 278 -> 246 with heads of 64 x 64.  Up to 32 rows they lose (24 x
 // 64: 181 us two columns of all rows, 193 four of half).  One warp per head of 64
 // columns instead of four with eight lanes a column: 425 -> 192 us at 151 sequences
-// of 180 tokens, 24 heads of 24 x 64 (the FMAs alone take about 80).
+// of 180 tokens, 24 heads of 24 x 64 (the FMAs alone take 54).
 // tokens staged at a time: more where few walks wait for each step's latency
 template <int R> __host__ __device__ constexpr int stage_tokens() { return R == 8 ? 32 : 16; }
 constexpr float kRun = 5.5f;          // bound on |log A| within a run
@@ -518,8 +518,8 @@ __global__ void __launch_bounds__(128) seg_states_kernel(const Args a) {
 // shorten the longest chain, at the price of a first pass that costs `first` of the
 // second's time a step, `fill` steps to start each walk, and the states' traffic
 // (`join` steps and a tenth for each segment).
-// Measured, one sequence of 8192 tokens, 24 heads of 128 x 64 in bf16: 134 us whole,
-// 95 in segments (27 first pass, 42 second).
+// Measured, one sequence of 8192 tokens, 24 heads of 128 x 64 in bf16: 186 us whole,
+// 71 in segments (first pass 26, states 3, second pass 40).
 static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64_t unit,
                               double first, double fill, double join, double &time) {
     time = 0.0;
@@ -551,10 +551,10 @@ static int64_t segment_tokens(const Args &a, int64_t walks, int64_t lanes, int64
 // widths or strides are others are laid out for it first, zeros behind Dk and Dv,
 // and o and h_last copied back: two launches and their traffic, where the recurrent
 // kernel took (us, both ways)
-//   8 x 379 tokens, 12 heads of 87 x 64                   247 -> 23
-//   15 x 2560, 6 heads of 64 x 14                         528 -> 66
-//   51221 in 23 sequences, 1 head of 89 x 104             330 -> 86
-//   40 x 568, 24 heads of 10 x 64                         355 -> 104
+//   8 x 379 tokens, 12 heads of 87 x 64                   207 -> 18
+//   15 x 2560, 6 heads of 64 x 14                         161 -> 67
+//   51221 in 23 sequences, 1 head of 89 x 104             286 -> 57
+//   40 x 568, 24 heads of 10 x 64                         295 -> 102
 struct Relay {
     struct Item {
         const void *src;
@@ -750,9 +750,9 @@ static Walks walks_of(const Args &a, bool narrow) {
 }
 
 // Short bf16 prompts the recurrent kernel does sooner: a walk of the tensor cores
-// takes its 128 tokens whole.  In us, 64 heads of 64 x 64: 1 token 4.0 against 8.7, 16
-// tokens 5.6 against 8.6, 32 tokens 7.8 against 8.4; 1024 heads of 16 x 120: 1 token 5.6
-// against 65, 64 tokens 32 against 55.
+// takes its 128 tokens whole.  In us, 64 heads of 64 x 64: 1 token 4.1 against 9.8, 16
+// tokens 5.7 against 9.4, 32 tokens 7.8 against 9.2; 1024 heads of 16 x 120: 1 token 5.3
+// against 71, 64 tokens 30 against 105.
 static bool short_prompt(const Args &a) {
     if (a.seqs == 0) return true;
     const double tokens = (double)(a.cu ? ceil_div(a.seqlen, a.seqs) : a.seqlen);

@@ -17,7 +17,7 @@
 //
 // Operands: P and S0 are two bf16 parts each (16 bits: 2^-16 of a term, so an output's
 // error is that of its own rounding, 1.66e-3 rms of 1.66e-3; with one part each it was
-// 2.3e-3, and 8 sequences of 8192 tokens took 306 us instead of 363).  V~ is three
+// 2.3e-3, and 8 sequences of 8192 tokens took 306 us instead of 357).  V~ is three
 // (24 bits), because the state is an fp32 output and lives for many chunks.  An
 // infinity stands in the first part alone.
 //
@@ -44,9 +44,10 @@
 // the device status.
 //
 // Bound: neither bytes nor MMAs (2700 cycles a chunk) but the chain of hand-overs
-// between the roles, about 4800 cycles = 2.6 us a chunk with 128-wide q and k, one
-// CTA an SM (shared memory and TMEM are full): Q K^T 1100, P 2400 (its scheduler's FMA
-// and ALU pipes, shared with V~ and the state), P V 700.  What brought it there, at 8
+// between the roles, about 5200 cycles = 2.7 us a chunk with 128-wide q and k, one
+// CTA an SM (shared memory and TMEM are full): Q K^T 1400 with the wait for q, P 2500
+// (its scheduler's FMA and ALU pipes, shared with V~ and the state), P V 900, the rest
+// from one to the next.  What brought it there, at 8
 // sequences of 8192 tokens, 24 heads of 128 x 64 (1.5 us of HBM time a chunk), with
 // P and S0 in one part:
 //   733 us  one role after the other, the state in registers

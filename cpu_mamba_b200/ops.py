@@ -365,11 +365,15 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
 
     cu_seqlens (int, N + 1 offsets on the device) packs N sequences along T with
     B = 1; rows before the first and behind the last one are zero in a new output
-    and untouched in ``out``, which must not overlap the inputs.  Otherwise N = B.
+    and untouched in ``out``, which must not overlap the inputs.  Sequences that
+    overlap leave the rows they share and their final states undefined.  Otherwise
+    N = B.
 
     Returns o (B, T, H, Dv), with the final state (N, H, Dk, Dv) float32 when
     ``return_final_state``.  An empty sequence's final state is its initial one.
-    Forward only."""
+    The state is float32 throughout; a bfloat16 output is off by its own rounding
+    and 2^-16 of its terms.  A kernel's wait that runs out leaves outputs incomplete
+    and is reported by ``_lib.device_status()``.  Forward only."""
     what = "decay_attention"
     dev = _device_of(what, q, k, v, g, initial_state, cu_seqlens, out)
     if v.dim() != 4 or q.dim() != 4 or k.dim() != 4 or g.dim() not in (1, 3):

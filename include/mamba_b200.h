@@ -429,7 +429,11 @@ int mb2_block_step_static(const mb2_block *blk, const void *x, void *out, float 
  * rows cu[i] .. cu[i+1]-1 of the seqlen rows; rows before the first and behind
  * the last sequence are zeroed when zero_tail is set and left alone otherwise.  Offsets are
  * clamped to 0 .. seqlen; a sequence whose end is not behind its start is
- * empty (its h_last is its h0).
+ * empty (its h_last is its h0).  Sequences that overlap leave the rows they
+ * share and their final states undefined.
+ * Magnitudes up to 1e36 (v and the state are held divided by up to e^-5.5).
+ * A wait inside the tensor-core kernel (bf16 prompts) that runs out, after about
+ * a second, leaves outputs incomplete; mb2_device_status reports it.
  * The workspace (256-byte aligned; MB2_ERR_WORKSPACE when smaller than asked
  * for) holds the states of sequences that are cut along their tokens and
  * tensors whose rows the tensor cores cannot read; ask for its size with the
