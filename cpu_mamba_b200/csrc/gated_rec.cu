@@ -716,32 +716,50 @@ forward_kernel(const Args a, const Plan p) {
         const unsigned or_ = odd_of<T, WIDE, Shape>(rr, p, t.axis, g, ch.c);
         const unsigned oi = odd_of<T, WIDE, Shape>(ri, p, t.axis, g, ch.c);
         const unsigned ox = odd_of<T, WIDE, Shape>(rx, p, t.axis, g, ch.c);
-        auto compute = [&](auto is_mild, int j, uint64_t &da, uint64_t &db) {
+        float far = 0.0f;                     // the largest 1 + e^-v of the input gates
+        auto compute = [&](auto is_mild, auto is_near, int j, uint64_t &da, uint64_t &db) {
             const uint64_t dr = one_plus_exp(value<T, WIDE>(sm.in[0][j][tid], or_, j), k);
             const uint64_t di = one_plus_exp(value<T, WIDE>(sm.in[1][j][tid], oi, j), k);
             const Decay e = decay_of<decltype(is_mild)::value>(
                 mul2(log2a, pack(rcp(lo(dr)), rcp(hi(dr)))), k);
             da = e.a;
-            db = mul2(input_factor(e.y, di), value<T, WIDE>(sm.in[2][j][tid], ox, j));
+            if constexpr (decltype(is_near)::value) far = max_of(far, lo(di), hi(di));
+            const uint64_t mi = decltype(is_near)::value ? near_input_factor(e.y, di)
+                                                         : input_factor(e.y, di);
+            db = mul2(mi, value<T, WIDE>(sm.in[2][j][tid], ox, j));
         };
         auto all = [&](auto is_mild) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j) {
                 uint64_t da, db;
-                compute(is_mild, j, da, db);
+                compute(is_mild, std::true_type(), j, da, db);
                 H = fma2(da, H, db);
                 A = mul2(A, da);
                 sm.ab[j][tid] = four(da, db);
             }
         };
-        if (plain || (n == RUN && !(mk.first | mk.none))) {
+        bool done = plain || (n == RUN && !(mk.first | mk.none));
+        if (done) {
             if (mild(log2a)) all(std::true_type());
             else all(std::false_type());
-        } else {                              // a sequence's start, or tokens of none
+            if (__any_sync(0xffffffffu, far > kFar)) {     // closed ones are 0 either way
+                bool some = false;
+#pragma unroll 1
+                for (int j = 0; j < RUN; ++j) {
+                    const uint64_t v = value<T, WIDE>(sm.in[1][j][tid], oi, j);
+                    some = some || (ch.in0 && lo(v) < -43.0f && lo(v) > -89.0f) ||
+                           (ch.in1 && hi(v) < -43.0f && hi(v) > -89.0f);
+                }
+                done = !__any_sync(0xffffffffu, some);
+            }
+        }
+        if (!done) {                          // a sequence's start, tokens of none, input
+            A = pair(1.0f), H = 0;            // gates between -89 and -43
 #pragma unroll 2
             for (int j = 0; j < RUN; ++j) {
                 uint64_t da = pair(1.0f), db = 0;
-                if (j < n && !(mk.none >> j & 1)) compute(std::false_type(), j, da, db);
+                if (j < n && !(mk.none >> j & 1))
+                    compute(std::false_type(), std::false_type(), j, da, db);
                 if (mk.first >> j & 1) {
                     if (a.h0) db = fma2(da, ch.load(a.h0 + seq_of(mk, j) * a.width), db);
                     H = db;

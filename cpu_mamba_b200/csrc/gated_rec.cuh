@@ -106,11 +106,30 @@ __device__ __forceinline__ bool mild(uint64_t log2a) {
 
 constexpr float kTiny = 7.52316384526264e-37f;        // 2^-120
 
-// sqrt(y) / d for y = 1 - a^2 and d = 1 + e^-v, v the input gate: one rsqrt for the
-// root and the sigmoid.  0 at y = 0 (a closed decay gate) and at d = inf.
-__device__ __forceinline__ uint64_t input_factor(uint64_t y, uint64_t d) {
+// sqrt(y) / d for y = 1 - a^2 and d = 1 + e^-v, v the input gate: one rsqrt for the root and
+// the sigmoid.  For d up to kFar (v above -43.6), beyond which y d^2 may be infinite and the
+// result 0; where d itself is infinite (v below -88.7) 0 is what it should be.  0 at y = 0 (a
+// closed decay gate).
+constexpr float kFar = 9.223372036854775808e18f;      // 2^63
+__device__ __forceinline__ uint64_t near_input_factor(uint64_t y, uint64_t d) {
     const uint64_t w = mul2(pack(fmaxf(lo(y), kTiny), fmaxf(hi(y), kTiny)), mul2(d, d));
     return mul2(y, pack(rsq(lo(w)), rsq(hi(w))));
+}
+// The same for all d: 0 where 1 / d is below the normal numbers (v below -87).  A value's
+// bits are near_input_factor's wherever that holds, whatever the value beside it.
+__device__ __forceinline__ uint64_t input_factor(uint64_t y, uint64_t d) {
+    uint64_t f = near_input_factor(y, d);
+    if (lo(d) > kFar || hi(d) > kFar) {
+        const uint64_t m = mul2(y, pack(rsq(fmaxf(lo(y), kTiny)), rsq(fmaxf(hi(y), kTiny))));
+        const uint64_t far = mul2(m, pack(rcp(lo(d)), rcp(hi(d))));
+        f = pack(lo(d) > kFar ? lo(far) : lo(f), hi(d) > kFar ? hi(far) : hi(f));
+    }
+    return f;
+}
+__device__ __forceinline__ float max_of(float a, float b, float c) {      // NaNs left out
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 struct Args {
