@@ -82,17 +82,22 @@ class LogitRules:
                                                 tokens[:, None], kept))
         self.lengths.add_(1).clamp_(max=capacity)
 
-    def _moving(self) -> list:
-        """What follows a beam: its history, and its mask where each row has its own."""
-        own = self.mask is not None and self.mask.is_contiguous()
-        return [self.tokens, self.lengths] + ([self.mask] if own else [])
+    def _own_mask(self) -> list:
+        """The mask where each row has its own (not one row expanded)."""
+        shared = self.mask is None or self.mask.stride(0) == 0
+        return [] if shared else [self.mask]
 
     def reorder(self, parents: torch.Tensor) -> None:
         """The rows' histories and masks follow their parents (B, beams)."""
-        ops.reorder_states(self._moving(), parents)
+        masks = self._own_mask()
+        together = [m.contiguous() for m in masks]        # rows of a wider buffer: a copy
+        ops.reorder_states([self.tokens, self.lengths] + together, parents)
+        for mask, moved in zip(masks, together):
+            if not mask.is_contiguous():
+                mask.copy_(moved)
 
     def _saved(self) -> list:
-        return [(t, t.clone()) for t in self._moving()]
+        return [(t, t.clone()) for t in [self.tokens, self.lengths] + self._own_mask()]
 
 
 class TiedEmbeddingSampler:
