@@ -12,6 +12,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, dtype_code, lib, ptr, require_cuda, stream_of
@@ -491,6 +492,13 @@ def _rec_forward(head, x, n, last, keep, dev):
     return h, h_last, saved
 
 
+def _refuse_duals(what: str, *tensors) -> None:
+    """Inside a forward-mode level: a dual tensor's tangent would be lost."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: forward-mode derivatives are not supported")
+
+
 class _GatedRecurrence(torch.autograd.Function):
     """Forward with the states the gradients need; one call computes them all."""
 
@@ -509,6 +517,8 @@ class _GatedRecurrence(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         if dh is None and dlast is None:
             return (None,) * 7
+        if forward_ad._current_level >= 0:
+            _refuse_duals("gated_recurrence backward", dh, dlast)
         x, ig, rg, decay, h0, cu, saved = ctx.saved_tensors
         sharpness, code, n, dev = ctx.rest
         want = ctx.needs_input_grad
@@ -558,12 +568,14 @@ def gated_recurrence(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torc
 
     Returns h (B, T, D) in x's dtype, with the final state (N, D) float32 when
     ``return_final_state``.  An empty sequence's final state is its initial one.
-    The state is float32 throughout.  Differentiable once, with respect to x, both
-    gates, decay and initial_state; a training step that is captured into a CUDA graph
-    needs leaves that no eager graph still holds, as torch's own functions do.  A
-    kernel's wait that runs out leaves outputs incomplete and is reported by
-    ``_lib.device_status()``."""
+    The state is float32 throughout.  Differentiable once, in reverse mode (dual tensors
+    are refused), with respect to x, both gates, decay and initial_state; a training step
+    that is captured into a CUDA graph needs leaves that no eager graph still holds, as
+    torch's own functions do.  A kernel's wait that runs out leaves outputs incomplete
+    and is reported by ``_lib.device_status()``."""
     what = "gated_recurrence"
+    if forward_ad._current_level >= 0:
+        _refuse_duals(what, x, input_gate, decay_gate, decay, initial_state)
     dev = _device_of(what, x, input_gate, decay_gate, decay, initial_state, cu_seqlens)
     code = _rec_check(what, x, input_gate, decay_gate, decay, sharpness, 2)
     n = x.shape[0]

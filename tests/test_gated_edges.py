@@ -1,6 +1,7 @@
 """The gated recurrence where it can go wrong beside test_gated_recurrence.py's cases."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from cpu_mamba_b200 import ops
 from test_gated_recurrence import BF16, F32, call, close, make, reference
@@ -46,3 +47,39 @@ def test_low_input_gates_among_others(dtype):
     same = torch.ones(2, 400, 72, dtype=torch.bool)
     same[0, 100:, 5], same[1, 250:, 70] = False, False
     assert torch.equal(got["h"][same], clean["h"][same])
+
+
+@pytest.mark.parametrize("which", ["x", "input_gate", "decay_gate", "decay", "initial_state"])
+def test_forward_mode_is_refused(which):
+    """A dual tensor's tangent is not dropped: the call is refused, without gradients too."""
+    v = {"x": torch.zeros(1, 2, 4), "input_gate": torch.zeros(1, 2, 4),
+         "decay_gate": torch.zeros(1, 2, 4), "decay": torch.zeros(4),
+         "initial_state": torch.zeros(1, 4)}
+    with fwd.dual_level():
+        v[which] = fwd.make_dual(v[which], torch.ones_like(v[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_recurrence(**v)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_recurrence(**v)
+
+
+@gpu
+def test_other_tensors_of_a_dual_level():
+    """A call that has no dual tensor among its own runs as always."""
+    x = torch.randn(1, 5, 8, device="cuda")
+    want = ops.gated_recurrence(x, x, x, x[0, 0])
+    with fwd.dual_level():
+        fwd.make_dual(torch.ones(2), torch.ones(2))
+        assert torch.equal(ops.gated_recurrence(x, x, x, x[0, 0]), want)
+
+
+@gpu
+def test_dual_gradients_are_refused():
+    x = torch.randn(1, 5, 8, device="cuda", requires_grad=True)
+    v = x.detach()
+    h, last = ops.gated_recurrence(x, v, v, v[0, 0], return_final_state=True)
+    with fwd.dual_level():
+        for y in (h, last):
+            dy = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, [x], [dy], retain_graph=True)
