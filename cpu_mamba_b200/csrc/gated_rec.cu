@@ -820,7 +820,8 @@ template <typename T, typename Slot> struct BackwardSmem {
     using Shape = Backward<T>;
     Slot gates[2][Shape::RUN][Shape::THREADS];
     Slot xd[2][2][Shape::RUN][Shape::THREADS];       // x, dh; two tiles'
-    float4 kept[2][Shape::RUN][Shape::THREADS];      // a, m i; 1 / m, r
+    // a, m i; m (1 - i), e^-v of the decay gate, and once the states are known 1 - i, 1 - r
+    float4 kept[2][Shape::RUN][Shape::THREADS];
     float4 agg[Shape::WARPS][32];          // A, A and the states' H, H
     float2 back[Shape::WARPS][32];         // the gradients' H, H
     float4 enter[Shape::WARPS][32];        // h before the warps' tokens, C behind them
@@ -955,28 +956,31 @@ backward_kernel(const Args a, const Plan p) {
         // the states: h -> A h + H, or to H alone; the gradients' C from the later tokens:
         // C -> A C + B, or to B alone before a last one
         uint64_t A = pair(1.0f), H = 0, B = 0, da[RUN];
-        // a, m i, 1 / m and r of a token
-        auto compute = [&](auto is_mild, int j, uint64_t &mi, uint64_t &rm, uint64_t &r) {
-            const uint64_t dr = one_plus_exp(value<T, WIDE>(sm.gates[0][j][tid], or_, j), k);
-            const uint64_t di = one_plus_exp(value<T, WIDE>(sm.gates[1][j][tid], oi, j), k);
-            r = pack(rcp(lo(dr)), rcp(hi(dr)));
-            const Decay e = decay_of<decltype(is_mild)::value>(mul2(log2a, r), k);
-            // 1 / m, or 0 where m is below 1e-18: nothing comes back through a closed gate (an
+        // a, m i, m (1 - i) and e^-v of the decay gate of a token
+        auto compute = [&](auto is_mild, int j, uint64_t &mi, uint64_t &mo, uint64_t &er) {
+            er = exp_neg(value<T, WIDE>(sm.gates[0][j][tid], or_, j), k);
+            const uint64_t ei = exp_neg(value<T, WIDE>(sm.gates[1][j][tid], oi, j), k);
+            const Decay e = decay_of<decltype(is_mild)::value>(
+                mul2(log2a, rcp2(add2(er, k.one))), k);
+            // m, or 0 where it is below 1e-18: nothing comes back through a closed gate (an
             // m^2 that is not normal would be 0 to the root, and 1 / m infinite)
-            rm = pack(lo(e.y) < kTiny ? 0.0f : rsq(lo(e.y)), hi(e.y) < kTiny ? 0.0f : rsq(hi(e.y)));
-            mi = mul2(mul2(e.y, rm), pack(rcp(lo(di)), rcp(hi(di))));
+            const uint64_t m = mul2(e.y, pack(lo(e.y) < kTiny ? 0.0f : rsq(lo(e.y)),
+                                              hi(e.y) < kTiny ? 0.0f : rsq(hi(e.y))));
+            const uint64_t i = rcp2(add2(ei, k.one));
+            mi = mul2(m, i);
+            mo = mul2(m, rest_of(ei, i));
             return e.a;
         };
         const bool plain = whole || (n == RUN && !(mk.first | mk.last | mk.none));
         auto all = [&](auto is_mild) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j) {
-                uint64_t mi, rm, r;
-                da[j] = compute(is_mild, j, mi, rm, r);
+                uint64_t mi, mo, er;
+                da[j] = compute(is_mild, j, mi, mo, er);
                 H = fma2(da[j], H, mul2(mi, value<T, WIDE>(xs[j][tid], ox, j)));
                 A = mul2(A, da[j]);
                 sm.kept[0][j][tid] = four(da[j], mi);
-                sm.kept[1][j][tid] = four(rm, r);
+                sm.kept[1][j][tid] = four(mo, er);
             }
 #pragma unroll
             for (int j = RUN - 1; j >= 0; --j)
@@ -988,9 +992,9 @@ backward_kernel(const Args a, const Plan p) {
         } else {
 #pragma unroll 2
             for (int j = 0; j < RUN; ++j) {
-                uint64_t a1 = pair(1.0f), mi = 0, rm = 0, r = 0;
+                uint64_t a1 = pair(1.0f), mi = 0, mo = 0, er = 0;
                 if (j >= n || (mk.none >> j & 1)) xs[j][tid] = ds[j][tid] = 0;
-                else a1 = compute(std::false_type(), j, mi, rm, r);
+                else a1 = compute(std::false_type(), j, mi, mo, er);
                 if (!a.dh) ds[j][tid] = 0;
                 const uint64_t b = mul2(mi, value<T, WIDE>(xs[j][tid], ox, j));
                 if (mk.first >> j & 1) {
@@ -1001,7 +1005,7 @@ backward_kernel(const Args a, const Plan p) {
                 }
                 A = mul2(A, a1);
                 sm.kept[0][j][tid] = four(a1, mi);
-                sm.kept[1][j][tid] = four(rm, r);
+                sm.kept[1][j][tid] = four(mo, er);
             }
 #pragma unroll 2
             for (int j = RUN - 1; j >= 0; --j) {
@@ -1026,28 +1030,30 @@ backward_kernel(const Args a, const Plan p) {
             const uint64_t g1 = mul2(log2a, pair(0.6931471824645996f));
             uint64_t h = pack(e.x, e.y), C = pack(e.z, e.w);
             // beside G the outputs need m i, x (1 - i), q = r (a h_{t-1} - a^2 i x / m) and
-            // g1 (1 - r)
+            // g1 (1 - r); m is the sum of its two parts
             uint64_t q[RUN];
             auto take = [&](int j) {
                 const float4 am = sm.kept[0][j][tid], mr = sm.kept[1][j][tid];
-                const uint64_t a1 = pack(am.x, am.y), mi = pack(am.z, am.w), rm = pack(mr.x, mr.y);
-                const uint64_t x = value<T, WIDE>(xs[j][tid], ox, j);
+                const uint64_t a1 = pack(am.x, am.y), mi = pack(am.z, am.w);
+                const uint64_t mo = pack(mr.x, mr.y), er = pack(mr.z, mr.w);
+                const uint64_t b = mul2(mi, value<T, WIDE>(xs[j][tid], ox, j));
+                const uint64_t rm = rcp2(add2(add2(mi, mo), pair(kFloor)));
+                const uint64_t r = rcp2(add2(er, k.one));
                 // h - a i x / m
-                const uint64_t less = fma2(mul2(a1, mul2(mul2(mul2(mi, rm), x), rm)), k.neg_one, h);
-                q[j] = mul2(mul2(pack(mr.z, mr.w), a1), less);
-                h = fma2(a1, h, mul2(mi, x));
+                const uint64_t less = fma2(mul2(a1, mul2(mul2(b, rm), rm)), k.neg_one, h);
+                q[j] = mul2(mul2(r, a1), less);
+                sm.kept[1][j][tid] = four(mul2(mo, rm), rest_of(er, r));
+                h = fma2(a1, h, b);
             };
             uint64_t dx[RUN], di[RUN], dr[RUN];
             auto give = [&](int j) {
-                const float4 am = sm.kept[0][j][tid], mr = sm.kept[1][j][tid];
-                const uint64_t mi = pack(am.z, am.w), r = pack(mr.z, mr.w);
+                const float4 am = sm.kept[0][j][tid], rest = sm.kept[1][j][tid];
                 const uint64_t x = value<T, WIDE>(xs[j][tid], ox, j);
-                const uint64_t i = mul2(mi, pack(mr.x, mr.y));
                 const uint64_t G = add2(C, value<T, WIDE>(ds[j][tid], od, j));
                 const uint64_t dl = mul2(G, q[j]);
-                dx[j] = mul2(G, mi);
-                di[j] = mul2(dx[j], fma2(mul2(i, x), k.neg_one, x));
-                dr[j] = mul2(dl, mul2(g1, fma2(r, k.neg_one, k.one)));
+                dx[j] = mul2(G, pack(am.z, am.w));
+                di[j] = mul2(dx[j], mul2(x, pack(rest.x, rest.y)));
+                dr[j] = mul2(dl, mul2(g1, pack(rest.z, rest.w)));
                 total = add2(total, dl);
                 C = mul2(pack(am.x, am.y), G);
             };

@@ -55,10 +55,21 @@ struct Factors {
     }
 };
 
+// e^-v
+__device__ __forceinline__ uint64_t exp_neg(uint64_t v, const Factors &k) {
+    const uint64_t t = mul2(v, k.neg_log2e);
+    return pack(ex2(lo(t)), ex2(hi(t)));
+}
 // 1 + e^-v; its reciprocal is sigmoid(v), exactly 0 at v = -inf
 __device__ __forceinline__ uint64_t one_plus_exp(uint64_t v, const Factors &k) {
-    const uint64_t t = mul2(v, k.neg_log2e);
-    return add2(pack(ex2(lo(t)), ex2(hi(t))), k.one);
+    return add2(exp_neg(v, k), k.one);
+}
+__device__ __forceinline__ uint64_t rcp2(uint64_t v) { return pack(rcp(lo(v)), rcp(hi(v))); }
+// 1 - sigmoid(v) = e^-v sigmoid(v) from both, to its own few units: sigmoid(v) taken from 1
+// would leave its rounding, 2^-24, where v is high.  0 where sigmoid(v) is.
+__device__ __forceinline__ uint64_t rest_of(uint64_t exp_neg_v, uint64_t sigmoid) {
+    constexpr float kMost = 8.507059173023462e37f;    // 2^126: infinity times 0 is not wanted
+    return mul2(pack(fminf(lo(exp_neg_v), kMost), fminf(hi(exp_neg_v), kMost)), sigmoid);
 }
 
 // a = 2^u and 1 - a^2 for u <= 0, both to within a few units of their own: near u = 0,
@@ -105,6 +116,7 @@ __device__ __forceinline__ bool mild(uint64_t log2a) {
 }
 
 constexpr float kTiny = 7.52316384526264e-37f;        // 2^-120
+constexpr float kFloor = 7.888609052210118e-31f;      // 2^-100, nothing beside kTiny's root
 
 // sqrt(y) / d for y = 1 - a^2 and d = 1 + e^-v, v the input gate: one rsqrt for the root and
 // the sigmoid.  For d up to kFar (v above -43.6), beyond which y d^2 may be infinite and the
@@ -121,7 +133,7 @@ __device__ __forceinline__ uint64_t input_factor(uint64_t y, uint64_t d) {
     uint64_t f = near_input_factor(y, d);
     if (lo(d) > kFar || hi(d) > kFar) {
         const uint64_t m = mul2(y, pack(rsq(fmaxf(lo(y), kTiny)), rsq(fmaxf(hi(y), kTiny))));
-        const uint64_t far = mul2(m, pack(rcp(lo(d)), rcp(hi(d))));
+        const uint64_t far = mul2(m, rcp2(d));
         f = pack(lo(d) > kFar ? lo(far) : lo(f), hi(d) > kFar ? hi(far) : hi(f));
     }
     return f;

@@ -1,10 +1,12 @@
 """The gated recurrence where it can go wrong beside test_gated_recurrence.py's cases."""
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 from cpu_mamba_b200 import ops
-from test_gated_recurrence import BF16, F32, call, close, make, reference
+from test_gated_recurrence import BF16, F32, HALF, U, call, close, make, reference
 
 gpu = pytest.mark.gpu
 
@@ -83,3 +85,89 @@ def test_dual_gradients_are_refused():
             dy = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, [x], [dy], retain_graph=True)
+
+
+def relative(got, want, rel):
+    """got within rel of want, and its rounding, all of one sign."""
+    d = (got.double().cpu() - want).abs()
+    ok = d <= (rel + HALF[got.dtype] * (1 + rel)) * want.abs() + 1e-37
+    assert bool(ok.all()), float((d / want.abs()).max())
+
+
+def sharper(v):
+    """sigmoid(-v) over 1 - sigmoid(v) in 64 bits, which is off by up to 1e-3 at v = 30."""
+    v = v.double().cpu()
+    return torch.sigmoid(-v) / (1 - torch.sigmoid(v))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 9, 200])
+def test_gradients_of_open_gates(dtype, T):
+    """Gates at 12 .. 30, whose 1 - sigmoid is 6e-6 .. 9e-14: the gates' gradients have that
+    as a factor, to its own few units.  Inputs of one sign, so that nothing cancels: u = 2^-24,
+    a sigmoid and 1 - sigmoid are off by 7 + 2 |v| units (the exponential's argument twice,
+    the exponential 4, sum, reciprocal and product), 1 - a^2 by the same and 19 more, G and h
+    by what a token's decay (8 units and |log a| times its own) and sum (2) add up to."""
+    B, D = 3, 64
+    g = torch.Generator().manual_seed(T)
+
+    def rand(*s):
+        return torch.rand(*s, generator=g).to(dtype).cuda()
+
+    case = {"B": B, "T": T, "D": D, "dtype": dtype, "state": True}
+    st = make(case)
+    high = (12 + 18 * torch.rand(B, T, D, generator=g)).to(dtype).cuda()
+    gate = 67 * U                                        # 7 + 2 * 30
+    # |log a| <= 0.11, so ea <= 0.11 (gate + 11 U) + 8 U; eb: half of y's, input gate's, 8
+    token = 0.11 * (gate + 11 * U) + 10 * U
+    eb = 0.5 * (gate + 19 * U) + gate + 8 * U
+    # dinput_gate = G m i x (1 - i): x and dh positive
+    for r in (st["r"], high):
+        s = {**st, "x": rand(B, T, D) + 0.5, "dh": rand(B, T, D) + 0.5, "i": high, "r": r,
+             "dlast": st["dlast"].abs()}
+        want, _ = reference(case, s)
+        # (an r at -5 multiplies |log a| by less, so that the same bounds hold)
+        relative(call(s, grad=True)["di"], want["di"] * sharper(high),
+                 T * token + eb + gate + 12 * U)
+    # ddecay_gate = G r (a h - a^2 i x / m) log a (1 - r): h positive, x negative and small
+    s = {**st, "x": -(rand(B, T, D) + 0.5) * 2.0 ** -40, "dh": rand(B, T, D) + 0.5, "r": high,
+         "h0": (st["h0"].abs() + 1) * 1e3, "dlast": st["dlast"].abs()}
+    want, _ = reference(case, s)
+    relative(call(s, grad=True)["dr"], want["dr"] * sharper(high),
+             2 * T * token + 2 * token + eb + 3 * gate + 40 * U)
+    # open altogether
+    s["i"], s["r"] = torch.full_like(high, math.inf), torch.full_like(high, math.inf)
+    got = call(s, grad=True)
+    assert bool((got["di"] == 0).all()) and bool((got["dr"] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_low_and_far_gates(dtype):
+    """Both gates over the whole range at once, -100 .. 100, and closed and open ones: finite,
+    within the reference's bounds wherever its own 64 bits tell 1 - sigmoid (gates below 12).
+    Decay gates whose 1 - a^2 is below 2^-120 count as closed: m, below 2^-60, counts as 0 in
+    h = .. + m i x, dx = G m i, dinput_gate = dx x (1 - i), and in ddecay_gate's G i x m / 2
+    (r log a / m is -m / 2 there).  |x| and |dh| are below 6, so |G| below 6 (T + 1); with the
+    sum over T tokens every output is off by less than 2^-60 36 (T + 1) T."""
+    B, T, D = 2, 230, 64
+    case = {"B": B, "T": T, "D": D, "dtype": dtype, "state": True}
+    st = make(case)
+    assert all(float(st[k].abs().max()) < 6 for k in ("x", "dh", "dlast"))
+    closed = 2.0 ** -60 * 36 * (T + 1) * T
+    g = torch.Generator().manual_seed(3)
+    far = 200 * torch.rand(2, B, T, D, generator=g) - 100
+    far[:, :, ::50], far[:, :, 1::50] = math.inf, -math.inf
+    # (from -80 to -100 sigmoids leave the normal numbers, where they count as 0)
+    far = torch.where((far < -80) & (far > -100), -80.0, far).to(dtype).cuda()
+    st["i"], st["r"] = far[0], far[1]
+    got = call(st, grad=True)
+    want, tol = reference(case, st)
+    for k, v in got.items():
+        assert bool(v.isfinite().all()), k
+    for k in ("h", "last", "dh0", "dx"):
+        close(k, got[k], want[k], tol[k] + closed, case)
+    low = ((far[0] < 12) & (far[1] < 12)).cpu()
+    for k in ("di", "dr"):
+        close(k, got[k][low.cuda()], want[k][low], tol[k][low] + closed, case)
