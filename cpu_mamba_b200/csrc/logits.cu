@@ -223,7 +223,10 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitArgs a) {
     }
     float temp = a.temp ? a.temp[row] : a.temp1;
     if (temp == 0.0f) temp = 1.0f;
-    // a product by the reciprocal, but for temperatures whose reciprocal may not be normal
+    // a product by the reciprocal, off by up to one unit and as torch divides by a number (so
+    // that a sampler has the same bits with rules and without); a corrected quotient, half a
+    // unit, took 66 instead of 61 us at 512 x 50257.  Divided where the reciprocal may not be
+    // normal
     const bool divide = !(fabsf(temp) > 1e-30f && fabsf(temp) < 1e30f);
     const float inverse = 1.0f / temp;
     T *dst = static_cast<T *>(a.out) + row * a.ld_out + slice0;

@@ -84,3 +84,20 @@ def test_beams_under_masks_of_their_own(kind):
     for row, words in zip(tokens.tolist(), mask.tolist()):
         assert len(set(row)) == n + 1
         assert {t for t in range(V) if not words[t // 32] >> (t % 32) & 1} == set(row)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [0.3, 0.7, 1.0, 1.9])
+def test_rules_that_ask_for_nothing(temperature):
+    """The same logits, bit for bit, and so the same tokens as without rules."""
+    model = Model(seed=14)
+    y = torch.randn(5, 48, generator=torch.Generator().manual_seed(15)).cuda()
+    plain = TiedEmbeddingSampler(model.E, temperature)
+    z = plain.logits(y)
+    rules = LogitRules(5, 8)
+    assert torch.equal(rules.adjust(z.clone(), temperature), z / temperature)
+    torch.manual_seed(1)
+    want = plain(y)[1]
+    torch.manual_seed(1)
+    assert torch.equal(TiedEmbeddingSampler(model.E, temperature, rules=rules)(y)[1], want)
+    assert torch.equal(rules.tokens[:, 0], want)
