@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import check, dtype_code, lib, ptr, require_cuda, stream_of
@@ -630,6 +631,7 @@ def gated_recurrence_step(x: torch.Tensor, input_gate: torch.Tensor, decay_gate:
         rc = lib().mb2_gated_recurrence_step(d, state.data_ptr(), _raw_stream(dev))
         if rc:
             check(rc, what)
+    increment_version(state)
     return h
 
 
@@ -734,7 +736,8 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             b64 = bias_tokens.dtype == i64
         if mask is not None:
             mask, ld_m = _row_tensor("mask", mask, (R, -(-V // 32)), (torch.int32,), dev)
-        if out is None:
+        given = out is not None
+        if not given:
             out, ld_out = logits.new_empty((R, V)), V
         else:
             ld_out, last = out.stride() if out.dim() == 2 else (0, 0)
@@ -752,6 +755,8 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         rc = lib().mb2_adjust_logits(d, _raw_stream(dev))
         if rc:
             check(rc, what)
+    if given:
+        increment_version(out)
     return out
 
 
@@ -939,4 +944,5 @@ def reorder_states(states, parents: torch.Tensor):
                                     parents.data_ptr(), B, K, _raw_stream(dev))
         if rc:
             check(rc, what)
+    increment_version(tensors)
     return states

@@ -171,3 +171,38 @@ def test_gradients_of_low_and_far_gates(dtype):
     low = ((far[0] < 12) & (far[1] < 12)).cpu()
     for k in ("di", "dr"):
         close(k, got[k][low.cuda()], want[k][low], tol[k][low] + closed, case)
+
+
+@gpu
+def test_states_advanced_in_place_are_seen_by_autograd():
+    """A state that a backward pass still needs and a step has advanced: an error, as for
+    torch's own operations in place, and no gradient of the wrong state."""
+    x = torch.randn(1, 5, 8, device="cuda")
+    decay = torch.full((8,), -5.0, device="cuda", requires_grad=True)
+    state = torch.randn(1, 8, device="cuda")
+    h = ops.gated_recurrence(x, x, x, decay, initial_state=state)
+    version = state._version
+    ops.gated_recurrence_step(x[:, 0], x[:, 0], x[:, 0], decay.detach(), state)
+    assert state._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h.sum(), [decay])
+    with torch.inference_mode():                          # (these have no versions)
+        state = torch.zeros(1, 8, device="cuda")
+    ops.gated_recurrence_step(x[:, 0], x[:, 0], x[:, 0], decay.detach(), state)
+
+
+@gpu
+def test_other_tensors_written_in_place_are_seen_by_autograd():
+    w = torch.randn(3, 40, device="cuda", requires_grad=True)
+    p = torch.sigmoid(w)                                  # keeps its output for the gradient
+    z = p.detach()
+    assert ops.adjust_logits(z, temperature=2.0, out=z) is z
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        p.sum().backward()
+    p = torch.sigmoid(w)
+    ops.adjust_logits(p.detach(), temperature=2.0)        # a new tensor: p is as it was
+    p.sum().backward()
+    p = torch.sigmoid(w)
+    ops.reorder_states([p.detach()], torch.tensor([[2, 1, 0]], device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        p.sum().backward()
