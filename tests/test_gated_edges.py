@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from cpu_mamba_b200 import ops
+from cpu_mamba_b200 import _lib, ops
 from test_gated_recurrence import BF16, F32, HALF, U, call, close, make, reference
 
 gpu = pytest.mark.gpu
@@ -206,3 +206,115 @@ def test_other_tensors_written_in_place_are_seen_by_autograd():
     ops.reorder_states([p.detach()], torch.tensor([[2, 1, 0]], device="cuda"))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         p.sum().backward()
+
+
+# Calls of many tiles: each CTA takes several, across sequences, strips and batch rows
+def check_channels(case, st, channels, got):
+    """The outputs of some channels (they do not touch) against the reference's."""
+    part = {k: v if v is None or k == "cu" else v[..., channels].contiguous()
+            for k, v in st.items()}
+    want, tol = reference({**case, "D": len(channels)}, part)
+    for k, v in got.items():
+        close(k, v[..., channels], want[k], tol[k], case)
+
+
+@gpu
+@pytest.mark.parametrize("D", [1536, 1537])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_tiles_than_ctas(dtype, D):
+    """2 x 1500 tokens are 30 tiles of 104 and more of fewer in 24 or 25 strips: from 720 to
+    1900 for 296 CTAs.  Dense, and as a pack of ragged sequences with rows of none."""
+    channels = [0, 1, 31, 32, 63, 64, 700, 767, 768, 1471, 1472, 1535, D - 1]
+    case = {"B": 2, "T": 1500, "D": D, "dtype": dtype, "state": True}
+    st = make(case)
+    check_channels(case, st, channels, call(st, grad=True))
+    case = {"B": 1, "T": 3000, "D": D, "dtype": dtype, "state": True,
+            "cu": [3, 700, 700, 1801, 1802, 2900, 2990]}
+    st = make(case)
+    check_channels(case, st, channels, call(st, grad=True))
+    assert _lib.device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("off", [-1, 0, 1])
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (F32, 128), (BF16, 64), (BF16, 136)])
+def test_packs_of_whole_tiles(dtype, D, off):
+    """Rows of 16-byte chunks and sequences of several tiles, so that most tiles need no marks;
+    they end at, one before and one behind the ends of tiles (104, 64, 56 and 40 tokens), tiles
+    begin with a sequence, end with one and hold several."""
+    cu = [0, 312 + off, 448 + off, 704 + off, 705 + off, 1064 + off, 1200 + off, 1664 + off, 1900]
+    for first, behind in ((0, 0), (5, 70)):
+        case = {"B": 1, "T": 1900 + behind, "D": D, "dtype": dtype, "state": True,
+                "cu": [first] + cu[1:]}
+        st = make(case)
+        want, tol = reference(case, st)
+        for k, v in call(st, grad=True).items():
+            close(k, v, want[k], tol[k], case)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,limit", [(F32, 1 << 21), (BF16, 1 << 22)])
+def test_strides_around_the_limit_of_short_offsets(dtype, limit):
+    """Token strides at which a tile's offsets (up to 104 rows) still fit 32 bits, and at which
+    they no longer do; the last rows are more than 2^31 elements away."""
+    T, D = 1100 if dtype == F32 else 600, 64
+    case = {"B": 1, "T": T, "D": D, "dtype": dtype, "state": True}
+    st = make(case)
+    want = call(st, grad=True)
+    store = torch.empty(T * limit, dtype=dtype, device="cuda")
+    assert (T - 1) * (limit - 8) > 1 << 31
+    for stride in (limit - 8, limit):
+        far = store.as_strided((1, T, D), (0, stride, 1))
+        for name in ("x", "i", "dh"):
+            far.copy_(st[name])
+            got = call({**st, name: far}, grad=True)
+            assert all(torch.equal(got[k], want[k]) for k in want), (stride, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_past_32_bits(dtype):
+    """Few tokens, and batch rows, more than 2^31 elements apart from first to last."""
+    far = (1 << 30) + 64
+    store = torch.empty(2 * far + 4096, dtype=dtype, device="cuda")
+    for B, T, strides in ((1, 3, (0, far, 1)), (3, 1, (far, 64, 1)), (3, 60, (far, 64, 1))):
+        case = {"B": B, "T": T, "D": 64, "dtype": dtype, "state": True}
+        st = make(case)
+        want = call(st, grad=True)
+        view = store.as_strided((B, T, 64), strides)
+        for name in ("x", "i", "r", "dh"):
+            view.copy_(st[name])
+            got = call({**st, name: view}, grad=True)
+            assert all(torch.equal(got[k], want[k]) for k in want), (B, T, name)
+
+
+# batches of which a CTA takes several sequences, the last ones unevenly
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,D", [(2400, 64), (2500, 75), (5001, 4), (700, 2048), (301, 4098)])
+def test_step_of_many_sequences(dtype, B, D):
+    """Two steps against the formula: bounds as reference's, for all sequences at once."""
+    g = torch.Generator().manual_seed(B + D)
+
+    def rand(*s, scale=1.0):
+        return (torch.randn(*s, generator=g) * scale).to(dtype).cuda()
+
+    x, i, r = rand(2, B, D), rand(2, B, D, scale=1.5), rand(2, B, D, scale=1.5)
+    decay = (torch.rand(D, generator=g) * 3 - 6).cuda()
+    state = torch.randn(B, D, generator=g).cuda()
+    want = state.double()
+    e = torch.zeros_like(want)
+    for t in range(2):
+        h = ops.gated_recurrence_step(x[t], i[t], r[t], decay, state)
+        vr, vi = r[t].double(), i[t].double()
+        la = -8 * torch.nn.functional.softplus(decay.double()) * torch.sigmoid(vr)
+        a = torch.exp(la)
+        b = (-torch.expm1(2 * la)).sqrt() * torch.sigmoid(vi) * x[t].double()
+        er, ei = (7 + 2 * vr.abs()) * U, (7 + 2 * vi.abs()) * U
+        eg = er + 11 * U
+        size = (a * want).abs() + b.abs()
+        e = (a * e + (la.abs() * eg + 8 * U) * (a * want).abs()
+             + (0.5 * (eg + 8 * U) + ei + 8 * U) * b.abs() + 2 * U * size)
+        want = a * want + b
+        assert bool(((state.double() - want).abs() <= e + 1e-37).all())
+        assert bool(((h.double() - want).abs() <= e + HALF[dtype] * (want.abs() + e)).all())
