@@ -421,6 +421,29 @@ template <typename T, bool WIDE>
 __device__ __forceinline__ uint64_t value(typename Lane<T, WIDE>::Slot s, unsigned odd, int j) {
     return Lane<T, WIDE>::get(s, odd >> j & 1);
 }
+// Whether a warp met input gates below -43.6 (where near_input_factor does not hold) that are
+// not closed (1 + e^-v infinite): the least distance of their bits from the first such value's,
+// which wraps around for all others.
+template <typename T, bool WIDE> struct FarGates {
+    static constexpr unsigned kFirst = 0x5f000001u, kMany = 0x7f800000u - kFirst;  // of 1 + e^-v
+    unsigned least = ~0u;
+    __device__ __forceinline__ void note(typename Lane<T, WIDE>::Slot, uint64_t d) {
+        least = __viaddmin_u32(lo_of(d), 0u - kFirst, __viaddmin_u32(hi_of(d), 0u - kFirst, least));
+    }
+    __device__ __forceinline__ bool some() const {
+        return __any_sync(0xffffffffu, least < kMany);
+    }
+};
+template <> struct FarGates<__nv_bfloat16, true> {     // both gates at once: -43 .. -88.5
+    static constexpr unsigned kFirst = 0xc22cu, kMany = 0xc2b2u - kFirst;
+    unsigned least = ~0u;
+    __device__ __forceinline__ void note(uint32_t gates, uint64_t) {
+        least = __viaddmin_u16x2(gates, (0x10000u - kFirst) * 0x10001u, least);
+    }
+    __device__ __forceinline__ bool some() const {
+        return __any_sync(0xffffffffu, (least & 0xffffu) < kMany || least >> 16 < kMany);
+    }
+};
 // rows of an output from a lane's values: token j of n
 template <typename T, bool WIDE, int RUN>
 __device__ __forceinline__ void put_rows(void *to, int64_t token, int64_t width, int n,
@@ -716,14 +739,14 @@ forward_kernel(const Args a, const Plan p) {
         const unsigned or_ = odd_of<T, WIDE, Shape>(rr, p, t.axis, g, ch.c);
         const unsigned oi = odd_of<T, WIDE, Shape>(ri, p, t.axis, g, ch.c);
         const unsigned ox = odd_of<T, WIDE, Shape>(rx, p, t.axis, g, ch.c);
-        float far = 0.0f;                     // the largest 1 + e^-v of the input gates
+        FarGates<T, WIDE> far;
         auto compute = [&](auto is_mild, auto is_near, int j, uint64_t &da, uint64_t &db) {
             const uint64_t dr = one_plus_exp(value<T, WIDE>(sm.in[0][j][tid], or_, j), k);
             const uint64_t di = one_plus_exp(value<T, WIDE>(sm.in[1][j][tid], oi, j), k);
             const Decay e = decay_of<decltype(is_mild)::value>(
                 mul2(log2a, pack(rcp(lo(dr)), rcp(hi(dr)))), k);
             da = e.a;
-            if constexpr (decltype(is_near)::value) far = max_of(far, lo(di), hi(di));
+            if constexpr (decltype(is_near)::value) far.note(sm.in[1][j][tid], di);
             const uint64_t mi = decltype(is_near)::value ? near_input_factor(e.y, di)
                                                          : input_factor(e.y, di);
             db = mul2(mi, value<T, WIDE>(sm.in[2][j][tid], ox, j));
@@ -742,16 +765,7 @@ forward_kernel(const Args a, const Plan p) {
         if (done) {
             if (mild(log2a)) all(std::true_type());
             else all(std::false_type());
-            if (__any_sync(0xffffffffu, far > kFar)) {     // closed ones are 0 either way
-                bool some = false;
-#pragma unroll 1
-                for (int j = 0; j < RUN; ++j) {
-                    const uint64_t v = value<T, WIDE>(sm.in[1][j][tid], oi, j);
-                    some = some || (ch.in0 && lo(v) < -43.0f && lo(v) > -89.0f) ||
-                           (ch.in1 && hi(v) < -43.0f && hi(v) > -89.0f);
-                }
-                done = !__any_sync(0xffffffffu, some);
-            }
+            done = !far.some();
         }
         if (!done) {                          // a sequence's start, tokens of none, input
             A = pair(1.0f), H = 0;            // gates between -89 and -43

@@ -122,7 +122,7 @@ constexpr float kFloor = 7.888609052210118e-31f;      // 2^-100, nothing beside 
 // the sigmoid.  For d up to kFar (v above -43.6), beyond which y d^2 may be infinite and the
 // result 0; where d itself is infinite (v below -88.7) 0 is what it should be.  0 at y = 0 (a
 // closed decay gate).
-constexpr float kFar = 9.223372036854775808e18f;      // 2^63
+constexpr float kFar = 9.223372036854775808e18f;      // 2^63, 0x5f000000
 __device__ __forceinline__ uint64_t near_input_factor(uint64_t y, uint64_t d) {
     const uint64_t w = mul2(pack(fmaxf(lo(y), kTiny), fmaxf(hi(y), kTiny)), mul2(d, d));
     return mul2(y, pack(rsq(lo(w)), rsq(hi(w))));
@@ -138,12 +138,6 @@ __device__ __forceinline__ uint64_t input_factor(uint64_t y, uint64_t d) {
     }
     return f;
 }
-__device__ __forceinline__ float max_of(float a, float b, float c) {      // NaNs left out
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 struct Args {
     const void *x, *ig, *rg;
     const float *decay;
