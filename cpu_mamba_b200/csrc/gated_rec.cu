@@ -19,12 +19,13 @@
 // multiplied by zero, which would let an infinity through).
 //
 // Measured (B200; a value: one channel of one token), with the rate that HBM allows:
-//   forward  fp32, 151 x 180 x 1536     123 us   103  HBM, 84 % of the copy rate
-//            bf16, 8 x 8192 x 1536      198      124  issue slots 50 %, MUFU 42 %, 28 warps an
+//   forward  fp32, 151 x 180 x 1536     124 us   103  HBM, 83 % of the copy rate
+//            bf16, 8 x 8192 x 1536      195      124  issue slots 52 %, MUFU 42 %, 28 warps an
 //                                                     SM that wait for one another's tiles
-//            bf16, 5 of 6500 x 1024     111       41  16 chains of tiles for 296 CTAs
+//            bf16, 5 of 6500 x 1024     116       41  16 chains of tiles for 296 CTAs
 //            bf16, 65536 x 64            44        5  one chain
-//   backward bf16, 8 x 4096 x 1536      228      108  issue 37 %, LSU 22 %, 16 warps an SM
+//            bf16, 8 x 8192 x 1535      473      124  one CTA an SM (slots of twice the bytes)
+//   backward bf16, 8 x 4096 x 1536      230      108  issue 40 %, MUFU 29 %, 16 warps an SM
 // What it took for the bf16 forward at 8 x 8192: a thread a channel 6710 us, tiles 593,
 // rare paths out of the unrolled loops 401, one barrier a tile and 16-byte fetches 293, a
 // carrying warp 263, a and b through shared memory and more warps 235, tiles without marks
@@ -42,12 +43,13 @@ namespace {
 constexpr int STRIP = 64;                     // channels of a tile
 // Warps that hold a tile's tokens, tokens of each, of a tile; CTAs of an SM.  One more
 // warp of the CTA carries the states.  As many warps as registers (bf16) or shared memory
-// (fp32: twice the bytes a token) let two CTAs have.  Forward, 8 x 8192 bf16: 13 warps 202
+// (fp32: twice the bytes a token) let two CTAs have; bf16 rows off 16 bytes come through
+// fp32's slots in bf16's shape, of which one CTA fits an SM.  Forward, 8 x 8192 bf16: 13 warps 202
 // us, 11 210, 9 (three CTAs) 215, 14 212 (spills); 151 x 180 fp32: 10 warps 139, 8 134.  The
 // backward pass keeps more of a token in registers, and there fewer warps of longer runs
 // win, for less is composed and carried a token; 8 x 4096 with gradients, bf16: 12 warps of
 // 4 tokens 385 us, 7 of 8 346, 6 of 8 359, 5 of 8 (three CTAs) 379; fp32: 8 of 4 454, 5 of 8
-// 429 (at an odd width 190 and 211).
+// 429 (at an odd width 190 and 211); with 1 - sigmoid kept by itself 353 and 431.
 template <typename T> struct Forward {
     static constexpr int WARPS = sizeof(T) == 2 ? 13 : 8, RUN = 8, THREADS = 32 * WARPS;
     static constexpr int TILE = WARPS * RUN, CTAS = 2;

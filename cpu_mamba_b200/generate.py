@@ -32,8 +32,14 @@ class LogitRules:
     ``prompt_tokens`` (rows, n) int64 with optional ``prompt_lengths`` (rows,) starts the
     histories (they count for the repetition penalty only).  The penalties are numbers or
     float32 (rows,); bias_tokens and bias (rows, n) and mask (rows, ceil(vocab / 32)) are
-    as in ops.adjust_logits, and may be changed in place between steps.  In a beam search
-    of B requests the rows are its B x beams beams, beam j of request b in row b x beams + j."""
+    as in ops.adjust_logits, and may be changed in place between steps; a number is part
+    of a loop's graph and stays what it was.  Histories go on from call to call: a new
+    prompt takes new rules (or ``tokens``, ``lengths`` and ``prompt_lengths`` set anew).
+
+    In a beam search of B requests the rows are its B x beams beams, beam j of request b
+    in row b x beams + j.  A request's beams start alike, with one prompt and one set of
+    penalties and biases; their histories follow them, and their masks where rows have
+    masks of their own."""
 
     def __init__(self, rows: int, capacity: int, device="cuda",
                  prompt_tokens: Optional[torch.Tensor] = None,

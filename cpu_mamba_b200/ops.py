@@ -563,9 +563,9 @@ def gated_recurrence(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torc
     contiguous last index; the gates before their sigmoid, -inf closing one
     exactly); decay: float32 (D,); initial_state: float32 (N, D), zeros when None.
 
-    cu_seqlens (int, N + 1 offsets on the device that do not fall) packs N sequences
-    along T with B = 1; rows before the first and behind the last one are zero, in
-    the gradients too.  Otherwise N = B.
+    cu_seqlens (int32, or int64 of values that fit it; N + 1 offsets on the device that
+    do not fall) packs N sequences along T with B = 1; rows before the first and behind
+    the last one are zero, in the gradients too.  Otherwise N = B.
 
     Returns h (B, T, D) in x's dtype, with the final state (N, D) float32 when
     ``return_final_state``.  An empty sequence's final state is its initial one.

@@ -529,7 +529,8 @@ int mb2_reorder_rows(void *const *tensors, const int64_t *row_bytes, int64_t n_t
  * h (batch, seqlen, width) in dtype, contiguous, overlapping no input.  The state
  * is fp32: h0 and h_last (n_seqs, width), each NULL for zeros or for none;
  * n_seqs is batch without cu_seqlens.  A gate of -inf is closed exactly (an input
- * that counts nothing, a state that stays).
+ * that counts nothing, a state that stays), and so is an input gate below -88, whose
+ * sigmoid is below the normal numbers.
  * cu_seqlens (device, n_seqs + 1 offsets that do not fall) packs sequences along
  * seqlen with batch 1; offsets are clamped to 0 .. seqlen, an empty sequence's
  * h_last is its h0, and rows before the first and behind the last sequence are
